@@ -50,6 +50,16 @@ extern "C" {
 #define S1KV_DTYPE_F32 0  /* the reference's storage type (include/core/tensor.h:5) */
 #define S1KV_DTYPE_BF16 1 /* round-to-nearest-even narrowed on append; widened like
                              bf16_to_float (include/io/safetensors.h:156-161) */
+#define S1KV_DTYPE_Q4 2   /* 4 bits a value.  A row (head_dim values x of one token and KV head, lo and hi its
+                             least and greatest) is held as codes 0..15 and two bf16 numbers:
+                               m = bf16(fp32((7 lo + 8 hi) / 15)), to nearest even;
+                               s = fp32(max((hi - m) / 7, (m - lo) / 8)), rounded up to bf16;
+                               code = 8 + the integer nearest to (x - m) / s (ties to even; 8 where s = 0);
+                               value = fp32(m + s (code - 8)), within s / 2 of x.
+                             A row holding a NaN, an infinity or a magnitude beyond bf16's largest reads back
+                             as NaN throughout.  head_dim a multiple of 8 up to 256, block_size a multiple
+                             of 4.  Every call of a pool takes it; attention reads the held values with
+                             fp32-level accuracy.  The no-allocation decode takes F32 and BF16 storage only. */
 
 /* ---- pool flags ---- */
 #define S1KV_POOL_HOST_ONLY 1 /* bookkeeping only: no device memory; kernel calls fail */
@@ -110,7 +120,12 @@ int s1kv_pool_storage(const s1kv_pool* pool, int32_t layer, void** k_base, void*
 
 /* Synchronous copy of the raw bytes of storage slots [slot0, slot0 +
  * n_slots) of one layer's K (which = S1KV_K) or V into host memory
- * (n_slots * num_kv_heads * head_dim elements of the pool dtype). */
+ * (n_slots * num_kv_heads * head_dim elements of the pool dtype).  A 4-bit
+ * pool is read by whole blocks: slot0 and n_slots multiples of block_size,
+ * n_slots * num_kv_heads * (head_dim / 2 + 4) bytes in storage order: per
+ * block and KV head the codes of its tokens (K: [token][head_dim / 2], low
+ * nibble first; V: [token pair][head_dim / 4][2 tokens][2 bytes]), then per
+ * token bf16 s and bf16 m. */
 int s1kv_pool_read(s1kv_pool* pool, int32_t layer, int32_t which, int64_t slot0, int64_t n_slots, void* host_out);
 
 /* s1kv_pool_check for the device error word of CUDA device `device`
@@ -180,7 +195,9 @@ int s1kv_prefix_match(s1kv_pool* pool, uint64_t dst, const int32_t* tokens, int6
 uint64_t s1kv_block_hash(uint64_t parent, const int32_t* tokens, int64_t n);
 
 /* save_prefix_cache (src/demo.cpp:33-41): for every layer in order, writes
- * seq's K then V as raw fp32 [length][num_kv_heads][head_dim]. */
+ * seq's K then V as raw fp32 [length][num_kv_heads][head_dim].  (A 4-bit pool
+ * writes the held values; loading them quantises them anew, so use the
+ * versioned file below to keep its rows as they are.) */
 int s1kv_prefix_save(s1kv_pool* pool, uint64_t seq, const char* path);
 /* load_prefix_cache (src/demo.cpp:10-31): reads n_tokens tokens of that
  * layout and appends them to seq in every layer.  S1KV_EINVAL if the file
@@ -390,6 +407,10 @@ int s1kv_batch_norm_rope_append(s1kv_batch* batch, int32_t layer, const float* q
  * arrays), on which it differs from the correctly rounded x / d. */
 int s1kv_debug_div_check(const float* xs, int64_t nx, const float* ds, int64_t nd, unsigned long long* mismatch,
                          void* stream);
+/* The rows this batch appended to `layer`, as the pool holds them: out
+ * [n_tokens][num_kv_heads][head_dim] fp32 (device), in the order of k and v
+ * (get_k / get_v of kv_block_pool.cpp:67-132 for the step's tokens). */
+int s1kv_batch_gather(s1kv_batch* batch, int32_t layer, int32_t which, float* out, void* stream);
 /* Append without RoPE (KVBlockPool::append data movement). */
 int s1kv_batch_append(s1kv_batch* batch, int32_t layer, const float* k, const float* v, void* stream);
 /* Paged GQA attention of the batch's query rows (post-RoPE q).  For decode
@@ -442,6 +463,33 @@ int s1kv_matmul_int8(const float* x, int64_t M, int64_t K, const int8_t* q, cons
  * (host memory) hold device pointers. */
 int s1kv_matmul_int8_group(const float* x, int64_t M, int64_t K, int32_t n_mats, const int8_t* const* q,
                            const float* const* scales, const int64_t* N, float* const* out, void* stream);
+
+/* Products in 8-bit integers, one scale per token and per output channel (no
+ * reference counterpart: the reference's int8 product keeps x in fp32).  For
+ * prompts and large batches: the product above takes x 8 rows at a time, this
+ * one runs whole tiles of tokens on the integer tensor cores.
+ *
+ * s1kv_quantize_tokens: x [M][K] fp32 -> q [M][ldq] int8 and one scale per
+ * row, scale = fp32(max|row| / 127) (1 for an all-zero row), q = the integer
+ * nearest to x / scale, ties to even; columns K .. ldq - 1 are set to 0.  A
+ * row with a NaN or an infinity gets scale NaN and zeros, so its products
+ * are NaN.  ldq: a multiple of 16, K <= ldq <= 131072; q 16-byte aligned. */
+int s1kv_quantize_tokens(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scales, void* stream);
+/* out [M][N] fp32 = (xq [M][K] times w [N][K], summed exactly in 32-bit
+ * integers) * x_scales[m] * w_scales[n], the two products rounded to fp32 in
+ * that order; the same bits on every run.  Weights are rows of an output
+ * channel (an nn.Linear weight's order): s1kv_quantize_rows of that [N][K]
+ * matrix makes q and scales.  K is the padded row length: a multiple of 16
+ * up to 131072, xq zero past the true K (w may hold anything there); xq and w
+ * 16-byte aligned. */
+int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, const int8_t* w,
+                     const float* w_scales, int64_t N, float* out, void* stream);
+/* Up to 4 products sharing xq in one launch (q/k/v, gate/up): out[i]
+ * [M][N[i]], the same results as separate calls; the arrays (host memory)
+ * hold device pointers. */
+int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, int32_t n_mats,
+                           const int8_t* const* w, const float* const* w_scales, const int64_t* N, float* const* out,
+                           void* stream);
 
 /* ======================== introspection ======================== */
 

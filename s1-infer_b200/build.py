@@ -43,7 +43,7 @@ def _stale(out, deps):
 
 
 def _headers(d):
-    return [os.path.join(d, f) for f in os.listdir(d) if f.endswith(".h")]
+    return [os.path.join(d, f) for f in os.listdir(d) if f.endswith((".h", ".cuh"))]
 
 
 def _run(cmd):

@@ -291,6 +291,7 @@ static int batch_append_impl(s1kv_batch* b, int32_t layer, const float* q_in, fl
     ap.Hkv = p->desc.num_kv_heads;
     ap.Hq = Hq;
     ap.D = p->desc.head_dim;
+    ap.block_size = p->desc.block_size;
     ap.err = p->d_err;
     if (rope) {
         ap.rope = rope_table(p->device, p->desc.head_dim, p->desc.rope_theta, std::max<int64_t>(b->max_pos, 1),
@@ -344,6 +345,7 @@ int s1kv_batch_norm_rope_append(s1kv_batch* b, int32_t layer, const float* q_in,
     ap.Hkv = p->desc.num_kv_heads;
     ap.Hq = Hq;
     ap.D = p->desc.head_dim;
+    ap.block_size = p->desc.block_size;
     ap.err = p->d_err;
     ap.rope = rope_table(p->device, p->desc.head_dim, p->desc.rope_theta, std::max<int64_t>(b->max_pos, 1), &ap.rope_cap,
                          stream, &st);
@@ -496,8 +498,9 @@ int s1kv_batch_attention_exchange(s1kv_batch* b, int32_t layer, const float* q, 
     if (Hq <= 0 || Hq % Hkv) return set_error(S1KV_EINVAL, "n_q_heads must be a multiple of num_kv_heads");
     const int G = Hq / Hkv;
     if (!b->decode_rows || !q) return set_error(S1KV_EINVAL, "exchange: decode batches only (one query row per sequence)");
-    if (!p->tmap_ok || !(decode_mma_supported(p->desc.dtype, D, G, p->desc.block_size) ||
-                         tma_attention_supported(p->desc.dtype, D, G, p->desc.block_size)))
+    if (p->desc.dtype == S1KV_DTYPE_Q4 ? !decode_q4_supported(D, G, p->desc.block_size)
+                                       : !p->tmap_ok || !(decode_mma_supported(p->desc.dtype, D, G, p->desc.block_size) ||
+                                                          tma_attention_supported(p->desc.dtype, D, G, p->desc.block_size)))
         return set_error(S1KV_EINVAL, "exchange: shape not served by the split-K decode kernels");
     if (head0 < 0 || head0 + Hq > heads_total || (int64_t)b->n_rows * heads_total * D > ex->slot_floats)
         return set_error(S1KV_EINVAL, "exchange: rows x heads x head_dim exceed the exchange slot");
@@ -597,6 +600,7 @@ int s1kv_append(s1kv_pool* p, int32_t layer, const float* k, const float* v, con
     ap.n = n;
     ap.Hkv = p->desc.num_kv_heads;
     ap.D = p->desc.head_dim;
+    ap.block_size = p->desc.block_size;
     ap.err = p->d_err;
     return launch_append(ap, p->desc.dtype, false, (cudaStream_t)stream, false);
 }
@@ -625,6 +629,7 @@ int s1kv_rope_append(s1kv_pool* p, int32_t layer, const float* q_in, float* q_ou
     ap.Hkv = p->desc.num_kv_heads;
     ap.Hq = Hq;
     ap.D = p->desc.head_dim;
+    ap.block_size = p->desc.block_size;
     ap.err = p->d_err;
     // Without an explicit bound the positions are token indices of
     // sequences in this pool, so the longest sequence bounds them; the
@@ -663,6 +668,18 @@ int s1kv_gather(s1kv_pool* p, int32_t layer, uint64_t seq, int32_t which, float*
     st = flush(p, (cudaStream_t)stream);
     if (st) return st;
     return launch_gather(p, layer, row, len, which, out, (cudaStream_t)stream);
+}
+
+int s1kv_batch_gather(s1kv_batch* b, int32_t layer, int32_t which, float* out, void* stream) {
+    if (!b) return set_error(S1KV_EINVAL, "null batch");
+    s1kv_pool* p = b->pool;
+    int st = check_layer(p, layer);
+    if (st) return st;
+    if (which != S1KV_K && which != S1KV_V) return set_error(S1KV_EINVAL, "s1kv_batch_gather: which is S1KV_K or S1KV_V");
+    if (b->n_tokens == 0) return S1KV_OK;
+    if (!out) return set_error(S1KV_EINVAL, "s1kv_batch_gather: null out");
+    S1KV_ON_DEVICE(p->device);
+    return launch_gather_slots(p, layer, b->d_slots, b->n_tokens, which, out, (cudaStream_t)stream);
 }
 
 int s1kv_cow_copy(s1kv_pool* p, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
@@ -739,7 +756,10 @@ int s1kv_pool_read(s1kv_pool* p, int32_t layer, int32_t which, int64_t slot0, in
         return set_error(S1KV_EINVAL, "s1kv_pool_read: slot range out of bounds");
     S1KV_ON_DEVICE(p->device);
     S1KV_CUDA(cudaDeviceSynchronize());
-    const size_t row = (size_t)p->desc.num_kv_heads * p->desc.head_dim * p->elem;
+    const int64_t bs = p->desc.block_size;
+    if (p->desc.dtype == S1KV_DTYPE_Q4 && (slot0 % bs || n_slots % bs))
+        return set_error(S1KV_EINVAL, "s1kv_pool_read: a 4-bit pool is read by whole blocks");
+    const size_t row = p->block_bytes / bs;  // 4-bit: a slot's share of its block
     const char* base = (which ? p->v : p->k) + (size_t)layer * p->layer_bytes + (size_t)slot0 * row;
     S1KV_CUDA(cudaMemcpy(host_out, base, (size_t)n_slots * row, cudaMemcpyDeviceToHost));
     return S1KV_OK;

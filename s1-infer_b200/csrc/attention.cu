@@ -635,6 +635,7 @@ int launch_attention_generic(const AttnParams& p, int dtype, cudaStream_t stream
 
 int launch_attention(s1kv_pool* pool, const AttnParams& p, int dtype, cudaStream_t stream) {
     if (p.n_rows <= 0) return S1KV_OK;
+    if (dtype == S1KV_DTYPE_Q4) return launch_decode_q4(p, stream);
     const int G = p.Hq / p.Hkv;
     if (p.table && pool->tmap_sw_ok && p.items && decode_mma_supported(dtype, p.D, G, p.block_size)) {
         // bf16 K/V, head_dim 128: tensor-core decode, then the shared combine
@@ -662,6 +663,7 @@ int launch_attention(s1kv_pool* pool, const AttnParams& p, int dtype, cudaStream
 // the kernels' chunk assignment is already conflict-free.
 int make_tensor_maps(s1kv_pool* p) {
     p->tmap_ok = false;
+    if (p->desc.dtype == S1KV_DTYPE_Q4) return S1KV_OK;  // plain loads in fragment order (q4_decode.cu)
     const int D = p->desc.head_dim;
     if (p->desc.block_size != 16 || !(D == 64 || D == 128)) return S1KV_OK;  // generic kernel only
     static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;

@@ -215,6 +215,7 @@ struct AppendParams {
     int64_t num_slots;
     int64_t n;
     int32_t Hkv, Hq, D;
+    int32_t block_size;    // 4-bit pools (a row's place inside its block's tile)
     int* err;
 };
 
@@ -289,7 +290,8 @@ struct s1kv_pool {
     // device storage
     char* k = nullptr;
     char* v = nullptr;
-    size_t elem = 4;
+    size_t elem = 4;          // bytes of one element (0: 4-bit rows, see q4.cuh)
+    size_t block_bytes = 0;   // bytes of one block of one layer of K (or V)
     size_t layer_bytes = 0;   // bytes of one layer of K (or V)
     int64_t num_slots = 0;    // max_blocks * block_size
     int32_t* d_table = nullptr;
@@ -399,6 +401,9 @@ int launch_rope(const float* x, float* out, const float2* table, int64_t table_c
                 int32_t H, int32_t D, int* err, cudaStream_t stream, const int32_t* pos = nullptr);
 int launch_gather(s1kv_pool* pool, int32_t layer, int32_t row, int64_t len, int which, float* out,
                   cudaStream_t stream);
+// The rows at slots[n] (device) as fp32.
+int launch_gather_slots(s1kv_pool* pool, int32_t layer, const int32_t* slots, int64_t n, int which, float* out,
+                        cudaStream_t stream);
 // Paged attention over a prepared work list; picks the TMA split-K decode
 // kernel when the shape allows it and the generic kernel otherwise.
 int launch_attention(s1kv_pool* pool, const AttnParams& p, int dtype, cudaStream_t stream);
@@ -426,6 +431,17 @@ int launch_decode_mma(const AttnParams& p, const CUtensorMap& tk_sw, const CUten
 // Exchange fields of a decode launch that publishes its rows (exchange.cu).
 int exchange_params(const s1kv_exchange* ex, uint32_t epoch, int32_t head0, int32_t heads_total, AttnParams* ap);
 void exchange_record(s1kv_exchange* ex, uint32_t epoch, int64_t words);
+
+// 4-bit pools (q4_kernels.cu, q4_decode.cu).
+int launch_append_q4(const AppendParams& p, bool rope, cudaStream_t stream, bool pdl);
+// Tokens of a block-table row (trow) or at slots (device) as fp32 rows.
+int launch_gather_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const int32_t* slots, int64_t n, int which,
+                     float* out, cudaStream_t stream);
+// Byte rows of prefix files, read from (trow) or written to (slots) the pool.
+int launch_rows_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const int32_t* slots, int64_t n, int which,
+                   void* rows, bool to_pool, cudaStream_t stream);
+bool decode_q4_supported(int D, int G, int block_size);
+int launch_decode_q4(const AttnParams& p, cudaStream_t stream);
 
 // Tensor-core prefix-hit prefill (prefill_tc.cu).
 bool prefill_tc_supported(int dtype, int D, int G, int block_size);

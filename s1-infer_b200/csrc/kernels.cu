@@ -13,6 +13,7 @@
 #include <unordered_map>
 
 #include "internal.h"
+#include "q4.cuh"
 
 namespace s1kv {
 
@@ -81,7 +82,7 @@ __global__ void cow_kernel(const int32_t* __restrict__ src, const int32_t* __res
 
 int launch_cow(s1kv_pool* p, const int32_t* d_src, const int32_t* d_dst, int64_t n, cudaStream_t stream) {
     if (n <= 0) return S1KV_OK;
-    size_t block_bytes = (size_t)p->desc.block_size * p->desc.num_kv_heads * p->desc.head_dim * p->elem;
+    const size_t block_bytes = p->block_bytes;
     if (block_bytes % 16)
         return set_error(S1KV_EINVAL, "s1kv_cow_copy: block bytes (%zu) not a multiple of 16", block_bytes);
     int64_t total = n * p->desc.num_layers * 2 * (int64_t)(block_bytes / 16);
@@ -247,6 +248,7 @@ static bool aligned16(const void* ptr) { return ((uintptr_t)ptr & 15) == 0; }
 int launch_append(const AppendParams& p, int dtype, bool rope, cudaStream_t stream, bool pdl) {
     if (p.n <= 0) return S1KV_OK;
     if (rope && (p.D % 2)) return set_error(S1KV_EINVAL, "RoPE needs an even head_dim");
+    if (dtype == S1KV_DTYPE_Q4) return launch_append_q4(p, rope, stream, pdl);
     bool vec = (p.D % 16 == 0) && aligned16(p.k) && aligned16(p.v) && (!p.q_in || (aligned16(p.q_in) && aligned16(p.q_out)));
     int64_t units = vec ? (2 * p.n * p.Hkv + (rope && p.q_in ? p.n * p.Hq : 0)) * (p.D / 16)
                         : (2 * p.n * p.Hkv + (rope && p.q_in ? p.n * p.Hq : 0)) * p.D;
@@ -393,6 +395,25 @@ __global__ void __launch_bounds__(256) norm_rope_append_kernel(const AppendParam
             for (int idx = lane; idx < nr * C4; idx += 32)
                 *reinterpret_cast<float4*>(dst + (int64_t)idx * 4) =
                     *reinterpret_cast<const float4*>(tile + (idx / C4) * RS + (idx % C4) * 4);
+        } else if constexpr (sizeof(T) == 1) {
+            // 4-bit rows (q4.cuh): D / 4 lanes quantise a row, four values each
+            constexpr int LANES = D / 4, RPW = 32 / LANES;
+            for (int r = lane / LANES; r - lane / LANES < nr; r += RPW) {  // warp-uniform trip count (shuffles inside)
+                const int rr = min(r, nr - 1);
+                const int64_t th = r0 + rr;
+                const int32_t slot = p.slots[th / H];
+                // a K row whose position was out of range stays unwritten
+                bool store = r < nr && (part == 2 || (uint64_t)p.pos[th / H] < (uint64_t)p.rope_cap);
+                if ((uint64_t)slot >= (uint64_t)p.num_slots) {
+                    if (r < nr && lane % LANES == 0) flag_error(p.err, kErrBounds);
+                    store = false;
+                }
+                int t = 0;
+                char* at = store ? q4_tile(part == 1 ? p.kpool : p.vpool, slot, (int)(th % H), H, p.block_size, D, &t) : nullptr;
+                const float4 a = *reinterpret_cast<const float4*>(tile + rr * RS + 4 * (lane % LANES));
+                const float x[1][4] = {{a.x, a.y, a.z, a.w}};
+                q4_store_row<LANES, 1>(x, LANES, at, t, part == 2, p.block_size, D, store);
+            }
         } else {
             // four elements per lane: 8-byte (bf16) or 16-byte stores; lane i
             // looks up row i's slot once and the warp shares it by shuffle
@@ -435,9 +456,11 @@ int launch_norm_rope_append(const AppendParams& p, int dtype, const float* qw, c
     } while (0)
     if (p.D == 128) {
         if (dtype == S1KV_DTYPE_F32) S1KV_NRA(float, 128);
+        else if (dtype == S1KV_DTYPE_Q4) S1KV_NRA(uint8_t, 128);
         else S1KV_NRA(uint16_t, 128);
     } else if (p.D == 64) {
         if (dtype == S1KV_DTYPE_F32) S1KV_NRA(float, 64);
+        else if (dtype == S1KV_DTYPE_Q4) S1KV_NRA(uint8_t, 64);
         else S1KV_NRA(uint16_t, 64);
     } else {
         return set_error(S1KV_EINVAL, "norm_rope_append: head_dim %d (64 or 128 supported)", p.D);
@@ -504,6 +527,8 @@ __global__ void gather_kernel(const T* __restrict__ pool, const int32_t* __restr
 
 int launch_gather(s1kv_pool* p, int32_t layer, int32_t row, int64_t len, int which, float* out, cudaStream_t stream) {
     if (len <= 0) return S1KV_OK;
+    if (p->desc.dtype == S1KV_DTYPE_Q4)
+        return launch_gather_q4(p, layer, p->d_table + (int64_t)row * p->max_bps, nullptr, len, which, out, stream);
     const char* base = (which ? p->v : p->k) + (size_t)layer * p->layer_bytes;
     const int32_t* trow = p->d_table + (int64_t)row * p->max_bps;
     int row_elems = p->desc.num_kv_heads * p->desc.head_dim;
@@ -515,6 +540,42 @@ int launch_gather(s1kv_pool* p, int32_t layer, int32_t row, int64_t len, int whi
     else
         gather_kernel<uint16_t><<<grid, 256, 0, stream>>>((const uint16_t*)base, trow, len, p->desc.block_size,
                                                          row_elems, (int32_t)p->desc.max_blocks, out, p->d_err);
+    g_launches++;
+    S1KV_CUDA(cudaGetLastError());
+    return S1KV_OK;
+}
+
+// The rows at slots[i] (a batch's appended tokens), widened to fp32.
+template <typename T>
+__global__ void gather_slots_kernel(const T* __restrict__ pool, const int32_t* __restrict__ slots, int64_t n, int row_elems,
+                                    int64_t num_slots, float* __restrict__ out, int* err) {
+    const int64_t total = n * row_elems;
+    for (int64_t u = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; u < total; u += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t i = u / row_elems, slot = slots[i];
+        if ((uint64_t)slot >= (uint64_t)num_slots) {
+            flag_error(err, kErrBounds);
+            out[u] = 0.0f;
+            continue;
+        }
+        const int64_t src = slot * row_elems + (u - i * row_elems);
+        if constexpr (sizeof(T) == 4) out[u] = reinterpret_cast<const float*>(pool)[src];
+        else out[u] = bf16_to_f32(reinterpret_cast<const uint16_t*>(pool)[src]);
+    }
+}
+
+int launch_gather_slots(s1kv_pool* p, int32_t layer, const int32_t* slots, int64_t n, int which, float* out,
+                        cudaStream_t stream) {
+    if (n <= 0) return S1KV_OK;
+    if (p->desc.dtype == S1KV_DTYPE_Q4) return launch_gather_q4(p, layer, nullptr, slots, n, which, out, stream);
+    const char* base = (which ? p->v : p->k) + (size_t)layer * p->layer_bytes;
+    const int row_elems = p->desc.num_kv_heads * p->desc.head_dim;
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((n * row_elems + 255) / 256, kSMs * 16));
+    if (p->desc.dtype == S1KV_DTYPE_F32)
+        gather_slots_kernel<float><<<grid, 256, 0, stream>>>((const float*)base, slots, n, row_elems, p->num_slots, out,
+                                                             p->d_err);
+    else
+        gather_slots_kernel<uint16_t><<<grid, 256, 0, stream>>>((const uint16_t*)base, slots, n, row_elems, p->num_slots,
+                                                                out, p->d_err);
     g_launches++;
     S1KV_CUDA(cudaGetLastError());
     return S1KV_OK;

@@ -403,8 +403,12 @@ int s1kv_pool_create(const s1kv_pool_desc* d, int device, s1kv_pool** out) {
     if (!d || !out) return set_error(S1KV_EINVAL, "s1kv_pool_create: null argument");
     *out = nullptr;
     if (d->num_layers < 1 || d->num_kv_heads < 1 || d->head_dim < 1 || d->block_size < 1 || d->max_blocks < 1 ||
-        d->max_blocks > INT32_MAX / 2 || (d->dtype != S1KV_DTYPE_F32 && d->dtype != S1KV_DTYPE_BF16))
+        d->max_blocks > INT32_MAX / 2 ||
+        (d->dtype != S1KV_DTYPE_F32 && d->dtype != S1KV_DTYPE_BF16 && d->dtype != S1KV_DTYPE_Q4))
         return set_error(S1KV_EINVAL, "s1kv_pool_create: bad descriptor");
+    if (d->dtype == S1KV_DTYPE_Q4 && (d->head_dim % 8 || d->head_dim > 256 || d->block_size % 4))
+        return set_error(S1KV_EINVAL, "s1kv_pool_create: a 4-bit pool needs a head_dim that is a multiple of 8 up to 256 "
+                                      "and a block_size that is a multiple of 4");
     int64_t slots = d->max_blocks * (int64_t)d->block_size;
     if (slots > INT32_MAX) return set_error(S1KV_EINVAL, "s1kv_pool_create: more than 2^31 slots per layer");
     auto* p = new s1kv_pool();
@@ -415,11 +419,14 @@ int s1kv_pool_create(const s1kv_pool_desc* d, int device, s1kv_pool** out) {
     if (p->desc.rope_theta == 0.0f) p->desc.rope_theta = 1.0e6f;
     p->device = device;
     p->host_only = (d->flags & S1KV_POOL_HOST_ONLY) != 0;
-    p->elem = d->dtype == S1KV_DTYPE_F32 ? 4 : 2;
+    p->elem = d->dtype == S1KV_DTYPE_F32 ? 4 : d->dtype == S1KV_DTYPE_BF16 ? 2 : 0;
     p->num_slots = slots;
     p->max_bps = (int32_t)std::min<int64_t>((p->desc.max_seq_len + d->block_size - 1) / d->block_size,
                                             d->max_blocks);
-    p->layer_bytes = (size_t)slots * d->num_kv_heads * d->head_dim * p->elem;
+    // one row: head_dim elements, or 4-bit codes and the row's scale and centre
+    const size_t row_bytes = d->dtype == S1KV_DTYPE_Q4 ? (size_t)d->head_dim / 2 + 4 : (size_t)d->head_dim * p->elem;
+    p->block_bytes = (size_t)d->block_size * d->num_kv_heads * row_bytes;
+    p->layer_bytes = p->block_bytes * d->max_blocks;
     // Free list bottom .. top; the reference pushes 0..max_blocks-1 in order.
     p->free_list.resize(d->max_blocks);
     if (d->initial_free_list) {

@@ -15,7 +15,7 @@
 //       20     4  num_kv_heads
 //       24     4  head_dim
 //       28     4  block_size of the writing pool (informational)
-//       32     4  dtype of the payload (S1KV_DTYPE_F32 or S1KV_DTYPE_BF16)
+//       32     4  dtype of the payload (S1KV_DTYPE_*)
 //       36     4  flags (bit 0: token ids present)
 //       40     8  n_tokens
 //       48     4  rope_theta (float)
@@ -23,7 +23,11 @@
 //       56     8  FNV-1a 64 of every byte after the header
 //       64        int32 token_ids[n_tokens] if flag bit 0
 //                 then per layer: K [n_tokens][num_kv_heads][head_dim],
-//                 V the same, in the payload dtype (bf16 stays 2 bytes)
+//                 V the same, in the payload dtype (bf16 stays 2 bytes; a
+//                 4-bit row is head_dim / 2 bytes of codes, low nibble
+//                 first, then bf16 s and bf16 m, and goes back into a 4-bit
+//                 pool unchanged)
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -31,6 +35,9 @@
 #include "internal.h"
 
 namespace s1kv {
+int flush(s1kv_pool* p, cudaStream_t stream);
+int seq_row(const s1kv_pool* p, uint64_t id, int32_t* row, int64_t* len);
+
 namespace {
 
 constexpr char kMagic[8] = {'S', '1', 'K', 'V', 'P', 'F', 'X', '\0'};
@@ -67,8 +74,15 @@ float from_bf16(uint16_t b) {
     return f;
 }
 
-// Reads and checks a whole file: header, token ids, payload as fp32.
-int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, std::vector<float>* payload) {
+// Bytes of one token's K (or V) of all heads in the payload.
+uint64_t payload_row(uint32_t dtype, uint64_t heads, uint64_t dim) {
+    return dtype == S1KV_DTYPE_Q4 ? heads * (dim / 2 + 4) : heads * dim * (dtype == S1KV_DTYPE_F32 ? 4 : 2);
+}
+
+// Reads and checks a whole file: header, token ids, payload as fp32 and as
+// it stands in the file.
+int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, std::vector<float>* payload,
+              std::vector<unsigned char>* raw = nullptr) {
     FILE* f = std::fopen(path, "rb");
     if (!f) return set_error(S1KV_EINVAL, "prefix file: cannot open %s", path);
     std::vector<unsigned char> all;
@@ -83,13 +97,14 @@ int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, st
     if (hd->version != kVersion || hd->header_bytes != kHeaderBytes)
         return set_error(S1KV_EINVAL, "prefix file %s: version %u / header %u not supported", path, hd->version,
                          hd->header_bytes);
-    if ((hd->dtype != S1KV_DTYPE_F32 && hd->dtype != S1KV_DTYPE_BF16) || hd->n_tokens < 0 || hd->head_dim == 0 ||
-        hd->num_kv_heads == 0 || hd->num_layers == 0)
+    if ((hd->dtype != S1KV_DTYPE_F32 && hd->dtype != S1KV_DTYPE_BF16 &&
+         (hd->dtype != S1KV_DTYPE_Q4 || hd->head_dim % 8)) ||
+        hd->n_tokens < 0 || hd->head_dim == 0 || hd->num_kv_heads == 0 || hd->num_layers == 0)
         return set_error(S1KV_EINVAL, "prefix file %s: bad header fields", path);
-    const uint64_t e = hd->dtype == S1KV_DTYPE_F32 ? 4 : 2;
     const uint64_t row = (uint64_t)hd->num_kv_heads * hd->head_dim;
+    const uint64_t row_bytes = payload_row(hd->dtype, hd->num_kv_heads, hd->head_dim);
     const uint64_t tok_bytes = (hd->flags & kHasTokens) ? (uint64_t)hd->n_tokens * 4 : 0;
-    const uint64_t body = tok_bytes + 2ull * hd->num_layers * (uint64_t)hd->n_tokens * row * e;
+    const uint64_t body = tok_bytes + 2ull * hd->num_layers * (uint64_t)hd->n_tokens * row_bytes;
     if (all.size() - kHeaderBytes != body)
         return set_error(S1KV_EINVAL, "prefix file %s: %llu payload bytes, header says %llu", path,
                          (unsigned long long)(all.size() - kHeaderBytes), (unsigned long long)body);
@@ -102,11 +117,21 @@ int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, st
         if (tok_bytes) std::memcpy(tokens->data(), p, tok_bytes);
     }
     p += tok_bytes;
+    if (raw) raw->assign(p, p + (body - tok_bytes));
     if (payload) {
         const uint64_t n = 2ull * hd->num_layers * (uint64_t)hd->n_tokens * row;
         payload->resize(n);
-        if (e == 4) {
+        if (hd->dtype == S1KV_DTYPE_F32) {
             std::memcpy(payload->data(), p, n * 4);
+        } else if (hd->dtype == S1KV_DTYPE_Q4) {
+            const uint64_t D = hd->head_dim;
+            for (uint64_t r = 0; r < n / D; r++, p += D / 2 + 4) {
+                uint16_t sm[2];
+                std::memcpy(sm, p + D / 2, 4);
+                const float s = from_bf16(sm[0]), m = from_bf16(sm[1]);
+                for (uint64_t d = 0; d < D; d++)
+                    (*payload)[r * D + d] = std::fmaf(s, (float)((int)(p[d / 2] >> (4 * (d & 1)) & 15) - 8), m);
+            }
         } else {
             for (uint64_t i = 0; i < n; i++) {
                 uint16_t b;
@@ -128,6 +153,7 @@ extern "C" {
 int s1kv_prefix_save_v1(s1kv_pool* p, uint64_t seq, const int32_t* token_ids, const char* path) {
     if (!p || !path) return set_error(S1KV_EINVAL, "s1kv_prefix_save_v1: null argument");
     if (p->host_only) return set_error(S1KV_EINVAL, "s1kv: host-only pool has no device storage");
+    S1KV_ON_DEVICE(p->device);
     const int64_t len = s1kv_seq_length(p, seq);
     if (!s1kv_seq_exists(p, seq)) return set_error(S1KV_ENOSEQ, "s1kv_prefix_save_v1: unknown sequence");
     const size_t row = (size_t)p->desc.num_kv_heads * p->desc.head_dim, n = (size_t)len * row;
@@ -150,7 +176,20 @@ int s1kv_prefix_save_v1(s1kv_pool* p, uint64_t seq, const int32_t* token_ids, co
     float* d = nullptr;
     cudaError_t e = cudaMalloc(&d, std::max<size_t>(n, 1) * sizeof(float));
     int st = S1KV_OK;
-    for (int32_t l = 0; l < p->desc.num_layers && e == cudaSuccess && st == S1KV_OK; l++) {
+    if (e == cudaSuccess && p->desc.dtype == S1KV_DTYPE_Q4) {
+        const size_t bytes = (size_t)len * payload_row(hd.dtype, hd.num_kv_heads, hd.head_dim);
+        int32_t trow = 0;
+        int64_t n_tok = 0;
+        st = flush(p, nullptr);
+        if (!st) st = seq_row(p, seq, &trow, &n_tok);
+        for (int32_t i = 0; i < 2 * p->desc.num_layers && e == cudaSuccess && st == S1KV_OK; i++) {
+            st = launch_rows_q4(p, i / 2, p->d_table + (int64_t)trow * p->max_bps, nullptr, len, i % 2, d, false, nullptr);
+            const size_t at = body.size();
+            body.resize(at + bytes);
+            if (!st) e = cudaMemcpy(body.data() + at, d, bytes, cudaMemcpyDeviceToHost);
+        }
+    }
+    for (int32_t l = 0; l < p->desc.num_layers && e == cudaSuccess && st == S1KV_OK && p->desc.dtype != S1KV_DTYPE_Q4; l++) {
         for (int which = 0; which < 2 && st == S1KV_OK; which++) {
             st = s1kv_gather(p, l, seq, which, d, nullptr);
             if (st) break;
@@ -204,7 +243,8 @@ int s1kv_prefix_load_v1(s1kv_pool* p, uint64_t seq, const char* path, int32_t re
     FileHeader hd{};
     std::vector<int32_t> tokens;
     std::vector<float> payload;
-    int st = read_file(path, &hd, &tokens, &payload);
+    std::vector<unsigned char> raw;
+    int st = read_file(path, &hd, &tokens, &payload, &raw);
     if (st) return st;
     if ((int32_t)hd.num_layers != p->desc.num_layers || (int32_t)hd.num_kv_heads != p->desc.num_kv_heads ||
         (int32_t)hd.head_dim != p->desc.head_dim)
@@ -217,6 +257,7 @@ int s1kv_prefix_load_v1(s1kv_pool* p, uint64_t seq, const char* path, int32_t re
     if (register_blocks && !(hd.flags & kHasTokens))
         return set_error(S1KV_EINVAL, "prefix file %s: no token ids to register", path);
     if (s1kv_seq_exists(p, seq)) return set_error(S1KV_EINVAL, "s1kv_prefix_load_v1: sequence exists");
+    S1KV_ON_DEVICE(p->device);
     const int64_t n_tok = hd.n_tokens;
     const size_t n = (size_t)n_tok * p->desc.num_kv_heads * p->desc.head_dim;
     s1kv_batch* b = nullptr;
@@ -225,7 +266,15 @@ int s1kv_prefix_load_v1(s1kv_pool* p, uint64_t seq, const char* path, int32_t re
     if (st) return st;
     float* d = nullptr;
     cudaError_t e = cudaMalloc(&d, std::max<size_t>(2 * n, 1) * sizeof(float));
-    for (int32_t l = 0; l < p->desc.num_layers && e == cudaSuccess && st == S1KV_OK; l++) {
+    // a 4-bit file's rows go into a 4-bit pool as they are
+    const bool as_is = hd.dtype == S1KV_DTYPE_Q4 && p->desc.dtype == S1KV_DTYPE_Q4;
+    const size_t bytes = (size_t)n_tok * payload_row(hd.dtype, hd.num_kv_heads, hd.head_dim);
+    for (int32_t i = 0; i < 2 * p->desc.num_layers && as_is && e == cudaSuccess && st == S1KV_OK; i++) {
+        e = cudaMemcpy(d, raw.data() + bytes * i, bytes, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) st = launch_rows_q4(p, i / 2, nullptr, b->d_slots, n_tok, i % 2, d, true, nullptr);
+        if (e == cudaSuccess && st == S1KV_OK) e = cudaDeviceSynchronize();
+    }
+    for (int32_t l = 0; l < p->desc.num_layers && !as_is && e == cudaSuccess && st == S1KV_OK; l++) {
         e = cudaMemcpy(d, payload.data() + 2 * n * l, 2 * n * sizeof(float), cudaMemcpyHostToDevice);
         if (e == cudaSuccess) st = s1kv_batch_append(b, l, d, d + n, nullptr);
         if (e == cudaSuccess && st == S1KV_OK) e = cudaDeviceSynchronize();

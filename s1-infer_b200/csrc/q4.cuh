@@ -1,0 +1,144 @@
+// q4.cuh -- the 4-bit K/V row format (device code shared by the append,
+// gather and attention kernels of S1KV_DTYPE_Q4 pools).
+//
+// A row is the D values x of one token and KV head.  With lo, hi its least
+// and greatest value:
+//   m = bf16(fp32((7 lo + 8 hi) / 15))          both to nearest even
+//   s = fp32(max((hi - m) / 7, (m - lo) / 8)) rounded UP to bf16
+//   code = 8 + nearest integer to (x - m) / s   (ties to even; 8 where s = 0 or NaN)
+//   held value = fp32(m + s (code - 8))
+// The codes -8 .. 7 around m reach lo and hi because s is rounded up, so
+// every held value is within s / 2 of x, with no clipping, whatever the
+// row's offset.  One (s, m) pair a row (4 bytes beside D / 2 bytes of codes)
+// keeps K's scale and zero term out of the tensor-core products: they act
+// on whole scores.  bf16 for both because its range is fp32's; the bound
+// above holds for the rounded pair.  A row with a NaN or an infinity (or a
+// value beyond bf16's largest, 3.39e38) is held as s = m = NaN: the whole
+// row reads back as NaN.
+//
+// Storage: one tile per (block, KV head), K and V apart:
+//   codes  bs * D / 2 bytes, then the rows' params  bs * {bf16 s, bf16 m}.
+//   K codes [token][D / 2]: nibble n of the row is value n (low first).
+//   V codes [token pair][D / 4][2 tokens][2 bytes]: four values (a quad) of
+//   a token are 16 bits, and a pair's tokens lie side by side in one 32-bit
+//   word: that word holds, for four dims, the two adjacent tokens that one
+//   fp16x2 register of a tensor-core fragment needs (K runs over dims, V
+//   over tokens), and no byte belongs to two tokens, so tokens of one tile
+//   may be appended by different threads, calls and launches.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "internal.h"
+
+namespace s1kv {
+
+struct Q4Row {  // one row's parameters
+    float s, m;
+    uint32_t packed;  // bf16 s | bf16 m << 16, as stored
+};
+
+__device__ __forceinline__ uint32_t q4_bf16_rn(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// (s, m) of a row from its extremes; `finite`: no value is NaN or infinite.
+// In 64 bits so that each of the two fp32 values is the real number's
+// rounding (the products by 1/15 and 1/7 are off by 2^-53).
+__device__ __forceinline__ Q4Row q4_params(float lo, float hi, bool finite) {
+    Q4Row r;
+    const double l = lo, h = hi;
+    const uint32_t mb = q4_bf16_rn(__double2float_rn((7.0 * l + 8.0 * h) * (1.0 / 15.0)));
+    r.m = __uint_as_float(mb << 16);
+    const double m = r.m;
+    const float need = __double2float_rn(fmax((h - m) * (1.0 / 7.0), (m - l) * 0.125));
+    const uint32_t sb = (__float_as_uint(need) + 0xFFFFu) >> 16;  // need >= 0: up
+    r.s = __uint_as_float(sb << 16);
+    if (!finite || !(r.s < INFINITY) || !(fabsf(r.m) < INFINITY)) {
+        r.packed = 0x7FC07FC0u;
+        r.s = r.m = __uint_as_float(0x7FC00000u);
+        return r;
+    }
+    r.packed = sb | (mb << 16);
+    return r;
+}
+
+// 0 .. 15; inv = 1 / s.  The fp32 quotient is within 2e-6 of the real one
+// (|q| < 8.6, three roundings): only one this near a tie (or not finite,
+// for a tiny s) is decided in 64 bits.
+__device__ __forceinline__ uint32_t q4_code(float x, const Q4Row& r, float inv) {
+    const float q = (x - r.m) * inv;
+    float n = rintf(q);
+    if (!(fabsf(q - n) < 0.49998f)) {
+        n = 0.0f;
+        if (r.s > 0.0f) n = (float)rint(((double)x - (double)r.m) / (double)r.s);
+    }
+    return (uint32_t)((int)fminf(fmaxf(n, -8.0f), 7.0f) + 8) & 15u;
+}
+
+__device__ __forceinline__ float q4_value(uint32_t code, float s, float m) {
+    return fmaf(s, (float)((int)code - 8), m);  // the product is exact (8 x 4 bits): one rounding
+}
+
+__device__ __forceinline__ float2 q4_unpack(uint32_t packed) {  // (s, m)
+    return make_float2(__uint_as_float(packed << 16), __uint_as_float(packed & 0xFFFF0000u));
+}
+
+// Bytes of one (block, KV head) tile and offsets inside it.
+__host__ __device__ __forceinline__ int q4_tile_bytes(int bs, int D) { return bs * (D / 2 + 4); }
+__device__ __forceinline__ int q4_k_quad(int t, int quad, int D) { return t * (D / 2) + quad * 2; }
+__device__ __forceinline__ int q4_v_quad(int t, int quad, int D) { return (t >> 1) * D + quad * 4 + (t & 1) * 2; }
+__device__ __forceinline__ int q4_param(int t, int bs, int D) { return bs * (D / 2) + t * 4; }
+
+// Tile of (slot, head) in one layer's storage and the token's place in it.
+__device__ __forceinline__ char* q4_tile(void* base, int64_t slot, int h, int Hkv, int bs, int D, int* t) {
+    const int64_t blk = slot / bs;
+    *t = (int)(slot - blk * bs);
+    return reinterpret_cast<char*>(base) + (blk * Hkv + h) * q4_tile_bytes(bs, D);
+}
+
+// Quantises one row held by `LANES` adjacent lanes of a warp, NQ quads a
+// lane (quad lane_in_row + i * LANES; quads from nq on are absent), and
+// stores it.  Every lane of the warp calls it; `store` is false for lanes
+// whose row is absent or out of range.
+template <int LANES, int NQ>
+__device__ __forceinline__ void q4_store_row(const float (&x)[NQ][4], int nq, char* tile, int t, bool is_v, int bs, int D,
+                                             bool store) {
+    const int lr = threadIdx.x % LANES;
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+        if (lr + i * LANES < nq) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                lo = fminf(lo, x[i][e]);
+                hi = fmaxf(hi, x[i][e]);
+                bad |= !(fabsf(x[i][e]) < INFINITY);
+            }
+        }
+    // a bad value spoils the row's maximum, which then spoils the row
+    if (bad) hi = INFINITY;
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const Q4Row r = q4_params(lo, hi, hi < INFINITY);
+    const float inv = __frcp_rn(r.s);
+    if (!store) return;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int quad = lr + i * LANES;
+        if (quad >= nq) continue;
+        uint32_t c = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) c |= q4_code(x[i][e], r, inv) << (4 * e);
+        *reinterpret_cast<uint16_t*>(tile + (is_v ? q4_v_quad(t, quad, D) : q4_k_quad(t, quad, D))) = (uint16_t)c;
+    }
+    if (lr == 0) *reinterpret_cast<uint32_t*>(tile + q4_param(t, bs, D)) = r.packed;
+}
+
+}  // namespace s1kv

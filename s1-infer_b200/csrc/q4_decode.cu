@@ -1,0 +1,488 @@
+// q4_decode.cu -- paged split-K GQA attention over a 4-bit cache (format:
+// q4.cuh) on warp-level tensor-core instructions (mma.sync m16n8k16, fp16 x
+// fp16 -> fp32).
+//
+// With u the raw codes, k = m_k + s_k (u - 8) and v = m_v + s_v (u - 8):
+//   score_t = s_k (q . u_t) + (m_k - 8 s_k) sum(q)
+//   out     = sum_t (p_t s_v) (u_t - 8) + sum_t p_t m_v,   over sum_t p_t
+// so the products run over small integers, exact in fp16, and the scales
+// act on scores.  V's codes are centred before the product (out is a small
+// sum of terms of both signs; 15-level unsigned sums would cancel against
+// 8 sum(p s_v) and lose 7 to 8 bits for a few thousand tokens).
+//
+// Precision: q (times log2(e) / sqrt(D)) and p s_v are each split into two
+// fp16 parts, 22 bits, of values scaled by a power of two that puts the
+// largest at 2^15: scores and outputs carry fp32-level error.
+//
+// Layout: one 16-token tile of a KV head is 16 D / 2 + 64 bytes of K and as
+// many of V, and the storage order is the fragments' own: a lane's codes of
+// the whole tile are two 16-byte loads of K and two of V (D = 128), straight
+// from global memory to registers, coalesced over the warp.
+//   K: lane (g, t) = (L / 4, L % 4) takes dims 32 t .. 32 t + 31 of tokens g
+//      and g + 8.  The sum over dims does not care for their order, so q's
+//      fragments simply follow K's: nibbles n and n + 4 of a word are the
+//      halves of one fp16x2 register.  (w & 0x000f000f) read as fp16 is
+//      u 2^-24 (a subnormal, exact), (w & 0x00f000f0) is u 2^-20: one
+//      instruction per two codes, the factors go into q and the scores.
+//   V: lane (g, t) takes dims 16 g .. 16 g + 15 of token pairs t and t + 4;
+//      a word holds four dims of the two adjacent tokens.  (w & 0x000f000f) |
+//      0x6400 is 1024 + u, and one fp16x2 operation makes it u - 8.
+// Query heads fill the N = 8 side: up to four heads take one mma with both
+// parts of q (or p) side by side in its columns, five to eight take two.
+//
+// Work: as the other decode kernels, a CTA takes one split-K item (row,
+// token range) of one KV head, its 4 warps the range's tiles in turn; warps
+// merge through shared memory, splits through combine.cuh.
+#include <cmath>
+
+#include "combine.cuh"
+#include "q4.cuh"
+
+namespace s1kv {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kNW = 4;
+constexpr int kTile = 16;
+constexpr int kMaxG = 32;              // query heads per KV head the merge's scratch covers (D = 64: 36 G of 2048 floats)
+constexpr float kRescaleAt = 8.0f;     // log2 units
+constexpr int kMinExp = 8;             // least exponent (biased) the V scales are taken relative to
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8x8 b16 matrix held as the warp's m8n8 fragment.
+__device__ __forceinline__ uint32_t movt(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (a, b) -> fp16 pair and the fp16 pair of what it leaves out.
+__device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack_h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t o) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(w), "r"(mask), "r"(o));  // (w & mask) | o
+    return y;
+}
+// Four codes of two tokens each: u - 8 as fp16x2, nibble n in out[n].
+__device__ __forceinline__ void centred(uint32_t w, uint32_t (&out)[4]) {
+    const __half2 one = __float2half2_rn(1.0f), m1032 = __float2half2_rn(-1032.0f);
+    const __half2 sixteenth = __float2half2_rn(0.0625f), m72 = __float2half2_rn(-72.0f);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t x = w >> (8 * i);
+        const uint32_t a = and_or(x, 0x000F000Fu, 0x64006400u), b = and_or(x, 0x00F000F0u, 0x64006400u);
+        const __half2 ha = __hfma2(*reinterpret_cast<const __half2*>(&a), one, m1032);
+        const __half2 hb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, m72);
+        out[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
+        out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+    }
+}
+
+// One tile's bytes of one lane: NWD words of K for tokens g and g + 8, of V
+// for pairs t and t + 4, and the params of tokens g and g + 8.
+template <int NWD>
+struct TileRegs {
+    uint32_t k0[NWD], k1[NWD], v0[NWD], v1[NWD];
+    uint32_t pk0, pk1, pv0, pv1;
+};
+
+template <int NWD>
+__device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[NWD]) {
+    if constexpr (NWD == 4) {
+        const uint4 x = __ldcs(reinterpret_cast<const uint4*>(at));
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+        const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
+        w[0] = x.x, w[1] = x.y;
+    }
+}
+
+}  // namespace
+
+// D = 32 NWD; heads of one pass (NT = 1: up to 4, NT = 2: up to 8).
+template <int D, int NT>
+__global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_constant__ AttnParams p, int G) {
+    constexpr int NWD = D / 32, KS = D / 16, GP = 4 * NT;
+    constexpr int kTileBytes = kTile * (D / 2 + 4), kParams = kTile * (D / 2);
+    extern __shared__ float smem_f[];
+    float* mo = smem_f;                    // [kNW][GP][D]
+    float* mml = mo + kNW * GP * D;        // [kNW][GP][2]
+    int* flag = reinterpret_cast<int*>(mml + kNW * GP * 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gq = lane >> 2, tq = lane & 3;
+    const int h = blockIdx.y;
+    const WorkItem item = p.items[blockIdx.x];
+    const int tok0 = item.split * p.split_tokens;
+    const int tok1 = min(tok0 + p.split_tokens, item.kv_len);
+    const int n_tiles = (tok1 - tok0 + kTile - 1) / kTile;
+    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kNW - 1) / kNW : 0;
+    const int32_t* tab = p.table + (int64_t)item.table_row * p.max_bps + (tok0 >> 4);
+    pdl_wait();
+    const RowMeta rm = p.rows[item.row];
+
+    for (int g0 = 0; g0 < G; g0 += GP) {
+        // q's fragments: column c of the N side is head g0 + c (NT = 2), or
+        // head g0 + c % 4 with the high part in columns 0-3 and the low part
+        // in 4-7 (NT = 1).
+        const int head = NT == 1 ? gq & 3 : gq;
+        const bool live = g0 + head < G;
+        const float* qrow = p.q + ((int64_t)item.row * p.Hq + h * G + g0 + (live ? head : 0)) * D;
+        float amax = 0.0f, qsum = 0.0f;
+        for (int d = tq; d < D; d += 4) {
+            const float x = live ? qrow[d] * p.scale_log2 : 0.0f;
+            amax = fmaxf(amax, fabsf(x));
+            qsum += x;
+        }
+        qsum += __shfl_xor_sync(kFull, qsum, 1);
+        qsum += __shfl_xor_sync(kFull, qsum, 2);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
+        // power of two that puts the pass's largest |q| in [2^14, 2^15)
+        const int qe = min(max((int)(__float_as_uint(amax) >> 23), 40), 240);
+        const float qscale = __uint_as_float((uint32_t)(127 + 14 + 127 - qe) << 23);
+        const float unscale = __uint_as_float((uint32_t)(qe - 14 + 24) << 23);  // 2^24 / qscale
+        uint32_t qf[NT][KS][2];
+#pragma unroll
+        for (int wi = 0; wi < NWD; wi++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int d = 8 * (NWD * tq + wi) + 2 * j + b;
+                    const float f = p.scale_log2 * (b ? 0.0625f : 1.0f);
+                    const float x0 = live ? qrow[d] * f * qscale : 0.0f, x1 = live ? qrow[d + 4] * f * qscale : 0.0f;
+                    uint32_t hi, lo;
+                    split_h2(x0, x1, hi, lo);
+                    if (NT == 1) {
+                        qf[0][2 * wi + j][b] = gq < 4 ? hi : lo;
+                    } else {
+                        qf[0][2 * wi + j][b] = hi;
+                        qf[NT - 1][2 * wi + j][b] = lo;
+                    }
+                }
+        // sum(q) of the two heads whose scores this lane holds (columns 2 tq, 2 tq + 1)
+        const float qs0 = __shfl_sync(kFull, qsum, (2 * tq) * 4 & 31), qs1 = __shfl_sync(kFull, qsum, (2 * tq + 1) * 4 & 31);
+
+        float o[KS][4];
+#pragma unroll
+        for (int mb = 0; mb < KS; mb++) o[mb][0] = o[mb][1] = o[mb][2] = o[mb][3] = 0.0f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, z0 = 0.0f, z1 = 0.0f;
+        int E = kMinExp;  // V scales are taken relative to 2^(E - 127)
+        float vmul = __uint_as_float((uint32_t)(260 - E) << 23);  // 2^(133 - E): the largest scaled s_v in [2^6, 2^7)
+
+        int32_t my_blk = 0;
+        auto fetch_ids = [&](int k) {  // block ids of this warp's tiles k .. k + 31, one a lane
+            my_blk = 0;
+            if (k + lane < my_tiles) {
+                my_blk = tab[warp + (k + lane) * kNW];
+                if ((uint32_t)my_blk >= (uint32_t)p.max_blocks) {
+                    atomicOr(p.err, kErrBounds);
+                    my_blk = 0;
+                }
+            }
+        };
+        auto load = [&](int k, TileRegs<NWD>& r) {
+            if ((k & 31) == 0) fetch_ids(k);
+            const int64_t off = ((int64_t)__shfl_sync(kFull, my_blk, k & 31) * p.Hkv + h) * kTileBytes;
+            const char* kt = reinterpret_cast<const char*>(p.kbase) + off;
+            const char* vt = reinterpret_cast<const char*>(p.vbase) + off;
+            load_words<NWD>(kt + gq * (D / 2) + tq * (4 * NWD), r.k0);
+            load_words<NWD>(kt + (gq + 8) * (D / 2) + tq * (4 * NWD), r.k1);
+            load_words<NWD>(vt + tq * D + gq * (4 * NWD), r.v0);
+            load_words<NWD>(vt + (tq + 4) * D + gq * (4 * NWD), r.v1);
+            r.pk0 = __ldcs(reinterpret_cast<const uint32_t*>(kt + kParams) + gq);
+            r.pk1 = __ldcs(reinterpret_cast<const uint32_t*>(kt + kParams) + gq + 8);
+            r.pv0 = __ldcs(reinterpret_cast<const uint32_t*>(vt + kParams) + gq);
+            r.pv1 = __ldcs(reinterpret_cast<const uint32_t*>(vt + kParams) + gq + 8);
+        };
+        TileRegs<NWD> nx;
+        if (my_tiles > 0) load(0, nx);
+        for (int k = 0; k < my_tiles; k++) {
+            const TileRegs<NWD> r = nx;
+            if (k + 1 < my_tiles) load(k + 1, nx);
+            const int valid = min(kTile, tok1 - (tok0 + (warp + k * kNW) * kTile));
+
+            // ---- scores: M = the 16 tokens, N = the 8 columns ----
+            float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int wi = 0; wi < NWD; wi++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t a = r.k0[wi] >> (8 * j), b = r.k1[wi] >> (8 * j);
+                    const uint32_t a0 = a & 0x000F000Fu, a1 = b & 0x000F000Fu, a2 = a & 0x00F000F0u, a3 = b & 0x00F000F0u;
+                    const int ks = 2 * wi + j;
+                    if (NT == 1) {
+                        mma16816(j ? sb : sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
+                    } else {
+                        mma16816(sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
+                        mma16816(sb, a0, a1, a2, a3, qf[NT - 1][ks][0], qf[NT - 1][ks][1]);
+                    }
+                }
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x[i] = sa[i] + sb[i];
+                if (NT == 1) x[i] += __shfl_xor_sync(kFull, x[i], 2);  // high + low part of q
+            }
+            // this lane: tokens gq (x[0], x[1]) and gq + 8 (x[2], x[3]) of its two heads
+            const float2 ka = q4_unpack(r.pk0), kb = q4_unpack(r.pk1);
+            const float sk0 = ka.x * unscale, sk1 = kb.x * unscale;
+            const float zk0 = fmaf(-8.0f, ka.x, ka.y), zk1 = fmaf(-8.0f, kb.x, kb.y);
+            x[0] = fmaf(x[0], sk0, zk0 * qs0);
+            x[1] = fmaf(x[1], sk0, zk0 * qs1);
+            x[2] = fmaf(x[2], sk1, zk1 * qs0);
+            x[3] = fmaf(x[3], sk1, zk1 * qs1);
+            float2 va = q4_unpack(r.pv0), vb = q4_unpack(r.pv1);
+            if (valid < kTile) {  // rows past the end hold anything, NaN included
+                if (gq >= valid) {
+                    x[0] = x[1] = -INFINITY;
+                    va = make_float2(0.0f, 0.0f);
+                }
+                if (gq + 8 >= valid) {
+                    x[2] = x[3] = -INFINITY;
+                    vb = make_float2(0.0f, 0.0f);
+                }
+            }
+            // the reference max of a head moves only when a score outgrows it
+            // by 2^8, and E only when an s_v outgrows it: both are rare
+            float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+            const int e = min((int)(__float_as_uint(fmaxf(va.x, vb.x)) >> 23), 254);
+            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || e > E)) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, off));
+                    mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, off));
+                }
+                const bool r0 = mx0 > m0 + kRescaleAt, r1 = mx1 > m1 + kRescaleAt;
+                float c0 = r0 ? ex2(m0 - mx0) : 1.0f, c1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
+                if (r0) m0 = mx0;
+                if (r1) m1 = mx1;
+                l0 *= c0;
+                l1 *= c1;
+                z0 *= c0;
+                z1 *= c1;
+                const int ne = max(E, (int)__reduce_max_sync(kFull, (unsigned)e));
+                const float ce = ne - E > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (ne - E)) << 23);
+                E = ne;
+                vmul = __uint_as_float((uint32_t)(260 - E) << 23);
+                c0 *= ce;
+                c1 *= ce;
+#pragma unroll
+                for (int mb = 0; mb < KS; mb++) {
+                    o[mb][0] *= c0;
+                    o[mb][1] *= c1;
+                    o[mb][2] *= c0;
+                    o[mb][3] *= c1;
+                }
+            }
+            const float p0 = ex2(x[0] - m0), p1 = ex2(x[1] - m1), p2 = ex2(x[2] - m0), p3 = ex2(x[3] - m1);
+            l0 += p0 + p2;
+            l1 += p1 + p3;
+            z0 = fmaf(p0, va.y, fmaf(p2, vb.y, z0));
+            z1 = fmaf(p1, va.y, fmaf(p3, vb.y, z1));
+            const float w0 = va.x * vmul, w1 = vb.x * vmul;
+            uint32_t h0, h1, e0, e1;
+            split_h2(p0 * w0, p1 * w0, h0, e0);
+            split_h2(p2 * w1, p3 * w1, h1, e1);
+            uint32_t bh0, bh1, bl0 = 0, bl1 = 0;
+            if (NT == 1) {
+                bh0 = movt(tq < 2 ? h0 : e0);
+                bh1 = movt(tq < 2 ? h1 : e1);
+            } else {
+                bh0 = movt(h0), bh1 = movt(h1), bl0 = movt(e0), bl1 = movt(e1);
+            }
+            // ---- O^T += V^T P^T: M = 16 dims per m-block, K = the 16 tokens ----
+#pragma unroll
+            for (int wi = 0; wi < NWD; wi++) {
+                uint32_t c0[4], c1[4];
+                centred(r.v0[wi], c0);
+                centred(r.v1[wi], c1);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bh0, bh1);
+                    if (NT == 2) mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bl0, bl1);
+                }
+            }
+        }
+
+        // ---- merge the warps through shared memory ----
+        const float back = __uint_as_float((uint32_t)(E - 6) << 23);  // 1 / vmul
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+            l0 += __shfl_xor_sync(kFull, l0, off);
+            l1 += __shfl_xor_sync(kFull, l1, off);
+            z0 += __shfl_xor_sync(kFull, z0, off);
+            z1 += __shfl_xor_sync(kFull, z1, off);
+        }
+#pragma unroll
+        for (int mb = 0; mb < KS; mb++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (NT == 1) o[mb][i] += __shfl_xor_sync(kFull, o[mb][i], 2);
+                o[mb][i] = fmaf(o[mb][i], back, i & 1 ? z1 : z0);
+            }
+        __syncthreads();  // the last pass's readers are done
+        if (2 * tq < GP) {  // dims D / 8 gq + 2 mb (rows g) and + 1 (rows g + 8) of heads 2 tq, 2 tq + 1
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int hc = 2 * tq + i;
+                float* dst = &mo[(warp * GP + hc) * D + (D / 8) * gq];
+#pragma unroll
+                for (int mb = 0; mb < KS; mb++) {
+                    dst[2 * mb] = o[mb][i];
+                    dst[2 * mb + 1] = o[mb][2 + i];
+                }
+                if (gq == 0) {
+                    mml[(warp * GP + hc) * 2] = i ? m1 : m0;
+                    mml[(warp * GP + hc) * 2 + 1] = i ? l1 : l0;
+                }
+            }
+        }
+        __syncthreads();
+        const int64_t part = (int64_t)(rm.part_off + item.split) * p.Hkv + h;
+        for (int idx = threadIdx.x; idx < min(GP, G - g0) * D; idx += kNW * 32) {
+            const int g = idx / D, d = idx % D;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kNW; w++) M = fmaxf(M, mml[(w * GP + g) * 2]);
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kNW; w++) {
+                const float mw = mml[(w * GP + g) * 2];
+                const float f = (mw == -INFINITY) ? 0.0f : ex2(mw - M);
+                L = fmaf(mml[(w * GP + g) * 2 + 1], f, L);
+                O = fmaf(mo[(w * GP + g) * D + d], f, O);
+            }
+            if (rm.n_split == 1) {
+                store_out(p, item.row, h * G + g0 + g, d, D, O / L);
+            } else {
+                p.part_o[(part * G + g0 + g) * D + d] = O;
+                if (d == 0) {
+                    p.part_ml[(part * G + g0 + g) * 2] = M;
+                    p.part_ml[(part * G + g0 + g) * 2 + 1] = L;
+                }
+            }
+        }
+    }
+    pdl_trigger();
+    if (p.counters && rm.n_split > 1) {
+        __syncthreads();
+        finish_split_row(p, item.row, h, item.split, rm.n_split, G, D, flag, mo, kNW * GP * D);
+    }
+}
+
+// ------------------------------------------------- any head_dim and block --
+// One warp per (query row, query head), tokens in order: shapes the kernel
+// above does not take (head_dim other than 64 and 128, blocks other than 16
+// tokens, more than kMaxG query heads per KV head).
+__global__ void attn_q4_generic_kernel(const AttnParams p) {
+    const int G = p.Hq / p.Hkv, D = p.D, nq = D / 4, bs = p.block_size;
+    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+    const RowMeta rm = p.rows[row];
+    const int32_t* tab = p.table + (int64_t)rm.table_row * p.max_bps;
+    for (int g = threadIdx.x >> 5; g < G; g += blockDim.x >> 5) {
+        const float* q = p.q + ((int64_t)row * p.Hq + h * G + g) * D;
+        float qv[2][4], o[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int quad = lane + 32 * i;
+                qv[i][e] = quad < nq ? q[4 * quad + e] : 0.0f;
+                o[i][e] = 0.0f;
+            }
+        float m = -INFINITY, l = 0.0f;
+        for (int j = 0; j < rm.kv_len; j++) {
+            const int32_t blk = tab[j / bs];
+            if ((uint32_t)blk >= (uint32_t)p.max_blocks) {
+                if (lane == 0) atomicOr(p.err, kErrBounds);
+                continue;
+            }
+            int t;
+            const int64_t slot = (int64_t)blk * bs + j % bs;
+            const char* kt = q4_tile(const_cast<void*>(p.kbase), slot, h, p.Hkv, bs, D, &t);
+            const char* vt = q4_tile(const_cast<void*>(p.vbase), slot, h, p.Hkv, bs, D, &t);
+            const float2 sk = q4_unpack(*reinterpret_cast<const uint32_t*>(kt + q4_param(t, bs, D)));
+            const float2 sv = q4_unpack(*reinterpret_cast<const uint32_t*>(vt + q4_param(t, bs, D)));
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int quad = lane + 32 * i;
+                if (quad >= nq) continue;
+                const uint32_t c = *reinterpret_cast<const uint16_t*>(kt + q4_k_quad(t, quad, D));
+#pragma unroll
+                for (int e = 0; e < 4; e++) s = fmaf(qv[i][e], q4_value((c >> (4 * e)) & 15u, sk.x, sk.y), s);
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(kFull, s, off);
+            s *= p.scale_log2;
+            const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : ex2(m - mn), pj = ex2(s - mn);
+            l = fmaf(l, c, pj);
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int quad = lane + 32 * i;
+                if (quad >= nq) continue;
+                const uint32_t cv = *reinterpret_cast<const uint16_t*>(vt + q4_v_quad(t, quad, D));
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[i][e] = fmaf(pj, q4_value((cv >> (4 * e)) & 15u, sv.x, sv.y), o[i][e] * c);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int quad = lane + 32 * i;
+            if (quad < nq)
+#pragma unroll
+                for (int e = 0; e < 4; e++) store_out(p, row, h * G + g, 4 * quad + e, D, o[i][e] / l);
+        }
+    }
+}
+
+bool decode_q4_supported(int D, int G, int block_size) {
+    return (D == 64 || D == 128) && block_size == kTile && G >= 1 && G <= kMaxG;
+}
+
+template <int D, int NT>
+static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
+    constexpr int smem = (kNW * 4 * NT * (D + 2) + 4) * 4;
+    const dim3 grid((unsigned)p.n_items, (unsigned)p.Hkv);
+    S1KV_CUDA(launch_pdl(decode_q4_kernel<D, NT>, grid, dim3(kNW * 32), smem, stream, p, G));
+    g_launches++;
+    S1KV_CUDA(cudaGetLastError());
+    return S1KV_OK;
+}
+
+int launch_decode_q4(const AttnParams& p, cudaStream_t stream) {
+    if (p.n_rows <= 0) return S1KV_OK;
+    const int G = p.Hq / p.Hkv;
+    if (p.items && decode_q4_supported(p.D, G, p.block_size)) {
+        if (p.D == 128) return G <= 4 ? launch_q4<128, 1>(p, G, stream) : launch_q4<128, 2>(p, G, stream);
+        return G <= 4 ? launch_q4<64, 1>(p, G, stream) : launch_q4<64, 2>(p, G, stream);
+    }
+    attn_q4_generic_kernel<<<dim3((unsigned)p.n_rows, (unsigned)p.Hkv), 32 * std::min(G, 8), 0, stream>>>(p);
+    g_launches++;
+    S1KV_CUDA(cudaGetLastError());
+    return S1KV_OK;
+}
+
+}  // namespace s1kv

@@ -26,7 +26,7 @@ _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "lib", "libs1kv.so")
 
 OK, ENOBLOCKS, ENOSEQ, EINVAL, ECUDA, ETIMEOUT, ENOMEM, EDEVICE = range(8)
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_Q4 = 0, 1, 2
 POOL_HOST_ONLY = 1
 K, V = 0, 1
 
@@ -123,12 +123,16 @@ SIGNATURES = {
     "s1kv_batch_norm_rope_append": (C.c_int, [vp, i32, vp, vp, i32, vp, vp, vp, vp, f32, vp]),
     "s1kv_debug_div_check": (C.c_int, [vp, i64, vp, i64, vp, vp]),
     "s1kv_batch_append": (C.c_int, [vp, i32, vp, vp, vp]),
+    "s1kv_batch_gather": (C.c_int, [vp, i32, i32, vp, vp]),
     "s1kv_batch_attention": (C.c_int, [vp, i32, vp, vp, i32, vp]),
     "s1kv_batch_layer_host": (C.c_int, [vp, i32, vp, vp, vp, vp, i32, vp]),
     "s1kv_batch_end": (C.c_int, [vp, vp]),
     "s1kv_quantize_rows": (C.c_int, [vp, i64, i64, vp, vp, vp]),
     "s1kv_matmul_int8": (C.c_int, [vp, i64, i64, vp, vp, i64, vp, vp]),
     "s1kv_matmul_int8_group": (C.c_int, [vp, i64, i64, i32, vp, vp, vp, vp, vp]),
+    "s1kv_quantize_tokens": (C.c_int, [vp, i64, i64, vp, i64, vp, vp]),
+    "s1kv_matmul_w8a8": (C.c_int, [vp, vp, i64, i64, vp, vp, i64, vp, vp]),
+    "s1kv_matmul_w8a8_group": (C.c_int, [vp, vp, i64, i64, i32, vp, vp, vp, vp, vp]),
     "s1kv_launch_count": (i64, []),
     "s1kv_batch_plan": (C.c_int, [vp, P(i32), P(i64)]),
 }
@@ -198,7 +202,8 @@ class Pool:
 
     def __init__(self, num_layers, num_kv_heads, head_dim, max_blocks, block_size=16, dtype="f32", device=None,
                  max_seqs=1024, max_seq_len=0, rope_theta=1.0e6, initial_free_list=None, host_only=False):
-        """device None = torch's current CUDA device (0 for a host-only pool)."""
+        """dtype "f32", "bf16" or "q4" (4 bits a value, S1KV_DTYPE_Q4).  device
+        None = torch's current CUDA device (0 for a host-only pool)."""
         self.L = lib()
         if device is None:
             if host_only:
@@ -208,7 +213,8 @@ class Pool:
                 device = torch.cuda.current_device()
         self.num_layers, self.Hkv, self.D = num_layers, num_kv_heads, head_dim
         self.max_blocks, self.bs = max_blocks, block_size
-        self.dtype = DTYPE_F32 if dtype in ("f32", "fp32", "float32", DTYPE_F32) else DTYPE_BF16
+        self.dtype = (DTYPE_F32 if dtype in ("f32", "fp32", "float32", DTYPE_F32) else
+                      DTYPE_Q4 if dtype in ("q4", DTYPE_Q4) else DTYPE_BF16)
         self.device = device
         d = PoolDesc(num_layers, num_kv_heads, head_dim, block_size, max_blocks, self.dtype, max_seqs, max_seq_len,
                      rope_theta, POOL_HOST_ONLY if host_only else 0, None)
@@ -321,10 +327,13 @@ class Pool:
 
     def read_storage(self, layer, which, slot0=0, n_slots=None):
         """Raw storage rows [slot0, slot0+n_slots) as numpy (float32 or the
-        uint16 bf16 bits)."""
+        uint16 bf16 bits); of a 4-bit pool whole blocks as uint8
+        [n_slots / block_size, Hkv, block_size * (D / 2 + 4)]."""
         n_slots = self.max_blocks * self.bs - slot0 if n_slots is None else n_slots
-        dt = np.float32 if self.dtype == DTYPE_F32 else np.uint16
-        out = np.empty((n_slots, self.Hkv, self.D), dt)
+        if self.dtype == DTYPE_Q4:
+            out = np.empty((n_slots // self.bs, self.Hkv, self.bs * (self.D // 2 + 4)), np.uint8)
+        else:
+            out = np.empty((n_slots, self.Hkv, self.D), np.float32 if self.dtype == DTYPE_F32 else np.uint16)
         check(self.L.s1kv_pool_read(self.h, layer, which, slot0, n_slots, out.ctypes.data_as(vp)))
         return out
 
@@ -418,6 +427,15 @@ class Batch:
 
     def append(self, layer, k, v):
         check(self.L.s1kv_batch_append(self.h, layer, _dptr(k), _dptr(v), _stream()))
+
+    def gather(self, layer, which, out=None):
+        """The rows this batch appended, as the pool holds them: fp32
+        [n_tokens, Hkv, D]."""
+        import torch
+        if out is None:
+            out = torch.empty((self.n_tokens, self.pool.Hkv, self.pool.D), dtype=torch.float32, device=self.pool.device)
+        check(self.L.s1kv_batch_gather(self.h, layer, which, _dptr(out), _stream()))
+        return out
 
     def attention(self, layer, q, out=None):
         import torch
@@ -609,6 +627,82 @@ def matmul_quantized_group(x, ws, outs=None):
     with torch.cuda.device(xd.device):
         check(lib().s1kv_matmul_int8_group(_dptr(xd), xd.shape[0], xd.shape[1], n, qa, sa, na, oa, _stream()))
     return outs
+
+
+class ChannelQuantizedTensor:
+    """An int8 weight with one scale per output channel: data int8 [N, K16]
+    (row n = channel n's K weights, zero padded to K16, K rounded up to a
+    multiple of 16) and scales fp32 [N], both on the GPU; k = K."""
+
+    def __init__(self, data, scales, k=None):
+        self.data, self.scales = data, scales
+        self.n, self.ld = int(data.shape[0]), int(data.shape[1])
+        self.k = self.ld if k is None else int(k)
+        if self.ld != (self.k + 15) // 16 * 16 or not data.is_contiguous() or not scales.is_contiguous():
+            raise S1KVError(EINVAL, "ChannelQuantizedTensor: contiguous rows of K rounded up to a multiple of 16 bytes")
+        if str(data.dtype) != "torch.int8" or str(scales.dtype) != "torch.float32" or tuple(scales.shape) != (self.n,):
+            raise S1KVError(EINVAL, "ChannelQuantizedTensor: int8 [N, K16] data and float32 [N] scales")
+
+
+def quantize_channels(t, device=None):
+    """A pre-transposed [K, N] weight to int8 with one scale per column n:
+    scale = max|w[:, n]| / 127 (1 for a zero column), round(value / scale)
+    ties away from zero (s1kv_quantize_rows on the channels' rows)."""
+    import torch
+    w = _cuda_f32(t, device)
+    if w.dim() != 2:
+        raise S1KVError(EINVAL, "quantize_channels needs a 2-D tensor")
+    k, n = w.shape
+    rows = torch.zeros((n, (k + 15) // 16 * 16), dtype=torch.float32, device=w.device)
+    rows[:, :k] = w.t()
+    q = quantize_tensor(rows, w.device.index)
+    return ChannelQuantizedTensor(q.data, q.scales, k)
+
+
+def quantize_tokens(x, device=None):
+    """x [M, K] float to (int8 [M, K rounded up to 16], fp32 scales [M]), one
+    scale per token (s1kv_quantize_tokens)."""
+    import torch
+    xd = _cuda_f32(x, device)
+    if xd.dim() != 2:
+        raise S1KVError(EINVAL, "quantize_tokens needs a 2-D tensor")
+    m, k = xd.shape
+    ld = (k + 15) // 16 * 16
+    q = torch.empty((m, ld), dtype=torch.int8, device=xd.device)
+    scales = torch.empty((m,), dtype=torch.float32, device=xd.device)
+    with torch.cuda.device(xd.device):
+        check(lib().s1kv_quantize_tokens(_dptr(xd), m, k, _dptr(q), ld, _dptr(scales), _stream()))
+    return q, scales
+
+
+def matmul_w8a8_group(x, ws, outs=None):
+    """Products of one x [M, K] float, quantised per token, with up to 4
+    ChannelQuantizedTensor weights of the same K in one launch (q/k/v,
+    gate/up) -> list of [M, N] fp32.  Summed exactly in 32-bit integers."""
+    import torch
+    xd = _cuda_f32(x, ws[0].data.device.index)
+    if xd.dim() != 2 or any(w.k != xd.shape[1] or w.data.device != xd.device for w in ws):
+        raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K] with K the weights' and all on one device")
+    m = xd.shape[0]
+    if outs is None:
+        outs = [torch.empty((m, w.n), dtype=torch.float32, device=xd.device) for w in ws]
+    elif len(outs) != len(ws) or any(o.shape != (m, w.n) or o.dtype != torch.float32 or not o.is_contiguous() or
+                                     o.device != xd.device for o, w in zip(outs, ws)):
+        raise S1KVError(EINVAL, "matmul_w8a8_group: outs must be contiguous float32 [M, N] on x's device")
+    n = len(ws)
+    wa = (vp * n)(*[w.data.data_ptr() for w in ws])
+    sa = (vp * n)(*[w.scales.data_ptr() for w in ws])
+    na = (i64 * n)(*[w.n for w in ws])
+    oa = (vp * n)(*[o.data_ptr() for o in outs])
+    with torch.cuda.device(xd.device):
+        q, scales = quantize_tokens(xd, xd.device.index)
+        check(lib().s1kv_matmul_w8a8_group(_dptr(q), _dptr(scales), m, ws[0].ld, n, wa, sa, na, oa, _stream()))
+    return outs
+
+
+def matmul_w8a8(x, w, out=None):
+    """matmul_w8a8_group with one weight -> [M, N] fp32."""
+    return matmul_w8a8_group(x, [w], None if out is None else [out])[0]
 
 
 # ================================================ KV-head-sharded serving ==
