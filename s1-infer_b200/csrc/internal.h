@@ -104,6 +104,8 @@ int* device_error_word(int device);
 // Reads and clears the no-allocation decode's error word on `device`
 // (noalloc.cu); *flags = 0 if that entry point never ran there.
 int noalloc_take_error(int device, int* flags);
+// The same of the 8-bit products' tensor-core kernels (w8a8.cu).
+int w8a8_take_error(int device, int* flags);
 
 // Split-K merging (combine.cuh): rows of up to kMergeGroup splits are
 // merged by one CTA; longer rows in two levels (groups of kMergeGroup

@@ -571,6 +571,10 @@ int s1kv_device_check(int device, int32_t* flags_out) {
     const int st = noalloc_take_error(device, &na);
     if (st) return st;
     h |= na;
+    int w8 = 0;
+    const int st8 = w8a8_take_error(device, &w8);
+    if (st8) return st8;
+    h |= w8;
     if (flags_out) *flags_out = h;
     if (h & kErrTimeout) return set_error(S1KV_ETIMEOUT, "s1kv: a bounded device wait timed out");
     if (h & kErrBounds) return set_error(S1KV_EDEVICE, "s1kv: a kernel saw an out-of-range slot or block");

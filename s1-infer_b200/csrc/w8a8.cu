@@ -12,6 +12,9 @@
 //
 // Weights are [N][K] rows of K bytes (an nn.Linear weight's own order; what
 // s1kv_quantize_rows makes of it), K a multiple of 16 padded with zeros in x.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 
 #include "internal.h"
@@ -46,6 +49,7 @@ __device__ __forceinline__ int token_code(float x, float s, float inv) {
 __global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __restrict__ x, int64_t M, int64_t K,
                                                               int8_t* __restrict__ q, int64_t ldq,
                                                               float* __restrict__ scales) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ float part[8];
     const int64_t m = blockIdx.x;
     const float* src = x + m * K;
@@ -67,44 +71,514 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __res
         q[m * ldq + k] = (int8_t)(fine && k < K ? token_code(src[k], s, inv) : 0);
 }
 
-// 64 x 64 outputs a CTA, 4 x 4 a thread, 64 bytes of K a step.
-__global__ void __launch_bounds__(256) w8a8_tile_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx, int M,
-                                                        int K, const __grid_constant__ W8Group grp) {
-    __shared__ int xs[64][17], ws[64][17];
+// ---------------------------------------------- few tokens: weight stream --
+// Up to 8 NTILE tokens (NTILE = 1 or 2): bound by the N K bytes of the
+// weights.  mma.sync m16n8k32 on int8 with the channels on the 16-row side
+// and the tokens on the 8-column side.  The sum over k does not care for the
+// order of k, so a lane's fragments are simply 16 adjacent bytes of its
+// channel's (and its token's) row: weights go from global memory to the
+// instruction's registers in 16-byte loads, nothing is staged or shuffled.
+// A CTA owns 16 channels, its 8 warps split K by 128-byte steps; the warps'
+// integer sums meet in shared memory.  The first steps' weights are
+// requested before the wait for the previous kernel (the token quantiser):
+// they do not depend on it.
+constexpr int kGemvWarps = 8;
+constexpr int kGemvPre = 4;  // 128-byte steps in flight a warp
+
+__device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NTILE>
+__global__ void __launch_bounds__(kGemvWarps * 32) w8a8_gemv_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
+                                                                   int M, int K, const __grid_constant__ W8Group grp) {
+    __shared__ int red[kGemvWarps][16][8 * NTILE + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int mi = 0;
 #pragma unroll
     for (int i = 1; i < kMaxMats; i++)
         if (i < grp.n && (int)blockIdx.x >= grp.m[i].tile0) mi = i;
     const W8Mat& mat = grp.m[mi];
-    const int n0 = ((int)blockIdx.x - mat.tile0) * 64, m0 = blockIdx.y * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int r = i >> 4, c = i & 15, k = k0 + 4 * c;
-            xs[r][c] = m0 + r < M && k < K ? *reinterpret_cast<const int*>(xq + (int64_t)(m0 + r) * K + k) : 0;
-            ws[r][c] = n0 + r < mat.N && k < K ? *reinterpret_cast<const int*>(mat.w + (int64_t)(n0 + r) * K + k) : 0;
+    const int n0 = ((int)blockIdx.x - mat.tile0) * 16;
+    // rows past the last channel read the last one's bytes and are not stored
+    const int8_t* w0 = mat.w + (int64_t)min(n0 + g, mat.N - 1) * K;
+    const int8_t* w1 = mat.w + (int64_t)min(n0 + g + 8, mat.N - 1) * K;
+    // step s of this warp: bytes 128 (warp + 8 s) .. + 127, in two 64-byte halves of 16 bytes a lane
+    const int steps = ((K + 127) / 128 - warp + kGemvWarps - 1) / kGemvWarps;
+    uint4 a[kGemvPre][2][2];
+    auto fetch = [&](int s, uint4 (&r)[2][2]) {
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+            const int k = 128 * (warp + kGemvWarps * s) + 64 * hf + 16 * t;
+            const bool in = s < steps && k < K;
+            r[hf][0] = in ? __ldcs(reinterpret_cast<const uint4*>(w0 + k)) : make_uint4(0, 0, 0, 0);
+            r[hf][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0, 0, 0, 0);
         }
-        __syncthreads();
+    };
 #pragma unroll
-        for (int c = 0; c < 16; c++)
+    for (int s = 0; s < kGemvPre; s++) fetch(s, a[s]);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int acc[NTILE][4] = {};
+    for (int s0 = 0; s0 < steps; s0 += kGemvPre) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+        for (int u = 0; u < kGemvPre; u++) {
+            const int s = s0 + u;
+            if (s >= steps) break;
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(xs[ty * 4 + i][c], ws[tx + 16 * j][c], acc[i][j]);
-        __syncthreads();
+            for (int hf = 0; hf < 2; hf++) {
+                const int k = 128 * (warp + kGemvWarps * s) + 64 * hf + 16 * t;
+                const uint4 x = a[u][hf][0], y = a[u][hf][1];
+#pragma unroll
+                for (int nt = 0; nt < NTILE; nt++) {
+                    // tokens past the last read the last one's bytes; their columns are not stored
+                    const uint4 b = k < K ? __ldg(reinterpret_cast<const uint4*>(xq + (int64_t)min(8 * nt + g, M - 1) * K + k))
+                                          : make_uint4(0, 0, 0, 0);
+                    imma16832(acc[nt], x.x, y.x, x.y, y.y, b.x, b.y);
+                    imma16832(acc[nt], x.z, y.z, x.w, y.w, b.z, b.w);
+                }
+            }
+            fetch(s + kGemvPre, a[u]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int nt = 0; nt < NTILE; nt++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m < M && n < mat.N)
-                mat.out[(int64_t)m * mat.N + n] = __fmul_rn(__fmul_rn((float)acc[i][j], sx[m]), mat.scales[n]);
+        for (int i = 0; i < 4; i++) red[warp][g + (i >> 1) * 8][8 * nt + 2 * t + (i & 1)] = acc[nt][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 8 * NTILE; i += kGemvWarps * 32) {
+        const int n = i & 15, m = i >> 4;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kGemvWarps; w++) sum += red[w][n][m];
+        if (m < M && n0 + n < mat.N)
+            mat.out[(int64_t)m * mat.N + n0 + n] = __fmul_rn(__fmul_rn((float)sum, sx[m]), mat.scales[n0 + n]);
+    }
+}
+
+// -------------------------------------------------- many tokens: tcgen05 --
+// tcgen05.mma kind::i8 with the 128 channels of a tile as M and NT tokens as
+// N, so one kernel serves from 17 tokens (NT = 32, bound by the weights'
+// bytes) to prompts (NT = 256, bound by the tensor cores), and a stored
+// output row is 128 adjacent channels.  Roles: a TMA warp fills a ring of
+// 128-byte deep stages (both operands K-major, 128B swizzle, rows past the
+// end zero filled), one warp issues the MMAs, four warps take finished
+// accumulators out of TMEM, scale and store them.
+//   * Tiles enough for the machine: persistent CTAs, two accumulators in
+//     TMEM so that a tile's output leaves while the next one's products run;
+//     eight token tiles at a time share the weights through L2.
+//   * Fewer tiles than SMs (few tokens): the K range of a tile is split over
+//     a cluster of up to 8 CTAs, each rank sends its partial sums of a token
+//     slice to that slice's owner through distributed shared memory, the
+//     owner adds them (integers: any order, the same bits) and stores.
+// Waits are bounded; a timeout raises an abort flag that every role polls
+// and the error word; copies in flight are waited for, TMEM is freed.
+constexpr uint32_t kSpin = 1u << 22;
+constexpr int kCh = 128;             // channels a tile
+constexpr int kKB = 128;             // bytes of K a stage
+constexpr int kTcThreads = 192;      // TMA warp, MMA warp, 4 epilogue warps
+
+template <int NT>
+struct TcCfg {
+    static constexpr int kStageBytes = kKB * (kCh + NT);
+    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 5 : 6;
+    static constexpr int kCols = 2 * NT;                       // two accumulators
+    static constexpr int kExchange = NT <= 128 ? kCh * NT * 4 : 0;  // split tiles: [rank][channel][slice] sums
+    static constexpr int kOffX = kStages * kStageBytes;
+    static constexpr int kOffBar = kOffX + kExchange;
+    static constexpr int kNumBars = 2 * kStages + 5;
+    static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
+};
+
+struct TcParams {
+    W8Group grp;       // tile0 counts tiles of 128 channels
+    const float* sx;
+    int M, k_blocks;   // stages of K
+    int ch_tiles, tok_tiles;
+};
+struct TcMaps {
+    CUtensorMap x, w[kMaxMats];
+};
+
+__device__ int g_w8a8_error;  // error word of this file's kernels (s1kv_device_check reads it)
+
+__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t phase) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(su32(b)), "r"(phase)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t phase) {
+    for (uint32_t i = 0; i < kSpin; i++)
+        if (bar_try(b, phase)) return true;
+    return false;
+}
+// The same for a whole warp, giving up when another role raised the flag; a
+// timeout raises it.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t phase, volatile int* abort_flag) {
+    bool ok = false;
+    for (uint32_t i = 0; i < kSpin && !ok; i++) {
+        ok = bar_try(b, phase);
+        if (!ok && *abort_flag) break;
+    }
+    if (!ok) *abort_flag = 1;
+    return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap* m, uint64_t* b, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(su32(b))
+        : "memory");
+}
+// Shared-memory descriptor: K-major, 128-byte swizzle (layout type 2), 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+// kind::i8 instruction descriptor: signed 8-bit A and B (1), 32-bit integer D (2), both K-major.
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Issued by one elected lane of a converged warp.
+__device__ __forceinline__ void mma_i8_w(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_w(uint64_t* b) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b))
+        : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 16 consecutive 32-bit columns of this thread's TMEM lane, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+template <int NT, bool SPLIT>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    w8a8_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ TcMaps maps) {
+    using C = TcCfg<NT>;
+    constexpr int ST = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+    uint64_t* empty = full + ST;
+    uint64_t* acc_full = empty + ST;    // [2]
+    uint64_t* acc_empty = acc_full + 2;  // [2]
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffBar + C::kNumBars * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(C::kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < C::kNumBars; i++) bar_init(&full[i], i == 2 * ST + 2 || i == 2 * ST + 3 ? 4u : 1u);  // acc_empty: one arrive a warp
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (SPLIT) {  // every rank runs before the first store into its shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // this CTA's tiles and its share of K
+    const int cs = SPLIT ? (int)gridDim.y : 1, rank = SPLIT ? (int)blockIdx.y : 0;
+    const int kb0 = (int)((int64_t)p.k_blocks * rank / cs), kb1 = (int)((int64_t)p.k_blocks * (rank + 1) / cs);
+    const int n_tiles = p.ch_tiles * p.tok_tiles;
+    auto tile_at = [&](int t, int& ch, int& tok) {  // eight token tiles side by side, their channels in turn
+        const int per = 8 * p.ch_tiles, grp = t / per, in = t - grp * per, wide = min(8, p.tok_tiles - grp * 8);
+        ch = in / wide;
+        tok = grp * 8 + in - ch * wide;
+    };
+    auto mat_of = [&](int ch) {
+        int mi = 0;
+#pragma unroll
+        for (int i = 1; i < kMaxMats; i++)
+            if (i < p.grp.n && ch >= p.grp.m[i].tile0) mi = i;
+        return mi;
+    };
+
+    if (warp == 0) {
+        // ================= TMA producer =================
+        int it = 0;  // stages used so far
+        bool ok = true;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
+            int ch, tok;
+            tile_at(t, ch, tok);
+            const int mi = mat_of(ch), n0 = (ch - p.grp.m[mi].tile0) * kCh;
+            for (int kb = kb0; kb < kb1; kb++, it++) {
+                const int s = it % ST;
+                if (it >= ST && !(ok = warp_wait(&empty[s], (uint32_t)((it / ST - 1) & 1), abort_flag))) break;
+                if (lane == 0) {
+                    const uint32_t at = su32(smem + s * C::kStageBytes);
+                    bar_expect(&full[s], C::kStageBytes);
+                    tma2(at, &maps.w[mi], &full[s], kb * kKB, n0);
+                    tma2(at + kCh * kKB, &maps.x, &full[s], kb * kKB, tok * NT);
+                }
+                __syncwarp();
+            }
         }
+        // every copy issued has landed before the CTA may exit (bounded)
+        for (int i = max(0, it - ST); i < it; i++) bar_wait(&full[i % ST], (uint32_t)((i / ST) & 1));
+    } else if (warp == 1) {
+        // ================= MMA issuer =================
+        constexpr uint32_t id = idesc_s8(kCh, NT);
+        int it = 0, done = 0;  // stages consumed, tiles issued
+        bool ok = true;
+        for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x, done++) {
+            const int buf = done & 1;
+            if (done >= 2 && !(ok = warp_wait(&acc_empty[buf], (uint32_t)((done / 2 - 1) & 1), abort_flag))) break;
+            tc_fence_after();
+            for (int kb = kb0; kb < kb1; kb++, it++) {
+                const int s = it % ST;
+                if (!(ok = warp_wait(&full[s], (uint32_t)((it / ST) & 1), abort_flag))) break;
+                tc_fence_after();
+                const uint64_t da = sdesc(su32(smem + s * C::kStageBytes)), db = sdesc(su32(smem + s * C::kStageBytes + kCh * kKB));
+#pragma unroll
+                for (int k = 0; k < kKB / 32; k++)  // 32 bytes of K an instruction
+                    mma_i8_w(tmem + buf * NT, da + 2 * k, db + 2 * k, id, kb > kb0 || k > 0);
+                mma_commit_w(&empty[s]);
+            }
+            if (ok) mma_commit_w(&acc_full[buf]);
+        }
+        // everything issued has finished before TMEM is freed (bounded)
+        mma_commit_w(drain);
+        bar_wait(drain, 0);
+    } else {
+        // ================= epilogue =================
+        const int sub = warp & 3;  // the TMEM lanes 32 sub .. + 31 are this warp's
+        const uint32_t lanes = (uint32_t)(32 * sub) << 16;
+        int done = 0;
+        for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, done++) {
+            const int buf = done & 1;
+            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
+            tc_fence_after();
+            int ch, tok;
+            tile_at(t, ch, tok);
+            const W8Mat& mat = p.grp.m[mat_of(ch)];
+            const int n = (ch - mat.tile0) * kCh + 32 * sub + lane;
+            const bool live = n < mat.N;
+            if (!SPLIT) {
+                const float sw = live ? mat.scales[n] : 0.0f;
+                float* out = mat.out + n;
+                const int m_end = min(NT, p.M - tok * NT);
+                for (int c = 0; c < m_end; c += 16) {
+                    int v[16];
+                    tmem_ld16(tmem + lanes + buf * NT + c, v);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int m = tok * NT + c + j;
+                        if (live && c + j < m_end) __stcs(out + (int64_t)m * mat.N, __fmul_rn(__fmul_rn((float)v[j], __ldg(p.sx + m)), sw));
+                    }
+                }
+            } else {
+                // columns [r * per, (r + 1) * per) of this tile are rank r's: [rank][column][channel]
+                const int per = NT / cs;
+                const uint32_t mine = su32(smem + C::kOffX) + (uint32_t)((rank * per * kCh + 32 * sub + lane) * 4);
+                for (int c = 0; c < NT; c += 16) {
+                    int v[16];
+                    tmem_ld16(tmem + lanes + c, v);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int owner = (c + j) / per;
+                        uint32_t at;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                                     : "=r"(at)
+                                     : "r"(mine + (uint32_t)((c + j - owner * per) * kCh * 4)), "r"(owner));
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&acc_empty[buf]);
+        }
+    }
+
+    // ---- tear-down: every path frees TMEM ----
+    __syncthreads();
+    if (SPLIT) {  // every rank's sums have arrived
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        int ch, tok;
+        tile_at(blockIdx.x, ch, tok);
+        const W8Mat& mat = p.grp.m[mat_of(ch)];
+        const int per = NT / cs;
+        const int* got = reinterpret_cast<const int*>(smem + C::kOffX);
+        for (int i = tid; i < per * kCh; i += kTcThreads) {
+            const int c = i / kCh, n = (ch - mat.tile0) * kCh + i % kCh, m = tok * NT + rank * per + c;
+            int sum = 0;
+            for (int r = 0; r < cs; r++) sum += got[r * per * kCh + i];
+            if (m < p.M && n < mat.N)
+                mat.out[(int64_t)m * mat.N + n] = __fmul_rn(__fmul_rn((float)sum, __ldg(p.sx + m)), mat.scales[n]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && *abort_flag) atomicOr(&g_w8a8_error, kErrTimeout);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------- launch --
+std::atomic<uint64_t> g_used_on{0};  // devices a tcgen05 launch ran on (its error word may be set there)
+
+int encode_rows(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t K, int box_rows) {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> cached{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 encode = cached.load(std::memory_order_acquire);
+    if (!encode) {
+        cudaDriverEntryPointQueryResult q;
+        void* fn = nullptr;
+        S1KV_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !fn)
+            return set_error(S1KV_ECUDA, "matmul_w8a8: cuTensorMapEncodeTiled unavailable");
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+        cached.store(encode, std::memory_order_release);
+    }
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)K};
+    cuuint32_t box[2] = {(cuuint32_t)kKB, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(S1KV_EINVAL, "matmul_w8a8: tensor map rejected (%d)", (int)r);
+    return S1KV_OK;
+}
+
+template <int NT, bool SPLIT>
+int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int ch_tiles, int cs, cudaStream_t stream) {
+    auto kern = w8a8_tc_kernel<NT, SPLIT>;
+    static std::atomic<uint64_t> attr_set{0};  // per device
+    int st = once_per_device(attr_set, [&] {
+        S1KV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<NT>::kSmem));
+        return S1KV_OK;
+    });
+    if (st) return st;
+    TcParams p{};
+    p.grp = grp;
+    p.sx = sx;
+    p.M = M;
+    p.k_blocks = (K + kKB - 1) / kKB;
+    p.ch_tiles = ch_tiles;
+    p.tok_tiles = (M + NT - 1) / NT;
+    TcMaps maps;
+    st = encode_rows(&maps.x, xq, M, K, NT);
+    for (int i = 0; i < grp.n && !st; i++) st = encode_rows(&maps.w[i], grp.m[i].w, grp.m[i].N, K, kCh);
+    if (st) return st;
+    for (int i = grp.n; i < kMaxMats; i++) maps.w[i] = maps.w[0];
+    int dev = 0;
+    S1KV_CUDA(cudaGetDevice(&dev));
+    if (dev < 64) g_used_on.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+    const int tiles = ch_tiles * p.tok_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = SPLIT ? dim3((unsigned)tiles, (unsigned)cs) : dim3((unsigned)std::min(tiles, 148));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = TcCfg<NT>::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)cs;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    S1KV_CUDA(cudaLaunchKernelEx(&cfg, kern, p, maps));
+    g_launches++;
+    return S1KV_OK;
+}
+
+template <int NTILE>
+int launch_gemv(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int tiles, cudaStream_t stream) {
+    S1KV_CUDA(launch_pdl(w8a8_gemv_kernel<NTILE>, dim3((unsigned)tiles), dim3(kGemvWarps * 32), 0, stream, xq, sx, M, K, grp));
+    g_launches++;
+    return S1KV_OK;
+}
+
+// Which kernel, by the tokens: up to 16 the weight stream; above, the
+// tensor-core tiles with the least NT that holds the tokens (256 at most),
+// and K split over a cluster while the tiles do not fill the 148 SMs.
+int matmul_w8a8(const int8_t* xq, const float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
+    const int rows = M <= 16 || K == 0 ? 16 : kCh;
+    int64_t tiles = 0;
+    for (int i = 0; i < grp.n; i++) {
+        grp.m[i].tile0 = (int)tiles;
+        tiles += (grp.m[i].N + rows - 1) / rows;
+    }
+    const int NT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    if (tiles * ((M + NT - 1) / NT) > INT32_MAX) return set_error(S1KV_EINVAL, "matmul_w8a8: more than 2^31 tiles");
+    if (K == 0) {  // empty sums
+        for (int i = 0; i < grp.n; i++)
+            S1KV_CUDA(cudaMemsetAsync(grp.m[i].out, 0, sizeof(float) * (size_t)M * grp.m[i].N, stream));
+        return S1KV_OK;
+    }
+    if (M <= 8) return launch_gemv<1>(xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 16) return launch_gemv<2>(xq, sx, M, K, grp, (int)tiles, stream);
+    const int k_blocks = (K + kKB - 1) / kKB;
+    int cs = 1;
+    if (NT <= 128)
+        while (cs < 8 && tiles * cs * 2 <= 148 + 74 && k_blocks >= cs * 4) cs *= 2;
+#define S1KV_TC(NT_)                                                                                       \
+    if (NT == NT_)                                                                                         \
+        return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, stream)                     \
+                      : launch_tc<NT_, false>(xq, sx, M, K, grp, (int)tiles, 1, stream);
+    S1KV_TC(32) S1KV_TC(64) S1KV_TC(128)
+#undef S1KV_TC
+    return launch_tc<256, false>(xq, sx, M, K, grp, (int)tiles, 1, stream);
 }
 
 }  // namespace
+
+int w8a8_take_error(int device, int* flags) {
+    *flags = 0;
+    if (device < 0 || device >= 64 || !(g_used_on.load(std::memory_order_relaxed) >> device & 1)) return S1KV_OK;
+    int h = 0;
+    S1KV_CUDA(cudaMemcpyFromSymbol(&h, g_w8a8_error, sizeof(int), 0, cudaMemcpyDeviceToHost));
+    if (h) {
+        const int zero = 0;
+        S1KV_CUDA(cudaMemcpyToSymbol(g_w8a8_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice));
+    }
+    *flags = h;
+    return S1KV_OK;
+}
 }  // namespace s1kv
 
 using namespace s1kv;
@@ -132,7 +606,6 @@ extern "C" int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, i
         return set_error(S1KV_EINVAL, "matmul_w8a8: M %lld, K %lld (a multiple of 16 up to %lld)", (long long)M, (long long)K,
                          (long long)kMaxK);
     W8Group grp = {};
-    int tiles = 0;
     for (int i = 0; i < n_mats; i++) {
         if (N[i] < 0 || N[i] > (1 << 30)) return set_error(S1KV_EINVAL, "matmul_w8a8: bad shape");
         if (M == 0 || N[i] == 0) continue;
@@ -140,21 +613,10 @@ extern "C" int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, i
             return set_error(S1KV_EINVAL, "matmul_w8a8: null pointer");
         if (((uintptr_t)xq | (uintptr_t)w[i]) & 15)
             return set_error(S1KV_EINVAL, "matmul_w8a8: xq and w must be 16-byte aligned");
-        grp.m[grp.n++] = {w[i], w_scales[i], out[i], (int)N[i], tiles};
-        tiles += (int)((N[i] + 63) / 64);
+        grp.m[grp.n++] = {w[i], w_scales[i], out[i], (int)N[i], 0};
     }
     if (grp.n == 0) return S1KV_OK;
-    const int64_t row_tiles = (M + 63) / 64;
-    for (int64_t r0 = 0; r0 < row_tiles; r0 += 65535) {  // grid.y's limit
-        const int64_t m0 = r0 * 64, m = std::min<int64_t>(M - m0, 65535 * 64);
-        W8Group g = grp;
-        for (int i = 0; i < g.n; i++) g.m[i].out += m0 * g.m[i].N;
-        w8a8_tile_kernel<<<dim3((unsigned)tiles, (unsigned)((m + 63) / 64)), 256, 0, (cudaStream_t)stream>>>(
-            xq + m0 * K, x_scales + m0, (int)m, (int)K, g);
-        g_launches++;
-        S1KV_CUDA(cudaGetLastError());
-    }
-    return S1KV_OK;
+    return matmul_w8a8(xq, x_scales, (int)M, (int)K, grp, (cudaStream_t)stream);
 }
 
 extern "C" int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, const int8_t* w,
