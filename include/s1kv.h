@@ -481,9 +481,21 @@ int s1kv_quantize_tokens(const float* x, int64_t M, int64_t K, int8_t* q, int64_
  * channel (an nn.Linear weight's order): s1kv_quantize_rows of that [N][K]
  * matrix makes q and scales.  K is the padded row length: a multiple of 16
  * up to 131072, xq zero past the true K (w may hold anything there); xq and w
- * 16-byte aligned. */
+ * 16-byte aligned.  The products are programmatic dependent launches that
+ * request weights while the previous kernel of the stream is still running: a
+ * caller's own programmatic-dependent kernel that writes weights must not come
+ * directly before them. */
 int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, const int8_t* w,
                      const float* w_scales, int64_t N, float* out, void* stream);
+/* Both in one call: x [M][K] fp32 (any K up to 131072) quantised per token and
+ * multiplied with up to 4 weights [N[i]][K rounded up to a multiple of 16].
+ * The codes and scales go to `workspace` (device, 16-byte aligned, at least
+ * s1kv_w8a8_workspace(M, K) bytes, borrowed until the stream work completes);
+ * for one or two tokens a single kernel does it all. */
+int64_t s1kv_w8a8_workspace(int64_t M, int64_t K);
+int s1kv_linear_w8a8_group(const float* x, int64_t M, int64_t K, void* workspace, int64_t workspace_bytes,
+                           int32_t n_mats, const int8_t* const* w, const float* const* w_scales, const int64_t* N,
+                           float* const* out, void* stream);
 /* Up to 4 products sharing xq in one launch (q/k/v, gate/up): out[i]
  * [M][N[i]], the same results as separate calls; the arrays (host memory)
  * hold device pointers. */

@@ -17,7 +17,7 @@ constexpr int kSMs = 148;
 // the L1 cache, before the quantisation.
 template <int LANES, int NQ, bool ROPE>
 __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
-    pdl_enter();
+    pdl_wait_trigger();
     const int D = p.D, half = D / 2, nq = D / 4;
     constexpr int RPW = 32 / LANES;
     const int lane = threadIdx.x & 31, lr = lane % LANES;

@@ -36,39 +36,91 @@ struct W8Group {
     int n;
 };
 
-// 0 .. 255 codes of one value; inv = 1 / s.  The fp32 quotient is within
-// 127 * 3 * 2^-24 = 2.3e-5 of the real one: only one this near a tie (or not
-// finite, for a tiny s) is decided in 64 bits.
+// x / s to the nearest integer where fp32 cannot tell (next to a tie, or 1 / s
+// overflowed), in 64 bits.
+__device__ __noinline__ float token_code_near_tie(float x, float s) {
+    return s > 0.0f ? (float)rint((double)x / (double)s) : 0.0f;
+}
+
+// Code of one value, -127 .. 127; inv = 1 / s.  The fp32 quotient is within
+// 127 * 3 * 2^-24 = 2.3e-5 of the real one.
 __device__ __forceinline__ int token_code(float x, float s, float inv) {
     const float q = x * inv;
     float n = rintf(q);
-    if (!(fabsf(q - n) < 0.49995f)) n = s > 0.0f ? (float)rint((double)x / (double)s) : 0.0f;
+    if (!(fabsf(q - n) < 0.49995f)) n = token_code_near_tie(x, s);
     return (int)fminf(fmaxf(n, -127.0f), 127.0f);
 }
 
-__global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __restrict__ x, int64_t M, int64_t K,
-                                                              int8_t* __restrict__ q, int64_t ldq,
-                                                              float* __restrict__ scales) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ float part[8];
-    const int64_t m = blockIdx.x;
-    const float* src = x + m * K;
-    float mx = 0.0f;
-    for (int64_t k = threadIdx.x; k < K; k += 256) {
-        const float a = fabsf(src[k]);
-        mx = a < INFINITY ? fmaxf(mx, a) : INFINITY;
-    }
+__device__ __forceinline__ uint32_t token_codes4(float4 x, float s, float inv) {
+    return (uint32_t)(token_code(x.x, s, inv) & 255) | (uint32_t)(token_code(x.y, s, inv) & 255) << 8 |
+           (uint32_t)(token_code(x.z, s, inv) & 255) << 16 | (uint32_t)(token_code(x.w, s, inv) & 255) << 24;
+}
+
+// |x| of the largest, infinite once any is not finite.
+__device__ __forceinline__ float top_of(float mx, float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? fmaxf(mx, a) : INFINITY;
+}
+
+// Maximum over the CTA's 256 threads; `part` is 8 floats of shared memory.
+__device__ __forceinline__ float cta_max(float mx, float* part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = mx;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) mx = fmaxf(mx, part[i]);
+    return mx;
+}
+
+__device__ __forceinline__ float token_scale(float mx) { return mx > 0.0f ? __fdiv_rn(mx, 127.0f) : 1.0f; }
+
+// A row a CTA.  NV > 0: rows of up to 1024 NV values, a multiple of 4 and
+// 16-byte aligned, stay in registers between the maximum and the codes (one
+// read of x); NV = 0: any row, read twice.
+template <int NV>
+__global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __restrict__ x, int64_t K, int8_t* __restrict__ q,
+                                                              int64_t ldq, float* __restrict__ scales) {
+    pdl_wait_trigger();
+    __shared__ float part[8];
+    const int64_t m = blockIdx.x;
+    const float* src = x + m * K;
+    float mx = 0.0f;
+    float4 v[NV > 0 ? NV : 1];
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int k = 4 * (threadIdx.x + 256 * i);
+            v[i] = k < K ? __ldcs(reinterpret_cast<const float4*>(src + k)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            mx = top_of(top_of(top_of(top_of(mx, v[i].x), v[i].y), v[i].z), v[i].w);
+        }
+    } else {
+        for (int64_t k = threadIdx.x; k < K; k += 256) mx = top_of(mx, src[k]);
+    }
+    mx = cta_max(mx, part);
     const bool fine = mx < INFINITY;
-    const float s = mx > 0.0f ? __fdiv_rn(mx, 127.0f) : 1.0f, inv = __frcp_rn(s);
+    const float s = token_scale(mx), inv = __frcp_rn(s);
     if (threadIdx.x == 0) scales[m] = fine ? s : __uint_as_float(0x7FC00000u);
-    for (int64_t k = threadIdx.x; k < ldq; k += 256)
-        q[m * ldq + k] = (int8_t)(fine && k < K ? token_code(src[k], s, inv) : 0);
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int k = 4 * (threadIdx.x + 256 * i);
+            if (k < ldq) *reinterpret_cast<uint32_t*>(q + m * ldq + k) = fine ? token_codes4(v[i], s, inv) : 0u;
+        }
+    } else {
+        for (int64_t k = threadIdx.x; k < ldq; k += 256)
+            q[m * ldq + k] = (int8_t)(fine && k < K ? token_code(src[k], s, inv) : 0);
+    }
+}
+
+int launch_quantize(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scales, cudaStream_t stream) {
+    const int nv = K % 4 || ((uintptr_t)x & 15) || ldq > 8192 ? 0 : ldq <= 1024 ? 1 : ldq <= 2048 ? 2 : ldq <= 4096 ? 4 : 8;
+    auto kern = nv == 0 ? quantize_tokens_kernel<0>
+                        : nv == 1 ? quantize_tokens_kernel<1>
+                                  : nv == 2 ? quantize_tokens_kernel<2> : nv == 4 ? quantize_tokens_kernel<4> : quantize_tokens_kernel<8>;
+    S1KV_CUDA(launch_pdl(kern, dim3((unsigned)M), dim3(256), 0, stream, x, K, q, ldq, scales));
+    g_launches++;
+    return S1KV_OK;
 }
 
 // ---------------------------------------------- few tokens: weight stream --
@@ -82,6 +134,10 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __res
 // integer sums meet in shared memory.  The first steps' weights are
 // requested before the wait for the previous kernel (the token quantiser):
 // they do not depend on it.
+// FUSED (one or two tokens of up to kFusedK values): each CTA quantises the
+// tokens itself, from x through L2 into its shared memory, while its first
+// weights are on their way: one launch instead of two.
+constexpr int kFusedK = 16384, kFusedM = 2;
 constexpr int kGemvWarps = 8;
 constexpr int kGemvPre = 4;  // 128-byte steps in flight a warp
 
@@ -93,9 +149,12 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NTILE>
-__global__ void __launch_bounds__(kGemvWarps * 32) w8a8_gemv_kernel(const int8_t* __restrict__ xq, const float* __restrict__ sx,
-                                                                   int M, int K, const __grid_constant__ W8Group grp) {
+template <int NTILE, bool FUSED>
+__global__ void __launch_bounds__(kGemvWarps * 32)
+    w8a8_gemv_kernel(const float* __restrict__ x, int x_len, const int8_t* __restrict__ xq, const float* __restrict__ sx, int M,
+                     int K, const __grid_constant__ W8Group grp) {
+    extern __shared__ uint4 own[];  // FUSED: the tokens' codes, K bytes each
+    __shared__ float part[8], own_scale[kFusedM];
     __shared__ int red[kGemvWarps][16][8 * NTILE + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int mi = 0;
@@ -121,8 +180,32 @@ __global__ void __launch_bounds__(kGemvWarps * 32) w8a8_gemv_kernel(const int8_t
     };
 #pragma unroll
     for (int s = 0; s < kGemvPre; s++) fetch(s, a[s]);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_wait_trigger();
+    if (FUSED) {
+        for (int m = 0; m < M; m++) {
+            const float* src = x + (int64_t)m * x_len;
+            float4 v[kFusedK / 1024];  // a row of up to 16 K values, 64 a thread: only what K needs is touched
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFusedK / 1024; i++) {
+                if (i * 1024 >= K) break;
+                const int k = 4 * (threadIdx.x + 256 * i);
+                v[i] = k < x_len ? *reinterpret_cast<const float4*>(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                mx = top_of(top_of(top_of(top_of(mx, v[i].x), v[i].y), v[i].z), v[i].w);
+            }
+            mx = cta_max(mx, part);
+            const bool fine = mx < INFINITY;
+            const float s = token_scale(mx), inv = __frcp_rn(s);
+            if (threadIdx.x == 0) own_scale[m] = fine ? s : __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int i = 0; i < kFusedK / 1024; i++) {
+                if (i * 1024 >= K) break;
+                const int k = 4 * (threadIdx.x + 256 * i);
+                if (k < K) reinterpret_cast<uint32_t*>(own)[(m * K + k) / 4] = fine ? token_codes4(v[i], s, inv) : 0u;
+            }
+            __syncthreads();  // codes written; part free for the next row
+        }
+    }
     int acc[NTILE][4] = {};
     for (int s0 = 0; s0 < steps; s0 += kGemvPre) {
 #pragma unroll
@@ -136,8 +219,9 @@ __global__ void __launch_bounds__(kGemvWarps * 32) w8a8_gemv_kernel(const int8_t
 #pragma unroll
                 for (int nt = 0; nt < NTILE; nt++) {
                     // tokens past the last read the last one's bytes; their columns are not stored
-                    const uint4 b = k < K ? __ldg(reinterpret_cast<const uint4*>(xq + (int64_t)min(8 * nt + g, M - 1) * K + k))
-                                          : make_uint4(0, 0, 0, 0);
+                    const int64_t at = (int64_t)min(8 * nt + g, M - 1) * K + k;
+                    const uint4 b = k >= K ? make_uint4(0, 0, 0, 0)
+                                           : FUSED ? own[at >> 4] : __ldg(reinterpret_cast<const uint4*>(xq + at));
                     imma16832(acc[nt], x.x, y.x, x.y, y.y, b.x, b.y);
                     imma16832(acc[nt], x.z, y.z, x.w, y.w, b.z, b.w);
                 }
@@ -156,7 +240,7 @@ __global__ void __launch_bounds__(kGemvWarps * 32) w8a8_gemv_kernel(const int8_t
 #pragma unroll
         for (int w = 0; w < kGemvWarps; w++) sum += red[w][n][m];
         if (m < M && n0 + n < mat.N)
-            mat.out[(int64_t)m * mat.N + n0 + n] = __fmul_rn(__fmul_rn((float)sum, sx[m]), mat.scales[n0 + n]);
+            mat.out[(int64_t)m * mat.N + n0 + n] = __fmul_rn(__fmul_rn((float)sum, FUSED ? own_scale[m] : sx[m]), mat.scales[n0 + n]);
     }
 }
 
@@ -182,12 +266,13 @@ constexpr int kCh = 128;             // channels a tile
 constexpr int kKB = 128;             // bytes of K a stage
 constexpr int kTcThreads = 192;      // TMA warp, MMA warp, 4 epilogue warps
 
-template <int NT>
+template <int NT, bool SPLIT>
 struct TcCfg {
     static constexpr int kStageBytes = kKB * (kCh + NT);
-    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 5 : 6;
-    static constexpr int kCols = 2 * NT;                       // two accumulators
-    static constexpr int kExchange = NT <= 128 ? kCh * NT * 4 : 0;  // split tiles: [rank][channel][slice] sums
+    // split tiles leave room for a second CTA on the SM where they can
+    static constexpr int kStages = NT == 256 ? 4 : !SPLIT ? 6 : NT == 128 ? 5 : NT == 64 ? 3 : 4;
+    static constexpr int kCols = (SPLIT ? 1 : 2) * NT;             // two accumulators for a chain of tiles
+    static constexpr int kExchange = SPLIT ? kCh * NT * 4 : 0;     // [rank][token of the slice][channel] sums
     static constexpr int kOffX = kStages * kStageBytes;
     static constexpr int kOffBar = kOffX + kExchange;
     static constexpr int kNumBars = 2 * kStages + 5;
@@ -286,7 +371,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
 template <int NT, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     w8a8_tc_kernel(const __grid_constant__ TcParams p, const __grid_constant__ TcMaps maps) {
-    using C = TcCfg<NT>;
+    using C = TcCfg<NT, SPLIT>;
     constexpr int ST = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -339,7 +424,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ================= TMA producer =================
         int it = 0;  // stages used so far
         bool ok = true;
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        // the weights of the first stages do not depend on the kernel before
+        // this one (the token quantiser): requested before the wait for it
+        int pre = 0;
+        {
+            int ch, tok;
+            tile_at(blockIdx.x, ch, tok);
+            const int mi = mat_of(ch), n0 = (ch - p.grp.m[mi].tile0) * kCh;
+            pre = min(ST, kb1 - kb0);
+            for (int s = 0; s < pre; s++)
+                if (lane == 0) {
+                    bar_expect(&full[s], C::kStageBytes);
+                    tma2(su32(smem + s * C::kStageBytes), &maps.w[mi], &full[s], (kb0 + s) * kKB, n0);
+                }
+            __syncwarp();
+        }
+        pdl_wait();
         for (int t = blockIdx.x; t < n_tiles && ok; t += gridDim.x) {
             int ch, tok;
             tile_at(t, ch, tok);
@@ -349,8 +449,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (it >= ST && !(ok = warp_wait(&empty[s], (uint32_t)((it / ST - 1) & 1), abort_flag))) break;
                 if (lane == 0) {
                     const uint32_t at = su32(smem + s * C::kStageBytes);
-                    bar_expect(&full[s], C::kStageBytes);
-                    tma2(at, &maps.w[mi], &full[s], kb * kKB, n0);
+                    if (it >= pre) {
+                        bar_expect(&full[s], C::kStageBytes);
+                        tma2(at, &maps.w[mi], &full[s], kb * kKB, n0);
+                    }
                     tma2(at + kCh * kKB, &maps.x, &full[s], kb * kKB, tok * NT);
                 }
                 __syncwarp();
@@ -384,6 +486,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bar_wait(drain, 0);
     } else {
         // ================= epilogue =================
+        pdl_wait_trigger();  // the scales of the tokens, and outputs the kernel before may still read
         const int sub = warp & 3;  // the TMEM lanes 32 sub .. + 31 are this warp's
         const uint32_t lanes = (uint32_t)(32 * sub) << 16;
         int done = 0;
@@ -436,6 +539,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---- tear-down: every path frees TMEM ----
     __syncthreads();
     if (SPLIT) {  // every rank's sums have arrived
+        pdl_wait();
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         int ch, tok;
@@ -489,7 +593,8 @@ int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& gr
     auto kern = w8a8_tc_kernel<NT, SPLIT>;
     static std::atomic<uint64_t> attr_set{0};  // per device
     int st = once_per_device(attr_set, [&] {
-        S1KV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<NT>::kSmem));
+        constexpr int bytes = TcCfg<NT, SPLIT>::kSmem;
+        S1KV_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         return S1KV_OK;
     });
     if (st) return st;
@@ -512,23 +617,27 @@ int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& gr
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = SPLIT ? dim3((unsigned)tiles, (unsigned)cs) : dim3((unsigned)std::min(tiles, 148));
     cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = TcCfg<NT>::kSmem;
+    cfg.dynamicSmemBytes = TcCfg<NT, SPLIT>::kSmem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = (unsigned)cs;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = (unsigned)cs;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = SPLIT ? 1 : 0;
+    cfg.numAttrs = SPLIT ? 2 : 1;
     S1KV_CUDA(cudaLaunchKernelEx(&cfg, kern, p, maps));
     g_launches++;
     return S1KV_OK;
 }
 
-template <int NTILE>
-int launch_gemv(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int tiles, cudaStream_t stream) {
-    S1KV_CUDA(launch_pdl(w8a8_gemv_kernel<NTILE>, dim3((unsigned)tiles), dim3(kGemvWarps * 32), 0, stream, xq, sx, M, K, grp));
+template <int NTILE, bool FUSED>
+int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int tiles,
+                cudaStream_t stream) {
+    S1KV_CUDA(launch_pdl(w8a8_gemv_kernel<NTILE, FUSED>, dim3((unsigned)tiles), dim3(kGemvWarps * 32),
+                         FUSED ? (size_t)M * K : 0, stream, x, x_len, xq, sx, M, K, grp));
     g_launches++;
     return S1KV_OK;
 }
@@ -536,7 +645,9 @@ int launch_gemv(const int8_t* xq, const float* sx, int M, int K, const W8Group& 
 // Which kernel, by the tokens: up to 16 the weight stream; above, the
 // tensor-core tiles with the least NT that holds the tokens (256 at most),
 // and K split over a cluster while the tiles do not fill the 148 SMs.
-int matmul_w8a8(const int8_t* xq, const float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
+// x (optional, rows of x_len values): the tokens that xq and sx will hold; they
+// are quantised here first, or by the weight stream itself.
+int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
     const int rows = M <= 16 || K == 0 ? 16 : kCh;
     int64_t tiles = 0;
     for (int i = 0; i < grp.n; i++) {
@@ -550,12 +661,19 @@ int matmul_w8a8(const int8_t* xq, const float* sx, int M, int K, W8Group& grp, c
             S1KV_CUDA(cudaMemsetAsync(grp.m[i].out, 0, sizeof(float) * (size_t)M * grp.m[i].N, stream));
         return S1KV_OK;
     }
-    if (M <= 8) return launch_gemv<1>(xq, sx, M, K, grp, (int)tiles, stream);
-    if (M <= 16) return launch_gemv<2>(xq, sx, M, K, grp, (int)tiles, stream);
+    // 32 KB of codes at most: within the static limit with the 5 KB of sums
+    if (x && M <= kFusedM && K <= kFusedK && x_len % 4 == 0 && ((uintptr_t)x & 15) == 0)
+        return launch_gemv<1, true>(x, x_len, nullptr, nullptr, M, K, grp, (int)tiles, stream);
+    if (x) {
+        const int st = launch_quantize(x, M, x_len, xq, K, sx, stream);
+        if (st) return st;
+    }
+    if (M <= 8) return launch_gemv<1, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 16) return launch_gemv<2, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
     int cs = 1;
     if (NT <= 128)
-        while (cs < 8 && tiles * cs * 2 <= 148 + 74 && k_blocks >= cs * 4) cs *= 2;
+        while (cs < 8 && tiles * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
 #define S1KV_TC(NT_)                                                                                       \
     if (NT == NT_)                                                                                         \
         return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, stream)                     \
@@ -591,15 +709,12 @@ extern "C" int s1kv_quantize_tokens(const float* x, int64_t M, int64_t K, int8_t
     if (M == 0) return S1KV_OK;
     if ((K > 0 && !x) || (ldq > 0 && !q) || !scales) return set_error(S1KV_EINVAL, "quantize_tokens: null pointer");
     if ((uintptr_t)q & 15) return set_error(S1KV_EINVAL, "quantize_tokens: q must be 16-byte aligned");
-    quantize_tokens_kernel<<<(unsigned)M, 256, 0, (cudaStream_t)stream>>>(x, M, K, q, ldq, scales);
-    g_launches++;
-    S1KV_CUDA(cudaGetLastError());
-    return S1KV_OK;
+    return launch_quantize(x, M, K, q, ldq, scales, (cudaStream_t)stream);
 }
 
-extern "C" int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, int32_t n_mats,
-                                      const int8_t* const* w, const float* const* w_scales, const int64_t* N,
-                                      float* const* out, void* stream) {
+static int w8a8_group(const float* x, int64_t x_len, int8_t* xq, float* x_scales, int64_t M, int64_t K, int32_t n_mats,
+                      const int8_t* const* w, const float* const* w_scales, const int64_t* N, float* const* out,
+                      void* stream) {
     if (!w || !w_scales || !N || !out) return set_error(S1KV_EINVAL, "matmul_w8a8: null array");
     if (n_mats < 1 || n_mats > kMaxMats) return set_error(S1KV_EINVAL, "matmul_w8a8: 1 to %d matrices per call", kMaxMats);
     if (M < 0 || M > (1 << 30) || K < 0 || K > kMaxK || K % 16)
@@ -616,7 +731,33 @@ extern "C" int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, i
         grp.m[grp.n++] = {w[i], w_scales[i], out[i], (int)N[i], 0};
     }
     if (grp.n == 0) return S1KV_OK;
-    return matmul_w8a8(xq, x_scales, (int)M, (int)K, grp, (cudaStream_t)stream);
+    return matmul_w8a8(x, (int)x_len, xq, x_scales, (int)M, (int)K, grp, (cudaStream_t)stream);
+}
+
+extern "C" int s1kv_matmul_w8a8_group(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, int32_t n_mats,
+                                      const int8_t* const* w, const float* const* w_scales, const int64_t* N,
+                                      float* const* out, void* stream) {
+    return w8a8_group(nullptr, 0, const_cast<int8_t*>(xq), const_cast<float*>(x_scales), M, K, n_mats, w, w_scales, N, out,
+                      stream);
+}
+
+extern "C" int64_t s1kv_w8a8_workspace(int64_t M, int64_t K) {
+    if (M < 0 || M > (1 << 30) || K < 0 || K > kMaxK) return 0;
+    return M * ((K + 15) / 16 * 16) + (4 * M + 15) / 16 * 16;
+}
+
+extern "C" int s1kv_linear_w8a8_group(const float* x, int64_t M, int64_t K, void* workspace, int64_t workspace_bytes,
+                                      int32_t n_mats, const int8_t* const* w, const float* const* w_scales, const int64_t* N,
+                                      float* const* out, void* stream) {
+    if (M < 0 || M > (1 << 30) || K < 0 || K > kMaxK)
+        return set_error(S1KV_EINVAL, "linear_w8a8: M %lld, K %lld (up to %lld)", (long long)M, (long long)K, (long long)kMaxK);
+    if (M > 0 && K > 0 && !x) return set_error(S1KV_EINVAL, "linear_w8a8: null x");
+    if (workspace_bytes < s1kv_w8a8_workspace(M, K) || (workspace_bytes > 0 && !workspace) || ((uintptr_t)workspace & 15))
+        return set_error(S1KV_EINVAL, "linear_w8a8: needs %lld bytes of 16-byte aligned workspace",
+                         (long long)s1kv_w8a8_workspace(M, K));
+    const int64_t ld = (K + 15) / 16 * 16;
+    int8_t* xq = (int8_t*)workspace;
+    return w8a8_group(x, K, xq, (float*)(xq + M * ld), M, ld, n_mats, w, w_scales, N, out, stream);
 }
 
 extern "C" int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, const int8_t* w,

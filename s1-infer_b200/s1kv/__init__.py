@@ -131,6 +131,8 @@ SIGNATURES = {
     "s1kv_matmul_int8": (C.c_int, [vp, i64, i64, vp, vp, i64, vp, vp]),
     "s1kv_matmul_int8_group": (C.c_int, [vp, i64, i64, i32, vp, vp, vp, vp, vp]),
     "s1kv_quantize_tokens": (C.c_int, [vp, i64, i64, vp, i64, vp, vp]),
+    "s1kv_w8a8_workspace": (i64, [i64, i64]),
+    "s1kv_linear_w8a8_group": (C.c_int, [vp, i64, i64, vp, i64, i32, vp, vp, vp, vp, vp]),
     "s1kv_matmul_w8a8": (C.c_int, [vp, vp, i64, i64, vp, vp, i64, vp, vp]),
     "s1kv_matmul_w8a8_group": (C.c_int, [vp, vp, i64, i64, i32, vp, vp, vp, vp, vp]),
     "s1kv_launch_count": (i64, []),
@@ -166,13 +168,14 @@ def _i32p(a):
     return a.ctypes.data_as(P(i32)) if a is not None else None
 
 
-def _stream():
+def _stream(device=None):
+    """torch's current stream on `device` (None = the current device)."""
     import torch
-    return vp(torch.cuda.current_stream().cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device)
 
 
 def _dptr(t):
-    return vp(t.data_ptr()) if t is not None else None
+    return t.data_ptr() if t is not None else None
 
 
 def _cuda_f32(x, device):
@@ -323,7 +326,7 @@ class Pool:
         return f.value
 
     def flush(self):
-        check(self.L.s1kv_flush(self.h, _stream()))
+        check(self.L.s1kv_flush(self.h, _stream(self.device)))
 
     def read_storage(self, layer, which, slot0=0, n_slots=None):
         """Raw storage rows [slot0, slot0+n_slots) as numpy (float32 or the
@@ -341,7 +344,7 @@ class Pool:
         import torch
         k, v = _cuda_f32(k, self.device), _cuda_f32(v, self.device)
         s = torch.as_tensor(slots, dtype=torch.int32).to(self.device)
-        check(self.L.s1kv_append(self.h, layer, _dptr(k), _dptr(v), _dptr(s), k.shape[0], _stream()))
+        check(self.L.s1kv_append(self.h, layer, _dptr(k), _dptr(v), _dptr(s), k.shape[0], _stream(self.device)))
 
     def rope_append(self, layer, k, v, slots, pos, q=None):
         import torch
@@ -352,20 +355,20 @@ class Pool:
         q_out = torch.empty_like(q_in) if q_in is not None else None
         max_pos = int(np.max(np.asarray(pos))) + 1 if len(pos) else 0
         check(self.L.s1kv_rope_append(self.h, layer, _dptr(q_in), _dptr(q_out), q_in.shape[1] if q_in is not None else 0,
-                                      _dptr(k), _dptr(v), _dptr(s), _dptr(p), k.shape[0], max_pos, _stream()))
+                                      _dptr(k), _dptr(v), _dptr(s), _dptr(p), k.shape[0], max_pos, _stream(self.device)))
         return q_out
 
     def gather(self, layer, seq, which):
         import torch
         out = torch.empty((self.length(seq), self.Hkv, self.D), dtype=torch.float32, device=self.device)
-        check(self.L.s1kv_gather(self.h, layer, seq, which, _dptr(out), _stream()))
+        check(self.L.s1kv_gather(self.h, layer, seq, which, _dptr(out), _stream(self.device)))
         return out
 
     def cow_copy(self, src, dst):
         import torch
         s = torch.as_tensor(src, dtype=torch.int32).to(self.device)
         d = torch.as_tensor(dst, dtype=torch.int32).to(self.device)
-        check(self.L.s1kv_cow_copy(self.h, _dptr(s), _dptr(d), s.numel(), _stream()))
+        check(self.L.s1kv_cow_copy(self.h, _dptr(s), _dptr(d), s.numel(), _stream(self.device)))
 
     def attention(self, layer, seqs, q_lens, q, n_q_heads):
         import torch
@@ -374,7 +377,7 @@ class Pool:
         q = _cuda_f32(q, self.device)
         out = torch.empty_like(q)
         check(self.L.s1kv_attention(self.h, layer, seqs.ctypes.data_as(P(u64)), _i32p(ql), seqs.size, _dptr(q),
-                                    _dptr(out), n_q_heads, _stream()))
+                                    _dptr(out), n_q_heads, _stream(self.device)))
         return out
 
     def batch(self, seqs, n_append=None, q_lens=None):
@@ -392,7 +395,7 @@ class Batch:
         self.ql = None if q_lens is None else np.ascontiguousarray(q_lens, dtype=np.int32)
         h = vp()
         check(self.L.s1kv_batch_begin(pool.h, self.seqs.ctypes.data_as(P(u64)), _i32p(self.na), _i32p(self.ql),
-                                      self.seqs.size, _stream(), C.byref(h)))
+                                      self.seqs.size, _stream(pool.device), C.byref(h)))
         self.h = h
         nt, nr = i64(), i64()
         check(self.L.s1kv_batch_sizes(h, C.byref(nt), C.byref(nr)))
@@ -410,7 +413,7 @@ class Batch:
         if q is not None and q_out is None:
             q_out = torch.empty_like(q)
         check(self.L.s1kv_batch_rope_append(self.h, layer, _dptr(q), _dptr(q_out), q.shape[1] if q is not None else 0,
-                                            _dptr(k), _dptr(v), _stream()))
+                                            _dptr(k), _dptr(v), _stream(self.pool.device)))
         return q_out
 
     def norm_rope_append(self, layer, k, v, k_norm_weight, q=None, q_norm_weight=None, eps=1e-6, q_out=None):
@@ -422,11 +425,11 @@ class Batch:
             q_out = torch.empty_like(q)
         check(self.L.s1kv_batch_norm_rope_append(self.h, layer, _dptr(q), _dptr(q_out),
                                                  q.shape[1] if q is not None else 0, _dptr(q_norm_weight), _dptr(k),
-                                                 _dptr(v), _dptr(k_norm_weight), eps, _stream()))
+                                                 _dptr(v), _dptr(k_norm_weight), eps, _stream(self.pool.device)))
         return q_out
 
     def append(self, layer, k, v):
-        check(self.L.s1kv_batch_append(self.h, layer, _dptr(k), _dptr(v), _stream()))
+        check(self.L.s1kv_batch_append(self.h, layer, _dptr(k), _dptr(v), _stream(self.pool.device)))
 
     def gather(self, layer, which, out=None):
         """The rows this batch appended, as the pool holds them: fp32
@@ -434,24 +437,24 @@ class Batch:
         import torch
         if out is None:
             out = torch.empty((self.n_tokens, self.pool.Hkv, self.pool.D), dtype=torch.float32, device=self.pool.device)
-        check(self.L.s1kv_batch_gather(self.h, layer, which, _dptr(out), _stream()))
+        check(self.L.s1kv_batch_gather(self.h, layer, which, _dptr(out), _stream(self.pool.device)))
         return out
 
     def attention(self, layer, q, out=None):
         import torch
         if out is None:
             out = torch.empty_like(q)
-        check(self.L.s1kv_batch_attention(self.h, layer, _dptr(q), _dptr(out), q.shape[1], _stream()))
+        check(self.L.s1kv_batch_attention(self.h, layer, _dptr(q), _dptr(out), q.shape[1], _stream(self.pool.device)))
         return out
 
     def layer_host(self, layer, h_q, h_k, h_v, h_out, n_q_heads):
         """End-to-end step of one layer from host (pinned) tensors."""
         check(self.L.s1kv_batch_layer_host(self.h, layer, _dptr(h_q), _dptr(h_k), _dptr(h_v), _dptr(h_out),
-                                           n_q_heads, _stream()))
+                                           n_q_heads, _stream(self.pool.device)))
 
     def end(self):
         if getattr(self, "h", None):
-            check(self.L.s1kv_batch_end(self.h, _stream()))
+            check(self.L.s1kv_batch_end(self.h, _stream(self.pool.device)))
             self.h = None
 
     def __enter__(self):
@@ -635,13 +638,14 @@ class ChannelQuantizedTensor:
     multiple of 16) and scales fp32 [N], both on the GPU; k = K."""
 
     def __init__(self, data, scales, k=None):
+        import torch
         self.data, self.scales = data, scales
-        self.n, self.ld = int(data.shape[0]), int(data.shape[1])
+        self.n, self.ld = data.shape
         self.k = self.ld if k is None else int(k)
         if self.ld != (self.k + 15) // 16 * 16 or not data.is_contiguous() or not scales.is_contiguous():
             raise S1KVError(EINVAL, "ChannelQuantizedTensor: contiguous rows of K rounded up to a multiple of 16 bytes")
-        if str(data.dtype) != "torch.int8" or str(scales.dtype) != "torch.float32" or tuple(scales.shape) != (self.n,):
-            raise S1KVError(EINVAL, "ChannelQuantizedTensor: int8 [N, K16] data and float32 [N] scales")
+        if data.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != (self.n,) or scales.device != data.device:
+            raise S1KVError(EINVAL, "ChannelQuantizedTensor: int8 [N, K16] data and float32 [N] scales on one device")
 
 
 def quantize_channels(t, device=None):
@@ -680,23 +684,36 @@ def matmul_w8a8_group(x, ws, outs=None):
     ChannelQuantizedTensor weights of the same K in one launch (q/k/v,
     gate/up) -> list of [M, N] fp32.  Summed exactly in 32-bit integers."""
     import torch
-    xd = _cuda_f32(x, ws[0].data.device.index)
-    if xd.dim() != 2 or any(w.k != xd.shape[1] or w.data.device != xd.device for w in ws):
-        raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K] with K the weights' and all on one device")
-    m = xd.shape[0]
+    dev, n = ws[0].data.device, len(ws)
+    if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.device == dev and x.is_contiguous()):
+        x = _cuda_f32(x, dev.index)
+    if x.dim() != 2:
+        raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K]")
+    m, k = x.shape
+    for w in ws:
+        if w.k != k or w.data.device != dev:
+            raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K] with K the weights' and all on one device")
     if outs is None:
-        outs = [torch.empty((m, w.n), dtype=torch.float32, device=xd.device) for w in ws]
-    elif len(outs) != len(ws) or any(o.shape != (m, w.n) or o.dtype != torch.float32 or not o.is_contiguous() or
-                                     o.device != xd.device for o, w in zip(outs, ws)):
+        outs = [x.new_empty((m, w.n)) for w in ws]
+    elif len(outs) != n or any(o.shape != (m, w.n) or o.dtype != torch.float32 or not o.is_contiguous() or o.device != dev
+                               for o, w in zip(outs, ws)):
         raise S1KVError(EINVAL, "matmul_w8a8_group: outs must be contiguous float32 [M, N] on x's device")
-    n = len(ws)
-    wa = (vp * n)(*[w.data.data_ptr() for w in ws])
-    sa = (vp * n)(*[w.scales.data_ptr() for w in ws])
-    na = (i64 * n)(*[w.n for w in ws])
-    oa = (vp * n)(*[o.data_ptr() for o in outs])
-    with torch.cuda.device(xd.device):
-        q, scales = quantize_tokens(xd, xd.device.index)
-        check(lib().s1kv_matmul_w8a8_group(_dptr(q), _dptr(scales), m, ws[0].ld, n, wa, sa, na, oa, _stream()))
+    L = lib()
+    size = L.s1kv_w8a8_workspace(m, k)
+    space = x.new_empty((size,), dtype=torch.int8)
+    args = (i64 * (4 * n))(*[w.data.data_ptr() for w in ws], *[w.scales.data_ptr() for w in ws], *[w.n for w in ws],
+                           *[o.data_ptr() for o in outs])
+    at = C.addressof(args)
+
+    def call():
+        check(L.s1kv_linear_w8a8_group(x.data_ptr(), m, k, space.data_ptr(), size, n, at, at + 8 * n, at + 16 * n, at + 24 * n,
+                                       _stream(dev.index)))
+
+    if dev.index == torch.cuda.current_device():
+        call()
+    else:
+        with torch.cuda.device(dev):
+            call()
     return outs
 
 

@@ -127,3 +127,15 @@ def test_q4_prefix_file_is_read_on_the_host(s1kv, tmp_path):
     for payload, d in ((body[:-1], dim), (body, 12)):
         with pytest.raises(s1kv.S1KVError):
             s1kv.prefix_file_info(write(payload, d))
+
+
+def test_linear_w8a8_refusals(s1kv):
+    L = s1kv.lib()
+    vp, i64 = C.c_void_p, C.c_int64
+    args = lambda n: ((vp * 1)(64), (vp * 1)(64), (i64 * 1)(n), (vp * 1)(64))  # noqa: E731
+    assert L.s1kv_w8a8_workspace(3, 17) == 3 * 32 + 16 and L.s1kv_w8a8_workspace(-1, 4) == 0
+    assert L.s1kv_linear_w8a8_group(64, 3, 17, 64, 111, 1, *args(8), None) == s1kv.EINVAL  # workspace too small
+    assert L.s1kv_linear_w8a8_group(64, 3, 17, 72, 112, 1, *args(8), None) == s1kv.EINVAL  # and not aligned
+    assert L.s1kv_linear_w8a8_group(None, 3, 17, 64, 112, 1, *args(8), None) == s1kv.EINVAL
+    assert L.s1kv_linear_w8a8_group(64, 3, 131073, 64, 1 << 40, 1, *args(8), None) == s1kv.EINVAL
+    assert L.s1kv_linear_w8a8_group(64, 3, 17, 64, 112, 1, *args(0), None) == s1kv.OK  # nothing to compute
