@@ -202,6 +202,7 @@ int s1kv_batch_begin(s1kv_pool* p, const uint64_t* seqs, const int32_t* n_append
             pseqs[i] = PrefillSeq{trow[i], (int32_t)lens[i], ql, q_start};
             q_start += ql;
             b->max_qlen = std::max(b->max_qlen, ql);
+            if (ql > 0) b->max_kv = std::max(b->max_kv, (int32_t)lens[i]);
         }
     }
     b->n_seqs = n_seqs;
@@ -463,6 +464,8 @@ int s1kv_batch_attention(s1kv_batch* b, int32_t layer, const float* q, float* ou
     // contraction: tensor-core prefill.  Decode rows stay on the split-K
     // kernel.
     // (q and out are read and written by TMA there: 16-byte aligned.)
+    if (!b->decode_rows && p->desc.dtype == S1KV_DTYPE_Q4 && prefill_q4_supported(D, G, p->desc.block_size))
+        return launch_prefill_q4(b, layer, q, out, Hq, scale_log2(D), b->max_kv, stream);
     if (!b->decode_rows && p->tmap_sw_ok && prefill_tc_supported(p->desc.dtype, D, G, p->desc.block_size) &&
         (((uintptr_t)q | (uintptr_t)out) & 15) == 0) {
         PrefillParams pp{};

@@ -264,10 +264,12 @@ struct Stager {
     void destroy();
 };
 
-// Growable device buffer; growth synchronises the device first.
+// Growable device buffer.  Growth is geometric and keeps the smaller buffers
+// until destroy(): a captured graph may still use them.
 struct DevBuf {
     void* p = nullptr;
     size_t cap = 0;
+    std::vector<void*> old;
     int ensure(size_t bytes);
     void destroy();
 };
@@ -385,6 +387,7 @@ struct s1kv_batch {
     const s1kv::PrefillSeq* d_pseqs = nullptr;
     int32_t n_seqs = 0;
     int32_t max_qlen = 0;
+    int32_t max_kv = 0;       // the longest context with query rows
     std::vector<s1kv::RowMeta> rows;  // host copy (for dispatch decisions)
     std::vector<s1kv::WorkItem> items;  // split-K work list (host copy)
     bool items_planned = false;       // rows' split fields and items computed
@@ -450,6 +453,9 @@ int launch_gather_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const 
 int launch_rows_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const int32_t* slots, int64_t n, int which,
                    void* rows, bool to_pool, cudaStream_t stream);
 bool decode_q4_supported(int D, int G, int block_size);
+bool prefill_q4_supported(int D, int G, int block_size);
+int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, int32_t Hq, float scale_log2, int32_t max_kv,
+                      cudaStream_t stream);
 int launch_decode_q4(const AttnParams& p, cudaStream_t stream);
 
 // Tensor-core prefix-hit prefill (prefill_tc.cu).

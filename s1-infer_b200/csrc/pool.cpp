@@ -125,17 +125,19 @@ void Stager::destroy() {
 int DevBuf::ensure(size_t bytes) {
     if (cap >= bytes) return S1KV_OK;
     S1KV_CUDA(cudaDeviceSynchronize());
-    if (p) cudaFree(p);
-    p = nullptr;
-    size_t c = std::max<size_t>({bytes + bytes / 4, 2 * cap, size_t(16) << 20});
-    cap = 0;
-    S1KV_CUDA(cudaMalloc(&p, c));
+    const size_t c = std::max<size_t>({bytes + bytes / 4, 2 * cap, size_t(16) << 20});
+    void* np = nullptr;
+    S1KV_CUDA(cudaMalloc(&np, c));
+    if (p) old.push_back(p);
+    p = np;
     cap = c;
     return S1KV_OK;
 }
 
 void DevBuf::destroy() {
     if (p) cudaFree(p);
+    for (void* o : old) cudaFree(o);
+    old.clear();
     p = nullptr;
     cap = 0;
 }

@@ -86,6 +86,28 @@ __device__ __forceinline__ float2 q4_unpack(uint32_t packed) {  // (s, m)
     return make_float2(__uint_as_float(packed << 16), __uint_as_float(packed & 0xFFFF0000u));
 }
 
+__device__ __forceinline__ uint32_t q4_and_or(uint32_t w, uint32_t mask, uint32_t o) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(w), "r"(mask), "r"(o));  // (w & mask) | o
+    return y;
+}
+// The eight codes of a word centred, u - 8, as fp16x2: nibble n of the low half
+// and of the high half in out[n] (V: four dims of two tokens; K: dims n and
+// n + 4 of eight).  0x6400 | u is the fp16 1024 + u, 0x6400 | 16 u is 1024 + 16 u.
+__device__ __forceinline__ void q4_centred(uint32_t w, uint32_t (&out)[4]) {
+    const __half2 one = __float2half2_rn(1.0f), m1032 = __float2half2_rn(-1032.0f);
+    const __half2 sixteenth = __float2half2_rn(0.0625f), m72 = __float2half2_rn(-72.0f);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t x = w >> (8 * i);
+        const uint32_t a = q4_and_or(x, 0x000F000Fu, 0x64006400u), b = q4_and_or(x, 0x00F000F0u, 0x64006400u);
+        const __half2 ha = __hfma2(*reinterpret_cast<const __half2*>(&a), one, m1032);
+        const __half2 hb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, m72);
+        out[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
+        out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+    }
+}
+
 // Bytes of one (block, KV head) tile and offsets inside it.
 __host__ __device__ __forceinline__ int q4_tile_bytes(int bs, int D) { return bs * (D / 2 + 4); }
 __device__ __forceinline__ int q4_k_quad(int t, int quad, int D) { return t * (D / 2) + quad * 2; }

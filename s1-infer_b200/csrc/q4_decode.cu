@@ -78,26 +78,6 @@ __device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = pack_h2(a - f.x, b - f.y);
 }
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t o) {
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(w), "r"(mask), "r"(o));  // (w & mask) | o
-    return y;
-}
-// Four codes of two tokens each: u - 8 as fp16x2, nibble n in out[n].
-__device__ __forceinline__ void centred(uint32_t w, uint32_t (&out)[4]) {
-    const __half2 one = __float2half2_rn(1.0f), m1032 = __float2half2_rn(-1032.0f);
-    const __half2 sixteenth = __float2half2_rn(0.0625f), m72 = __float2half2_rn(-72.0f);
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t x = w >> (8 * i);
-        const uint32_t a = and_or(x, 0x000F000Fu, 0x64006400u), b = and_or(x, 0x00F000F0u, 0x64006400u);
-        const __half2 ha = __hfma2(*reinterpret_cast<const __half2*>(&a), one, m1032);
-        const __half2 hb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, m72);
-        out[2 * i] = *reinterpret_cast<const uint32_t*>(&ha);
-        out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
-    }
-}
-
 // One tile's bytes of one lane: NWD words of K for tokens g and g + 8, of V
 // for pairs t and t + 4, and the params of tokens g and g + 8.
 template <int NWD>
@@ -315,8 +295,8 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
 #pragma unroll
             for (int wi = 0; wi < NWD; wi++) {
                 uint32_t c0[4], c1[4];
-                centred(r.v0[wi], c0);
-                centred(r.v1[wi], c1);
+                q4_centred(r.v0[wi], c0);
+                q4_centred(r.v1[wi], c1);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bh0, bh1);

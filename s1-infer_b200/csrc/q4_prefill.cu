@@ -1,0 +1,752 @@
+// q4_prefill.cu -- chunked-prefill attention over a 4-bit cache (format:
+// q4.cuh) on tcgen05: query chunks of more than one token, row i of a
+// sequence's q_len new tokens seeing tokens 0 .. (kv_len - q_len) + i.
+//
+//   score_t = s_k (q . c_t) + m_k sum(q),  out = sum_t (p_t s_v) c_t + sum_t p_t m_v
+// with the centred codes c = u - 8 (-8 .. 7, exact in fp16), so the scales
+// act on whole score columns and the products run over fp16 integers.  q and
+// p s_v are each split into two fp16 parts (22 bits) and both parts are
+// multiplied: fp32-level results for twice the tensor-core work of a bf16
+// cache's prefill, 8 Hq D products a (query, visible token) in place of 4.
+// That is what bounds the kernel; K/V bytes are a seventh of bf16's.
+//
+// A CTA takes a chunk of queries of one sequence and KV head as two tiles A
+// and B of 128 accumulator rows, a row a (query, head) pair: 128 / G queries
+// times the G query heads of the KV head (any G up to 128).
+//   * Two warpgroups run the softmax, one per tile, a thread a row: scores
+//     from TMEM, scaled per token, the online softmax in the exp2 domain
+//     (reference max moved only past 2^8), p s_v split and stored over the
+//     scores: 64 columns of high parts, 64 of low parts.
+//   * One warpgroup widens K/V: a thread loads a token's codes straight from
+//     its block (the next tile's loads are in flight while it waits for the
+//     buffer), makes fp16 of them and writes the 128-byte-swizzled tiles the
+//     MMAs read.  K's dims stand in the order 0 4 1 5 2 6 3 7 of each eight,
+//     as they come out of a word; q is stored alike.
+//   * One warp issues the MMAs: PV_A(t) S_A(t+1) PV_B(t) S_B(t+1), so one
+//     tile's softmax runs under the other's products, and K and V need one
+//     buffer each: K(t+1) is written under PV_A(t), V(t+1) under S_B(t+1).
+// Few chunks over a long context: the tiles are split over CTAs as well, a
+// second kernel joins the partial rows.
+// Waits are bounded; a timeout raises an abort flag that every role polls
+// and the device error word.  TMEM is freed on every path.
+#include <cmath>
+
+#include "q4.cuh"
+
+namespace s1kv {
+namespace {
+
+constexpr uint32_t kSpin = 1u << 22;
+constexpr int kM = 128, kN = 128;  // rows per tile, tokens per K/V tile
+constexpr int kThreads = 512;      // softmax A, softmax B, widening, MMA (+ 3 idle warps)
+constexpr int kColO = 256;         // TMEM: S_A [0, 128) S_B [128, 256) O_A O_B
+constexpr int kTmemCols = 512;
+constexpr float kRescaleAt = 8.0f;
+constexpr int kMinExp = 8;
+constexpr int kIdsCached = 1024;   // block ids kept in shared memory (16K tokens)
+
+template <int D>
+struct Cfg {
+    static constexpr int kAtoms = D / 64;             // 128-byte swizzle atoms across a row
+    static constexpr int kQBytes = kAtoms * kM * 128;  // one part of one query tile
+    static constexpr int kKBytes = kAtoms * kN * 128;
+    static constexpr int kOffQ = 0;                    // A high, A low, B high, B low
+    static constexpr int kOffK = 4 * kQBytes;
+    static constexpr int kOffV = kOffK + kKBytes;
+    static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
+    static constexpr int kOffIds = kOffPar + 2 * (kN * 16 + 64);
+    static constexpr int kOffBar = kOffIds + kIdsCached * 4;
+    // k_full k_empty v_full v_empty par_full[2] s_full[2] p_half[2] p_full[2] pv_done[2] drain
+    static constexpr int kNumBars = 15;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM slot, abort flag
+    static constexpr int kSmem = kOffMisc + 16 + 1024;
+};
+
+__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t phase) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(su32(b)), "r"(phase)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t phase) {
+    for (uint32_t i = 0; i < kSpin; i++)
+        if (bar_try(b, phase)) return true;
+    return false;
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t phase, volatile int* abort_flag) {
+    bool ok = false;
+    for (uint32_t i = 0; i < kSpin && !ok; i++) {
+        ok = bar_try(b, phase);
+        if (!ok && *abort_flag) break;
+    }
+    if (!ok) *abort_flag = 1;
+    return __all_sync(0xffffffffu, ok);
+}
+// Shared-memory descriptor, 128-byte swizzle (layout type 2).
+__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16 |
+           (uint64_t)((sbo_bytes >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16 instruction descriptor: fp16 A and B (0), fp32 D (1).
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int b_mn_major) {
+    return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Issued by one elected lane of a converged warp: D (TMEM) (+)= A B with A in
+// shared memory (ss) or TMEM (ts), B in shared memory.
+__device__ __forceinline__ void mma_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_w(uint64_t* b) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b))
+        : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 consecutive fp32 columns of this thread's TMEM lane; the wait is apart.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, "
+        "[%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+    uint32_t w[16];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(v[16 * h + i]);
+        tmem_st16(taddr + 16 * h, w);
+    }
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack_h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
+
+// Byte offset of 16-byte chunk `chunk` of row `r` in a tile of `rows` rows
+// held as 128B-swizzled atoms of 64 elements.
+__device__ __forceinline__ uint32_t chunk_at(int r, int chunk, int rows) {
+    return (uint32_t)((chunk >> 3) * rows * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+}
+
+// One row's softmax state.  un: scores are in units of 1 / un (q was scaled
+// by a power of two); qs: sum of the scaled q.
+struct RowState {
+    float m, l, z, vmul, un, qs;
+    int E;
+};
+// The parameters of a tile, two adjacent tokens side by side.
+struct TilePar {
+    float4 k[kN / 2];  // s_k, s_k', m_k, m_k'
+    float4 v[kN / 2];  // s_v, s_v', m_v, m_v'
+    int e[4];          // largest exponents of the finite s_v (one a widening warp)
+    int pad[12];
+};
+
+// A tile's 128 scores of one row -> P over them: of each 32 columns the first
+// 16 take the high parts of p s_v, the others the low parts.  Two passes over
+// the columns, 32 at a time: scale per token, maximum, store back; then the
+// weights.  (Holding all 128 scores in registers takes the code out of the
+// instruction cache and the warps into spills: 24000 cycles a tile pair.)
+// EDGE: only tokens up to `last` (of this tile) are seen; the others may hold
+// anything, NaN included.
+template <bool EDGE, int D>
+__device__ __forceinline__ void softmax_tile(uint32_t tS, const TilePar& par, int last, RowState& st, bool first, uint32_t tO,
+                                             uint64_t* p_half, uint64_t* p_full, int lane) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    int e = EDGE ? 0 : max(max(par.e[0], par.e[1]), max(par.e[2], par.e[3]));
+    const float2 qs2 = make_float2(st.qs, st.qs);
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        float v[32];
+        tmem_ld32(tS + 32 * q, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float4 a = par.k[16 * q + i];
+            float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(a.x, a.y),
+                                  __fmul2_rn(make_float2(a.z, a.w), qs2));
+            if (EDGE) {
+                const float4 b = par.v[16 * q + i];
+                if (32 * q + 2 * i > last) x.x = -INFINITY;
+                else if (b.x < INFINITY) e = max(e, (int)(__float_as_uint(b.x) >> 23));
+                if (32 * q + 2 * i + 1 > last) x.y = -INFINITY;
+                else if (b.y < INFINITY) e = max(e, (int)(__float_as_uint(b.y) >> 23));
+            }
+            mx[i & 3] = fmaxf(fmaxf(mx[i & 3], x.x), x.y);
+            v[2 * i] = x.x;
+            v[2 * i + 1] = x.y;
+        }
+        tmem_st32(tS + 32 * q, v);
+    }
+    tmem_st_wait();
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * st.un;
+    const bool raise = top > st.m + kRescaleAt || e > st.E;
+    float corr = 1.0f;
+    if (raise) {
+        if (top > st.m + kRescaleAt) {
+            corr = ex2(st.m - top);  // 0 on the first tile (m = -inf)
+            st.m = top;
+            st.l *= corr;
+            st.z *= corr;
+        }
+        const int ne = max(st.E, e);
+        corr *= ne - st.E > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (ne - st.E)) << 23);
+        st.E = ne;
+        st.vmul = __uint_as_float((uint32_t)(260 - ne) << 23);
+    }
+    const bool rescale = !first && __any_sync(0xffffffffu, raise);
+    const float mref = st.m == -INFINITY ? 0.0f : st.m;  // nothing visible yet: p = 0
+    const float2 un2 = make_float2(st.un, st.un), nm2 = make_float2(-mref, -mref), vm2 = make_float2(st.vmul, st.vmul);
+    float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        float v[32];
+        tmem_ld32(tS + 32 * q, v);
+        tmem_ld_wait();
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float4 a = par.v[16 * q + i];
+            const float2 y = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), un2, nm2);
+            const float2 p = make_float2(ex2(y.x), ex2(y.y));
+            l2 = __fadd2_rn(l2, p);
+            float2 w = __fmul2_rn(__fmul2_rn(p, make_float2(a.x, a.y)), vm2), m = make_float2(a.z, a.w);
+            if (EDGE) {  // 0 times what an unseen token holds
+                if (32 * q + 2 * i > last) w.x = m.x = 0.0f;
+                if (32 * q + 2 * i + 1 > last) w.y = m.y = 0.0f;
+            }
+            z2 = __ffma2_rn(p, m, z2);
+            const __half2 h = __floats2half2_rn(w.x, w.y);
+            const float2 f = __half22float2(h);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+            const float2 r = __fadd2_rn(w, make_float2(-f.x, -f.y));
+            lo[i] = pack_h2(r.x, r.y);
+        }
+        tmem_st16(tS + 32 * q, hi);
+        tmem_st16(tS + 32 * q + 16, lo);
+        if (q == 1 && !rescale) {  // the first 64 tokens are handed over while the rest is computed
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(p_half);
+        }
+    }
+    if (rescale) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            float ov[32];
+            tmem_ld32(tO + c, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++) ov[i] *= corr;
+            tmem_st32(tO + c, ov);
+        }
+    }
+    tmem_st_wait();
+    st.l += l2.x + l2.y;
+    st.z += z2.x + z2.y;
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) {
+        if (rescale) bar_arrive(p_half);
+        bar_arrive(p_full);
+    }
+}
+
+}  // namespace
+
+struct PrefillQ4Params {
+    const float* q;          // [rows][Hq][D] fp32, post-RoPE
+    float* out;
+    const int32_t* table;
+    const PrefillSeq* seqs;
+    const char* kbase;       // this layer's tiles
+    const char* vbase;
+    float* part_o;           // n_split > 1: [split][rows][Hq][D], unnormalised
+    float* part_ml;          // [split][rows][Hq][2]  (max in log2 units, sum)
+    int64_t n_rows;
+    int32_t max_chunks, n_split;
+    int32_t max_bps, max_blocks;
+    int32_t Hq, Hkv, G, QT;  // QT = 128 / G queries a tile
+    float scale_log2;
+    int* err;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_constant__ PrefillQ4Params p) {
+    using C = Cfg<D>;
+    constexpr int kTileBytes = 16 * (D / 2 + 4);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+    uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *par_full = bars + 4;
+    uint64_t *s_full = bars + 6, *p_half = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *drain = bars + 14;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+    TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
+    static_assert(sizeof(TilePar) == kN * 16 + 64, "two tiles' parameters");
+    int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // the chunks with the most visible tokens first
+    const int seq_i = blockIdx.x / p.max_chunks, chunk = p.max_chunks - 1 - blockIdx.x % p.max_chunks;
+    const int h = blockIdx.y;
+    pdl_wait_trigger();
+    const PrefillSeq sm = p.seqs[seq_i];
+    const int G = p.G, QT = p.QT, q0 = chunk * 2 * QT;
+    if (q0 >= sm.q_len) return;  // uniform: no TMEM allocated yet
+    const int prefix = sm.kv_len - sm.q_len;
+    const int kv_end = min(sm.kv_len, prefix + q0 + 2 * QT);
+    const int all_tiles = (kv_end + kN - 1) / kN;
+    const int tb = (int)((int64_t)all_tiles * blockIdx.z / p.n_split), te = (int)((int64_t)all_tiles * (blockIdx.z + 1) / p.n_split);
+    const int n_tiles = te - tb;
+    const bool two_tiles = q0 + QT < sm.q_len;
+    const int32_t* tab = p.table + (int64_t)sm.table_row * p.max_bps;
+    const int n_blocks = (kv_end + 15) / 16, b0 = tb * (kN / 16);
+
+    // ---- set-up ----
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        // the widening and softmax warps arrive once a warp, the MMA commits once
+        for (int i = 0; i < C::kNumBars; i++)
+            bar_init(&bars[i], i == 0 || i == 2 || i == 4 || i == 5 || (i >= 8 && i < 12) ? 4u : 1u);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    auto lookup = [&](int b) -> int32_t {  // -1: no such block
+        if (b >= n_blocks) return -1;
+        const int32_t blk = tab[b];
+        if ((uint32_t)blk >= (uint32_t)p.max_blocks) {
+            atomicOr(p.err, kErrBounds);
+            return -1;
+        }
+        return blk;
+    };
+    for (int i = tid; i < min(n_tiles * (kN / 16), kIdsCached); i += kThreads) ids[i] = lookup(b0 + i);
+    // Row 128 X + r is query X QT + r / G, head r % G; thread tid < 256 keeps
+    // that of row tid.  A warp brings its own 32 rows, eight in flight, each
+    // scaled by the power of two that puts its largest |q| in [2^14, 2^15).
+    float q_un = 1.0f, q_sum = 0.0f;
+    if (warp < 8) {
+        const int r = tid & 127, qi = (tid >> 7) * QT + r / G;
+        const int mine = r < QT * G && q0 + qi < sm.q_len ? (sm.q_start + q0 + qi) * p.Hq + h * G + r % G : -1;
+        uint8_t* hi_at = smem + C::kOffQ + 2 * (tid >> 7) * C::kQBytes;
+        // lane L takes dims 8 (L / 4) + L % 4 and + 4 (a register pair of K's order), of 64 dims at a time
+        const int d0 = 8 * (lane >> 2) + (lane & 3);
+#pragma unroll 1
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            float x[8][2 * C::kAtoms];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int at = __shfl_sync(0xffffffffu, mine, j0 + j);
+#pragma unroll
+                for (int a = 0; a < 2 * C::kAtoms; a++)
+                    x[j][a] = at < 0 ? 0.0f : p.q[(int64_t)at * D + 64 * (a >> 1) + 4 * (a & 1) + d0] * p.scale_log2;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float mx = 0.0f, sum = 0.0f;
+#pragma unroll
+                for (int a = 0; a < 2 * C::kAtoms; a++) {
+                    mx = fmaxf(mx, fabsf(x[j][a]));
+                    sum += x[j][a];
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                }
+                const int qe = min(max((int)(__float_as_uint(mx) >> 23), 40), 240);
+                const float scale = __uint_as_float((uint32_t)(268 - qe) << 23);
+                if (lane == j0 + j) {
+                    q_un = __uint_as_float((uint32_t)(qe - 14) << 23);  // 1 / scale
+                    q_sum = sum * scale;
+                }
+#pragma unroll
+                for (int a = 0; a < C::kAtoms; a++) {
+                    uint32_t hi, lo;
+                    split_h2(x[j][2 * a] * scale, x[j][2 * a + 1] * scale, hi, lo);
+                    const uint32_t at = chunk_at((tid & 96) + j0 + j, 8 * a + (lane >> 2), kM) + 4 * (lane & 3);
+                    *reinterpret_cast<uint32_t*>(hi_at + at) = hi;
+                    *reinterpret_cast<uint32_t*>(hi_at + C::kQBytes + at) = lo;
+                }
+            }
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= 12) {
+        if (warp == 12) {
+            // ================= MMA issuer =================
+            constexpr uint32_t idS = idesc_f16(kM, kN, 0), idO = idesc_f16(kM, D, 1);
+            const uint64_t dk = sdesc(su32(smem + C::kOffK), 16, 1024), dv = sdesc(su32(smem + C::kOffV), kN * 128, 1024);
+            auto issue_s = [&](int X) {
+                const uint64_t dq = sdesc(su32(smem + C::kOffQ + 2 * X * C::kQBytes), 16, 1024);
+#pragma unroll
+                for (int part = 1; part >= 0; part--)  // the small parts first: the sums are cut, not rounded
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++) {
+                        const uint32_t step = (ks >> 2) * (kM * 128 / 16) + (ks & 3) * 2;
+                        mma_ss_w(tmem + X * 128, dq + part * (C::kQBytes / 16) + step, dk + step, idS, part == 0 || ks > 0);
+                    }
+                mma_commit_w(&s_full[X]);
+            };
+            auto issue_pv = [&](int X, int t, int half) {  // 64 tokens, both parts of P
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int ks = 4 * half + k;
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+                        mma_ts_w(tmem + kColO + X * 128, tmem + X * 128 + (ks >> 1) * 32 + part * 16 + (ks & 1) * 8,
+                                 dv + ks * (16 * 128 / 16), idO, t > 0 || ks > 0 || part > 0);
+                }
+                if (half) mma_commit_w(&pv_done[X]);
+            };
+            bool ok = n_tiles > 0 && warp_wait(k_full, 0, abort_flag);
+            if (ok) {
+                tc_fence_after();
+                issue_s(0);
+                if (two_tiles) issue_s(1);
+                mma_commit_w(k_empty);
+            }
+            for (int t = 0; t < n_tiles && ok; t++) {
+                const uint32_t ph = (uint32_t)(t & 1);
+                const bool more = t + 1 < n_tiles;
+                for (int X = 0; X < (two_tiles ? 2 : 1) && ok; X++) {
+                    ok = warp_wait(&p_half[X], ph, abort_flag) && (X || warp_wait(v_full, ph, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(X, t, 0);
+                    ok = warp_wait(&p_full[X], ph, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(X, t, 1);
+                    if (X == (two_tiles ? 1 : 0)) mma_commit_w(v_empty);  // after the last product that reads V(t)
+                    if (more) {  // S_X(t + 1) overwrites P_X(t), which PV_X(t) ahead of it reads
+                        ok = X || warp_wait(k_full, ph ^ 1u, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(X);
+                        if (X == (two_tiles ? 1 : 0)) mma_commit_w(k_empty);
+                    }
+                }
+            }
+            // everything issued has finished before TMEM is freed (bounded)
+            mma_commit_w(drain);
+            bar_wait(drain, 0);
+        }
+    } else if (warp >= 8) {
+        // ================= widening: K, V and the rows' scales =================
+        const int i = tid - 256;  // this thread's token of a tile (K), token pair and half (V)
+        const int vp = i & 63, vh = i >> 6;
+        constexpr int NK = D / 32;  // 16-byte loads of a token's K codes; as many of half a V pair's
+        uint4 kr[NK], vr[NK];
+        uint32_t pk = 0, pv = 0;
+        auto block = [&](int t, int b) -> int32_t {  // block b of local tile t
+            const int j = t * (kN / 16) + b;
+            return j < kIdsCached ? ids[j] : lookup(b0 + j);
+        };
+        auto load_k = [&](int t) {
+            const int32_t blk = block(t, i >> 4);
+            pk = pv = 0;
+#pragma unroll
+            for (int c = 0; c < NK; c++) kr[c] = make_uint4(0, 0, 0, 0);
+            if (blk < 0) return;
+            const int64_t off = ((int64_t)blk * p.Hkv + h) * kTileBytes;
+            const uint4* src = reinterpret_cast<const uint4*>(p.kbase + off + (i & 15) * (D / 2));
+#pragma unroll
+            for (int c = 0; c < NK; c++) kr[c] = src[c];
+            if ((tb + t) * kN + i < kv_end) {  // rows past the end hold anything
+                pk = *reinterpret_cast<const uint32_t*>(p.kbase + off + 16 * (D / 2) + (i & 15) * 4);
+                pv = *reinterpret_cast<const uint32_t*>(p.vbase + off + 16 * (D / 2) + (i & 15) * 4);
+            }
+        };
+        auto load_v = [&](int t) {
+            const int32_t blk = block(t, vp >> 3);
+#pragma unroll
+            for (int c = 0; c < NK; c++) vr[c] = make_uint4(0, 0, 0, 0);
+            if (blk < 0) return;
+            const uint4* src = reinterpret_cast<const uint4*>(p.vbase + ((int64_t)blk * p.Hkv + h) * kTileBytes + (vp & 7) * D +
+                                                              vh * (D / 2));
+#pragma unroll
+            for (int c = 0; c < NK; c++) vr[c] = src[c];
+        };
+        if (n_tiles > 0) {
+            load_k(0);
+            load_v(0);
+        }
+        for (int t = 0; t < n_tiles; t++) {
+            const uint32_t ph = (uint32_t)(t & 1);
+            if (t > 0 && !warp_wait(k_empty, ph ^ 1u, abort_flag)) break;
+            // parameters of slot t & 1: the softmax of tile t - 2 is done with
+            // them (S(t - 1), which k_empty tracks, was issued after it)
+            const float2 ka = q4_unpack(pk), va = q4_unpack(pv);
+            float* at_k = reinterpret_cast<float*>(&par[ph].k[i >> 1]) + (i & 1);
+            float* at_v = reinterpret_cast<float*>(&par[ph].v[i >> 1]) + (i & 1);
+            at_k[0] = ka.x, at_k[2] = ka.y;
+            at_v[0] = va.x, at_v[2] = va.y;
+            const int e = __reduce_max_sync(0xffffffffu, va.x < INFINITY ? __float_as_uint(va.x) >> 23 : 0u);
+            if (lane == 0) par[ph].e[warp & 3] = e;
+            uint8_t* kt = smem + C::kOffK;
+#pragma unroll
+            for (int c = 0; c < NK; c++) {
+                const uint32_t w[4] = {kr[c].x, kr[c].y, kr[c].z, kr[c].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t x[4];
+                    q4_centred(w[j], x);
+                    *reinterpret_cast<uint4*>(kt + chunk_at(i, 4 * c + j, kN)) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+            if (t + 1 < n_tiles) load_k(t + 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                bar_arrive(&par_full[ph]);
+                bar_arrive(k_full);
+            }
+            if (t > 0 && !warp_wait(v_empty, ph ^ 1u, abort_flag)) break;
+            uint8_t* vt = smem + C::kOffV;
+            const int ta = 2 * vp;  // the pair's tokens: rows ta and ta + 1
+#pragma unroll
+            for (int c = 0; c < NK; c++) {
+                const uint32_t w[4] = {vr[c].x, vr[c].y, vr[c].z, vr[c].w};
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {  // two quads: eight dims of both tokens
+                    uint32_t x[4], y[4];
+                    q4_centred(w[j], x);
+                    q4_centred(w[j + 1], y);
+                    const int chunk = vh * (D / 16) + 2 * c + j / 2;
+                    *reinterpret_cast<uint4*>(vt + chunk_at(ta, chunk, kN)) =
+                        make_uint4(prmt(x[0], x[1], 0x5410), prmt(x[2], x[3], 0x5410), prmt(y[0], y[1], 0x5410),
+                                   prmt(y[2], y[3], 0x5410));
+                    *reinterpret_cast<uint4*>(vt + chunk_at(ta + 1, chunk, kN)) =
+                        make_uint4(prmt(x[0], x[1], 0x7632), prmt(x[2], x[3], 0x7632), prmt(y[0], y[1], 0x7632),
+                                   prmt(y[2], y[3], 0x7632));
+                }
+            }
+            if (t + 1 < n_tiles) load_v(t + 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(v_full);
+        }
+    } else {
+        // ================= softmax warpgroups =================
+        const int X = tid >> 7, r = tid & 127, qi = X * QT + r / G;
+        const bool valid = r < QT * G && q0 + qi < sm.q_len;
+        const int row_limit = valid ? prefix + q0 + qi : kv_end - 1;  // last visible token
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t tS = tmem + lanes + X * 128, tO = tmem + lanes + kColO + X * 128;
+        RowState st{-INFINITY, 0.0f, 0.0f, __uint_as_float((uint32_t)(260 - kMinExp) << 23), q_un, q_sum, kMinExp};
+        const bool active = X == 0 || two_tiles;
+        bool ok = true;
+        for (int t = 0; active && t < n_tiles; t++) {
+            const uint32_t ph = (uint32_t)(t & 1);
+            // S_X(t) done also means PV_X(t - 1) done: O_X and P_X are free
+            if (!warp_wait(&par_full[ph], (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(&s_full[X], ph, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int base = (tb + t) * kN;
+            if (base + kN - 1 > prefix + q0)  // some row of the chunk does not see all of it
+                softmax_tile<true, D>(tS, par[ph], row_limit - base, st, t == 0, tO, &p_half[X], &p_full[X], lane);
+            else
+                softmax_tile<false, D>(tS, par[ph], 0, st, t == 0, tO, &p_half[X], &p_full[X], lane);
+        }
+        const int64_t at = ((int64_t)(sm.q_start + q0 + qi) * p.Hq + h * G + r % G);
+        if (active && n_tiles == 0 && valid) {  // an empty share of a split
+            const int64_t row = (int64_t)blockIdx.z * p.n_rows * p.Hq + at;
+            for (int d = 0; d < D; d++) p.part_o[row * D + d] = 0.0f;
+            p.part_ml[row * 2] = -INFINITY;
+            p.part_ml[row * 2 + 1] = 0.0f;
+        }
+        if (active && n_tiles > 0 && ok && warp_wait(&pv_done[X], (uint32_t)((n_tiles - 1) & 1), abort_flag)) {
+            tc_fence_after();
+            const float back = __uint_as_float((uint32_t)(st.E - 6) << 23);  // 1 / vmul
+            const bool split = p.n_split > 1;
+            const int64_t row = split ? (int64_t)blockIdx.z * p.n_rows * p.Hq + at : at;
+            float* dst = (split ? p.part_o : p.out) + row * D;
+            const float inv = split ? 1.0f : 1.0f / st.l;
+            if (split && valid) {
+                p.part_ml[row * 2] = st.m;
+                p.part_ml[row * 2 + 1] = st.l;
+            }
+            const bool vec = ((uintptr_t)dst & 15) == 0;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float ov[32];
+                tmem_ld32(tO + c, ov);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; j++) ov[j] = fmaf(ov[j], back, st.z) * inv;
+                if (!valid) continue;
+                if (vec) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(dst + c + j) = make_float4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) dst[c + j] = ov[j];
+                }
+            }
+        }
+    }
+
+    // ---- tear-down: every path frees TMEM ----
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && *abort_flag) atomicOr(p.err, kErrTimeout);
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+}
+
+// Joins the n_split partial rows of a split chunk: a warp a (row, head).
+__global__ void __launch_bounds__(256) join_q4_kernel(const PrefillQ4Params p, int D) {
+    pdl_wait_trigger();
+    const int64_t rows = p.n_rows * p.Hq, row = blockIdx.x * (int64_t)8 + threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float M = -INFINITY;
+    for (int s = 0; s < p.n_split; s++) M = fmaxf(M, p.part_ml[(s * rows + row) * 2]);
+    float L = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.n_split; s++) {
+        const float ms = p.part_ml[(s * rows + row) * 2], f = ms == -INFINITY ? 0.0f : ex2(ms - M);
+        L = fmaf(p.part_ml[(s * rows + row) * 2 + 1], f, L);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (lane + 32 * i < D) o[i] = fmaf(p.part_o[(s * rows + row) * D + lane + 32 * i], f, o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (lane + 32 * i < D) p.out[row * D + lane + 32 * i] = o[i] / L;
+}
+
+bool prefill_q4_supported(int D, int G, int block_size) {
+    return (D == 64 || D == 128) && block_size == 16 && G >= 1 && G <= kM;
+}
+
+template <int D>
+static int launch_prefill(const PrefillQ4Params& p, int n_seqs, cudaStream_t stream) {
+    static std::atomic<uint64_t> attr_set{0};  // per device
+    int st = once_per_device(attr_set, [] {
+        S1KV_CUDA(cudaFuncSetAttribute(prefill_q4_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+        return S1KV_OK;
+    });
+    if (st) return st;
+    const dim3 grid((unsigned)(n_seqs * p.max_chunks), (unsigned)p.Hkv, (unsigned)p.n_split);
+    S1KV_CUDA(launch_pdl(prefill_q4_kernel<D>, grid, dim3(kThreads), Cfg<D>::kSmem, stream, p));
+    g_launches++;
+    if (p.n_split > 1) {
+        const int64_t rows = p.n_rows * p.Hq;
+        S1KV_CUDA(launch_pdl(join_q4_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, p, D));
+        g_launches++;
+    }
+    return S1KV_OK;
+}
+
+// `max_kv`: the longest context of the batch.
+int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, int32_t Hq, float scale_log2, int32_t max_kv,
+                      cudaStream_t stream) {
+    s1kv_pool* pool = b->pool;
+    PrefillQ4Params p{};
+    p.q = q;
+    p.out = out;
+    p.table = pool->d_table;
+    p.seqs = b->d_pseqs;
+    p.kbase = pool->k + (size_t)layer * pool->layer_bytes;
+    p.vbase = pool->v + (size_t)layer * pool->layer_bytes;
+    p.n_rows = b->n_rows;
+    p.max_bps = pool->max_bps;
+    p.max_blocks = (int32_t)pool->desc.max_blocks;
+    p.Hq = Hq;
+    p.Hkv = pool->desc.num_kv_heads;
+    p.G = Hq / p.Hkv;
+    p.QT = kM / p.G;
+    p.max_chunks = (b->max_qlen + 2 * p.QT - 1) / (2 * p.QT);
+    p.scale_log2 = scale_log2;
+    p.err = pool->d_err;
+    if (b->n_seqs == 0 || p.max_chunks == 0) return S1KV_OK;
+    // Fewer chunks than SMs: split their tiles, at least 4 a CTA, so that all
+    // SMs have work (a chunk's K/V reading and products run on one SM else).
+    const int D = pool->desc.head_dim;
+    const int64_t ctas = std::max<int64_t>(1, (b->n_rows + 2 * p.QT - 1) / (2 * p.QT)) * p.Hkv;
+    const int64_t tiles = (max_kv + kN - 1) / kN;
+    p.n_split = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(148 / ctas, tiles / 4), 64));
+    if (p.n_split > 1) {
+        const size_t rows = (size_t)p.n_split * p.n_rows * Hq;
+        const int st = pool->scratch.ensure(rows * (D + 2) * sizeof(float));
+        if (st) return st;
+        p.part_o = (float*)pool->scratch.p;
+        p.part_ml = p.part_o + rows * D;
+    }
+    return D == 128 ? launch_prefill<128>(p, b->n_seqs, stream) : launch_prefill<64>(p, b->n_seqs, stream);
+}
+
+}  // namespace s1kv
