@@ -341,6 +341,7 @@ struct s1kv_pool {
     s1kv::DevBuf scratch;             // split-K partials
     s1kv::DevBuf counters;            // split-K arrival counters (kept at zero)
     s1kv::DevBuf late_meta;           // rows + work list planned after batch_begin
+    s1kv::DevBuf aside;               // 4-bit prefill: sums set aside by running CTAs, and their slots' locks
     s1kv::DevBuf io;                  // host-pointer step buffers: two slots
     // s1kv_batch_layer_host: inputs go up on copy_stream and outputs come back
     // on d2h_stream, overlapped with the kernels of neighbouring calls.

@@ -511,6 +511,7 @@ int s1kv_pool_destroy(s1kv_pool* p) {
         p->scratch.destroy();
         p->counters.destroy();
         p->late_meta.destroy();
+        p->aside.destroy();
         p->io.destroy();
         if (p->k) cudaFree(p->k);
         if (p->v) cudaFree(p->v);
@@ -541,7 +542,7 @@ int s1kv_pool_stats_get(const s1kv_pool* p, s1kv_pool_stats* out) {
     out->device_bytes = p->host_only ? 0
                                      : (int64_t)(2 * p->layer_bytes * p->desc.num_layers +
                                                  (size_t)p->desc.max_seqs * p->max_bps * 4 + p->scratch.cap +
-                                                 p->io.cap);
+                                                 p->aside.cap + p->io.cap);
     return S1KV_OK;
 }
 

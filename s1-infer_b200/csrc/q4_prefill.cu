@@ -2,13 +2,14 @@
 // q4.cuh) on tcgen05: query chunks of more than one token, row i of a
 // sequence's q_len new tokens seeing tokens 0 .. (kv_len - q_len) + i.
 //
-//   score_t = s_k (q . c_t) + m_k sum(q),  out = sum_t (p_t s_v) c_t + sum_t p_t m_v
-// with the centred codes c = u - 8 (-8 .. 7, exact in fp16), so the scales
-// act on whole score columns and the products run over fp16 integers.  q and
-// p s_v are each split into two fp16 parts (22 bits) and both parts are
+//   score_t = q . (s_k c_t) + m_k sum(q),  out = sum_t p_t (s_v c_t) + sum_t p_t m_v
+// with the centred codes c = u - 8.  s c is exact in fp16: seven significant
+// codes are 3 bits, the eighth a power of two, s is 8 bits, fp16 has 11.  q
+// and p are each split into two fp16 parts (22 bits) and both parts are
 // multiplied: fp32-level results for twice the tensor-core work of a bf16
 // cache's prefill, 8 Hq D products a (query, visible token) in place of 4.
-// That is what bounds the kernel; K/V bytes are a seventh of bf16's.
+// That and the softmax's instructions bound the kernel; K/V bytes are a
+// seventh of bf16's.
 //
 // A CTA takes a chunk of queries of one sequence and KV head as two tiles A
 // and B of 128 accumulator rows, a row a (query, head) pair: 128 / G queries
@@ -38,11 +39,15 @@ namespace {
 
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kM = 128, kN = 128;  // rows per tile, tokens per K/V tile
-constexpr int kThreads = 512;      // softmax A, softmax B, widening, MMA (+ 3 idle warps)
+constexpr int kSoftmaxWarps = 8, kWidenWarps = 4, kMmaWarp = 12;
+constexpr int kThreads = 32 * 13;
+constexpr int kFlush = 4;          // tiles a chain of sums in TMEM
 constexpr int kColO = 256;         // TMEM: S_A [0, 128) S_B [128, 256) O_A O_B
 constexpr int kTmemCols = 512;
 constexpr float kRescaleAt = 8.0f;
-constexpr int kMinExp = 8;
+constexpr int kMinExp = 20;         // least exponent (biased) scales are taken relative to
+constexpr int kUp = 11;             // the largest scale stands as 2^11 .. 2^12 in the fp16 tiles: 8 s below 2^15
+constexpr float kPUp = 6.0f;        // p is kept 2^6 times as large (at most 2^14), also in its sums
 constexpr int kIdsCached = 1024;   // block ids kept in shared memory (16K tokens)
 
 template <int D>
@@ -54,11 +59,11 @@ struct Cfg {
     static constexpr int kOffK = 4 * kQBytes;
     static constexpr int kOffV = kOffK + kKBytes;
     static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
-    static constexpr int kOffIds = kOffPar + 2 * (kN * 16 + 64);
+    static constexpr int kOffIds = kOffPar + 2 * (kN * 12 + 32);
     static constexpr int kOffBar = kOffIds + kIdsCached * 4;
-    // k_full k_empty v_full v_empty par_full[2] s_full[2] p_half[2] p_full[2] pv_done[2] drain
-    static constexpr int kNumBars = 15;
-    static constexpr int kOffMisc = kOffBar + kNumBars * 8;  // TMEM slot, abort flag
+    // k_full k_empty v_full v_empty par_full[2] s_full[2] p_half[2] p_full[2] pv_done[2] drain q_full
+    static constexpr int kNumBars = 16;
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8 + 8;  // TMEM slot, abort flag, set-aside slot
     static constexpr int kSmem = kOffMisc + 16 + 1024;
 };
 
@@ -92,10 +97,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t phase, volatile 
     if (!ok) *abort_flag = 1;
     return __all_sync(0xffffffffu, ok);
 }
-// Shared-memory descriptor, 128-byte swizzle (layout type 2).
-__device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16 |
-           (uint64_t)((sbo_bytes >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory descriptor, 128-byte swizzle (layout type 2), 8-row groups
+// 1024 bytes apart: the low word holds the address and the leading offset,
+// the high word is the same for all (64-bit descriptors kept for every K step
+// spill; a low word is one addition).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo_bytes) {
+    return ((addr >> 4) & 0x3FFF) | (lbo_bytes >> 4) << 16;
 }
 // kind::f16 instruction descriptor: fp16 A and B (0), fp32 D (1).
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int b_mn_major) {
@@ -103,18 +111,20 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int b_mn_major) {
 }
 // Issued by one elected lane of a converged warp: D (TMEM) (+)= A B with A in
 // shared memory (ss) or TMEM (ts), B in shared memory.
-__device__ __forceinline__ void mma_ss_w(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss_w(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts_w(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts_w(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHi)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit_w(uint64_t* b) {
@@ -128,27 +138,37 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 
 // 32 consecutive fp32 columns of this thread's TMEM lane; the wait is apart.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-    uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, "
         "[%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this thread's TMEM loads.  The registers pass through, so that
+// nothing that uses them can be moved ahead of the wait.
+__device__ __forceinline__ void tmem_ld_wait16(float* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-        : "memory");
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]));
+}
+__device__ __forceinline__ void tmem_ld_wait32(float* v) {
+    tmem_ld_wait16(v);
+    tmem_ld_wait16(v + 16);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
     uint32_t w[16];
@@ -178,6 +198,12 @@ __device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_
 }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+
 // Byte offset of 16-byte chunk `chunk` of row `r` in a tile of `rows` rows
 // held as 128B-swizzled atoms of 64 elements.
 __device__ __forceinline__ uint32_t chunk_at(int r, int chunk, int rows) {
@@ -185,102 +211,125 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int chunk, int rows) {
 }
 
 // One row's softmax state.  un: scores are in units of 1 / un (q was scaled
-// by a power of two); qs: sum of the scaled q.
+// by a power of two); qs: sum of the scaled q.  mb, Eb: what the row's
+// set-aside sums refer to.
 struct RowState {
-    float m, l, z, vmul, un, qs;
-    int E;
+    float m, l, z, un, qs, mb;
+    int E, Eb;
 };
-// The parameters of a tile, two adjacent tokens side by side.
+// The parameters of a tile's rows.
 struct TilePar {
-    float4 k[kN / 2];  // s_k, s_k', m_k, m_k'
-    float4 v[kN / 2];  // s_v, s_v', m_v, m_v'
-    int e[4];          // largest exponents of the finite s_v (one a widening warp)
-    int pad[12];
+    float mk[kN], mv[kN];
+    float sv[kN];   // (the widening warps' own)
+    float f[4];     // K's tokens 32 g .. + 31 stand in the tile as s_k c / f[g], a power of two
+    int e[4];       // largest exponent of the s_v of tokens 32 g .. + 31
 };
 
+// 2^(m' - m) 2^(E' - E): from sums that refer to (m', E') to (m, E).
+__device__ __forceinline__ float rebase(float m_old, int e_old, float m, int e) {
+    const float c = m_old == m ? 1.0f : ex2(m_old - m);  // 0 from m' = -inf
+    return e - e_old > 126 ? 0.0f : c * __uint_as_float((uint32_t)(127 - (e - e_old)) << 23);
+}
+
 // A tile's 128 scores of one row -> P over them: of each 32 columns the first
-// 16 take the high parts of p s_v, the others the low parts.  Two passes over
-// the columns, 32 at a time: scale per token, maximum, store back; then the
-// weights.  (Holding all 128 scores in registers takes the code out of the
-// instruction cache and the warps into spills: 24000 cycles a tile pair.)
-// EDGE: only tokens up to `last` (of this tile) are seen; the others may hold
-// anything, NaN included.
+// 16 take the high parts of p, the others the low parts.  Two passes over the
+// columns, 32 at a time with the next 32 on their way: the maximum, then the
+// weights (adding m_k sum(q) anew costs less than storing the scores back, a
+// round trip to TMEM).  The loops stay rolled: unrolled over 128 scores the
+// code runs from beyond the instruction cache.  EDGE: only tokens up to `last`
+// (of this tile) are seen; the others may hold anything, NaN included.  fresh:
+// O starts anew with this tile.
 template <bool EDGE, int D>
-__device__ __forceinline__ void softmax_tile(uint32_t tS, const TilePar& par, int last, RowState& st, bool first, uint32_t tO,
+__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int last, RowState& st, bool fresh,
                                              uint64_t* p_half, uint64_t* p_full, int lane) {
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    int e = EDGE ? 0 : max(max(par.e[0], par.e[1]), max(par.e[2], par.e[3]));
-    const float2 qs2 = make_float2(st.qs, st.qs);
+    float v[2][32];
+    float top = -INFINITY;
+    tmem_ld32(tS, v[0]);
 #pragma unroll 1
-    for (int q = 0; q < 4; q++) {
-        float v[32];
-        tmem_ld32(tS + 32 * q, v);
-        tmem_ld_wait();
+    for (int c = 0; c < kN; c += 64) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float4 a = par.k[16 * q + i];
-            float2 x = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(a.x, a.y),
-                                  __fmul2_rn(make_float2(a.z, a.w), qs2));
-            if (EDGE) {
-                const float4 b = par.v[16 * q + i];
-                if (32 * q + 2 * i > last) x.x = -INFINITY;
-                else if (b.x < INFINITY) e = max(e, (int)(__float_as_uint(b.x) >> 23));
-                if (32 * q + 2 * i + 1 > last) x.y = -INFINITY;
-                else if (b.y < INFINITY) e = max(e, (int)(__float_as_uint(b.y) >> 23));
+        for (int u = 0; u < 2; u++) {
+            const int c0 = c + 32 * u;
+            const float f = par.f[c0 / 32], qs = __fdividef(st.qs, f);
+            const float2 qs2 = make_float2(qs, qs);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld_wait32(v[u]);
+            tmem_ld32(tS + ((c0 + 32) & (kN - 1)), v[u ^ 1]);  // after the last, the first again for the second pass
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
+                float2 x = __ffma2_rn(make_float2(k.x, k.y), qs2, make_float2(v[u][i], v[u][i + 1]));
+                float2 y = __ffma2_rn(make_float2(k.z, k.w), qs2, make_float2(v[u][i + 2], v[u][i + 3]));
+                if (EDGE) {
+                    if (c0 + i > last) x.x = -INFINITY;
+                    if (c0 + i + 1 > last) x.y = -INFINITY;
+                    if (c0 + i + 2 > last) y.x = -INFINITY;
+                    if (c0 + i + 3 > last) y.y = -INFINITY;
+                }
+                mx[(i >> 1) & 2] = fmaxf(fmaxf(mx[(i >> 1) & 2], x.x), x.y);
+                mx[((i >> 1) & 2) + 1] = fmaxf(fmaxf(mx[((i >> 1) & 2) + 1], y.x), y.y);
             }
-            mx[i & 3] = fmaxf(fmaxf(mx[i & 3], x.x), x.y);
-            v[2 * i] = x.x;
-            v[2 * i + 1] = x.y;
+            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (st.un * f));
         }
-        tmem_st32(tS + 32 * q, v);
     }
-    tmem_st_wait();
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * st.un;
+    const int e = max(st.E, max(max(par.e[0], par.e[1]), max(par.e[2], par.e[3])));
     const bool raise = top > st.m + kRescaleAt || e > st.E;
     float corr = 1.0f;
     if (raise) {
-        if (top > st.m + kRescaleAt) {
-            corr = ex2(st.m - top);  // 0 on the first tile (m = -inf)
-            st.m = top;
-            st.l *= corr;
-            st.z *= corr;
-        }
-        const int ne = max(st.E, e);
-        corr *= ne - st.E > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (ne - st.E)) << 23);
-        st.E = ne;
-        st.vmul = __uint_as_float((uint32_t)(260 - ne) << 23);
+        const float m = top > st.m + kRescaleAt ? top : st.m;
+        const float c = m == st.m ? 1.0f : ex2(st.m - m);  // 0 on the first tile (m = -inf)
+        corr = rebase(st.m, st.E, m, e);
+        st.l *= c;
+        st.z *= c;
+        st.m = m;
+        st.E = e;
     }
-    const bool rescale = !first && __any_sync(0xffffffffu, raise);
-    const float mref = st.m == -INFINITY ? 0.0f : st.m;  // nothing visible yet: p = 0
-    const float2 un2 = make_float2(st.un, st.un), nm2 = make_float2(-mref, -mref), vm2 = make_float2(st.vmul, st.vmul);
+    const bool rescale = !fresh && __any_sync(0xffffffffu, raise);
+    const float nm = kPUp - (st.m == -INFINITY ? 0.0f : st.m);  // nothing visible yet: p = 0
+    const float2 nm2 = make_float2(nm, nm);
     float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
 #pragma unroll 1
-    for (int q = 0; q < 4; q++) {
-        float v[32];
-        tmem_ld32(tS + 32 * q, v);
-        tmem_ld_wait();
-        uint32_t hi[16], lo[16];
+    for (int c = 0; c < kN; c += 64) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float4 a = par.v[16 * q + i];
-            const float2 y = __ffma2_rn(make_float2(v[2 * i], v[2 * i + 1]), un2, nm2);
-            const float2 p = make_float2(ex2(y.x), ex2(y.y));
-            l2 = __fadd2_rn(l2, p);
-            float2 w = __fmul2_rn(__fmul2_rn(p, make_float2(a.x, a.y)), vm2), m = make_float2(a.z, a.w);
-            if (EDGE) {  // 0 times what an unseen token holds
-                if (32 * q + 2 * i > last) w.x = m.x = 0.0f;
-                if (32 * q + 2 * i + 1 > last) w.y = m.y = 0.0f;
+        for (int u = 0; u < 2; u++) {
+            const int c0 = c + 32 * u;
+            const float f = par.f[c0 / 32], qs = __fdividef(st.qs, f), un = st.un * f;
+            const float2 qs2 = make_float2(qs, qs), un2 = make_float2(un, un);
+            uint32_t hi[8], lo[8];
+            tmem_ld_wait32(v[u]);
+            if (c0 + 32 < kN) tmem_ld32(tS + c0 + 32, v[u ^ 1]);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
+                const float4 mv = *reinterpret_cast<const float4*>(&par.mv[c0 + i]);
+#pragma unroll
+                for (int w = 0; w < 4; w += 2) {
+                    const int j = c0 + i + w;
+                    float2 x = __ffma2_rn(w ? make_float2(k.z, k.w) : make_float2(k.x, k.y), qs2,
+                                          make_float2(v[u][i + w], v[u][i + w + 1]));
+                    float2 m = w ? make_float2(mv.z, mv.w) : make_float2(mv.x, mv.y);
+                    x = __ffma2_rn(x, un2, nm2);
+                    if (EDGE) {
+                        if (j > last) x.x = -INFINITY, m.x = 0.0f;
+                        if (j + 1 > last) x.y = -INFINITY, m.y = 0.0f;
+                    }
+                    const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                    l2 = __fadd2_rn(l2, p);
+                    z2 = __ffma2_rn(p, m, z2);
+                    // high part: the leading 11 bits by a mask, low part: the rest
+                    const float2 t = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
+                                                 __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
+                    const float2 r = __fadd2_rn(p, make_float2(-t.x, -t.y));
+                    hi[(i + w) / 2 & 7] = pack_h2(t.x, t.y);
+                    lo[(i + w) / 2 & 7] = pack_h2(r.x, r.y);
+                }
+                if (i == 12 || i == 28) {
+                    tmem_st8(tS + c0 + (i & 16) / 2, hi);
+                    tmem_st8(tS + c0 + 16 + (i & 16) / 2, lo);
+                }
             }
-            z2 = __ffma2_rn(p, m, z2);
-            const __half2 h = __floats2half2_rn(w.x, w.y);
-            const float2 f = __half22float2(h);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-            const float2 r = __fadd2_rn(w, make_float2(-f.x, -f.y));
-            lo[i] = pack_h2(r.x, r.y);
         }
-        tmem_st16(tS + 32 * q, hi);
-        tmem_st16(tS + 32 * q + 16, lo);
-        if (q == 1 && !rescale) {  // the first 64 tokens are handed over while the rest is computed
+        if (c == 0 && !rescale) {  // the first 64 tokens are handed over while the rest is computed
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -292,7 +341,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, const TilePar& par, in
         for (int c = 0; c < D; c += 32) {
             float ov[32];
             tmem_ld32(tO + c, ov);
-            tmem_ld_wait();
+            tmem_ld_wait32(ov);
 #pragma unroll
             for (int i = 0; i < 32; i++) ov[i] *= corr;
             tmem_st32(tO + c, ov);
@@ -324,6 +373,9 @@ struct PrefillQ4Params {
     int32_t max_chunks, n_split;
     int32_t max_bps, max_blocks;
     int32_t Hq, Hkv, G, QT;  // QT = 128 / G queries a tile
+    float* aside;            // [n_aside][D][256] sums set aside by running CTAs
+    int32_t* aside_lock;     // [n_aside] 1 while a CTA holds the slot
+    int32_t n_aside;
     float scale_log2;
     int* err;
 };
@@ -336,11 +388,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
     uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *par_full = bars + 4;
-    uint64_t *s_full = bars + 6, *p_half = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *drain = bars + 14;
+    uint64_t *s_full = bars + 6, *p_half = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *drain = bars + 14, *q_full = bars + 15;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+    volatile int* aside_slot = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 8);
     TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
-    static_assert(sizeof(TilePar) == kN * 16 + 64, "two tiles' parameters");
+    static_assert(sizeof(TilePar) == kN * 12 + 32, "two tiles' parameters");
     int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -361,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     const int n_blocks = (kv_end + 15) / 16, b0 = tb * (kN / 16);
 
     // ---- set-up ----
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(kTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -369,8 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     if (tid == 0) {
         // the widening and softmax warps arrive once a warp, the MMA commits once
         for (int i = 0; i < C::kNumBars; i++)
-            bar_init(&bars[i], i == 0 || i == 2 || i == 4 || i == 5 || (i >= 8 && i < 12) ? 4u : 1u);
+            bar_init(&bars[i], i == 0 || i == 2 || i == 4 || i == 5 ? (uint32_t)kWidenWarps : i >= 8 && i < 12 ? 4u : i == 15 ? (uint32_t)kSoftmaxWarps : 1u);
         *abort_flag = 0;
+        // A slot for the sums that chains of tiles set aside.  One CTA fits an
+        // SM and there are as many slots as SMs, so one is free
+        // (without one the sums merely run on).
+        int got = -1;
+        if (n_tiles > kFlush) {
+            uint32_t sm_id;
+            asm volatile("mov.u32 %0, %%smid;" : "=r"(sm_id));
+            for (int i = 0; i < p.n_aside && got < 0; i++) {
+                const int at = (int)((sm_id + i) % p.n_aside);
+                if (atomicCAS(&p.aside_lock[at], 0, 1) == 0) got = at;
+            }
+        }
+        *aside_slot = got;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     auto lookup = [&](int b) -> int32_t {  // -1: no such block
@@ -383,69 +449,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         return blk;
     };
     for (int i = tid; i < min(n_tiles * (kN / 16), kIdsCached); i += kThreads) ids[i] = lookup(b0 + i);
-    // Row 128 X + r is query X QT + r / G, head r % G; thread tid < 256 keeps
-    // that of row tid.  A warp brings its own 32 rows, eight in flight, each
-    // scaled by the power of two that puts its largest |q| in [2^14, 2^15).
-    float q_un = 1.0f, q_sum = 0.0f;
-    if (warp < 8) {
-        const int r = tid & 127, qi = (tid >> 7) * QT + r / G;
-        const int mine = r < QT * G && q0 + qi < sm.q_len ? (sm.q_start + q0 + qi) * p.Hq + h * G + r % G : -1;
-        uint8_t* hi_at = smem + C::kOffQ + 2 * (tid >> 7) * C::kQBytes;
-        // lane L takes dims 8 (L / 4) + L % 4 and + 4 (a register pair of K's order), of 64 dims at a time
-        const int d0 = 8 * (lane >> 2) + (lane & 3);
-#pragma unroll 1
-        for (int j0 = 0; j0 < 32; j0 += 8) {
-            float x[8][2 * C::kAtoms];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int at = __shfl_sync(0xffffffffu, mine, j0 + j);
-#pragma unroll
-                for (int a = 0; a < 2 * C::kAtoms; a++)
-                    x[j][a] = at < 0 ? 0.0f : p.q[(int64_t)at * D + 64 * (a >> 1) + 4 * (a & 1) + d0] * p.scale_log2;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float mx = 0.0f, sum = 0.0f;
-#pragma unroll
-                for (int a = 0; a < 2 * C::kAtoms; a++) {
-                    mx = fmaxf(mx, fabsf(x[j][a]));
-                    sum += x[j][a];
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                }
-                const int qe = min(max((int)(__float_as_uint(mx) >> 23), 40), 240);
-                const float scale = __uint_as_float((uint32_t)(268 - qe) << 23);
-                if (lane == j0 + j) {
-                    q_un = __uint_as_float((uint32_t)(qe - 14) << 23);  // 1 / scale
-                    q_sum = sum * scale;
-                }
-#pragma unroll
-                for (int a = 0; a < C::kAtoms; a++) {
-                    uint32_t hi, lo;
-                    split_h2(x[j][2 * a] * scale, x[j][2 * a + 1] * scale, hi, lo);
-                    const uint32_t at = chunk_at((tid & 96) + j0 + j, 8 * a + (lane >> 2), kM) + 4 * (lane & 3);
-                    *reinterpret_cast<uint32_t*>(hi_at + at) = hi;
-                    *reinterpret_cast<uint32_t*>(hi_at + C::kQBytes + at) = lo;
-                }
-            }
-        }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const int slot = *aside_slot;
+    const int chain = slot < 0 ? INT32_MAX : kFlush;  // tiles until O starts anew
 
-    if (warp >= 12) {
-        if (warp == 12) {
+    if (warp == kMmaWarp) {
+        {
             // ================= MMA issuer =================
             constexpr uint32_t idS = idesc_f16(kM, kN, 0), idO = idesc_f16(kM, D, 1);
-            const uint64_t dk = sdesc(su32(smem + C::kOffK), 16, 1024), dv = sdesc(su32(smem + C::kOffV), kN * 128, 1024);
+            const uint32_t dk = desc_lo(su32(smem + C::kOffK), 16), dv = desc_lo(su32(smem + C::kOffV), kN * 128);
             auto issue_s = [&](int X) {
-                const uint64_t dq = sdesc(su32(smem + C::kOffQ + 2 * X * C::kQBytes), 16, 1024);
+                const uint32_t dq = desc_lo(su32(smem + C::kOffQ + 2 * X * C::kQBytes), 16);
 #pragma unroll
                 for (int part = 1; part >= 0; part--)  // the small parts first: the sums are cut, not rounded
 #pragma unroll
@@ -455,18 +472,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                     }
                 mma_commit_w(&s_full[X]);
             };
-            auto issue_pv = [&](int X, int t, int half) {  // 64 tokens, both parts of P
+            auto issue_pv = [&](int X, bool fresh, int half) {  // 64 tokens, both parts of P
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int ks = 4 * half + k;
 #pragma unroll
-                    for (int part = 0; part < 2; part++)
+                    for (int part = 1; part >= 0; part--)
                         mma_ts_w(tmem + kColO + X * 128, tmem + X * 128 + (ks >> 1) * 32 + part * 16 + (ks & 1) * 8,
-                                 dv + ks * (16 * 128 / 16), idO, t > 0 || ks > 0 || part > 0);
+                                 dv + ks * (16 * 128 / 16), idO, !fresh || ks > 0 || part == 0);
                 }
                 if (half) mma_commit_w(&pv_done[X]);
             };
-            bool ok = n_tiles > 0 && warp_wait(k_full, 0, abort_flag);
+            bool ok = n_tiles > 0 && warp_wait(q_full, 0, abort_flag) && warp_wait(k_full, 0, abort_flag);
             if (ok) {
                 tc_fence_after();
                 issue_s(0);
@@ -480,11 +497,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                     ok = warp_wait(&p_half[X], ph, abort_flag) && (X || warp_wait(v_full, ph, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(X, t, 0);
+                    issue_pv(X, t % chain == 0, 0);
                     ok = warp_wait(&p_full[X], ph, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(X, t, 1);
+                    issue_pv(X, t % chain == 0, 1);
                     if (X == (two_tiles ? 1 : 0)) mma_commit_w(v_empty);  // after the last product that reads V(t)
                     if (more) {  // S_X(t + 1) overwrites P_X(t), which PV_X(t) ahead of it reads
                         ok = X || warp_wait(k_full, ph ^ 1u, abort_flag);
@@ -499,13 +516,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             mma_commit_w(drain);
             bar_wait(drain, 0);
         }
-    } else if (warp >= 8) {
+    } else if (warp >= kSoftmaxWarps) {
         // ================= widening: K, V and the rows' scales =================
-        const int i = tid - 256;  // this thread's token of a tile (K), token pair and half (V)
+        const int i = tid - 32 * kSoftmaxWarps;  // this thread's token of a tile (K), token pair and half (V)
         const int vp = i & 63, vh = i >> 6;
         constexpr int NK = D / 32;  // 16-byte loads of a token's K codes; as many of half a V pair's
         uint4 kr[NK], vr[NK];
         uint32_t pk = 0, pv = 0;
+        int E = kMinExp;  // largest exponent of s_v so far: V stands as s_v c 2^(138 - E), as the softmax warps know
         auto block = [&](int t, int b) -> int32_t {  // block b of local tile t
             const int j = t * (kN / 16) + b;
             return j < kIdsCached ? ids[j] : lookup(b0 + j);
@@ -544,13 +562,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             if (t > 0 && !warp_wait(k_empty, ph ^ 1u, abort_flag)) break;
             // parameters of slot t & 1: the softmax of tile t - 2 is done with
             // them (S(t - 1), which k_empty tracks, was issued after it)
+            TilePar& par_t = par[ph];
             const float2 ka = q4_unpack(pk), va = q4_unpack(pv);
-            float* at_k = reinterpret_cast<float*>(&par[ph].k[i >> 1]) + (i & 1);
-            float* at_v = reinterpret_cast<float*>(&par[ph].v[i >> 1]) + (i & 1);
-            at_k[0] = ka.x, at_k[2] = ka.y;
-            at_v[0] = va.x, at_v[2] = va.y;
-            const int e = __reduce_max_sync(0xffffffffu, va.x < INFINITY ? __float_as_uint(va.x) >> 23 : 0u);
-            if (lane == 0) par[ph].e[warp & 3] = e;
+            // a V row that cannot be held (s = m = NaN) stands as zeros: its NaN
+            // reaches the rows that see it through m alone
+            const bool fine = va.x < INFINITY;
+            par_t.mk[i] = ka.y;
+            par_t.mv[i] = va.y;
+            par_t.sv[i] = fine ? va.x : 0.0f;
+            const uint32_t ek = __reduce_max_sync(0xffffffffu, ka.x < INFINITY ? __float_as_uint(ka.x) >> 23 : 0u);
+            const uint32_t ev = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(va.x) >> 23 : 0u);
+            const uint32_t kx = max(ek, (uint32_t)kMinExp);
+            if (lane == 0) {
+                par_t.f[warp & 3] = pow2((int)kx - 127 - kUp);
+                par_t.e[warp & 3] = (int)ev;
+            }
+            const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - (int)kx));
             uint8_t* kt = smem + C::kOffK;
 #pragma unroll
             for (int c = 0; c < NK; c++) {
@@ -559,7 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 for (int j = 0; j < 4; j++) {
                     uint32_t x[4];
                     q4_centred(w[j], x);
-                    *reinterpret_cast<uint4*>(kt + chunk_at(i, 4 * c + j, kN)) = make_uint4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<uint4*>(kt + chunk_at(i, 4 * c + j, kN)) =
+                        make_uint4(mul_h2(x[0], sk), mul_h2(x[1], sk), mul_h2(x[2], sk), mul_h2(x[3], sk));
                 }
             }
             if (t + 1 < n_tiles) load_k(t + 1);
@@ -569,7 +597,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 bar_arrive(&par_full[ph]);
                 bar_arrive(k_full);
             }
+            // every warp's part of the parameters, then V's buffer
+            if (!warp_wait(&par_full[ph], (uint32_t)((t >> 1) & 1), abort_flag)) break;
             if (t > 0 && !warp_wait(v_empty, ph ^ 1u, abort_flag)) break;
+            E = max(E, max(max(par_t.e[0], par_t.e[1]), max(par_t.e[2], par_t.e[3])));
+            const float v_up = pow2(127 + kUp - E);
+            const __half2 sv = __floats2half2_rn(par_t.sv[2 * vp] * v_up, par_t.sv[2 * vp + 1] * v_up);
             uint8_t* vt = smem + C::kOffV;
             const int ta = 2 * vp;  // the pair's tokens: rows ta and ta + 1
 #pragma unroll
@@ -580,6 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                     uint32_t x[4], y[4];
                     q4_centred(w[j], x);
                     q4_centred(w[j + 1], y);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) x[n] = mul_h2(x[n], sv), y[n] = mul_h2(y[n], sv);
                     const int chunk = vh * (D / 16) + 2 * c + j / 2;
                     *reinterpret_cast<uint4*>(vt + chunk_at(ta, chunk, kN)) =
                         make_uint4(prmt(x[0], x[1], 0x5410), prmt(x[2], x[3], 0x5410), prmt(y[0], y[1], 0x5410),
@@ -595,40 +630,134 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             if (lane == 0) bar_arrive(v_full);
         }
     } else {
-        // ================= softmax warpgroups =================
-        const int X = tid >> 7, r = tid & 127, qi = X * QT + r / G;
+        // ================= softmax warps =================
+        // Row 128 X + r is query X QT + r / G, head r % G; thread tid keeps that of
+        // row tid.  A warp brings its own 32 rows of q, eight in flight, each
+        // scaled by the power of two that puts its largest |q| in [2^14, 2^15).
+        const int X = warp >> 2, r = tid & 127, qi = X * QT + r / G;
         const bool valid = r < QT * G && q0 + qi < sm.q_len;
+        float q_un = 1.0f, q_sum = 0.0f;
+        {
+            const int mine = valid ? (sm.q_start + q0 + qi) * p.Hq + h * G + r % G : -1;
+            uint8_t* hi_at = smem + C::kOffQ + 2 * X * C::kQBytes;
+            // lane L takes dims 8 (L / 4) + L % 4 and + 4 (a register pair of K's order), of 64 dims at a time
+            const int d0 = 8 * (lane >> 2) + (lane & 3);
+#pragma unroll 1
+            for (int j0 = 0; j0 < 32; j0 += 8) {
+                float x[8][2 * C::kAtoms], mx[8], sum[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int at = __shfl_sync(0xffffffffu, mine, j0 + j);
+                    mx[j] = sum[j] = 0.0f;
+#pragma unroll
+                    for (int a = 0; a < 2 * C::kAtoms; a++) {
+                        x[j][a] = at < 0 ? 0.0f : p.q[(int64_t)at * D + 64 * (a >> 1) + 4 * (a & 1) + d0] * p.scale_log2;
+                        mx[j] = fmaxf(mx[j], fabsf(x[j][a]));
+                        sum[j] += x[j][a];
+                    }
+                }
+                // eight rows' maxima and sums at once: halve the rows and the lanes that hold them, then the lanes
+#pragma unroll
+                for (int n = 4; n > 0; n >>= 1) {
+                    const bool up = lane & (4 * n);
+#pragma unroll
+                    for (int j = 0; j < n; j++) {
+                        const float m_keep = up ? mx[j + n] : mx[j], m_give = up ? mx[j] : mx[j + n];
+                        const float s_keep = up ? sum[j + n] : sum[j], s_give = up ? sum[j] : sum[j + n];
+                        mx[j] = fmaxf(m_keep, __shfl_xor_sync(0xffffffffu, m_give, 4 * n));
+                        sum[j] = s_keep + __shfl_xor_sync(0xffffffffu, s_give, 4 * n);
+                    }
+                }
+#pragma unroll
+                for (int o = 2; o > 0; o >>= 1) {
+                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+                    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+                }
+                // lanes 4 j .. 4 j + 3 hold row j0 + j
+                const int qe = min(max((int)(__float_as_uint(mx[0]) >> 23), 40), 240);
+                const float scale = __uint_as_float((uint32_t)(268 - qe) << 23), un = __uint_as_float((uint32_t)(qe - 14) << 23);
+                const float un_j = __shfl_sync(0xffffffffu, un, 4 * (lane & 7)), sum_j = __shfl_sync(0xffffffffu, sum[0] * scale, 4 * (lane & 7));
+                if ((lane & 24) == j0) {
+                    q_un = un_j;  // 1 / scale
+                    q_sum = sum_j;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float sc = __shfl_sync(0xffffffffu, scale, 4 * j);
+#pragma unroll
+                    for (int a = 0; a < C::kAtoms; a++) {
+                        uint32_t hi, lo;
+                        split_h2(x[j][2 * a] * sc, x[j][2 * a + 1] * sc, hi, lo);
+                        const uint32_t at = chunk_at(32 * (warp & 3) + j0 + j, 8 * a + (lane >> 2), kM) + 4 * (lane & 3);
+                        *reinterpret_cast<uint32_t*>(hi_at + at) = hi;
+                        *reinterpret_cast<uint32_t*>(hi_at + C::kQBytes + at) = lo;
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(q_full);
+        }
         const int row_limit = valid ? prefix + q0 + qi : kv_end - 1;  // last visible token
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + lanes + X * 128, tO = tmem + lanes + kColO + X * 128;
-        RowState st{-INFINITY, 0.0f, 0.0f, __uint_as_float((uint32_t)(260 - kMinExp) << 23), q_un, q_sum, kMinExp};
+        RowState st{-INFINITY, 0.0f, 0.0f, q_un, q_sum, -INFINITY, kMinExp, kMinExp};
         const bool active = X == 0 || two_tiles;
+        float4* aside = reinterpret_cast<float4*>(p.aside) + (int64_t)slot * (D / 4) * (2 * kM) + tid;  // columns 4 c ..: + 256 c
         bool ok = true;
         for (int t = 0; active && t < n_tiles; t++) {
             const uint32_t ph = (uint32_t)(t & 1);
+            const bool fresh = t % chain == 0;
             // S_X(t) done also means PV_X(t - 1) done: O_X and P_X are free
             if (!warp_wait(&par_full[ph], (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(&s_full[X], ph, abort_flag)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
+            if (fresh && t > 0) {
+                // The tensor cores cut their sums instead of rounding them, so a
+                // long chain drifts: set the sums aside with rounded additions
+                // (in L2, nothing waited for) and start anew.
+                const float c = rebase(st.mb, st.Eb, st.m, st.E);
+                const bool add = t > chain && __all_sync(0xffffffffu, c == 1.0f);
+                if (t > chain && !add) __threadfence();
+#pragma unroll 1
+                for (int d = 0; d < D / 4; d += 8) {
+                    float ov[32];
+                    tmem_ld32(tO + 4 * d, ov);
+                    tmem_ld_wait16(ov);
+                    tmem_ld_wait16(ov + 16);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float4* at = aside + (d + i) * (2 * kM);
+                        float4 o = make_float4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+                        if (add) {
+                            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(o.x), "f"(o.y),
+                                         "f"(o.z), "f"(o.w)
+                                         : "memory");
+                        } else {
+                            if (t > chain) {
+                                const float4 old = __ldcg(at);
+                                o = make_float4(fmaf(old.x, c, o.x), fmaf(old.y, c, o.y), fmaf(old.z, c, o.z), fmaf(old.w, c, o.w));
+                            }
+                            __stcg(at, o);
+                        }
+                    }
+                }
+                st.mb = st.m;
+                st.Eb = st.E;
+            }
             const int base = (tb + t) * kN;
             if (base + kN - 1 > prefix + q0)  // some row of the chunk does not see all of it
-                softmax_tile<true, D>(tS, par[ph], row_limit - base, st, t == 0, tO, &p_half[X], &p_full[X], lane);
+                softmax_tile<true, D>(tS, tO, par[ph], row_limit - base, st, fresh, &p_half[X], &p_full[X], lane);
             else
-                softmax_tile<false, D>(tS, par[ph], 0, st, t == 0, tO, &p_half[X], &p_full[X], lane);
+                softmax_tile<false, D>(tS, tO, par[ph], 0, st, fresh, &p_half[X], &p_full[X], lane);
         }
         const int64_t at = ((int64_t)(sm.q_start + q0 + qi) * p.Hq + h * G + r % G);
-        if (active && n_tiles == 0 && valid) {  // an empty share of a split
-            const int64_t row = (int64_t)blockIdx.z * p.n_rows * p.Hq + at;
-            for (int d = 0; d < D; d++) p.part_o[row * D + d] = 0.0f;
-            p.part_ml[row * 2] = -INFINITY;
-            p.part_ml[row * 2 + 1] = 0.0f;
-        }
+        const bool split = p.n_split > 1;
         if (active && n_tiles > 0 && ok && warp_wait(&pv_done[X], (uint32_t)((n_tiles - 1) & 1), abort_flag)) {
             tc_fence_after();
-            const float back = __uint_as_float((uint32_t)(st.E - 6) << 23);  // 1 / vmul
-            const bool split = p.n_split > 1;
+            const float back = pow2(st.E - 127 - kUp);
             const int64_t row = split ? (int64_t)blockIdx.z * p.n_rows * p.Hq + at : at;
             float* dst = (split ? p.part_o : p.out) + row * D;
             const float inv = split ? 1.0f : 1.0f / st.l;
@@ -636,24 +765,41 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 p.part_ml[row * 2] = st.m;
                 p.part_ml[row * 2 + 1] = st.l;
             }
-            const bool vec = ((uintptr_t)dst & 15) == 0;
+            const bool vec = ((uintptr_t)dst & 15) == 0, had = n_tiles > chain;
+            const float c = rebase(st.mb, st.Eb, st.m, st.E);
+            if (had) __threadfence();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int d = 0; d < D / 4; d += 8) {
                 float ov[32];
-                tmem_ld32(tO + c, ov);
-                tmem_ld_wait();
+                float4 old[8];
+                if (had)
 #pragma unroll
-                for (int j = 0; j < 32; j++) ov[j] = fmaf(ov[j], back, st.z) * inv;
-                if (!valid) continue;
-                if (vec) {
+                    for (int i = 0; i < 8; i++) old[i] = __ldcg(aside + (d + i) * (2 * kM));
+                tmem_ld32(tO + 4 * d, ov);
+                tmem_ld_wait16(ov);
+                tmem_ld_wait16(ov + 16);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(dst + c + j) = make_float4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) dst[c + j] = ov[j];
+                for (int i = 0; i < 8; i++) {
+                    float4 o = make_float4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+                    if (had)
+                        o = make_float4(fmaf(old[i].x, c, o.x), fmaf(old[i].y, c, o.y), fmaf(old[i].z, c, o.z), fmaf(old[i].w, c, o.w));
+                    o = make_float4(fmaf(o.x, back, st.z) * inv, fmaf(o.y, back, st.z) * inv, fmaf(o.z, back, st.z) * inv,
+                                    fmaf(o.w, back, st.z) * inv);
+                    if (!valid) continue;
+                    if (vec) {
+                        *reinterpret_cast<float4*>(dst + 4 * (d + i)) = o;
+                    } else {
+                        dst[4 * (d + i)] = o.x, dst[4 * (d + i) + 1] = o.y;
+                        dst[4 * (d + i) + 2] = o.z, dst[4 * (d + i) + 3] = o.w;
+                    }
                 }
             }
+        }
+        if (active && n_tiles == 0 && valid) {  // an empty share of a split
+            const int64_t row = (int64_t)blockIdx.z * p.n_rows * p.Hq + at;
+            for (int d = 0; d < D; d++) p.part_o[row * D + d] = 0.0f;
+            p.part_ml[row * 2] = -INFINITY;
+            p.part_ml[row * 2 + 1] = 0.0f;
         }
     }
 
@@ -661,7 +807,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && *abort_flag) atomicOr(p.err, kErrTimeout);
-    if (warp == 12) {
+    if (tid == 0 && slot >= 0) {  // every thread is done with the slot
+        __threadfence();
+        atomicExch(&p.aside_lock[slot], 0);
+    }
+    if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
@@ -739,6 +889,19 @@ int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, 
     const int64_t ctas = std::max<int64_t>(1, (b->n_rows + 2 * p.QT - 1) / (2 * p.QT)) * p.Hkv;
     const int64_t tiles = (max_kv + kN - 1) / kN;
     p.n_split = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(148 / ctas, tiles / 4), 64));
+    // slots for the sums that long chains set aside, one an SM
+    int sms = 0;
+    S1KV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, pool->device));
+    const size_t slots = (size_t)sms * D * 2 * kM * sizeof(float);
+    if (!pool->aside.p) {
+        const int st = pool->aside.ensure(slots + sms * sizeof(int32_t));
+        if (st) return st;
+        S1KV_CUDA(cudaMemset((char*)pool->aside.p + slots, 0, sms * sizeof(int32_t)));
+        S1KV_CUDA(cudaDeviceSynchronize());
+    }
+    p.aside = (float*)pool->aside.p;
+    p.aside_lock = (int32_t*)((char*)pool->aside.p + slots);
+    p.n_aside = sms;
     if (p.n_split > 1) {
         const size_t rows = (size_t)p.n_split * p.n_rows * Hq;
         const int st = pool->scratch.ensure(rows * (D + 2) * sizeof(float));
