@@ -2,22 +2,24 @@
 // q4.cuh) on tcgen05: query chunks of more than one token, row i of a
 // sequence's q_len new tokens seeing tokens 0 .. (kv_len - q_len) + i.
 //
-//   score_t = q . (s_k c_t) + m_k sum(q),  out = sum_t p_t (s_v c_t) + sum_t p_t m_v
+//   score_t = q . (s_k c_t) + m_k sum(q),  out = sum_t (p_t s_v) c_t + sum_t p_t m_v
 // with the centred codes c = u - 8.  s c is exact in fp16: seven significant
 // codes are 3 bits, the eighth a power of two, s is 8 bits, fp16 has 11.  q
-// and p are each split into two fp16 parts (22 bits) and both parts are
+// and p s_v are each split into two fp16 parts (22 bits) and both parts are
 // multiplied: fp32-level results for twice the tensor-core work of a bf16
 // cache's prefill, 8 Hq D products a (query, visible token) in place of 4.
+// V stands as plain codes and s_v goes to p: the tensor cores cut the bits of
+// a product that lie below the running sum, and products of 15 bits lose a
+// quarter of what products of 22 lose over the hundreds of steps of a sum.
 // That and the softmax's instructions bound the kernel; K/V bytes are a
 // seventh of bf16's.
 //
 // A CTA takes a chunk of queries of one sequence and KV head as two tiles A
 // and B of 128 accumulator rows, a row a (query, head) pair: 128 / G queries
 // times the G query heads of the KV head (any G up to 128).
-//   * Two warpgroups run the softmax, one per tile, a thread a row: scores
-//     from TMEM, scaled per token, the online softmax in the exp2 domain
-//     (reference max moved only past 2^8), p s_v split and stored over the
-//     scores: 64 columns of high parts, 64 of low parts.
+//   * Four warpgroups run the softmax, two per tile, two threads a row:
+//     scores from TMEM, the online softmax in the exp2 domain (reference max
+//     moved only past 2^8), p split and stored over the scores.
 //   * One warpgroup widens K/V: a thread loads a token's codes straight from
 //     its block (the next tile's loads are in flight while it waits for the
 //     buffer), makes fp16 of them and writes the 128-byte-swizzled tiles the
@@ -39,15 +41,19 @@ namespace {
 
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kM = 128, kN = 128;  // rows per tile, tokens per K/V tile
-constexpr int kSoftmaxWarps = 8, kWidenWarps = 4, kMmaWarp = 12;
-constexpr int kThreads = 32 * 13;
+constexpr int kSoftmaxWarps = 16, kWidenWarps = 4, kMmaWarp = 20;  // two softmax threads a row
+constexpr int kThreads = 32 * 24;  // (three idle warps complete the MMA's warpgroup)
+// Registers by role.  At launch 80 a thread, 768 * 80 = 61440 in all;
+// 512 * 96 + 128 * 64 + 128 * 32 = 61440.  Spilled registers cost dearly here:
+// shared memory leaves the L1 cache too little for them.
+constexpr int kRegsSoftmax = 96, kRegsWiden = 64, kRegsMma = 32;
 constexpr int kFlush = 4;          // tiles a chain of sums in TMEM
 constexpr int kColO = 256;         // TMEM: S_A [0, 128) S_B [128, 256) O_A O_B
 constexpr int kTmemCols = 512;
 constexpr float kRescaleAt = 8.0f;
 constexpr int kMinExp = 20;         // least exponent (biased) scales are taken relative to
-constexpr int kUp = 11;             // the largest scale stands as 2^11 .. 2^12 in the fp16 tiles: 8 s below 2^15
-constexpr float kPUp = 6.0f;        // p is kept 2^6 times as large (at most 2^14), also in its sums
+constexpr int kUp = 11;             // K's largest s stands as 2^11 .. 2^12 in its fp16 tile: 8 s below 2^15
+constexpr int kVUp = 6;             // V's largest s counts as 2^6 .. 2^7 beside p: p s below 2^15
 constexpr int kIdsCached = 1024;   // block ids kept in shared memory (16K tokens)
 
 template <int D>
@@ -59,42 +65,54 @@ struct Cfg {
     static constexpr int kOffK = 4 * kQBytes;
     static constexpr int kOffV = kOffK + kKBytes;
     static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
-    static constexpr int kOffIds = kOffPar + 2 * (kN * 12 + 32);
+    static constexpr int kOffXch = kOffPar + 2 * (kN * 12 + 32);  // floats [4][2 halves][256 rows]
+    static constexpr int kOffRef = kOffXch + 4 * 4 * 2 * kM * 2;  // float2 [512] (max, exponent)
+    static constexpr int kOffIds = kOffRef + 512 * 8;
     static constexpr int kOffBar = kOffIds + kIdsCached * 4;
-    // k_full k_empty v_full v_empty par_full[2] s_full[2] p_half[2] p_full[2] pv_done[2] drain q_full
-    static constexpr int kNumBars = 16;
+    // k_full k_empty v_full v_empty par_full[2] s_full[2] p_full[2] pv_done[2] drain q_full pair[8]
+    static constexpr int kNumBars = 22;
     static constexpr int kOffMisc = kOffBar + kNumBars * 8 + 8;  // TMEM slot, abort flag, set-aside slot
     static constexpr int kSmem = kOffMisc + 16 + 1024;
 };
 
 __device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n) : "memory");
+// Barriers and the abort flag are held as 32-bit shared addresses (registers
+// are short).
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
 }
-__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t phase) {
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t phase) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(su32(b)), "r"(phase)
+        : "r"(b), "r"(phase)
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t phase) {
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t phase) {
     for (uint32_t i = 0; i < kSpin; i++)
         if (bar_try(b, phase)) return true;
     return false;
 }
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+__device__ __forceinline__ void bar_arrive(uint32_t b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t phase, volatile int* abort_flag) {
-    bool ok = false;
+__device__ __forceinline__ int flag_get(uint32_t flag) {
+    int v;
+    asm volatile("ld.volatile.shared.b32 %0, [%1];" : "=r"(v) : "r"(flag) : "memory");
+    return v;
+}
+__device__ __forceinline__ void flag_set(uint32_t flag, int v) {
+    asm volatile("st.volatile.shared.b32 [%0], %1;" ::"r"(flag), "r"(v) : "memory");
+}
+__device__ __forceinline__ bool warp_wait(uint32_t b, uint32_t phase, uint32_t abort_flag) {
+    bool ok = bar_try(b, phase);
     for (uint32_t i = 0; i < kSpin && !ok; i++) {
         ok = bar_try(b, phase);
-        if (!ok && *abort_flag) break;
+        if (!ok && flag_get(abort_flag)) break;
     }
-    if (!ok) *abort_flag = 1;
+    if (!ok) flag_set(abort_flag, 1);
     return __all_sync(0xffffffffu, ok);
 }
 // Shared-memory descriptor, 128-byte swizzle (layout type 2), 8-row groups
@@ -127,25 +145,21 @@ __device__ __forceinline__ void mma_ts_w(uint32_t d, uint32_t a, uint32_t b, uin
         "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit_w(uint64_t* b) {
+__device__ __forceinline__ void mma_commit_w(uint32_t b) {
     asm volatile(
         "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(b))
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(b)
         : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 consecutive fp32 columns of this thread's TMEM lane; the wait is apart.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+// 16 consecutive fp32 columns of this thread's TMEM lane; the wait is apart.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, "
-        "[%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
-          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
-          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
-          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr));
 }
 // Waits for this thread's TMEM loads.  The registers pass through, so that
@@ -165,19 +179,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]));
-}
-__device__ __forceinline__ void tmem_ld_wait32(float* v) {
-    tmem_ld_wait16(v);
-    tmem_ld_wait16(v + 16);
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
-    uint32_t w[16];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(v[16 * h + i]);
-        tmem_st16(taddr + 16 * h, w);
-    }
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -210,19 +211,28 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int chunk, int rows) {
     return (uint32_t)((chunk >> 3) * rows * 128 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
 }
 
-// One row's softmax state.  un: scores are in units of 1 / un (q was scaled
-// by a power of two); qs: sum of the scaled q.  mb, Eb: what the row's
-// set-aside sums refer to.
+template <int REGS>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// A softmax thread's state: half of each tile's tokens of a row.  un: scores are in units of 1 / un (q was scaled
+// by a power of two); qs: sum of the scaled q.
 struct RowState {
-    float m, l, z, un, qs, mb;
-    int E, Eb;
+    float m, l, z, un, qs;  // l and z: of this thread's tokens
+    int E;
 };
 // The parameters of a tile's rows.
 struct TilePar {
     float mk[kN], mv[kN];
-    float sv[kN];   // (the widening warps' own)
+    float sv[kN];   // s_v 2^(133 - E)
     float f[4];     // K's tokens 32 g .. + 31 stand in the tile as s_k c / f[g], a power of two
-    int e[4];       // largest exponent of the s_v of tokens 32 g .. + 31
+    int E;          // largest exponent of s_v so far
+    int pad[3];
 };
 
 // 2^(m' - m) 2^(E' - E): from sums that refer to (m', E') to (m, E).
@@ -231,32 +241,34 @@ __device__ __forceinline__ float rebase(float m_old, int e_old, float m, int e) 
     return e - e_old > 126 ? 0.0f : c * __uint_as_float((uint32_t)(127 - (e - e_old)) << 23);
 }
 
-// A tile's 128 scores of one row -> P over them: of each 32 columns the first
-// 16 take the high parts of p, the others the low parts.  Two passes over the
-// columns, 32 at a time with the next 32 on their way: the maximum, then the
-// weights (adding m_k sum(q) anew costs less than storing the scores back, a
-// round trip to TMEM).  The loops stay rolled: unrolled over 128 scores the
-// code runs from beyond the instruction cache.  EDGE: only tokens up to `last`
-// (of this tile) are seen; the others may hold anything, NaN included.  fresh:
-// O starts anew with this tile.
+// Half a tile's scores of one row (64 tokens from token t0) -> P over them: of
+// each 16 columns the first 8 take the high parts of p, the others the low
+// parts.  Two passes over the columns, 16 at a time with the next 16 on their
+// way: the maximum (exchanged with the row's other thread), then the weights
+// (adding m_k sum(q) anew costs less than storing the scores back, a round
+// trip to TMEM).  The loops stay rolled: unrolled over all scores the code
+// runs from beyond the instruction cache.  EDGE: only tokens up to `last` (of
+// this tile) are seen; the others may hold anything, NaN included.  fresh: O
+// starts anew with this tile.
 template <bool EDGE, int D>
-__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int last, RowState& st, bool fresh,
-                                             uint64_t* p_half, uint64_t* p_full, int lane) {
-    float v[2][32];
+__device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int t0, int last, RowState& st,
+                                             bool fresh, float* xch, int xch_other, uint32_t pair, uint32_t phase,
+                                             uint32_t p_full, uint32_t abort_flag, int lane) {
+    float v[2][16];
     float top = -INFINITY;
-    tmem_ld32(tS, v[0]);
+    tmem_ld16(tS, v[0]);
 #pragma unroll 1
-    for (int c = 0; c < kN; c += 64) {
+    for (int c = 0; c < 64; c += 32) {
+        const float f = par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f);
+        const float2 qs2 = make_float2(qs, qs);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int c0 = c + 32 * u;
-            const float f = par.f[c0 / 32], qs = __fdividef(st.qs, f);
-            const float2 qs2 = make_float2(qs, qs);
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld_wait32(v[u]);
-            tmem_ld32(tS + ((c0 + 32) & (kN - 1)), v[u ^ 1]);  // after the last, the first again for the second pass
+            const int c0 = t0 + c + 16 * u;
+            tmem_ld_wait16(v[u]);
+            tmem_ld16(tS + ((c + 16 * u + 16) & 63), v[u ^ 1]);  // after the last, the first again for the second pass
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+            for (int i = 0; i < 16; i += 4) {
                 const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
                 float2 x = __ffma2_rn(make_float2(k.x, k.y), qs2, make_float2(v[u][i], v[u][i + 1]));
                 float2 y = __ffma2_rn(make_float2(k.z, k.w), qs2, make_float2(v[u][i + 2], v[u][i + 3]));
@@ -269,10 +281,15 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const Til
                 mx[(i >> 1) & 2] = fmaxf(fmaxf(mx[(i >> 1) & 2], x.x), x.y);
                 mx[((i >> 1) & 2) + 1] = fmaxf(fmaxf(mx[((i >> 1) & 2) + 1], y.x), y.y);
             }
-            top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (st.un * f));
         }
+        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (st.un * f));
     }
-    const int e = max(st.E, max(max(par.e[0], par.e[1]), max(par.e[2], par.e[3])));
+    *xch = top;
+    __syncwarp();
+    if (lane == 0) bar_arrive(pair);
+    if (!warp_wait(pair, phase, abort_flag)) return false;
+    top = fmaxf(top, xch[xch_other]);
+    const int e = par.E;
     const bool raise = top > st.m + kRescaleAt || e > st.E;
     float corr = 1.0f;
     if (raise) {
@@ -285,23 +302,36 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const Til
         st.E = e;
     }
     const bool rescale = !fresh && __any_sync(0xffffffffu, raise);
-    const float nm = kPUp - (st.m == -INFINITY ? 0.0f : st.m);  // nothing visible yet: p = 0
+    const float nm = st.m == -INFINITY ? 0.0f : -st.m;  // nothing visible yet: p = 0
     const float2 nm2 = make_float2(nm, nm);
     float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
+    if (rescale) {  // this thread's half of O's columns
 #pragma unroll 1
-    for (int c = 0; c < kN; c += 64) {
+        for (int c = 0; c < D / 2; c += 16) {
+            float ov[16];
+            tmem_ld16(tO + c, ov);
+            tmem_ld_wait16(ov);
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = __float_as_uint(ov[i] * corr);
+            tmem_st16(tO + c, w);
+        }
+    }
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 32) {
+        const float f = par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f), un = st.un * f;
+        const float2 qs2 = make_float2(qs, qs), un2 = make_float2(un, un);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int c0 = c + 32 * u;
-            const float f = par.f[c0 / 32], qs = __fdividef(st.qs, f), un = st.un * f;
-            const float2 qs2 = make_float2(qs, qs), un2 = make_float2(un, un);
+            const int c0 = t0 + c + 16 * u;
             uint32_t hi[8], lo[8];
-            tmem_ld_wait32(v[u]);
-            if (c0 + 32 < kN) tmem_ld32(tS + c0 + 32, v[u ^ 1]);
+            tmem_ld_wait16(v[u]);
+            if (u == 0 || c == 0) tmem_ld16(tS + c + 16 * u + 16, v[u ^ 1]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
+            for (int i = 0; i < 16; i += 4) {
                 const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
                 const float4 mv = *reinterpret_cast<const float4*>(&par.mv[c0 + i]);
+                const float4 sv = *reinterpret_cast<const float4*>(&par.sv[c0 + i]);
 #pragma unroll
                 for (int w = 0; w < 4; w += 2) {
                     const int j = c0 + i + w;
@@ -316,35 +346,17 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const Til
                     const float2 p = make_float2(ex2(x.x), ex2(x.y));
                     l2 = __fadd2_rn(l2, p);
                     z2 = __ffma2_rn(p, m, z2);
-                    // high part: the leading 11 bits by a mask, low part: the rest
-                    const float2 t = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
-                                                 __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
-                    const float2 r = __fadd2_rn(p, make_float2(-t.x, -t.y));
-                    hi[(i + w) / 2 & 7] = pack_h2(t.x, t.y);
-                    lo[(i + w) / 2 & 7] = pack_h2(r.x, r.y);
-                }
-                if (i == 12 || i == 28) {
-                    tmem_st8(tS + c0 + (i & 16) / 2, hi);
-                    tmem_st8(tS + c0 + 16 + (i & 16) / 2, lo);
+                    const float2 ps = __fmul2_rn(p, w ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y));
+                    // the high part rounded, not cut: the low parts' signs then
+                    // vary and what the sums cut from them cancels
+                    const __half2 t = __floats2half2_rn(ps.x, ps.y);
+                    const float2 tf = __half22float2(t), r = __fadd2_rn(ps, make_float2(-tf.x, -tf.y));
+                    hi[(i + w) / 2] = *reinterpret_cast<const uint32_t*>(&t);
+                    lo[(i + w) / 2] = pack_h2(r.x, r.y);
                 }
             }
-        }
-        if (c == 0 && !rescale) {  // the first 64 tokens are handed over while the rest is computed
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(p_half);
-        }
-    }
-    if (rescale) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-            float ov[32];
-            tmem_ld32(tO + c, ov);
-            tmem_ld_wait32(ov);
-#pragma unroll
-            for (int i = 0; i < 32; i++) ov[i] *= corr;
-            tmem_st32(tO + c, ov);
+            tmem_st8(tS + c + 16 * u, hi);
+            tmem_st8(tS + c + 16 * u + 8, lo);
         }
     }
     tmem_st_wait();
@@ -352,10 +364,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, const Til
     st.z += z2.x + z2.y;
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) {
-        if (rescale) bar_arrive(p_half);
-        bar_arrive(p_full);
-    }
+    if (lane == 0) bar_arrive(p_full);
+    return true;
 }
 
 }  // namespace
@@ -386,11 +396,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     constexpr int kTileBytes = 16 * (D / 2 + 4);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-    uint64_t *k_full = bars, *k_empty = bars + 1, *v_full = bars + 2, *v_empty = bars + 3, *par_full = bars + 4;
-    uint64_t *s_full = bars + 6, *p_half = bars + 8, *p_full = bars + 10, *pv_done = bars + 12, *drain = bars + 14, *q_full = bars + 15;
+    const uint32_t bars = su32(smem) + C::kOffBar;
+    const uint32_t k_full = bars, k_empty = bars + 8, v_full = bars + 16, v_empty = bars + 24;
+    const uint32_t par_full = bars + 32, s_full = bars + 48, p_full = bars + 64, pv_done = bars + 80;  // of two each
+    const uint32_t drain = bars + 96, q_full = bars + 104, pairs = bars + 112;
+    const uint32_t abort_flag = su32(smem) + C::kOffMisc + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+    float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
     volatile int* aside_slot = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 8);
     TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
     static_assert(sizeof(TilePar) == kN * 12 + 32, "two tiles' parameters");
@@ -422,8 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     if (tid == 0) {
         // the widening and softmax warps arrive once a warp, the MMA commits once
         for (int i = 0; i < C::kNumBars; i++)
-            bar_init(&bars[i], i == 0 || i == 2 || i == 4 || i == 5 ? (uint32_t)kWidenWarps : i >= 8 && i < 12 ? 4u : i == 15 ? (uint32_t)kSoftmaxWarps : 1u);
-        *abort_flag = 0;
+            bar_init(bars + 8 * i, i == 0 || i == 2 || i == 4 || i == 5 ? (uint32_t)kWidenWarps : i == 8 || i == 9 ? 8u : i == 13 ? (uint32_t)kSoftmaxWarps : i > 13 ? 2u : 1u);
+        flag_set(abort_flag, 0);
         // A slot for the sums that chains of tiles set aside.  One CTA fits an
         // SM and there are as many slots as SMs, so one is free
         // (without one the sums merely run on).
@@ -456,32 +468,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     const int slot = *aside_slot;
     const int chain = slot < 0 ? INT32_MAX : kFlush;  // tiles until O starts anew
 
-    if (warp == kMmaWarp) {
-        {
+    if (warp >= kMmaWarp) {
+        regs_dec<kRegsMma>();
+        if (warp == kMmaWarp) {
             // ================= MMA issuer =================
             constexpr uint32_t idS = idesc_f16(kM, kN, 0), idO = idesc_f16(kM, D, 1);
             const uint32_t dk = desc_lo(su32(smem + C::kOffK), 16), dv = desc_lo(su32(smem + C::kOffV), kN * 128);
+            const uint32_t dq0 = desc_lo(su32(smem + C::kOffQ), 16);
+            // (rolled: descriptors of every step at once would spill)
             auto issue_s = [&](int X) {
-                const uint32_t dq = desc_lo(su32(smem + C::kOffQ + 2 * X * C::kQBytes), 16);
-#pragma unroll
+                const uint32_t dq = dq0 + (uint32_t)X * (2 * C::kQBytes / 16);
+#pragma unroll 1
                 for (int part = 1; part >= 0; part--)  // the small parts first: the sums are cut, not rounded
+#pragma unroll 1
+                    for (int a = 0; a < C::kAtoms; a++) {
+                        const uint32_t da = dq + (uint32_t)part * (C::kQBytes / 16) + (uint32_t)a * (kM * 128 / 16);
+                        const uint32_t db = dk + (uint32_t)a * (kN * 128 / 16);
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ks++) {
-                        const uint32_t step = (ks >> 2) * (kM * 128 / 16) + (ks & 3) * 2;
-                        mma_ss_w(tmem + X * 128, dq + part * (C::kQBytes / 16) + step, dk + step, idS, part == 0 || ks > 0);
+                        for (int k = 0; k < 4; k++)
+                            mma_ss_w(tmem + X * 128, da + 2 * k, db + 2 * k, idS, part == 0 || a > 0 || k > 0);
                     }
-                mma_commit_w(&s_full[X]);
+                mma_commit_w(s_full + 8 * X);
             };
-            auto issue_pv = [&](int X, bool fresh, int half) {  // 64 tokens, both parts of P
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int ks = 4 * half + k;
-#pragma unroll
-                    for (int part = 1; part >= 0; part--)
-                        mma_ts_w(tmem + kColO + X * 128, tmem + X * 128 + (ks >> 1) * 32 + part * 16 + (ks & 1) * 8,
-                                 dv + ks * (16 * 128 / 16), idO, !fresh || ks > 0 || part == 0);
+            auto issue_pv = [&](int X, bool fresh) {  // both parts of P, the small ones first
+#pragma unroll 2
+                for (int ks = 0; ks < 8; ks++) {
+                    const uint32_t a = tmem + X * 128 + ks * 16, db = dv + ks * (16 * 128 / 16);
+                    mma_ts_w(tmem + kColO + X * 128, a + 8, db, idO, !fresh || ks > 0);
+                    mma_ts_w(tmem + kColO + X * 128, a, db, idO, true);
                 }
-                if (half) mma_commit_w(&pv_done[X]);
+                mma_commit_w(pv_done + 8 * X);
             };
             bool ok = n_tiles > 0 && warp_wait(q_full, 0, abort_flag) && warp_wait(k_full, 0, abort_flag);
             if (ok) {
@@ -494,14 +510,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 const uint32_t ph = (uint32_t)(t & 1);
                 const bool more = t + 1 < n_tiles;
                 for (int X = 0; X < (two_tiles ? 2 : 1) && ok; X++) {
-                    ok = warp_wait(&p_half[X], ph, abort_flag) && (X || warp_wait(v_full, ph, abort_flag));
+                    ok = warp_wait(p_full + 8 * X, ph, abort_flag) && (X || warp_wait(v_full, ph, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(X, t % chain == 0, 0);
-                    ok = warp_wait(&p_full[X], ph, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_pv(X, t % chain == 0, 1);
+                    issue_pv(X, t % chain == 0);
                     if (X == (two_tiles ? 1 : 0)) mma_commit_w(v_empty);  // after the last product that reads V(t)
                     if (more) {  // S_X(t + 1) overwrites P_X(t), which PV_X(t) ahead of it reads
                         ok = X || warp_wait(k_full, ph ^ 1u, abort_flag);
@@ -518,19 +530,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         }
     } else if (warp >= kSoftmaxWarps) {
         // ================= widening: K, V and the rows' scales =================
+        regs_dec<kRegsWiden>();
         const int i = tid - 32 * kSoftmaxWarps;  // this thread's token of a tile (K), token pair and half (V)
         const int vp = i & 63, vh = i >> 6;
         constexpr int NK = D / 32;  // 16-byte loads of a token's K codes; as many of half a V pair's
-        uint4 kr[NK], vr[NK];
-        uint32_t pk = 0, pv = 0;
-        int E = kMinExp;  // largest exponent of s_v so far: V stands as s_v c 2^(138 - E), as the softmax warps know
+        uint4 kr[NK];  // one tile of K or V at a time: K's next loads wait for V's conversion, registers are short
+        uint4 (&vr)[NK] = kr;
+        uint32_t pk = 0, pv[4];  // this thread's token of K; V's tokens lane + 32 j (every warp works out the tile's largest s_v)
+        int E = kMinExp;         // largest exponent of s_v so far
         auto block = [&](int t, int b) -> int32_t {  // block b of local tile t
             const int j = t * (kN / 16) + b;
             return j < kIdsCached ? ids[j] : lookup(b0 + j);
         };
         auto load_k = [&](int t) {
             const int32_t blk = block(t, i >> 4);
-            pk = pv = 0;
+            pk = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int32_t b = block(t, 2 * j + (lane >> 4));
+                pv[j] = b < 0 || (tb + t) * kN + 32 * j + lane >= kv_end
+                            ? 0u
+                            : *reinterpret_cast<const uint32_t*>(p.vbase + ((int64_t)b * p.Hkv + h) * kTileBytes + 16 * (D / 2) + (lane & 15) * 4);
+            }
 #pragma unroll
             for (int c = 0; c < NK; c++) kr[c] = make_uint4(0, 0, 0, 0);
             if (blk < 0) return;
@@ -538,10 +559,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             const uint4* src = reinterpret_cast<const uint4*>(p.kbase + off + (i & 15) * (D / 2));
 #pragma unroll
             for (int c = 0; c < NK; c++) kr[c] = src[c];
-            if ((tb + t) * kN + i < kv_end) {  // rows past the end hold anything
+            if ((tb + t) * kN + i < kv_end)  // rows past the end hold anything
                 pk = *reinterpret_cast<const uint32_t*>(p.kbase + off + 16 * (D / 2) + (i & 15) * 4);
-                pv = *reinterpret_cast<const uint32_t*>(p.vbase + off + 16 * (D / 2) + (i & 15) * 4);
-            }
         };
         auto load_v = [&](int t) {
             const int32_t blk = block(t, vp >> 3);
@@ -553,30 +572,32 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
 #pragma unroll
             for (int c = 0; c < NK; c++) vr[c] = src[c];
         };
-        if (n_tiles > 0) {
-            load_k(0);
-            load_v(0);
-        }
+        if (n_tiles > 0) load_k(0);
         for (int t = 0; t < n_tiles; t++) {
             const uint32_t ph = (uint32_t)(t & 1);
             if (t > 0 && !warp_wait(k_empty, ph ^ 1u, abort_flag)) break;
             // parameters of slot t & 1: the softmax of tile t - 2 is done with
             // them (S(t - 1), which k_empty tracks, was issued after it)
             TilePar& par_t = par[ph];
-            const float2 ka = q4_unpack(pk), va = q4_unpack(pv);
-            // a V row that cannot be held (s = m = NaN) stands as zeros: its NaN
-            // reaches the rows that see it through m alone
-            const bool fine = va.x < INFINITY;
+            const float2 ka = q4_unpack(pk);
+            uint32_t ev = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = q4_unpack(pv[j]).x;
+                ev = max(ev, x < INFINITY ? __float_as_uint(x) >> 23 : 0u);
+            }
+            E = max(E, (int)__reduce_max_sync(0xffffffffu, ev));
+            const int wi = warp & 3;
+            const float2 va = q4_unpack(wi == 0 ? pv[0] : wi == 1 ? pv[1] : wi == 2 ? pv[2] : pv[3]);
             par_t.mk[i] = ka.y;
             par_t.mv[i] = va.y;
-            par_t.sv[i] = fine ? va.x : 0.0f;
+            // a V row that cannot be held (s = m = NaN) counts as zeros here: its NaN
+            // reaches the rows that see it through m
+            par_t.sv[i] = va.x < INFINITY ? va.x * pow2(127 + kVUp - E) : 0.0f;
+            if (i == 0) par_t.E = E;
             const uint32_t ek = __reduce_max_sync(0xffffffffu, ka.x < INFINITY ? __float_as_uint(ka.x) >> 23 : 0u);
-            const uint32_t ev = __reduce_max_sync(0xffffffffu, fine ? __float_as_uint(va.x) >> 23 : 0u);
             const uint32_t kx = max(ek, (uint32_t)kMinExp);
-            if (lane == 0) {
-                par_t.f[warp & 3] = pow2((int)kx - 127 - kUp);
-                par_t.e[warp & 3] = (int)ev;
-            }
+            if (lane == 0) par_t.f[wi] = pow2((int)kx - 127 - kUp);
             const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - (int)kx));
             uint8_t* kt = smem + C::kOffK;
 #pragma unroll
@@ -590,19 +611,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                         make_uint4(mul_h2(x[0], sk), mul_h2(x[1], sk), mul_h2(x[2], sk), mul_h2(x[3], sk));
                 }
             }
-            if (t + 1 < n_tiles) load_k(t + 1);
+            load_v(t);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                bar_arrive(&par_full[ph]);
+                bar_arrive(par_full + 8 * ph);
                 bar_arrive(k_full);
             }
-            // every warp's part of the parameters, then V's buffer
-            if (!warp_wait(&par_full[ph], (uint32_t)((t >> 1) & 1), abort_flag)) break;
             if (t > 0 && !warp_wait(v_empty, ph ^ 1u, abort_flag)) break;
-            E = max(E, max(max(par_t.e[0], par_t.e[1]), max(par_t.e[2], par_t.e[3])));
-            const float v_up = pow2(127 + kUp - E);
-            const __half2 sv = __floats2half2_rn(par_t.sv[2 * vp] * v_up, par_t.sv[2 * vp + 1] * v_up);
             uint8_t* vt = smem + C::kOffV;
             const int ta = 2 * vp;  // the pair's tokens: rows ta and ta + 1
 #pragma unroll
@@ -613,8 +629,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                     uint32_t x[4], y[4];
                     q4_centred(w[j], x);
                     q4_centred(w[j + 1], y);
-#pragma unroll
-                    for (int n = 0; n < 4; n++) x[n] = mul_h2(x[n], sv), y[n] = mul_h2(y[n], sv);
                     const int chunk = vh * (D / 16) + 2 * c + j / 2;
                     *reinterpret_cast<uint4*>(vt + chunk_at(ta, chunk, kN)) =
                         make_uint4(prmt(x[0], x[1], 0x5410), prmt(x[2], x[3], 0x5410), prmt(y[0], y[1], 0x5410),
@@ -624,17 +638,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                                    prmt(y[2], y[3], 0x7632));
                 }
             }
-            if (t + 1 < n_tiles) load_v(t + 1);
+            if (t + 1 < n_tiles) load_k(t + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(v_full);
         }
     } else {
+        regs_inc<kRegsSoftmax>();
         // ================= softmax warps =================
-        // Row 128 X + r is query X QT + r / G, head r % G; thread tid keeps that of
-        // row tid.  A warp brings its own 32 rows of q, eight in flight, each
+        // Softmax warp w: tile X = w / 8, rows 32 (w % 4) .. + 31 of it (a row a
+        // lane, as TMEM has it), tokens 64 half .. + 63 of every tile, half =
+        // (w / 4) % 2.  Row 128 X + r is query X QT + r / G, head r % G.  The
+        // two warps of 32 rows bring 16 of q's rows each, eight in flight, each
         // scaled by the power of two that puts its largest |q| in [2^14, 2^15).
-        const int X = warp >> 2, r = tid & 127, qi = X * QT + r / G;
+        const int X = warp >> 3, half = (warp >> 2) & 1, r = 32 * (warp & 3) + lane, qi = X * QT + r / G;
+        const uint32_t pair = pairs + 8 * (4 * X + (warp & 3));  // of the two warps
+        float* x_mine = xch + half * 2 * kM + X * kM + r;  // slot s: + s * 4 kM; the other half's:
+        const int x_other = (half ? -2 : 2) * kM;
         const bool valid = r < QT * G && q0 + qi < sm.q_len;
         float q_un = 1.0f, q_sum = 0.0f;
         {
@@ -643,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             // lane L takes dims 8 (L / 4) + L % 4 and + 4 (a register pair of K's order), of 64 dims at a time
             const int d0 = 8 * (lane >> 2) + (lane & 3);
 #pragma unroll 1
-            for (int j0 = 0; j0 < 32; j0 += 8) {
+            for (int j0 = 16 * half; j0 < 16 * half + 16; j0 += 8) {
                 float x[8][2 * C::kAtoms], mx[8], sum[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -677,9 +697,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 const int qe = min(max((int)(__float_as_uint(mx[0]) >> 23), 40), 240);
                 const float scale = __uint_as_float((uint32_t)(268 - qe) << 23), un = __uint_as_float((uint32_t)(qe - 14) << 23);
                 const float un_j = __shfl_sync(0xffffffffu, un, 4 * (lane & 7)), sum_j = __shfl_sync(0xffffffffu, sum[0] * scale, 4 * (lane & 7));
-                if ((lane & 24) == j0) {
-                    q_un = un_j;  // 1 / scale
-                    q_sum = sum_j;
+                if ((lane & 24) == j0) {  // for this row's other thread too
+                    x_mine[2 * 4 * kM] = x_mine[2 * 4 * kM + x_other] = un_j;  // 1 / scale
+                    x_mine[3 * 4 * kM] = x_mine[3 * 4 * kM + x_other] = sum_j;
                 }
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -696,20 +716,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) bar_arrive(q_full);
+            if (lane == 0) {
+                bar_arrive(q_full);
+                bar_arrive(pair);
+            }
         }
+        bool ok = warp_wait(pair, 0, abort_flag);
+        q_un = x_mine[2 * 4 * kM];
+        q_sum = x_mine[3 * 4 * kM];
         const int row_limit = valid ? prefix + q0 + qi : kv_end - 1;  // last visible token
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t tS = tmem + lanes + X * 128, tO = tmem + lanes + kColO + X * 128;
-        RowState st{-INFINITY, 0.0f, 0.0f, q_un, q_sum, -INFINITY, kMinExp, kMinExp};
+        const uint32_t tS = tmem + lanes + X * 128 + 64 * half, tO = tmem + lanes + kColO + X * 128 + half * (D / 2);
+        RowState st{-INFINITY, 0.0f, 0.0f, q_un, q_sum, kMinExp};
         const bool active = X == 0 || two_tiles;
-        float4* aside = reinterpret_cast<float4*>(p.aside) + (int64_t)slot * (D / 4) * (2 * kM) + tid;  // columns 4 c ..: + 256 c
-        bool ok = true;
-        for (int t = 0; active && t < n_tiles; t++) {
+        float4* aside = reinterpret_cast<float4*>(p.aside) + ((int64_t)slot * (D / 4) + half * (D / 8)) * (2 * kM) + X * kM + r;  // columns 4 c ..: + 256 c
+        float2* ref = reinterpret_cast<float2*>(smem + C::kOffRef) + tid;  // what this thread's set-aside sums refer to
+        for (int t = 0; active && ok && t < n_tiles; t++) {
             const uint32_t ph = (uint32_t)(t & 1);
             const bool fresh = t % chain == 0;
             // S_X(t) done also means PV_X(t - 1) done: O_X and P_X are free
-            if (!warp_wait(&par_full[ph], (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(&s_full[X], ph, abort_flag)) {
+            if (!warp_wait(par_full + 8 * ph, (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(s_full + 8 * X, ph, abort_flag)) {
                 ok = false;
                 break;
             }
@@ -718,17 +744,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 // The tensor cores cut their sums instead of rounding them, so a
                 // long chain drifts: set the sums aside with rounded additions
                 // (in L2, nothing waited for) and start anew.
-                const float c = rebase(st.mb, st.Eb, st.m, st.E);
+                const float c = t > chain ? rebase(ref->x, __float_as_int(ref->y), st.m, st.E) : 1.0f;
                 const bool add = t > chain && __all_sync(0xffffffffu, c == 1.0f);
                 if (t > chain && !add) __threadfence();
 #pragma unroll 1
-                for (int d = 0; d < D / 4; d += 8) {
-                    float ov[32];
-                    tmem_ld32(tO + 4 * d, ov);
+                for (int d = 0; d < D / 8; d += 4) {
+                    float ov[16];
+                    tmem_ld16(tO + 4 * d, ov);
                     tmem_ld_wait16(ov);
-                    tmem_ld_wait16(ov + 16);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 4; i++) {
                         float4* at = aside + (d + i) * (2 * kM);
                         float4 o = make_float4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
                         if (add) {
@@ -744,48 +769,60 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                         }
                     }
                 }
-                st.mb = st.m;
-                st.Eb = st.E;
+                *ref = make_float2(st.m, __int_as_float(st.E));
             }
             const int base = (tb + t) * kN;
+            // (the pair's phase 0 was q's)
             if (base + kN - 1 > prefix + q0)  // some row of the chunk does not see all of it
-                softmax_tile<true, D>(tS, tO, par[ph], row_limit - base, st, fresh, &p_half[X], &p_full[X], lane);
+                ok = softmax_tile<true, D>(tS, tO, par[ph], 64 * half, row_limit - base, st, fresh, x_mine + ph * 4 * kM, x_other, pair,
+                                           ph ^ 1u, p_full + 8 * X, abort_flag, lane);
             else
-                softmax_tile<false, D>(tS, tO, par[ph], 0, st, fresh, &p_half[X], &p_full[X], lane);
+                ok = softmax_tile<false, D>(tS, tO, par[ph], 64 * half, 0, st, fresh, x_mine + ph * 4 * kM, x_other, pair, ph ^ 1u,
+                                            p_full + 8 * X, abort_flag, lane);
         }
-        const int64_t at = ((int64_t)(sm.q_start + q0 + qi) * p.Hq + h * G + r % G);
+        int tid_;  // (where the row lies is worked out anew, not kept over the loop)
+        asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid_));
+        const int X_ = tid_ >> 8, half_ = (tid_ >> 7) & 1, r_ = tid_ & 127, qi_ = X_ * QT + r_ / G;
+        const bool valid_ = r_ < QT * G && q0 + qi_ < sm.q_len;
+        const int64_t at = ((int64_t)(sm.q_start + q0 + qi_) * p.Hq + h * G + r_ % G);
         const bool split = p.n_split > 1;
-        if (active && n_tiles > 0 && ok && warp_wait(&pv_done[X], (uint32_t)((n_tiles - 1) & 1), abort_flag)) {
+        if (active && n_tiles > 0 && ok && warp_wait(pv_done + 8 * X_, (uint32_t)((n_tiles - 1) & 1), abort_flag)) {
             tc_fence_after();
-            const float back = pow2(st.E - 127 - kUp);
+            // the row's sums from its two threads
+            x_mine[2 * 4 * kM] = st.l;
+            x_mine[3 * 4 * kM] = st.z;
+            __syncwarp();
+            if (lane == 0) bar_arrive(pair);
+            warp_wait(pair, (uint32_t)((n_tiles + 1) & 1), abort_flag);
+            const float l = st.l + x_mine[2 * 4 * kM + x_other], z = st.z + x_mine[3 * 4 * kM + x_other];
+            const float back = pow2(st.E - 127 - kVUp);
             const int64_t row = split ? (int64_t)blockIdx.z * p.n_rows * p.Hq + at : at;
-            float* dst = (split ? p.part_o : p.out) + row * D;
-            const float inv = split ? 1.0f : 1.0f / st.l;
-            if (split && valid) {
+            float* dst = (split ? p.part_o : p.out) + row * D + half_ * (D / 2);
+            const float inv = split ? 1.0f : 1.0f / l;
+            if (split && valid_ && half_ == 0) {
                 p.part_ml[row * 2] = st.m;
-                p.part_ml[row * 2 + 1] = st.l;
+                p.part_ml[row * 2 + 1] = l;
             }
             const bool vec = ((uintptr_t)dst & 15) == 0, had = n_tiles > chain;
-            const float c = rebase(st.mb, st.Eb, st.m, st.E);
+            const float c = had ? rebase(ref->x, __float_as_int(ref->y), st.m, st.E) : 1.0f;
             if (had) __threadfence();
 #pragma unroll 1
-            for (int d = 0; d < D / 4; d += 8) {
-                float ov[32];
-                float4 old[8];
+            for (int d = 0; d < D / 8; d += 4) {
+                float ov[16];
+                float4 old[4];
                 if (had)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) old[i] = __ldcg(aside + (d + i) * (2 * kM));
-                tmem_ld32(tO + 4 * d, ov);
+                    for (int i = 0; i < 4; i++) old[i] = __ldcg(aside + (d + i) * (2 * kM));
+                tmem_ld16(tO + 4 * d, ov);
                 tmem_ld_wait16(ov);
-                tmem_ld_wait16(ov + 16);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < 4; i++) {
                     float4 o = make_float4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
                     if (had)
                         o = make_float4(fmaf(old[i].x, c, o.x), fmaf(old[i].y, c, o.y), fmaf(old[i].z, c, o.z), fmaf(old[i].w, c, o.w));
-                    o = make_float4(fmaf(o.x, back, st.z) * inv, fmaf(o.y, back, st.z) * inv, fmaf(o.z, back, st.z) * inv,
-                                    fmaf(o.w, back, st.z) * inv);
-                    if (!valid) continue;
+                    o = make_float4(fmaf(o.x, back, z) * inv, fmaf(o.y, back, z) * inv, fmaf(o.z, back, z) * inv,
+                                    fmaf(o.w, back, z) * inv);
+                    if (!valid_) continue;
                     if (vec) {
                         *reinterpret_cast<float4*>(dst + 4 * (d + i)) = o;
                     } else {
@@ -795,9 +832,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 }
             }
         }
-        if (active && n_tiles == 0 && valid) {  // an empty share of a split
+        if (active && n_tiles == 0 && valid_) {  // an empty share of a split
             const int64_t row = (int64_t)blockIdx.z * p.n_rows * p.Hq + at;
-            for (int d = 0; d < D; d++) p.part_o[row * D + d] = 0.0f;
+            for (int d = 0; d < D / 2; d++) p.part_o[row * D + half_ * (D / 2) + d] = 0.0f;
             p.part_ml[row * 2] = -INFINITY;
             p.part_ml[row * 2 + 1] = 0.0f;
         }
@@ -806,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     // ---- tear-down: every path frees TMEM ----
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && *abort_flag) atomicOr(p.err, kErrTimeout);
+    if (tid == 0 && flag_get(abort_flag)) atomicOr(p.err, kErrTimeout);
     if (tid == 0 && slot >= 0) {  // every thread is done with the slot
         __threadfence();
         atomicExch(&p.aside_lock[slot], 0);
