@@ -15,9 +15,10 @@
 // largest at 2^15: scores and outputs carry fp32-level error.
 //
 // Layout: one 16-token tile of a KV head is 16 D / 2 + 64 bytes of K and as
-// many of V, and the storage order is the fragments' own: a lane's codes of
-// the whole tile are two 16-byte loads of K and two of V (D = 128), straight
-// from global memory to registers, coalesced over the warp.
+// many of V, contiguous, and the storage order is the fragments' own: a lane's
+// codes of the whole tile are two 16-byte reads of K and two of V (D = 128),
+// without bank conflicts.  Each warp brings its tiles with two bulk copies each
+// into a ring of its own in shared memory, kNS tiles ahead.
 //   K: lane (g, t) = (L / 4, L % 4) takes dims 32 t .. 32 t + 31 of tokens g
 //      and g + 8.  The sum over dims does not care for their order, so q's
 //      fragments simply follow K's: nibbles n and n + 4 of a word are the
@@ -44,9 +45,11 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kNW = 4;
 constexpr int kTile = 16;
-constexpr int kMaxG = 32;              // query heads per KV head the merge's scratch covers (D = 64: 36 G of 2048 floats)
+constexpr int kMaxG = 128;             // query heads per KV head the merge's scratch covers (D = 64: 36 G of 4608 floats)
 constexpr float kRescaleAt = 8.0f;     // log2 units
 constexpr int kMinExp = 8;             // least exponent (biased) the V scales are taken relative to
+constexpr uint32_t kSpin = 1u << 22;
+constexpr int kNS = 4;                 // tiles in flight a warp
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -78,21 +81,37 @@ __device__ __forceinline__ void split_h2(float a, float b, uint32_t& hi, uint32_
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = pack_h2(a - f.x, b - f.y);
 }
-// One tile's bytes of one lane: NWD words of K for tokens g and g + 8, of V
-// for pairs t and t + 4, and the params of tokens g and g + 8.
-template <int NWD>
-struct TileRegs {
-    uint32_t k0[NWD], k1[NWD], v0[NWD], v1[NWD];
-    uint32_t pk0, pk1, pv0, pv1;
-};
-
+__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t phase) {
+    for (uint32_t i = 0; i < kSpin; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(b), "r"(phase)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t b) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(b)
+                 : "memory");
+}
 template <int NWD>
 __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[NWD]) {
     if constexpr (NWD == 4) {
-        const uint4 x = __ldcs(reinterpret_cast<const uint4*>(at));
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
         w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else {
-        const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
         w[0] = x.x, w[1] = x.y;
     }
 }
@@ -101,14 +120,18 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[NWD]) {
 
 // D = 32 NWD; heads of one pass (NT = 1: up to 4, NT = 2: up to 8).
 template <int D, int NT>
-__global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_constant__ AttnParams p, int G) {
+__global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_constant__ AttnParams p, int G) {
     constexpr int NWD = D / 32, KS = D / 16, GP = 4 * NT;
-    constexpr int kTileBytes = kTile * (D / 2 + 4), kParams = kTile * (D / 2);
-    extern __shared__ float smem_f[];
-    float* mo = smem_f;                    // [kNW][GP][D]
-    float* mml = mo + kNW * GP * D;        // [kNW][GP][2]
-    int* flag = reinterpret_cast<int*>(mml + kNW * GP * 2);
+    constexpr int kTileBytes = kTile * (D / 2 + 4), kParams = kTile * (D / 2), kStage = 2 * kTileBytes;
+    constexpr int kRing = kNW * kNS * kStage;
+    static_assert(kRing >= kNW * GP * (D + 2) * 4, "the warps' partial rows lie over the rings");
+    extern __shared__ __align__(128) char smem[];
+    float* mo = reinterpret_cast<float*>(smem);  // [kNW][GP][D], over the rings once they are done
+    float* mml = mo + kNW * GP * D;              // [kNW][GP][2]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const char* ring = smem + warp * kNS * kStage;
+    const uint32_t bars = su32(smem) + kRing + warp * kNS * 8;
+    int* flag = reinterpret_cast<int*>(smem + kRing + kNW * kNS * 8);
     const int gq = lane >> 2, tq = lane & 3;
     const int h = blockIdx.y;
     const WorkItem item = p.items[blockIdx.x];
@@ -117,21 +140,70 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
     const int n_tiles = (tok1 - tok0 + kTile - 1) / kTile;
     const int my_tiles = n_tiles > warp ? (n_tiles - warp + kNW - 1) / kNW : 0;
     const int32_t* tab = p.table + (int64_t)item.table_row * p.max_bps + (tok0 >> 4);
+
+    int32_t my_blk = 0;
+    auto fetch_ids = [&](int k) {  // block ids of this warp's tiles k .. k + 31, one a lane
+        my_blk = 0;
+        if (k + lane < my_tiles) {
+            my_blk = tab[warp + (k + lane) * kNW];
+            if ((uint32_t)my_blk >= (uint32_t)p.max_blocks) {
+                atomicOr(p.err, kErrBounds);
+                my_blk = 0;
+            }
+        }
+    };
+    auto issue = [&](int k, int it) {  // tile k of this warp into the stage of copy `it`
+        const int64_t off = ((int64_t)__shfl_sync(kFull, my_blk, k & 31) * p.Hkv + h) * kTileBytes;
+        if (lane == 0) {
+            const uint32_t b = bars + (it % kNS) * 8, dst = su32(ring) + (it % kNS) * kStage;
+            bar_expect(b, kStage);
+            bulk_copy(dst, reinterpret_cast<const char*>(p.kbase) + off, kTileBytes, b);
+            bulk_copy(dst + kTileBytes, reinterpret_cast<const char*>(p.vbase) + off, kTileBytes, b);
+        }
+    };
+    if (lane == 0) {
+        for (int i = 0; i < kNS; i++) bar_init(bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    fetch_ids(0);
+    // Tiles that lie below the tokens this batch appends are requested before
+    // the wait for the previous kernel: nothing that may still run writes them
+    // (split_k_attention states why).
+    const int n_first = min(kNS, my_tiles);
+    int pre = 0;
+    if (p.prewait)
+        while (pre < n_first && tok0 + (warp + pre * kNW) * kTile + kTile <= item.kv_len - p.prewait_margin) pre++;
+    for (int k = 0; k < pre; k++) issue(k, k);
     pdl_wait();
     const RowMeta rm = p.rows[item.row];
+    bool failed = false;
+    int it0 = 0;  // copies consumed by earlier passes
 
     for (int g0 = 0; g0 < G; g0 += GP) {
+        const int tiles = failed ? 0 : my_tiles;  // (the CTA's warps stay together whatever happens)
+        if (g0 > 0) fetch_ids(0);
+        for (int k = g0 > 0 ? 0 : pre; k < min(n_first, tiles); k++) issue(k, it0 + k);
         // q's fragments: column c of the N side is head g0 + c (NT = 2), or
         // head g0 + c % 4 with the high part in columns 0-3 and the low part
-        // in 4-7 (NT = 1).
+        // in 4-7 (NT = 1).  This lane's column and dims 8 NWD tq .. are one
+        // contiguous piece of a row of q.
         const int head = NT == 1 ? gq & 3 : gq;
         const bool live = g0 + head < G;
-        const float* qrow = p.q + ((int64_t)item.row * p.Hq + h * G + g0 + (live ? head : 0)) * D;
+        const float* qrow = p.q + ((int64_t)item.row * p.Hq + h * G + g0 + (live ? head : 0)) * D + 8 * NWD * tq;
+        float x[8 * NWD];
         float amax = 0.0f, qsum = 0.0f;
-        for (int d = tq; d < D; d += 4) {
-            const float x = live ? qrow[d] * p.scale_log2 : 0.0f;
-            amax = fmaxf(amax, fabsf(x));
-            qsum += x;
+        const bool vec = ((uintptr_t)p.q & 15) == 0;
+#pragma unroll
+        for (int d = 0; d < 8 * NWD; d += 4) {
+            const float4 f = vec ? *reinterpret_cast<const float4*>(qrow + d) : make_float4(qrow[d], qrow[d + 1], qrow[d + 2], qrow[d + 3]);
+            x[d] = f.x, x[d + 1] = f.y, x[d + 2] = f.z, x[d + 3] = f.w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[d + e] = live ? x[d + e] * p.scale_log2 : 0.0f;
+                amax = fmaxf(amax, fabsf(x[d + e]));
+                qsum += x[d + e];
+            }
         }
         qsum += __shfl_xor_sync(kFull, qsum, 1);
         qsum += __shfl_xor_sync(kFull, qsum, 2);
@@ -148,11 +220,10 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const int d = 8 * (NWD * tq + wi) + 2 * j + b;
-                    const float f = p.scale_log2 * (b ? 0.0625f : 1.0f);
-                    const float x0 = live ? qrow[d] * f * qscale : 0.0f, x1 = live ? qrow[d + 4] * f * qscale : 0.0f;
+                    const int d = 8 * wi + 2 * j + b;
+                    const float f = qscale * (b ? 0.0625f : 1.0f);
                     uint32_t hi, lo;
-                    split_h2(x0, x1, hi, lo);
+                    split_h2(x[d] * f, x[d + 4] * f, hi, lo);
                     if (NT == 1) {
                         qf[0][2 * wi + j][b] = gq < 4 ? hi : lo;
                     } else {
@@ -170,37 +241,19 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
         int E = kMinExp;  // V scales are taken relative to 2^(E - 127)
         float vmul = __uint_as_float((uint32_t)(260 - E) << 23);  // 2^(133 - E): the largest scaled s_v in [2^6, 2^7)
 
-        int32_t my_blk = 0;
-        auto fetch_ids = [&](int k) {  // block ids of this warp's tiles k .. k + 31, one a lane
-            my_blk = 0;
-            if (k + lane < my_tiles) {
-                my_blk = tab[warp + (k + lane) * kNW];
-                if ((uint32_t)my_blk >= (uint32_t)p.max_blocks) {
-                    atomicOr(p.err, kErrBounds);
-                    my_blk = 0;
-                }
+        int done = 0;
+        for (int k = 0; k < tiles; k++) {
+            const int stage = (it0 + k) % kNS;
+            if (!bar_wait(bars + 8 * stage, (uint32_t)(((it0 + k) / kNS) & 1))) {
+                failed = true;
+                break;
             }
-        };
-        auto load = [&](int k, TileRegs<NWD>& r) {
-            if ((k & 31) == 0) fetch_ids(k);
-            const int64_t off = ((int64_t)__shfl_sync(kFull, my_blk, k & 31) * p.Hkv + h) * kTileBytes;
-            const char* kt = reinterpret_cast<const char*>(p.kbase) + off;
-            const char* vt = reinterpret_cast<const char*>(p.vbase) + off;
-            load_words<NWD>(kt + gq * (D / 2) + tq * (4 * NWD), r.k0);
-            load_words<NWD>(kt + (gq + 8) * (D / 2) + tq * (4 * NWD), r.k1);
-            load_words<NWD>(vt + tq * D + gq * (4 * NWD), r.v0);
-            load_words<NWD>(vt + (tq + 4) * D + gq * (4 * NWD), r.v1);
-            r.pk0 = __ldcs(reinterpret_cast<const uint32_t*>(kt + kParams) + gq);
-            r.pk1 = __ldcs(reinterpret_cast<const uint32_t*>(kt + kParams) + gq + 8);
-            r.pv0 = __ldcs(reinterpret_cast<const uint32_t*>(vt + kParams) + gq);
-            r.pv1 = __ldcs(reinterpret_cast<const uint32_t*>(vt + kParams) + gq + 8);
-        };
-        TileRegs<NWD> nx;
-        if (my_tiles > 0) load(0, nx);
-        for (int k = 0; k < my_tiles; k++) {
-            const TileRegs<NWD> r = nx;
-            if (k + 1 < my_tiles) load(k + 1, nx);
+            done = k + 1;
+            const char *kt = ring + stage * kStage, *vt = kt + kTileBytes;
             const int valid = min(kTile, tok1 - (tok0 + (warp + k * kNW) * kTile));
+            uint32_t k0[NWD], k1[NWD], v0[NWD], v1[NWD];
+            load_words<NWD>(kt + gq * (D / 2) + tq * (4 * NWD), k0);
+            load_words<NWD>(kt + (gq + 8) * (D / 2) + tq * (4 * NWD), k1);
 
             // ---- scores: M = the 16 tokens, N = the 8 columns ----
             float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
@@ -208,7 +261,7 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
             for (int wi = 0; wi < NWD; wi++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const uint32_t a = r.k0[wi] >> (8 * j), b = r.k1[wi] >> (8 * j);
+                    const uint32_t a = k0[wi] >> (8 * j), b = k1[wi] >> (8 * j);
                     const uint32_t a0 = a & 0x000F000Fu, a1 = b & 0x000F000Fu, a2 = a & 0x00F000F0u, a3 = b & 0x00F000F0u;
                     const int ks = 2 * wi + j;
                     if (NT == 1) {
@@ -225,14 +278,24 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
                 if (NT == 1) x[i] += __shfl_xor_sync(kFull, x[i], 2);  // high + low part of q
             }
             // this lane: tokens gq (x[0], x[1]) and gq + 8 (x[2], x[3]) of its two heads
-            const float2 ka = q4_unpack(r.pk0), kb = q4_unpack(r.pk1);
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(kt + kParams);
+            const uint32_t* vp = reinterpret_cast<const uint32_t*>(vt + kParams);
+            const float2 ka = q4_unpack(kp[gq]), kb = q4_unpack(kp[gq + 8]);
             const float sk0 = ka.x * unscale, sk1 = kb.x * unscale;
             const float zk0 = fmaf(-8.0f, ka.x, ka.y), zk1 = fmaf(-8.0f, kb.x, kb.y);
             x[0] = fmaf(x[0], sk0, zk0 * qs0);
             x[1] = fmaf(x[1], sk0, zk0 * qs1);
             x[2] = fmaf(x[2], sk1, zk1 * qs0);
             x[3] = fmaf(x[3], sk1, zk1 * qs1);
-            float2 va = q4_unpack(r.pv0), vb = q4_unpack(r.pv1);
+            float2 va = q4_unpack(vp[gq]), vb = q4_unpack(vp[gq + 8]);
+            load_words<NWD>(vt + tq * D + gq * (4 * NWD), v0);
+            load_words<NWD>(vt + (tq + 4) * D + gq * (4 * NWD), v1);
+            __syncwarp();  // the stage is in registers: its next tile may come
+            if (k + kNS < my_tiles) {
+                if (((k + kNS) & 31) == 0) fetch_ids(k + kNS);
+                if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                issue(k + kNS, it0 + k + kNS);
+            }
             if (valid < kTile) {  // rows past the end hold anything, NaN included
                 if (gq >= valid) {
                     x[0] = x[1] = -INFINITY;
@@ -295,8 +358,8 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
 #pragma unroll
             for (int wi = 0; wi < NWD; wi++) {
                 uint32_t c0[4], c1[4];
-                q4_centred(r.v0[wi], c0);
-                q4_centred(r.v1[wi], c1);
+                q4_centred(v0[wi], c0);
+                q4_centred(v1[wi], c1);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bh0, bh1);
@@ -305,7 +368,16 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
             }
         }
 
-        // ---- merge the warps through shared memory ----
+        it0 += my_tiles;
+        if (failed && tiles > 0) {
+            // copies still in flight land before the CTA exits (bounded)
+            if (lane == 0) atomicOr(p.err, kErrTimeout);
+            for (int k = done + 1; k < min(my_tiles, done + kNS); k++)
+                bar_wait(bars + 8 * ((it0 - my_tiles + k) % kNS), (uint32_t)(((it0 - my_tiles + k) / kNS) & 1));
+            m0 = m1 = -INFINITY;
+            l0 = l1 = z0 = z1 = 0.0f;
+        }
+        // ---- merge the warps through shared memory (over the rings) ----
         const float back = __uint_as_float((uint32_t)(E - 6) << 23);  // 1 / vmul
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
@@ -321,7 +393,7 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
                 if (NT == 1) o[mb][i] += __shfl_xor_sync(kFull, o[mb][i], 2);
                 o[mb][i] = fmaf(o[mb][i], back, i & 1 ? z1 : z0);
             }
-        __syncthreads();  // the last pass's readers are done
+        __syncthreads();  // every warp's tiles are consumed
         if (2 * tq < GP) {  // dims D / 8 gq + 2 mb (rows g) and + 1 (rows g + 8) of heads 2 tq, 2 tq + 1
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -363,11 +435,11 @@ __global__ void __launch_bounds__(kNW * 32) decode_q4_kernel(const __grid_consta
                 }
             }
         }
+        __syncthreads();  // before the next pass's copies overwrite the partial rows
     }
     pdl_trigger();
     if (p.counters && rm.n_split > 1) {
-        __syncthreads();
-        finish_split_row(p, item.row, h, item.split, rm.n_split, G, D, flag, mo, kNW * GP * D);
+        finish_split_row(p, item.row, h, item.split, rm.n_split, G, D, flag, mo, kRing / 4);
     }
 }
 
@@ -444,7 +516,13 @@ bool decode_q4_supported(int D, int G, int block_size) {
 
 template <int D, int NT>
 static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
-    constexpr int smem = (kNW * 4 * NT * (D + 2) + 4) * 4;
+    constexpr int smem = kNW * kNS * (2 * kTile * (D / 2 + 4) + 8) + 16;
+    static std::atomic<uint64_t> attr_set{0};  // per device
+    const int st = once_per_device(attr_set, [] {
+        S1KV_CUDA(cudaFuncSetAttribute(decode_q4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        return S1KV_OK;
+    });
+    if (st) return st;
     const dim3 grid((unsigned)p.n_items, (unsigned)p.Hkv);
     S1KV_CUDA(launch_pdl(decode_q4_kernel<D, NT>, grid, dim3(kNW * 32), smem, stream, p, G));
     g_launches++;
