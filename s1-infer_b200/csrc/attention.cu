@@ -579,9 +579,8 @@ bool tma_attention_supported(int dtype, int D, int G, int block_size) {
 }
 
 int tma_warps_per_cta(int dtype, int D) {
-    (void)dtype;
     (void)D;
-    return 4;
+    return dtype == S1KV_DTYPE_Q4 ? 8 : 4;  // (4-bit: 4 warps that take tiles in pairs)
 }
 
 template <typename T, int D, int G>

@@ -17,8 +17,10 @@
 // Layout: one 16-token tile of a KV head is 16 D / 2 + 64 bytes of K and as
 // many of V, contiguous, and the storage order is the fragments' own: a lane's
 // codes of the whole tile are two 16-byte reads of K and two of V (D = 128),
-// without bank conflicts.  Each warp brings its tiles with two bulk copies each
-// into a ring of its own in shared memory, kNS tiles ahead.
+// without bank conflicts.  Each warp brings pairs of tiles, two bulk copies a
+// tile, into a ring of its own in shared memory, kNS pairs ahead, and takes a
+// pair at a time: what a step costs besides the codes (waits, the maximum's
+// vote) is shared by 32 tokens.
 //   K: lane (g, t) = (L / 4, L % 4) takes dims 32 t .. 32 t + 31 of tokens g
 //      and g + 8.  The sum over dims does not care for their order, so q's
 //      fragments simply follow K's: nibbles n and n + 4 of a word are the
@@ -45,11 +47,11 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kNW = 4;
 constexpr int kTile = 16;
-constexpr int kMaxG = 128;             // query heads per KV head the merge's scratch covers (D = 64: 36 G of 4608 floats)
+constexpr int kMaxG = 128;             // query heads per KV head the merge's scratch covers (D = 64: 36 G of 6912 floats)
 constexpr float kRescaleAt = 8.0f;     // log2 units
 constexpr int kMinExp = 8;             // least exponent (biased) the V scales are taken relative to
 constexpr uint32_t kSpin = 1u << 22;
-constexpr int kNS = 4;                 // tiles in flight a warp
+constexpr int kNS = 3;                 // stages a warp, of two tiles each
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -122,7 +124,7 @@ __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[NWD]) {
 template <int D, int NT>
 __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_constant__ AttnParams p, int G) {
     constexpr int NWD = D / 32, KS = D / 16, GP = 4 * NT;
-    constexpr int kTileBytes = kTile * (D / 2 + 4), kParams = kTile * (D / 2), kStage = 2 * kTileBytes;
+    constexpr int kTileBytes = kTile * (D / 2 + 4), kParams = kTile * (D / 2), kStage = 4 * kTileBytes;
     constexpr int kRing = kNW * kNS * kStage;
     static_assert(kRing >= kNW * GP * (D + 2) * 4, "the warps' partial rows lie over the rings");
     extern __shared__ __align__(128) char smem[];
@@ -138,25 +140,32 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
     const int tok0 = item.split * p.split_tokens;
     const int tok1 = min(tok0 + p.split_tokens, item.kv_len);
     const int n_tiles = (tok1 - tok0 + kTile - 1) / kTile;
-    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kNW - 1) / kNW : 0;
+    const int n_pairs = (n_tiles + 1) / 2;  // this warp: pairs warp, warp + kNW ..
+    const int my_pairs = n_pairs > warp ? (n_pairs - warp + kNW - 1) / kNW : 0;
     const int32_t* tab = p.table + (int64_t)item.table_row * p.max_bps + (tok0 >> 4);
 
     int32_t my_blk = 0;
-    auto fetch_ids = [&](int k) {  // block ids of this warp's tiles k .. k + 31, one a lane
-        my_blk = 0;
-        if (k + lane < my_tiles) {
-            my_blk = tab[warp + (k + lane) * kNW];
+    auto fetch_ids = [&](int k) {  // block ids of this warp's pairs k .. k + 15, two a pair (-1: no second tile)
+        const int tile = 2 * (warp + (k + (lane >> 1)) * kNW) + (lane & 1);
+        my_blk = -1;
+        if (tile < n_tiles) {
+            my_blk = tab[tile];
             if ((uint32_t)my_blk >= (uint32_t)p.max_blocks) {
                 atomicOr(p.err, kErrBounds);
                 my_blk = 0;
             }
         }
     };
-    auto issue = [&](int k, int it) {  // tile k of this warp into the stage of copy `it`
-        const int64_t off = ((int64_t)__shfl_sync(kFull, my_blk, k & 31) * p.Hkv + h) * kTileBytes;
-        if (lane == 0) {
-            const uint32_t b = bars + (it % kNS) * 8, dst = su32(ring) + (it % kNS) * kStage;
-            bar_expect(b, kStage);
+    auto issue = [&](int k, int it) {  // pair k of this warp into the stage of copy `it`
+        // lanes 0 and 1 bring the pair's first and second tile
+        const int32_t blk = __shfl_sync(kFull, my_blk, 2 * (k & 15) + (lane & 1));
+        const bool both = __shfl_sync(kFull, blk, 1) >= 0;
+        const uint32_t b = bars + (it % kNS) * 8;
+        if (lane == 0) bar_expect(b, both ? kStage : kStage / 2);
+        __syncwarp();
+        if (lane < 2 && blk >= 0) {
+            const int64_t off = ((int64_t)blk * p.Hkv + h) * kTileBytes;
+            const uint32_t dst = su32(ring) + (it % kNS) * kStage + lane * 2 * kTileBytes;
             bulk_copy(dst, reinterpret_cast<const char*>(p.kbase) + off, kTileBytes, b);
             bulk_copy(dst + kTileBytes, reinterpret_cast<const char*>(p.vbase) + off, kTileBytes, b);
         }
@@ -170,10 +179,10 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
     // Tiles that lie below the tokens this batch appends are requested before
     // the wait for the previous kernel: nothing that may still run writes them
     // (split_k_attention states why).
-    const int n_first = min(kNS, my_tiles);
+    const int n_first = min(kNS, my_pairs);
     int pre = 0;
     if (p.prewait)
-        while (pre < n_first && tok0 + (warp + pre * kNW) * kTile + kTile <= item.kv_len - p.prewait_margin) pre++;
+        while (pre < n_first && tok0 + (warp + pre * kNW + 1) * 2 * kTile <= item.kv_len - p.prewait_margin) pre++;
     for (int k = 0; k < pre; k++) issue(k, k);
     pdl_wait();
     const RowMeta rm = p.rows[item.row];
@@ -181,9 +190,9 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
     int it0 = 0;  // copies consumed by earlier passes
 
     for (int g0 = 0; g0 < G; g0 += GP) {
-        const int tiles = failed ? 0 : my_tiles;  // (the CTA's warps stay together whatever happens)
+        const int pairs = failed ? 0 : my_pairs;  // (the CTA's warps stay together whatever happens)
         if (g0 > 0) fetch_ids(0);
-        for (int k = g0 > 0 ? 0 : pre; k < min(n_first, tiles); k++) issue(k, it0 + k);
+        for (int k = g0 > 0 ? 0 : pre; k < min(n_first, pairs); k++) issue(k, it0 + k);
         // q's fragments: column c of the N side is head g0 + c (NT = 2), or
         // head g0 + c % 4 with the high part in columns 0-3 and the low part
         // in 4-7 (NT = 1).  This lane's column and dims 8 NWD tq .. are one
@@ -237,80 +246,76 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
         float o[KS][4];
 #pragma unroll
         for (int mb = 0; mb < KS; mb++) o[mb][0] = o[mb][1] = o[mb][2] = o[mb][3] = 0.0f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, z0 = 0.0f, z1 = 0.0f;
+        // heads 2 tq, 2 tq + 1: reference max (log2 units, the same in the 8
+        // lanes of a head), this lane's share of sum(p) and sum(p m_v)
+        float m0 = -INFINITY, m1 = -INFINITY;
+        float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
+        const float2 un2 = make_float2(unscale, unscale), qs2 = make_float2(qs0, qs1), off2 = make_float2(-8.0f * qs0, -8.0f * qs1);
+        const float2 low = NT == 1 ? (tq < 2 ? make_float2(0.f, 0.f) : make_float2(-1.f, -1.f)) : make_float2(-1.f, -1.f);
         int E = kMinExp;  // V scales are taken relative to 2^(E - 127)
         float vmul = __uint_as_float((uint32_t)(260 - E) << 23);  // 2^(133 - E): the largest scaled s_v in [2^6, 2^7)
-
         int done = 0;
-        for (int k = 0; k < tiles; k++) {
-            const int stage = (it0 + k) % kNS;
-            if (!bar_wait(bars + 8 * stage, (uint32_t)(((it0 + k) / kNS) & 1))) {
+        for (int k = 0; k < pairs; k++) {
+            const int it = it0 + k, stage = it % kNS;
+            if (!bar_wait(bars + 8 * stage, (uint32_t)((it / kNS) & 1))) {
                 failed = true;
                 break;
             }
             done = k + 1;
-            const char *kt = ring + stage * kStage, *vt = kt + kTileBytes;
-            const int valid = min(kTile, tok1 - (tok0 + (warp + k * kNW) * kTile));
-            uint32_t k0[NWD], k1[NWD], v0[NWD], v1[NWD];
-            load_words<NWD>(kt + gq * (D / 2) + tq * (4 * NWD), k0);
-            load_words<NWD>(kt + (gq + 8) * (D / 2) + tq * (4 * NWD), k1);
+            const char* kt = ring + stage * kStage;
+            const int rest = tok1 - (tok0 + (warp + k * kNW) * 2 * kTile);  // tokens of the pair: 32, fewer at the end
 
-            // ---- scores: M = the 16 tokens, N = the 8 columns ----
-            float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+            // ---- scores: M = the 16 tokens of a tile, N = the 8 columns ----
+            float2 x[2][2], va[2], vb[2];  // [tile][token gq, gq + 8] of heads (2 tq, 2 tq + 1); (s_v, m_v) of the tokens
 #pragma unroll
-            for (int wi = 0; wi < NWD; wi++)
+            for (int u = 0; u < 2; u++) {
+                const char* at = kt + u * 2 * kTileBytes;
+                uint32_t k0[NWD], k1[NWD];
+                load_words<NWD>(at + gq * (D / 2) + tq * (4 * NWD), k0);
+                load_words<NWD>(at + (gq + 8) * (D / 2) + tq * (4 * NWD), k1);
+                const uint32_t* kp = reinterpret_cast<const uint32_t*>(at + kParams) + gq;
+                const uint32_t* vp = reinterpret_cast<const uint32_t*>(at + kTileBytes + kParams) + gq;
+                const float2 ka = q4_unpack(kp[0]), kb = q4_unpack(kp[8]);
+                va[u] = q4_unpack(vp[0]);
+                vb[u] = q4_unpack(vp[8]);
+                float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const uint32_t a = k0[wi] >> (8 * j), b = k1[wi] >> (8 * j);
-                    const uint32_t a0 = a & 0x000F000Fu, a1 = b & 0x000F000Fu, a2 = a & 0x00F000F0u, a3 = b & 0x00F000F0u;
-                    const int ks = 2 * wi + j;
-                    if (NT == 1) {
-                        mma16816(j ? sb : sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
-                    } else {
-                        mma16816(sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
-                        mma16816(sb, a0, a1, a2, a3, qf[NT - 1][ks][0], qf[NT - 1][ks][1]);
+                for (int wi = 0; wi < NWD; wi++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t a = k0[wi] >> (8 * j), b = k1[wi] >> (8 * j);
+                        const uint32_t a0 = a & 0x000F000Fu, a1 = b & 0x000F000Fu, a2 = a & 0x00F000F0u, a3 = b & 0x00F000F0u;
+                        const int ks = 2 * wi + j;
+                        if (NT == 1) {
+                            mma16816(j ? sb : sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
+                        } else {
+                            mma16816(sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
+                            mma16816(sb, a0, a1, a2, a3, qf[NT - 1][ks][0], qf[NT - 1][ks][1]);
+                        }
                     }
+                float2 s0 = __fadd2_rn(make_float2(sa[0], sa[1]), make_float2(sb[0], sb[1]));
+                float2 s1 = __fadd2_rn(make_float2(sa[2], sa[3]), make_float2(sb[2], sb[3]));
+                if (NT == 1) {  // high + low part of q
+                    s0 = __fadd2_rn(s0, make_float2(__shfl_xor_sync(kFull, s0.x, 2), __shfl_xor_sync(kFull, s0.y, 2)));
+                    s1 = __fadd2_rn(s1, make_float2(__shfl_xor_sync(kFull, s1.x, 2), __shfl_xor_sync(kFull, s1.y, 2)));
                 }
-            float x[4];
+                // s (q . u - 8 sum(q)) + m sum(q)
+                x[u][0] = __ffma2_rn(make_float2(ka.x, ka.x), __ffma2_rn(s0, un2, off2), __fmul2_rn(make_float2(ka.y, ka.y), qs2));
+                x[u][1] = __ffma2_rn(make_float2(kb.x, kb.x), __ffma2_rn(s1, un2, off2), __fmul2_rn(make_float2(kb.y, kb.y), qs2));
+            }
+            if (rest < 2 * kTile) {  // rows past the end hold anything, NaN included
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[i] = sa[i] + sb[i];
-                if (NT == 1) x[i] += __shfl_xor_sync(kFull, x[i], 2);  // high + low part of q
-            }
-            // this lane: tokens gq (x[0], x[1]) and gq + 8 (x[2], x[3]) of its two heads
-            const uint32_t* kp = reinterpret_cast<const uint32_t*>(kt + kParams);
-            const uint32_t* vp = reinterpret_cast<const uint32_t*>(vt + kParams);
-            const float2 ka = q4_unpack(kp[gq]), kb = q4_unpack(kp[gq + 8]);
-            const float sk0 = ka.x * unscale, sk1 = kb.x * unscale;
-            const float zk0 = fmaf(-8.0f, ka.x, ka.y), zk1 = fmaf(-8.0f, kb.x, kb.y);
-            x[0] = fmaf(x[0], sk0, zk0 * qs0);
-            x[1] = fmaf(x[1], sk0, zk0 * qs1);
-            x[2] = fmaf(x[2], sk1, zk1 * qs0);
-            x[3] = fmaf(x[3], sk1, zk1 * qs1);
-            float2 va = q4_unpack(vp[gq]), vb = q4_unpack(vp[gq + 8]);
-            load_words<NWD>(vt + tq * D + gq * (4 * NWD), v0);
-            load_words<NWD>(vt + (tq + 4) * D + gq * (4 * NWD), v1);
-            __syncwarp();  // the stage is in registers: its next tile may come
-            if (k + kNS < my_tiles) {
-                if (((k + kNS) & 31) == 0) fetch_ids(k + kNS);
-                if (lane == 0) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                issue(k + kNS, it0 + k + kNS);
-            }
-            if (valid < kTile) {  // rows past the end hold anything, NaN included
-                if (gq >= valid) {
-                    x[0] = x[1] = -INFINITY;
-                    va = make_float2(0.0f, 0.0f);
-                }
-                if (gq + 8 >= valid) {
-                    x[2] = x[3] = -INFINITY;
-                    vb = make_float2(0.0f, 0.0f);
+                for (int u = 0; u < 2; u++) {
+                    if (16 * u + gq >= rest) x[u][0] = make_float2(-INFINITY, -INFINITY), va[u] = make_float2(0.f, 0.f);
+                    if (16 * u + gq + 8 >= rest) x[u][1] = make_float2(-INFINITY, -INFINITY), vb[u] = make_float2(0.f, 0.f);
                 }
             }
             // the reference max of a head moves only when a score outgrows it
             // by 2^8, and E only when an s_v outgrows it: both are rare
-            float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
-            const int e = min((int)(__float_as_uint(fmaxf(va.x, vb.x)) >> 23), 254);
-            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || e > E)) {
+            float mx0 = fmaxf(fmaxf(x[0][0].x, x[0][1].x), fmaxf(x[1][0].x, x[1][1].x));
+            float mx1 = fmaxf(fmaxf(x[0][0].y, x[0][1].y), fmaxf(x[1][0].y, x[1][1].y));
+            const float sv = fmaxf(fmaxf(va[0].x, vb[0].x), fmaxf(va[1].x, vb[1].x));
+            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || (int)(__float_as_uint(sv) >> 23) > E)) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, off));
@@ -320,10 +325,9 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
                 float c0 = r0 ? ex2(m0 - mx0) : 1.0f, c1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
                 if (r0) m0 = mx0;
                 if (r1) m1 = mx1;
-                l0 *= c0;
-                l1 *= c1;
-                z0 *= c0;
-                z1 *= c1;
+                l2 = make_float2(l2.x * c0, l2.y * c1);
+                z2 = make_float2(z2.x * c0, z2.y * c1);
+                const int e = min((int)(__float_as_uint(sv) >> 23), 254);
                 const int ne = max(E, (int)__reduce_max_sync(kFull, (unsigned)e));
                 const float ce = ne - E > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (ne - E)) << 23);
                 E = ne;
@@ -338,45 +342,70 @@ __global__ void __launch_bounds__(kNW * 32, 4) decode_q4_kernel(const __grid_con
                     o[mb][3] *= c1;
                 }
             }
-            const float p0 = ex2(x[0] - m0), p1 = ex2(x[1] - m1), p2 = ex2(x[2] - m0), p3 = ex2(x[3] - m1);
-            l0 += p0 + p2;
-            l1 += p1 + p3;
-            z0 = fmaf(p0, va.y, fmaf(p2, vb.y, z0));
-            z1 = fmaf(p1, va.y, fmaf(p3, vb.y, z1));
-            const float w0 = va.x * vmul, w1 = vb.x * vmul;
-            uint32_t h0, h1, e0, e1;
-            split_h2(p0 * w0, p1 * w0, h0, e0);
-            split_h2(p2 * w1, p3 * w1, h1, e1);
-            uint32_t bh0, bh1, bl0 = 0, bl1 = 0;
-            if (NT == 1) {
-                bh0 = movt(tq < 2 ? h0 : e0);
-                bh1 = movt(tq < 2 ? h1 : e1);
-            } else {
-                bh0 = movt(h0), bh1 = movt(h1), bl0 = movt(e0), bl1 = movt(e1);
+            // p, then p s_v in two fp16 parts: rows of P^T, transposed in
+            // registers into the B fragments of O^T += V^T P^T.  NT = 1: lanes
+            // of columns 0-3 give the high part, of 4-7 the low part.
+            const float2 nm = make_float2(-m0, -m1);
+            auto weights = [&](float2 xs, float2 sm, uint32_t& first, uint32_t& second) {
+                const float2 y = __fadd2_rn(xs, nm), pr = make_float2(ex2(y.x), ex2(y.y));
+                l2 = __fadd2_rn(l2, pr);
+                z2 = __ffma2_rn(pr, make_float2(sm.y, sm.y), z2);
+                const float w = sm.x * vmul;
+                const float2 ps = __fmul2_rn(pr, make_float2(w, w));
+                const __half2 hi = __floats2half2_rn(ps.x, ps.y);
+                const float2 r = __ffma2_rn(__half22float2(hi), low, ps);  // NT = 1, columns 0-3: ps itself
+                second = pack_h2(r.x, r.y);
+                first = *reinterpret_cast<const uint32_t*>(&hi);
+            };
+            uint32_t b0[2][2], b1[2][2];  // [tile][high, low (NT = 2)]: tokens 2 tq .. and 2 tq + 8 ..
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                uint32_t h0, e0, h1, e1;
+                weights(x[u][0], va[u], h0, e0);
+                weights(x[u][1], vb[u], h1, e1);
+                if (NT == 1) {
+                    b0[u][0] = movt(e0), b1[u][0] = movt(e1);
+                } else {
+                    b0[u][0] = movt(h0), b1[u][0] = movt(h1);
+                    b0[u][1] = movt(e0), b1[u][1] = movt(e1);
+                }
             }
             // ---- O^T += V^T P^T: M = 16 dims per m-block, K = the 16 tokens ----
 #pragma unroll
-            for (int wi = 0; wi < NWD; wi++) {
-                uint32_t c0[4], c1[4];
-                q4_centred(v0[wi], c0);
-                q4_centred(v1[wi], c1);
+            for (int u = 0; u < 2; u++) {
+                const char* at = kt + u * 2 * kTileBytes + kTileBytes;
+                uint32_t v0[NWD], v1[NWD];
+                load_words<NWD>(at + tq * D + gq * (4 * NWD), v0);
+                load_words<NWD>(at + (tq + 4) * D + gq * (4 * NWD), v1);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bh0, bh1);
-                    if (NT == 2) mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], bl0, bl1);
+                for (int wi = 0; wi < NWD; wi++) {
+                    uint32_t c0[4], c1[4];
+                    q4_centred(v0[wi], c0);
+                    q4_centred(v1[wi], c1);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], b0[u][0], b1[u][0]);
+                        if (NT == 2) mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], b0[u][1], b1[u][1]);
+                    }
                 }
+            }
+            __syncwarp();  // the stage is read: its next pair may come
+            if (k + kNS < pairs) {
+                if (((k + kNS) & 15) == 0) fetch_ids(k + kNS);
+                if (lane < 2) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                issue(k + kNS, it + kNS);
             }
         }
 
-        it0 += my_tiles;
-        if (failed && tiles > 0) {
+        if (failed && pairs > 0) {
             // copies still in flight land before the CTA exits (bounded)
             if (lane == 0) atomicOr(p.err, kErrTimeout);
-            for (int k = done + 1; k < min(my_tiles, done + kNS); k++)
-                bar_wait(bars + 8 * ((it0 - my_tiles + k) % kNS), (uint32_t)(((it0 - my_tiles + k) / kNS) & 1));
+            for (int k = done + 1; k < min(pairs, done + kNS); k++) bar_wait(bars + 8 * ((it0 + k) % kNS), (uint32_t)(((it0 + k) / kNS) & 1));
             m0 = m1 = -INFINITY;
-            l0 = l1 = z0 = z1 = 0.0f;
+            l2 = z2 = make_float2(0.f, 0.f);
         }
+        it0 += pairs;
+        float l0 = l2.x, l1 = l2.y, z0 = z2.x, z1 = z2.y;
         // ---- merge the warps through shared memory (over the rings) ----
         const float back = __uint_as_float((uint32_t)(E - 6) << 23);  // 1 / vmul
 #pragma unroll
@@ -516,7 +545,7 @@ bool decode_q4_supported(int D, int G, int block_size) {
 
 template <int D, int NT>
 static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
-    constexpr int smem = kNW * kNS * (2 * kTile * (D / 2 + 4) + 8) + 16;
+    constexpr int smem = kNW * kNS * (4 * kTile * (D / 2 + 4) + 8) + 16;
     static std::atomic<uint64_t> attr_set{0};  // per device
     const int st = once_per_device(attr_set, [] {
         S1KV_CUDA(cudaFuncSetAttribute(decode_q4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
