@@ -45,9 +45,15 @@ int check_layer(const s1kv_pool* p, int32_t layer) {
 // block ids per warp and look further ones up as they go), and no more than
 // kMaxSplitsPerRow splits of the longest row (the merge's counters and
 // groups are sized for that).
-int32_t plan_split_tiles(int64_t total_tiles, int64_t max_row_tiles, int32_t Hkv, int nw) {
+// 4-bit pools: a tile is a quarter of bf16's bytes, so what a CTA costs besides
+// its tiles weighs more.  About two CTAs an SM until a CTA has 32 tiles, then
+// longer splits only past the 8 waves: 33 rows of up to 2049 tokens, 4 KV heads
+// of 64, took 17.7 us at 8 waves and 11.1 at two CTAs an SM; 64 rows of up to
+// 8192, 8 KV heads of 128, 85.7 at 8 waves, 125 at two CTAs an SM.
+int32_t plan_split_tiles(int64_t total_tiles, int64_t max_row_tiles, int32_t Hkv, int nw, bool q4) {
     int64_t target = (int64_t)kSMs * 8;
     int64_t s = (total_tiles * Hkv + target - 1) / target;
+    if (q4) s = std::max<int64_t>(s, std::min<int64_t>(32, (total_tiles * Hkv + 2 * kSMs - 1) / (2 * kSMs)));
     s = std::max<int64_t>(s, nw);
     s = std::min<int64_t>(s, 32 * nw);
     s = std::max<int64_t>(s, (max_row_tiles + kMaxSplitsPerRow - 1) / kMaxSplitsPerRow);
@@ -66,7 +72,8 @@ void plan_items(const s1kv_pool* p, s1kv_batch* b) {
         total_tiles += (m.kv_len + bs - 1) / bs;
         max_row_tiles = std::max<int64_t>(max_row_tiles, (m.kv_len + bs - 1) / bs);
     }
-    b->split_tokens = plan_split_tiles(total_tiles, max_row_tiles, p->desc.num_kv_heads, nw) * 16;
+    b->split_tokens = plan_split_tiles(total_tiles, max_row_tiles, p->desc.num_kv_heads, nw,
+                                       p->desc.dtype == S1KV_DTYPE_Q4) * 16;
     std::vector<WorkItem>& items = b->items;
     items.clear();
     int64_t n_part = 0;
