@@ -163,4 +163,65 @@ __device__ __forceinline__ void q4_store_row(const float (&x)[NQ][4], int nq, ch
     if (lr == 0) *reinterpret_cast<uint32_t*>(tile + q4_param(t, bs, D)) = r.packed;
 }
 
+// The same for a row held by D / 16 adjacent lanes, 16 contiguous values
+// (four quads) a lane: a warp takes 512 / D rows, so the reductions and the
+// 64-bit arithmetic of the parameters serve that many rows at once (a row a
+// warp ran at a quarter of the speed).  Codes are made in packed fp32:
+// (x - m) / s + 8, rounded by adding 1.5 * 2^23; a row with a value within
+// 1e-4 of a tie is done again value by value.
+template <int LANES>
+__device__ __forceinline__ void q4_store_row16(const float (&x)[16], char* tile, int t, bool is_v, int bs, int D, bool store) {
+    const int lr = threadIdx.x % LANES;
+    float lo = x[0], hi = x[0];
+    float2 bad2 = make_float2(0.f, 0.f);  // 0, or NaN from a value that is not finite
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        lo = fminf(fminf(lo, x[i]), x[i + 1]);
+        hi = fmaxf(fmaxf(hi, x[i]), x[i + 1]);
+        bad2 = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(0.f, 0.f), bad2);
+    }
+    if (!(bad2.x + bad2.y == 0.0f)) hi = INFINITY;  // spoils the row's maximum, which then spoils the row
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const Q4Row r = q4_params(lo, hi, hi < INFINITY);
+    const float inv = __frcp_rn(r.s);
+    if (!store) return;
+    const float2 m2 = make_float2(-r.m, -r.m), inv2 = make_float2(inv, inv), eight = make_float2(8.f, 8.f);
+    const float kRound = 12582912.0f;  // 1.5 * 2^23
+    const float2 up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
+    float far = 0.0f;
+    uint32_t c[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        float u[4];
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const float2 v = __ffma2_rn(__fadd2_rn(make_float2(x[4 * q + e], x[4 * q + e + 1]), m2), inv2, eight);
+            const float2 n = __fadd2_rn(__fadd2_rn(v, up), down), d = __fadd2_rn(v, make_float2(-n.x, -n.y));
+            far = fmaxf(fmaxf(far, fabsf(d.x)), fabsf(d.y));
+            u[e] = n.x, u[e + 1] = n.y;
+        }
+        c[q] = (uint32_t)fmaf(4096.f, u[3], fmaf(256.f, u[2], fmaf(16.f, u[1], u[0])));
+    }
+    // (not finite where s is 0 or too small to invert, or the row is spoilt)
+    if (!(far < 0.4999f) || !(fabsf(inv) < INFINITY)) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            c[q] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) c[q] |= q4_code(x[4 * q + e], r, inv) << (4 * e);
+        }
+    }
+    if (is_v) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) *reinterpret_cast<uint16_t*>(tile + q4_v_quad(t, 4 * lr + q, D)) = (uint16_t)c[q];
+    } else {
+        *reinterpret_cast<uint2*>(tile + q4_k_quad(t, 4 * lr, D)) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    }
+    if (lr == 0) *reinterpret_cast<uint32_t*>(tile + q4_param(t, bs, D)) = r.packed;
+}
+
 }  // namespace s1kv

@@ -9,29 +9,31 @@ namespace s1kv {
 constexpr int kSMs = 148;
 
 // -------------------------------------------------------------- append ----
-// A row (one token and head of k, v or, rotated only, q) per LANES lanes,
-// one quad of values a lane: its extremes are two shuffle reductions, and
-// K's 64 code bytes of a row (D = 128) leave as one segment.  RoPE
-// (src/nn/RoPE.cpp:32-33: out1 = x1 c - x2 s, out2 = x2 c + x1 s, each
-// operation rounded on its own) reads its partner quad D / 2 away through
-// the L1 cache, before the quantisation.
-template <int LANES, int NQ, bool ROPE>
+// A row (one token and head of k, v or, rotated only, q) on LANES lanes.
+// LANES = D / 16 (D of 64, 128, 256): 16 contiguous values a lane.  LANES = 32,
+// any other D: two quads a lane, 128 values apart.  RoPE (src/nn/RoPE.cpp:32-33:
+// out1 = x1 c - x2 s, out2 = x2 c + x1 s, each operation rounded on its own)
+// reads its partner values D / 2 away through the L1 cache, before the
+// quantisation.  Bound by the fp32 rows read (8 bytes a K and V value pair
+// against 1 written).
+template <int LANES, bool ROPE>
 __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
     pdl_wait_trigger();
+    constexpr bool kWide = LANES < 32;               // 16 contiguous values
+    constexpr int NQ = kWide ? 4 : 2, RPW = 32 / LANES;
     const int D = p.D, half = D / 2, nq = D / 4;
-    constexpr int RPW = 32 / LANES;
     const int lane = threadIdx.x & 31, lr = lane % LANES;
-    const int64_t kv_rows = p.n * p.Hkv, q_rows = ROPE && p.q_in ? p.n * p.Hq : 0, total = 2 * kv_rows + q_rows;
-    const int64_t warp = blockIdx.x * (int64_t)(blockDim.x / 32) + threadIdx.x / 32, warps = (int64_t)gridDim.x * (blockDim.x / 32);
-    for (int64_t u0 = warp * RPW; u0 < total; u0 += warps * RPW) {  // warp-uniform (shuffles inside)
-        const int64_t u = u0 + lane / LANES;
+    const uint32_t kv_rows = (uint32_t)(p.n * p.Hkv), q_rows = ROPE && p.q_in ? (uint32_t)(p.n * p.Hq) : 0u;
+    const uint32_t total = 2 * kv_rows + q_rows;  // (launch_append_q4 keeps it below 2^31)
+    const uint32_t warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, warps = gridDim.x * (blockDim.x / 32);
+    for (uint32_t u0 = warp * RPW; u0 < total; u0 += warps * RPW) {  // warp-uniform (shuffles inside)
+        const uint32_t u = u0 + lane / LANES;
         const bool have = u < total;
         const int part = u < kv_rows ? 0 : u < 2 * kv_rows ? 1 : 2;  // K, V, Q
-        const int64_t th = part == 0 ? u : part == 1 ? u - kv_rows : u - 2 * kv_rows;
-        const int H = part == 2 ? p.Hq : p.Hkv;
-        const int64_t t = have ? th / H : 0;
+        const uint32_t th = !have ? 0u : part == 0 ? u : part == 1 ? u - kv_rows : u - 2 * kv_rows;
+        const uint32_t H = part == 2 ? p.Hq : p.Hkv, t = th / H;
         const int h = (int)(th - t * H);
-        const float* src = (part == 0 ? p.k : part == 1 ? p.v : p.q_in) + (have ? th : 0) * D;
+        const float* src = (part == 0 ? p.k : part == 1 ? p.v : p.q_in) + (int64_t)th * D;
         const bool rot = ROPE && part != 1;
         const int32_t pos = rot && have ? p.pos[t] : 0;
         bool ok = have;
@@ -39,24 +41,38 @@ __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
             if (lr == 0) atomicOr(p.err, kErrBounds);
             ok = false;
         }
-        float x[NQ][4];
+        float x[4 * NQ];
 #pragma unroll
         for (int i = 0; i < NQ; i++) {
-            const int quad = lr + i * LANES, d = 4 * quad;
-            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+            const int quad = kWide ? 4 * lr + i : lr + i * LANES, d = 4 * quad;
+            x[4 * i] = x[4 * i + 1] = x[4 * i + 2] = x[4 * i + 3] = 0.0f;
             if (quad >= nq || !ok) continue;
+            if (kWide) {  // 16-byte aligned (launch_append_q4)
+                const float4 f = *reinterpret_cast<const float4*>(src + d);
+                x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[i][e] = src[d + e];
+                for (int e = 0; e < 4; e++) x[4 * i + e] = src[d + e];
+            }
             if (rot) {
                 const bool first = d < half;
                 const float* other = src + (first ? d + half : d - half);
                 const float2* cs = p.rope + (int64_t)pos * half + (first ? d : d - half);
+                float o[4];
+                if (kWide) {
+                    const float4 f = *reinterpret_cast<const float4*>(other);
+                    o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 c = __ldg(cs + e);
-                    const float o = other[e];
-                    x[i][e] = first ? __fsub_rn(__fmul_rn(x[i][e], c.x), __fmul_rn(o, c.y))
-                                    : __fadd_rn(__fmul_rn(x[i][e], c.x), __fmul_rn(o, c.y));
+                    for (int e = 0; e < 4; e++) o[e] = other[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float4 c = __ldg(reinterpret_cast<const float4*>(cs + e));  // two (cos, sin)
+                    const float a0 = __fmul_rn(x[4 * i + e], c.x), b0 = __fmul_rn(o[e], c.y);
+                    const float a1 = __fmul_rn(x[4 * i + e + 1], c.z), b1 = __fmul_rn(o[e + 1], c.w);
+                    x[4 * i + e] = first ? __fsub_rn(a0, b0) : __fadd_rn(a0, b0);
+                    x[4 * i + e + 1] = first ? __fsub_rn(a1, b1) : __fadd_rn(a1, b1);
                 }
             }
         }
@@ -75,69 +91,105 @@ __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
         if (ok && part == 2)
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                const int quad = lr + i * LANES;
-                if (quad < nq)
+                const int quad = kWide ? 4 * lr + i : lr + i * LANES;
+                if (quad >= nq) continue;
+                float* dst = p.q_out + (int64_t)th * D + 4 * quad;
+                if (kWide) *reinterpret_cast<float4*>(dst) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                else
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p.q_out[th * D + 4 * quad + e] = x[i][e];
+                    for (int e = 0; e < 4; e++) dst[e] = x[4 * i + e];
             }
-        q4_store_row<LANES, NQ>(x, nq, tile, tt, part == 1, p.block_size, D, store);
+        if constexpr (kWide) {
+            q4_store_row16<LANES>(x, tile, tt, part == 1, p.block_size, D, store);
+        } else {
+            const float y[2][4] = {{x[0], x[1], x[2], x[3]}, {x[4], x[5], x[6], x[7]}};
+            q4_store_row<32, 2>(y, nq, tile, tt, part == 1, p.block_size, D, store);
+        }
     }
 }
 
-int launch_append_q4(const AppendParams& p, bool rope, cudaStream_t stream, bool pdl) {
-    if (p.n <= 0) return S1KV_OK;
-    const int64_t rows = 2 * p.n * p.Hkv + (rope && p.q_in ? p.n * p.Hq : 0);
-    const int rpw = p.D == 64 ? 2 : 1;
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((rows + 8 * rpw - 1) / (8 * rpw), kSMs * 16));
-#define S1KV_APPEND(L, N, R)                                                                            \
-    do {                                                                                               \
-        if (pdl) S1KV_CUDA(launch_pdl(append_q4_kernel<L, N, R>, dim3(grid), dim3(256), 0, stream, p)); \
-        else append_q4_kernel<L, N, R><<<grid, 256, 0, stream>>>(p);                                   \
+int launch_append_q4(const AppendParams& all, bool rope, cudaStream_t stream, bool pdl) {
+    // row numbers in 32 bits: a call of more than 2^31 rows goes in pieces
+    const int64_t per = 2 * (int64_t)all.Hkv + (rope && all.q_in ? all.Hq : 0), most = ((int64_t)1 << 30) / per;
+    const bool wide = (all.D == 64 || all.D == 128 || all.D == 256) &&
+                      ((((uintptr_t)all.k | (uintptr_t)all.v | (uintptr_t)(all.q_in ? all.q_in : all.k) |
+                         (uintptr_t)(all.q_in ? all.q_out : all.k)) & 15) == 0);
+    const int lanes = wide ? all.D / 16 : 32;
+    for (int64_t t0 = 0; t0 < all.n; t0 += most) {
+        AppendParams p = all;
+        p.n = std::min<int64_t>(most, all.n - t0);
+        p.k += t0 * p.Hkv * p.D;
+        p.v += t0 * p.Hkv * p.D;
+        if (p.q_in) p.q_in += t0 * p.Hq * p.D, p.q_out += t0 * p.Hq * p.D;
+        p.slots += t0;
+        if (p.pos) p.pos += t0;
+        const int64_t rows = p.n * per, per_cta = 8 * (32 / lanes);
+        const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((rows + per_cta - 1) / per_cta, kSMs * 16));
+#define S1KV_APPEND(L, R)                                                                            \
+    do {                                                                                             \
+        if (pdl) S1KV_CUDA(launch_pdl(append_q4_kernel<L, R>, dim3(grid), dim3(256), 0, stream, p)); \
+        else append_q4_kernel<L, R><<<grid, 256, 0, stream>>>(p);                                    \
     } while (0)
-#define S1KV_APPEND_R(R)                       \
-    do {                                       \
-        if (p.D == 64) S1KV_APPEND(16, 1, R);  \
-        else if (p.D <= 128) S1KV_APPEND(32, 1, R); \
-        else S1KV_APPEND(32, 2, R);            \
+#define S1KV_APPEND_R(R)                    \
+    do {                                    \
+        if (lanes == 4) S1KV_APPEND(4, R);  \
+        else if (lanes == 8) S1KV_APPEND(8, R);   \
+        else if (lanes == 16) S1KV_APPEND(16, R); \
+        else S1KV_APPEND(32, R);            \
     } while (0)
-    if (rope) S1KV_APPEND_R(true);
-    else S1KV_APPEND_R(false);
+        if (rope) S1KV_APPEND_R(true);
+        else S1KV_APPEND_R(false);
 #undef S1KV_APPEND_R
 #undef S1KV_APPEND
-    g_launches++;
-    S1KV_CUDA(cudaGetLastError());
+        g_launches++;
+        S1KV_CUDA(cudaGetLastError());
+    }
     return S1KV_OK;
 }
 
 // -------------------------------------------------------------- gather ----
-// One thread per quad: token i of a sequence (block-table row `trow`) or of
-// a batch (`slots`), widened to fp32.
-__global__ void gather_q4_kernel(const char* __restrict__ base, bool is_v, const int32_t* __restrict__ trow,
-                                 const int32_t* __restrict__ slots, int64_t n, int bs, int Hkv, int D, int64_t num_slots,
-                                 float* __restrict__ out, int* err) {
-    const int nq = D / 4;
-    const int64_t total = n * Hkv * nq;
-    for (int64_t u = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; u < total; u += (int64_t)gridDim.x * blockDim.x) {
-        const int quad = (int)(u % nq);
-        const int64_t th = u / nq, i = th / Hkv;
-        const int h = (int)(th - i * Hkv);
-        const int64_t slot = slots ? slots[i] : (int64_t)trow[i / bs] * bs + i % bs;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if ((uint64_t)slot >= (uint64_t)num_slots) {
-            atomicOr(err, kErrBounds);
-        } else {
-            int t;
-            const char* tile = q4_tile(const_cast<char*>(base), slot, h, Hkv, bs, D, &t);
-            const uint32_t c = *reinterpret_cast<const uint16_t*>(tile + (is_v ? q4_v_quad(t, quad, D) : q4_k_quad(t, quad, D)));
-            const float2 sm = q4_unpack(*reinterpret_cast<const uint32_t*>(tile + q4_param(t, bs, D)));
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = q4_value((c >> (4 * e)) & 15u, sm.x, sm.y);
+// Token i of a sequence (block-table row `trow`) or of a batch (`slots`), widened
+// to fp32: a warp a (token, head) row, one quad a lane at a time, several rows
+// in turn; the row's place is worked out once for its lanes.
+__global__ void __launch_bounds__(256) gather_q4_kernel(const char* __restrict__ base, bool is_v, const int32_t* __restrict__ trow,
+                                                        const int32_t* __restrict__ slots, uint32_t n_rows, uint32_t row0, int bs,
+                                                        int Hkv, int D, int64_t num_slots, float* __restrict__ out, int* err) {
+    const int nq = D / 4, lane = threadIdx.x & 31;
+    const uint32_t warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, warps = gridDim.x * (blockDim.x / 32);
+    const bool vec = ((uintptr_t)out & 15) == 0;
+    for (uint32_t r0 = warp * 4; r0 < n_rows; r0 += warps * 4) {
+        // lane j < 4 looks row r0 + j up
+        int64_t off = -1;
+        int t = 0;
+        if (lane < 4 && r0 + lane < n_rows) {
+            const uint32_t th = row0 + r0 + lane, i = th / Hkv;
+            const int32_t slot = slots ? slots[i] : trow[i / bs] * bs + (int)(i % bs);
+            if ((uint64_t)slot >= (uint64_t)num_slots) {
+                atomicOr(err, kErrBounds);
+            } else {
+                const int32_t blk = slot / bs;
+                t = slot - blk * bs;
+                off = ((int64_t)blk * Hkv + (int)(th - i * Hkv)) * q4_tile_bytes(bs, D);
+            }
         }
-        if (((uintptr_t)out & 15) == 0)
-            *reinterpret_cast<float4*>(out + u * 4) = make_float4(v[0], v[1], v[2], v[3]);
-        else
 #pragma unroll
-            for (int e = 0; e < 4; e++) out[u * 4 + e] = v[e];
+        for (int j = 0; j < 4; j++) {
+            const int64_t at = __shfl_sync(0xffffffffu, off, j);
+            const int tt = __shfl_sync(0xffffffffu, t, j);
+            if (r0 + j >= n_rows) break;
+            const char* tile = base + at;
+            float2 sm = make_float2(0.0f, 0.0f);
+            if (at >= 0) sm = q4_unpack(*reinterpret_cast<const uint32_t*>(tile + q4_param(tt, bs, D)));
+            for (int quad = lane; quad < nq; quad += 32) {
+                uint32_t c = 0x8888u;  // zeros where the slot is out of range
+                if (at >= 0) c = *reinterpret_cast<const uint16_t*>(tile + (is_v ? q4_v_quad(tt, quad, D) : q4_k_quad(tt, quad, D)));
+                const float4 v = make_float4(q4_value(c & 15u, sm.x, sm.y), q4_value((c >> 4) & 15u, sm.x, sm.y),
+                                             q4_value((c >> 8) & 15u, sm.x, sm.y), q4_value(c >> 12, sm.x, sm.y));
+                float* dst = out + (int64_t)(r0 + j) * D + 4 * quad;
+                if (vec) __stcs(reinterpret_cast<float4*>(dst), v);
+                else dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
+            }
+        }
     }
 }
 
@@ -145,12 +197,17 @@ int launch_gather_q4(s1kv_pool* p, int32_t layer, const int32_t* trow, const int
                      float* out, cudaStream_t stream) {
     if (n <= 0) return S1KV_OK;
     const char* base = (which ? p->v : p->k) + (size_t)layer * p->layer_bytes;
-    const int64_t total = n * p->desc.num_kv_heads * (p->desc.head_dim / 4);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((total + 255) / 256, kSMs * 16));
-    gather_q4_kernel<<<grid, 256, 0, stream>>>(base, which != 0, trow, slots, n, p->desc.block_size, p->desc.num_kv_heads,
-                                               p->desc.head_dim, p->num_slots, out, p->d_err);
-    g_launches++;
-    S1KV_CUDA(cudaGetLastError());
+    const int64_t rows = n * p->desc.num_kv_heads;
+    if (rows > UINT32_MAX) return set_error(S1KV_EINVAL, "gather: more than 2^32 rows");
+    for (int64_t r0 = 0; r0 < rows; r0 += (int64_t)1 << 30) {
+        const uint32_t part = (uint32_t)std::min<int64_t>((int64_t)1 << 30, rows - r0);
+        const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)part + 31) / 32, kSMs * 16));
+        gather_q4_kernel<<<grid, 256, 0, stream>>>(base, which != 0, trow, slots, part, (uint32_t)r0, p->desc.block_size,
+                                                   p->desc.num_kv_heads, p->desc.head_dim, p->num_slots,
+                                                   out + r0 * p->desc.head_dim, p->d_err);
+        g_launches++;
+        S1KV_CUDA(cudaGetLastError());
+    }
     return S1KV_OK;
 }
 
