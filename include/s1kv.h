@@ -491,7 +491,7 @@ int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t
  * multiplied with up to 4 weights [N[i]][K rounded up to a multiple of 16].
  * The codes and scales go to `workspace` (device, 16-byte aligned, at least
  * s1kv_w8a8_workspace(M, K) bytes, borrowed until the stream work completes);
- * for one or two tokens a single kernel does it all. */
+ * a single token may take one kernel for it all. */
 int64_t s1kv_w8a8_workspace(int64_t M, int64_t K);
 int s1kv_linear_w8a8_group(const float* x, int64_t M, int64_t K, void* workspace, int64_t workspace_bytes,
                            int32_t n_mats, const int8_t* const* w, const float* const* w_scales, const int64_t* N,

@@ -124,7 +124,7 @@ int launch_quantize(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq
 }
 
 // ---------------------------------------------- few tokens: weight stream --
-// Up to 8 NTILE tokens (NTILE = 1 or 2): bound by the N K bytes of the
+// Up to 8 NTILE tokens (NTILE = 1, 2 or 4): bound by the N K bytes of the
 // weights.  mma.sync m16n8k32 on int8 with the channels on the 16-row side
 // and the tokens on the 8-column side.  The sum over k does not care for the
 // order of k, so a lane's fragments are simply 16 adjacent bytes of its
@@ -134,12 +134,14 @@ int launch_quantize(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq
 // integer sums meet in shared memory.  The first steps' weights are
 // requested before the wait for the previous kernel (the token quantiser):
 // they do not depend on it.
-// FUSED (one or two tokens of up to kFusedK values): each CTA quantises the
-// tokens itself, from x through L2 into its shared memory, while its first
-// weights are on their way: one launch instead of two.
-constexpr int kFusedK = 16384, kFusedM = 2;
+// FUSED (one token of up to kFusedK values): each CTA quantises the token
+// itself, from x through L2 into its shared memory, while its first weights
+// are on their way: one launch instead of two.
+// Three CTAs an SM with two steps in flight a warp stream better than two with
+// four (8 tokens, K = 4096, 6144 channels: 7.8 against 11.0 us, 3.3 TB/s).
+constexpr int kFusedK = 4096, kFusedM = 1;
 constexpr int kGemvWarps = 8;
-constexpr int kGemvPre = 4;  // 128-byte steps in flight a warp
+constexpr int kGemvPre = 2;  // 128-byte steps in flight a warp
 
 __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -150,7 +152,7 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
 }
 
 template <int NTILE, bool FUSED>
-__global__ void __launch_bounds__(kGemvWarps * 32)
+__global__ void __launch_bounds__(kGemvWarps * 32, 3)
     w8a8_gemv_kernel(const float* __restrict__ x, int x_len, const int8_t* __restrict__ xq, const float* __restrict__ sx, int M,
                      int K, const __grid_constant__ W8Group grp) {
     extern __shared__ uint4 own[];  // FUSED: the tokens' codes, K bytes each
@@ -642,27 +644,34 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
     return S1KV_OK;
 }
 
-// Which kernel, by the tokens: up to 16 the weight stream; above, the
-// tensor-core tiles with the least NT that holds the tokens (256 at most),
-// and K split over a cluster while the tiles do not fill the 148 SMs.
+// Which kernel, by the tokens: up to 32 the weight stream (32 tokens, K = 4096,
+// 6144 channels: 13.8 us against 14.6 in tiles; 16: 9.3 us); above, the
+// tensor-core tiles.  NT is the least that holds the tokens (256 at most),
+// halved down to 64 while the tiles leave SMs without work, and K is split
+// over a cluster while the tiles still do not fill them (two CTAs an SM fit
+// for NT up to 64).
 // x (optional, rows of x_len values): the tokens that xq and sx will hold; they
 // are quantised here first, or by the weight stream itself.
 int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
-    const int rows = M <= 16 || K == 0 ? 16 : kCh;
+    const int rows = M <= 32 || K == 0 ? 16 : kCh;
     int64_t tiles = 0;
     for (int i = 0; i < grp.n; i++) {
         grp.m[i].tile0 = (int)tiles;
         tiles += (grp.m[i].N + rows - 1) / rows;
     }
-    const int NT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    int NT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    while (NT > 64 && tiles * ((M + NT - 1) / NT) < 111) NT /= 2;
     if (tiles * ((M + NT - 1) / NT) > INT32_MAX) return set_error(S1KV_EINVAL, "matmul_w8a8: more than 2^31 tiles");
     if (K == 0) {  // empty sums
         for (int i = 0; i < grp.n; i++)
             S1KV_CUDA(cudaMemsetAsync(grp.m[i].out, 0, sizeof(float) * (size_t)M * grp.m[i].N, stream));
         return S1KV_OK;
     }
-    // 32 KB of codes at most: within the static limit with the 5 KB of sums
-    if (x && M <= kFusedM && K <= kFusedK && x_len % 4 == 0 && ((uintptr_t)x & 15) == 0)
+    // One token: a kernel of its own for the codes costs more than making them
+    // in every CTA as long as all CTAs are resident at once (K = 1024, 4096
+    // channels: 2.6 against 3.3 us; K = 4096, 6144 channels: 7.2 against 7.4;
+    // 14336 channels: 15.6 against 14.8).
+    if (x && M <= kFusedM && K <= kFusedK && tiles <= 3 * 148 && x_len % 4 == 0 && ((uintptr_t)x & 15) == 0)
         return launch_gemv<1, true>(x, x_len, nullptr, nullptr, M, K, grp, (int)tiles, stream);
     if (x) {
         const int st = launch_quantize(x, M, x_len, xq, K, sx, stream);
@@ -670,10 +679,11 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
     }
     if (M <= 8) return launch_gemv<1, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     if (M <= 16) return launch_gemv<2, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 32) return launch_gemv<4, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
     int cs = 1;
     if (NT <= 128)
-        while (cs < 8 && tiles * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
+        while (cs < 8 && tiles * ((M + NT - 1) / NT) * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
 #define S1KV_TC(NT_)                                                                                       \
     if (NT == NT_)                                                                                         \
         return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, stream)                     \

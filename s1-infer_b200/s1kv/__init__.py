@@ -642,10 +642,12 @@ class ChannelQuantizedTensor:
         self.data, self.scales = data, scales
         self.n, self.ld = data.shape
         self.k = self.ld if k is None else int(k)
+        self.device = data.get_device()  # CUDA device index
         if self.ld != (self.k + 15) // 16 * 16 or not data.is_contiguous() or not scales.is_contiguous():
             raise S1KVError(EINVAL, "ChannelQuantizedTensor: contiguous rows of K rounded up to a multiple of 16 bytes")
-        if data.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != (self.n,) or scales.device != data.device:
-            raise S1KVError(EINVAL, "ChannelQuantizedTensor: int8 [N, K16] data and float32 [N] scales on one device")
+        if (data.dtype is not torch.int8 or scales.dtype is not torch.float32 or scales.shape != (self.n,) or
+                self.device < 0 or scales.get_device() != self.device):
+            raise S1KVError(EINVAL, "ChannelQuantizedTensor: int8 [N, K16] data and float32 [N] scales on one GPU")
 
 
 def quantize_channels(t, device=None):
@@ -684,36 +686,34 @@ def matmul_w8a8_group(x, ws, outs=None):
     ChannelQuantizedTensor weights of the same K in one launch (q/k/v,
     gate/up) -> list of [M, N] fp32.  Summed exactly in 32-bit integers."""
     import torch
-    dev, n = ws[0].data.device, len(ws)
-    if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.device == dev and x.is_contiguous()):
-        x = _cuda_f32(x, dev.index)
+    n, dev, ld = len(ws), ws[0].device, ws[0].ld
+    if not (isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.get_device() == dev and x.is_contiguous()):
+        x = _cuda_f32(x, dev)
     if x.dim() != 2:
         raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K]")
     m, k = x.shape
     for w in ws:
-        if w.k != k or w.data.device != dev:
+        if w.k != k or w.device != dev:
             raise S1KVError(EINVAL, "matmul_w8a8_group: x must be [M, K] with K the weights' and all on one device")
     if outs is None:
         outs = [x.new_empty((m, w.n)) for w in ws]
-    elif len(outs) != n or any(o.shape != (m, w.n) or o.dtype != torch.float32 or not o.is_contiguous() or o.device != dev
-                               for o, w in zip(outs, ws)):
-        raise S1KVError(EINVAL, "matmul_w8a8_group: outs must be contiguous float32 [M, N] on x's device")
-    L = lib()
-    size = L.s1kv_w8a8_workspace(m, k)
-    space = x.new_empty((size,), dtype=torch.int8)
+    else:
+        if len(outs) != n:
+            raise S1KVError(EINVAL, "matmul_w8a8_group: one out for each weight")
+        for o, w in zip(outs, ws):
+            if o.shape != (m, w.n) or o.dtype is not torch.float32 or not o.is_contiguous() or o.get_device() != dev:
+                raise S1KVError(EINVAL, "matmul_w8a8_group: outs must be contiguous float32 [M, N] on x's device")
+    size = m * ld + (4 * m + 15) // 16 * 16  # s1kv_w8a8_workspace
+    space = x.new_empty((size // 4,))
     args = (i64 * (4 * n))(*[w.data.data_ptr() for w in ws], *[w.scales.data_ptr() for w in ws], *[w.n for w in ws],
                            *[o.data_ptr() for o in outs])
     at = C.addressof(args)
-
-    def call():
-        check(L.s1kv_linear_w8a8_group(x.data_ptr(), m, k, space.data_ptr(), size, n, at, at + 8 * n, at + 16 * n, at + 24 * n,
-                                       _stream(dev.index)))
-
-    if dev.index == torch.cuda.current_device():
-        call()
+    call = (x.data_ptr(), m, k, space.data_ptr(), size, n, at, at + 8 * n, at + 16 * n, at + 24 * n, _stream(dev))
+    if dev == torch.cuda.current_device():
+        check(lib().s1kv_linear_w8a8_group(*call))
     else:
         with torch.cuda.device(dev):
-            call()
+            check(lib().s1kv_linear_w8a8_group(*call))
     return outs
 
 
