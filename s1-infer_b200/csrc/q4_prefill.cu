@@ -220,11 +220,14 @@ __device__ __forceinline__ void regs_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-// A softmax thread's state: half of each tile's tokens of a row.  un: scores are in units of 1 / un (q was scaled
-// by a power of two); qs: sum of the scaled q.
+// A softmax thread's state: half of each tile's tokens of a row.  un: scores
+// are in units of 1 / un (q was scaled by a power of two); qs: sum of the
+// scaled q.
 struct RowState {
-    float m, l, z, un, qs;  // l and z: of this thread's tokens
+    float m;
+    float2 l, z;  // of this thread's even and odd tokens
     int E;
+    float un, qs;
 };
 // The parameters of a tile's rows.
 struct TilePar {
@@ -235,88 +238,51 @@ struct TilePar {
     int pad[3];
 };
 
+// 2^(m' - m): from what refers to m' to m; reference maxima are whole numbers.
+__device__ __forceinline__ float from_max(float m_old, float m) {
+    return m_old == m ? 1.0f : m - m_old < 127.0f ? pow2((int)(m_old - m)) : 0.0f;  // (0 from m' = -inf)
+}
 // 2^(m' - m) 2^(E' - E): from sums that refer to (m', E') to (m, E).
 __device__ __forceinline__ float rebase(float m_old, int e_old, float m, int e) {
-    const float c = m_old == m ? 1.0f : ex2(m_old - m);  // 0 from m' = -inf
-    return e - e_old > 126 ? 0.0f : c * __uint_as_float((uint32_t)(127 - (e - e_old)) << 23);
+    return e - e_old > 126 ? 0.0f : from_max(m_old, m) * pow2(e_old - e);
+}
+
+// The first `cols` columns of this thread's P times a power of two (exact but
+// for subnormals): its reference max rose after they were stored.
+__device__ __forceinline__ void scale_p(uint32_t tS, int cols, float f) {
+    tmem_st_wait();
+    const __half2 f2 = __float2half2_rn(f);
+#pragma unroll 1
+    for (int c = 0; c < cols; c += 16) {
+        float w[16];
+        tmem_ld16(tS + c, w);
+        tmem_ld_wait16(w);
+        uint32_t y[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) y[i] = mul_h2(__float_as_uint(w[i]), f2);
+        tmem_st16(tS + c, y);
+    }
 }
 
 // Half a tile's scores of one row (64 tokens from token t0) -> P over them: of
-// each 16 columns the first 8 take the high parts of p, the others the low
-// parts.  Two passes over the columns, 16 at a time with the next 16 on their
-// way: the maximum (exchanged with the row's other thread), then the weights
-// (adding m_k sum(q) anew costs less than storing the scores back, a round
-// trip to TMEM).  The loops stay rolled: unrolled over all scores the code
-// runs from beyond the instruction cache.  EDGE: only tokens up to `last` (of
-// this tile) are seen; the others may hold anything, NaN included.  fresh: O
-// starts anew with this tile.
+// each 16 columns the first 8 take the high parts of p s_v, the others the low
+// parts.  One pass, 16 columns at a time with the next 16 on their way.  The
+// reference max (a whole number of log2 units) moves only when a score outgrows
+// it by 2^8, seldom after the first tile: then what this tile has stored so far
+// is scaled; at the end the row's two threads agree on the larger reference.
+// (A pass of its own for the maximum, agreed on before the weights, took 2200
+// of 5400 cycles a tile.)  The loop stays rolled: unrolled over all scores the
+// code runs from beyond the instruction cache.  EDGE: only tokens up to `last`
+// (of this tile) are seen; the others may hold anything, NaN included.  fresh:
+// O starts anew with this tile.
 template <bool EDGE, int D>
 __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int t0, int last, RowState& st,
                                              bool fresh, float* xch, int xch_other, uint32_t pair, uint32_t phase,
                                              uint32_t p_full, uint32_t abort_flag, int lane) {
     float v[2][16];
-    float top = -INFINITY;
+    float m = st.m;
+    float2 l2 = st.l, z2 = st.z;
     tmem_ld16(tS, v[0]);
-#pragma unroll 1
-    for (int c = 0; c < 64; c += 32) {
-        const float f = par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f);
-        const float2 qs2 = make_float2(qs, qs);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int c0 = t0 + c + 16 * u;
-            tmem_ld_wait16(v[u]);
-            tmem_ld16(tS + ((c + 16 * u + 16) & 63), v[u ^ 1]);  // after the last, the first again for the second pass
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
-                float2 x = __ffma2_rn(make_float2(k.x, k.y), qs2, make_float2(v[u][i], v[u][i + 1]));
-                float2 y = __ffma2_rn(make_float2(k.z, k.w), qs2, make_float2(v[u][i + 2], v[u][i + 3]));
-                if (EDGE) {
-                    if (c0 + i > last) x.x = -INFINITY;
-                    if (c0 + i + 1 > last) x.y = -INFINITY;
-                    if (c0 + i + 2 > last) y.x = -INFINITY;
-                    if (c0 + i + 3 > last) y.y = -INFINITY;
-                }
-                mx[(i >> 1) & 2] = fmaxf(fmaxf(mx[(i >> 1) & 2], x.x), x.y);
-                mx[((i >> 1) & 2) + 1] = fmaxf(fmaxf(mx[((i >> 1) & 2) + 1], y.x), y.y);
-            }
-        }
-        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * (st.un * f));
-    }
-    *xch = top;
-    __syncwarp();
-    if (lane == 0) bar_arrive(pair);
-    if (!warp_wait(pair, phase, abort_flag)) return false;
-    top = fmaxf(top, xch[xch_other]);
-    const int e = par.E;
-    const bool raise = top > st.m + kRescaleAt || e > st.E;
-    float corr = 1.0f;
-    if (raise) {
-        const float m = top > st.m + kRescaleAt ? top : st.m;
-        const float c = m == st.m ? 1.0f : ex2(st.m - m);  // 0 on the first tile (m = -inf)
-        corr = rebase(st.m, st.E, m, e);
-        st.l *= c;
-        st.z *= c;
-        st.m = m;
-        st.E = e;
-    }
-    const bool rescale = !fresh && __any_sync(0xffffffffu, raise);
-    const float nm = st.m == -INFINITY ? 0.0f : -st.m;  // nothing visible yet: p = 0
-    const float2 nm2 = make_float2(nm, nm);
-    float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
-    if (rescale) {  // this thread's half of O's columns
-#pragma unroll 1
-        for (int c = 0; c < D / 2; c += 16) {
-            float ov[16];
-            tmem_ld16(tO + c, ov);
-            tmem_ld_wait16(ov);
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = __float_as_uint(ov[i] * corr);
-            tmem_st16(tO + c, w);
-        }
-    }
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
         const float f = par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f), un = st.un * f;
@@ -324,44 +290,92 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int c0 = t0 + c + 16 * u;
-            uint32_t hi[8], lo[8];
+            float2 x[8];
+            float top = -INFINITY;
             tmem_ld_wait16(v[u]);
             if (u == 0 || c == 0) tmem_ld16(tS + c + 16 * u + 16, v[u ^ 1]);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + i]);
-                const float4 mv = *reinterpret_cast<const float4*>(&par.mv[c0 + i]);
-                const float4 sv = *reinterpret_cast<const float4*>(&par.sv[c0 + i]);
+            for (int i = 0; i < 8; i += 2) {
+                const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + 2 * i]);
+                x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, make_float2(v[u][2 * i], v[u][2 * i + 1]));
+                x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, make_float2(v[u][2 * i + 2], v[u][2 * i + 3]));
+                if (EDGE) {
+                    if (c0 + 2 * i > last) x[i].x = -INFINITY;
+                    if (c0 + 2 * i + 1 > last) x[i].y = -INFINITY;
+                    if (c0 + 2 * i + 2 > last) x[i + 1].x = -INFINITY;
+                    if (c0 + 2 * i + 3 > last) x[i + 1].y = -INFINITY;
+                }
+                top = fmaxf(fmaxf(top, fmaxf(x[i].x, x[i].y)), fmaxf(x[i + 1].x, x[i + 1].y));
+            }
+            top *= un;
+            const bool raise = top > m + kRescaleAt;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float mn = raise ? ceilf(top) : m, r = from_max(m, mn);
+                l2 = make_float2(l2.x * r, l2.y * r);
+                z2 = make_float2(z2.x * r, z2.y * r);
+                scale_p(tS, c + 16 * u, r);
+                m = mn;
+            }
+            const float nm = m == -INFINITY ? 0.0f : -m;  // nothing visible yet: p = 0
+            const float2 nm2 = make_float2(nm, nm);
+            uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int w = 0; w < 4; w += 2) {
-                    const int j = c0 + i + w;
-                    float2 x = __ffma2_rn(w ? make_float2(k.z, k.w) : make_float2(k.x, k.y), qs2,
-                                          make_float2(v[u][i + w], v[u][i + w + 1]));
-                    float2 m = w ? make_float2(mv.z, mv.w) : make_float2(mv.x, mv.y);
-                    x = __ffma2_rn(x, un2, nm2);
-                    if (EDGE) {
-                        if (j > last) x.x = -INFINITY, m.x = 0.0f;
-                        if (j + 1 > last) x.y = -INFINITY, m.y = 0.0f;
+            for (int i = 0; i < 8; i += 2) {
+                const float4 mv = *reinterpret_cast<const float4*>(&par.mv[c0 + 2 * i]);
+                const float4 sv = *reinterpret_cast<const float4*>(&par.sv[c0 + 2 * i]);
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const float2 y = __ffma2_rn(x[i + w], un2, nm2);
+                    float2 mm = w ? make_float2(mv.z, mv.w) : make_float2(mv.x, mv.y);
+                    if (EDGE) {  // 0 times what an unseen token holds
+                        if (c0 + 2 * (i + w) > last) mm.x = 0.0f;
+                        if (c0 + 2 * (i + w) + 1 > last) mm.y = 0.0f;
                     }
-                    const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                    const float2 p = make_float2(ex2(y.x), ex2(y.y));
                     l2 = __fadd2_rn(l2, p);
-                    z2 = __ffma2_rn(p, m, z2);
+                    z2 = __ffma2_rn(p, mm, z2);
                     const float2 ps = __fmul2_rn(p, w ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y));
                     // the high part rounded, not cut: the low parts' signs then
                     // vary and what the sums cut from them cancels
                     const __half2 t = __floats2half2_rn(ps.x, ps.y);
-                    const float2 tf = __half22float2(t), r = __fadd2_rn(ps, make_float2(-tf.x, -tf.y));
-                    hi[(i + w) / 2] = *reinterpret_cast<const uint32_t*>(&t);
-                    lo[(i + w) / 2] = pack_h2(r.x, r.y);
+                    const float2 tf = __half22float2(t), r = __ffma2_rn(tf, make_float2(-1.0f, -1.0f), ps);
+                    hi[i + w] = *reinterpret_cast<const uint32_t*>(&t);
+                    lo[i + w] = pack_h2(r.x, r.y);
                 }
             }
             tmem_st8(tS + c + 16 * u, hi);
             tmem_st8(tS + c + 16 * u + 8, lo);
         }
     }
+    *xch = m;
+    __syncwarp();
+    if (lane == 0) bar_arrive(pair);
+    if (!warp_wait(pair, phase, abort_flag)) return false;
+    const float other = xch[xch_other];
+    const int e = par.E;
+    if (!__all_sync(0xffffffffu, m == other && m == st.m && e == st.E)) {
+        const float row_m = fmaxf(m, other), r = from_max(m, row_m), corr = rebase(st.m, st.E, row_m, e);
+        l2 = make_float2(l2.x * r, l2.y * r);
+        z2 = make_float2(z2.x * r, z2.y * r);
+        if (__any_sync(0xffffffffu, r != 1.0f)) scale_p(tS, 64, r);
+        if (!fresh && __any_sync(0xffffffffu, corr != 1.0f)) {  // this thread's half of O's columns
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+                float ov[16];
+                tmem_ld16(tO + c, ov);
+                tmem_ld_wait16(ov);
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[i] = __float_as_uint(ov[i] * corr);
+                tmem_st16(tO + c, w);
+            }
+        }
+        st.m = row_m;
+        st.E = e;
+    }
     tmem_st_wait();
-    st.l += l2.x + l2.y;
-    st.z += z2.x + z2.y;
+    st.l = l2;
+    st.z = z2;
     tc_fence_before();
     __syncwarp();
     if (lane == 0) bar_arrive(p_full);
@@ -380,7 +394,7 @@ struct PrefillQ4Params {
     float* part_o;           // n_split > 1: [split][rows][Hq][D], unnormalised
     float* part_ml;          // [split][rows][Hq][2]  (max in log2 units, sum)
     int64_t n_rows;
-    int32_t max_chunks, n_split;
+    int32_t n_seqs, max_chunks, n_split;
     int32_t max_bps, max_blocks;
     int32_t Hq, Hkv, G, QT;  // QT = 128 / G queries a tile
     float* aside;            // [n_aside][D][256] sums set aside by running CTAs
@@ -395,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     using C = Cfg<D>;
     constexpr int kTileBytes = 16 * (D / 2 + 4);
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem = smem_raw + (-su32(smem_raw) & 1023u);  // (a sum: the compiler still sees shared memory)
     const uint32_t bars = su32(smem) + C::kOffBar;
     const uint32_t k_full = bars, k_empty = bars + 8, v_full = bars + 16, v_empty = bars + 24;
     const uint32_t par_full = bars + 32, s_full = bars + 48, p_full = bars + 64, pv_done = bars + 80;  // of two each
@@ -409,9 +423,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    // the chunks with the most visible tokens first
-    const int seq_i = blockIdx.x / p.max_chunks, chunk = p.max_chunks - 1 - blockIdx.x % p.max_chunks;
-    const int h = blockIdx.y;
+    // the chunks with the most visible tokens first, all sequences' and heads'
+    // (a head after the other, the last one's long chunks start when the SMs run empty)
+    const int h = blockIdx.x % p.Hkv, seq_i = blockIdx.x / p.Hkv % p.n_seqs;
+    const int chunk = p.max_chunks - 1 - blockIdx.x / p.Hkv / p.n_seqs;
     pdl_wait_trigger();
     const PrefillSeq sm = p.seqs[seq_i];
     const int G = p.G, QT = p.QT, q0 = chunk * 2 * QT;
@@ -419,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     const int prefix = sm.kv_len - sm.q_len;
     const int kv_end = min(sm.kv_len, prefix + q0 + 2 * QT);
     const int all_tiles = (kv_end + kN - 1) / kN;
-    const int tb = (int)((int64_t)all_tiles * blockIdx.z / p.n_split), te = (int)((int64_t)all_tiles * (blockIdx.z + 1) / p.n_split);
+    const int tb = (int)((int64_t)all_tiles * blockIdx.y / p.n_split), te = (int)((int64_t)all_tiles * (blockIdx.y + 1) / p.n_split);
     const int n_tiles = te - tb;
     const bool two_tiles = q0 + QT < sm.q_len;
     const int32_t* tab = p.table + (int64_t)sm.table_row * p.max_bps;
@@ -649,70 +664,71 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         // Softmax warp w: tile X = w / 8, rows 32 (w % 4) .. + 31 of it (a row a
         // lane, as TMEM has it), tokens 64 half .. + 63 of every tile, half =
         // (w / 4) % 2.  Row 128 X + r is query X QT + r / G, head r % G.  The
-        // two warps of 32 rows bring 16 of q's rows each, eight in flight, each
+        // two warps of 32 rows bring 16 of q's rows each, all in flight, each
         // scaled by the power of two that puts its largest |q| in [2^14, 2^15).
         const int X = warp >> 3, half = (warp >> 2) & 1, r = 32 * (warp & 3) + lane, qi = X * QT + r / G;
         const uint32_t pair = pairs + 8 * (4 * X + (warp & 3));  // of the two warps
         float* x_mine = xch + half * 2 * kM + X * kM + r;  // slot s: + s * 4 kM; the other half's:
         const int x_other = (half ? -2 : 2) * kM;
         const bool valid = r < QT * G && q0 + qi < sm.q_len;
-        float q_un = 1.0f, q_sum = 0.0f;
         {
             const int mine = valid ? (sm.q_start + q0 + qi) * p.Hq + h * G + r % G : -1;
             uint8_t* hi_at = smem + C::kOffQ + 2 * X * C::kQBytes;
-            // lane L takes dims 8 (L / 4) + L % 4 and + 4 (a register pair of K's order), of 64 dims at a time
-            const int d0 = 8 * (lane >> 2) + (lane & 3);
-#pragma unroll 1
-            for (int j0 = 16 * half; j0 < 16 * half + 16; j0 += 8) {
-                float x[8][2 * C::kAtoms], mx[8], sum[8];
+            // D / 4 lanes a row, four dims a lane; x[j]: row RW j + lane / LR of the 16
+            constexpr int LR = D / 4, RW = 32 / LR, NJ = 16 / RW;
+            const int d0 = 4 * (lane % LR);
+            const bool vec = ((uintptr_t)p.q & 15) == 0;
+            float4 x[NJ];
+            float mx[NJ], sum[NJ];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int at = __shfl_sync(0xffffffffu, mine, j0 + j);
-                    mx[j] = sum[j] = 0.0f;
+            for (int j = 0; j < NJ; j++) {
+                const int at = __shfl_sync(0xffffffffu, mine, 16 * half + RW * j + lane / LR);
+                const float* src = p.q + (int64_t)at * D + d0;
+                x[j] = at < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                     : vec    ? *reinterpret_cast<const float4*>(src)
+                              : make_float4(src[0], src[1], src[2], src[3]);
+            }
 #pragma unroll
-                    for (int a = 0; a < 2 * C::kAtoms; a++) {
-                        x[j][a] = at < 0 ? 0.0f : p.q[(int64_t)at * D + 64 * (a >> 1) + 4 * (a & 1) + d0] * p.scale_log2;
-                        mx[j] = fmaxf(mx[j], fabsf(x[j][a]));
-                        sum[j] += x[j][a];
-                    }
+            for (int j = 0; j < NJ; j++) {
+                x[j] = make_float4(x[j].x * p.scale_log2, x[j].y * p.scale_log2, x[j].z * p.scale_log2, x[j].w * p.scale_log2);
+                mx[j] = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+                sum[j] = (x[j].x + x[j].y) + (x[j].z + x[j].w);
+            }
+            // all rows' maxima and sums at once: halve the rows a lane holds and the lanes that hold a row
+#pragma unroll
+            for (int n = NJ / 2; n > 0; n >>= 1) {
+                const bool up = lane & (2 * n);
+#pragma unroll
+                for (int j = 0; j < n; j++) {
+                    const float m_keep = up ? mx[j + n] : mx[j], m_give = up ? mx[j] : mx[j + n];
+                    const float s_keep = up ? sum[j + n] : sum[j], s_give = up ? sum[j] : sum[j + n];
+                    mx[j] = fmaxf(m_keep, __shfl_xor_sync(0xffffffffu, m_give, 2 * n));
+                    sum[j] = s_keep + __shfl_xor_sync(0xffffffffu, s_give, 2 * n);
                 }
-                // eight rows' maxima and sums at once: halve the rows and the lanes that hold them, then the lanes
+            }
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
+            sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+            // lanes 2 j and 2 j + 1 (of a row's lanes) hold x[j]'s row
+            const int qe = min(max((int)(__float_as_uint(mx[0]) >> 23), 40), 240);
+            const float scale = __uint_as_float((uint32_t)(268 - qe) << 23);
+            if (!(lane & 1)) {  // for both of the row's threads
+                float* at = xch + 2 * 4 * kM + X * kM + 32 * (warp & 3) + 16 * half + RW * (lane % LR / 2) + lane / LR;
+                at[0] = at[2 * kM] = __uint_as_float((uint32_t)(qe - 14) << 23);  // 1 / scale
+                at[4 * kM] = at[6 * kM] = sum[0] * scale;
+            }
 #pragma unroll
-                for (int n = 4; n > 0; n >>= 1) {
-                    const bool up = lane & (4 * n);
-#pragma unroll
-                    for (int j = 0; j < n; j++) {
-                        const float m_keep = up ? mx[j + n] : mx[j], m_give = up ? mx[j] : mx[j + n];
-                        const float s_keep = up ? sum[j + n] : sum[j], s_give = up ? sum[j] : sum[j + n];
-                        mx[j] = fmaxf(m_keep, __shfl_xor_sync(0xffffffffu, m_give, 4 * n));
-                        sum[j] = s_keep + __shfl_xor_sync(0xffffffffu, s_give, 4 * n);
-                    }
-                }
-#pragma unroll
-                for (int o = 2; o > 0; o >>= 1) {
-                    mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-                    sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
-                }
-                // lanes 4 j .. 4 j + 3 hold row j0 + j
-                const int qe = min(max((int)(__float_as_uint(mx[0]) >> 23), 40), 240);
-                const float scale = __uint_as_float((uint32_t)(268 - qe) << 23), un = __uint_as_float((uint32_t)(qe - 14) << 23);
-                const float un_j = __shfl_sync(0xffffffffu, un, 4 * (lane & 7)), sum_j = __shfl_sync(0xffffffffu, sum[0] * scale, 4 * (lane & 7));
-                if ((lane & 24) == j0) {  // for this row's other thread too
-                    x_mine[2 * 4 * kM] = x_mine[2 * 4 * kM + x_other] = un_j;  // 1 / scale
-                    x_mine[3 * 4 * kM] = x_mine[3 * 4 * kM + x_other] = sum_j;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float sc = __shfl_sync(0xffffffffu, scale, 4 * j);
-#pragma unroll
-                    for (int a = 0; a < C::kAtoms; a++) {
-                        uint32_t hi, lo;
-                        split_h2(x[j][2 * a] * sc, x[j][2 * a + 1] * sc, hi, lo);
-                        const uint32_t at = chunk_at(32 * (warp & 3) + j0 + j, 8 * a + (lane >> 2), kM) + 4 * (lane & 3);
-                        *reinterpret_cast<uint32_t*>(hi_at + at) = hi;
-                        *reinterpret_cast<uint32_t*>(hi_at + C::kQBytes + at) = lo;
-                    }
-                }
+            for (int j = 0; j < NJ; j++) {
+                const float sc = __shfl_sync(0xffffffffu, scale, (lane & ~(LR - 1)) + 2 * j);
+                // K's order of dims: an even lane takes 0 4 1 5 of eight, the next one 2 6 3 7
+                const bool odd = lane & 1;
+                const float g0 = __shfl_xor_sync(0xffffffffu, odd ? x[j].x : x[j].z, 1);
+                const float g1 = __shfl_xor_sync(0xffffffffu, odd ? x[j].y : x[j].w, 1);
+                uint2 hi, lo;
+                split_h2((odd ? g0 : x[j].x) * sc, (odd ? x[j].z : g0) * sc, hi.x, lo.x);
+                split_h2((odd ? g1 : x[j].y) * sc, (odd ? x[j].w : g1) * sc, hi.y, lo.y);
+                const uint32_t at = chunk_at(32 * (warp & 3) + 16 * half + RW * j + lane / LR, lane % LR / 2, kM) + 8 * (lane & 1);
+                *reinterpret_cast<uint2*>(hi_at + at) = hi;
+                *reinterpret_cast<uint2*>(hi_at + C::kQBytes + at) = lo;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -722,28 +738,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             }
         }
         bool ok = warp_wait(pair, 0, abort_flag);
-        q_un = x_mine[2 * 4 * kM];
-        q_sum = x_mine[3 * 4 * kM];
         const int row_limit = valid ? prefix + q0 + qi : kv_end - 1;  // last visible token
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + lanes + X * 128 + 64 * half, tO = tmem + lanes + kColO + X * 128 + half * (D / 2);
-        RowState st{-INFINITY, 0.0f, 0.0f, q_un, q_sum, kMinExp};
+        RowState st{-INFINITY, make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), kMinExp, x_mine[2 * 4 * kM], x_mine[3 * 4 * kM]};
         const bool active = X == 0 || two_tiles;
         float4* aside = reinterpret_cast<float4*>(p.aside) + ((int64_t)slot * (D / 4) + half * (D / 8)) * (2 * kM) + X * kM + r;  // columns 4 c ..: + 256 c
         float2* ref = reinterpret_cast<float2*>(smem + C::kOffRef) + tid;  // what this thread's set-aside sums refer to
         for (int t = 0; active && ok && t < n_tiles; t++) {
             const uint32_t ph = (uint32_t)(t & 1);
             const bool fresh = t % chain == 0;
-            // S_X(t) done also means PV_X(t - 1) done: O_X and P_X are free
-            if (!warp_wait(par_full + 8 * ph, (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(s_full + 8 * X, ph, abort_flag)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            if (fresh && t > 0) {
+            if (fresh && t > 0 && (ok = warp_wait(pv_done + 8 * X, ph ^ 1u, abort_flag))) {
+                tc_fence_after();
                 // The tensor cores cut their sums instead of rounding them, so a
                 // long chain drifts: set the sums aside with rounded additions
-                // (in L2, nothing waited for) and start anew.
+                // (in L2, nothing waited for) and start anew.  S_X(t) runs meanwhile.
                 const float c = t > chain ? rebase(ref->x, __float_as_int(ref->y), st.m, st.E) : 1.0f;
                 const bool add = t > chain && __all_sync(0xffffffffu, c == 1.0f);
                 if (t > chain && !add) __threadfence();
@@ -771,6 +780,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 }
                 *ref = make_float2(st.m, __int_as_float(st.E));
             }
+            // S_X(t) done also means PV_X(t - 1) done: O_X and P_X are free
+            if (!ok || !warp_wait(par_full + 8 * ph, (uint32_t)((t >> 1) & 1), abort_flag) || !warp_wait(s_full + 8 * X, ph, abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
             const int base = (tb + t) * kN;
             // (the pair's phase 0 was q's)
             if (base + kN - 1 > prefix + q0)  // some row of the chunk does not see all of it
@@ -784,56 +799,72 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid_));
         const int X_ = tid_ >> 8, half_ = (tid_ >> 7) & 1, r_ = tid_ & 127, qi_ = X_ * QT + r_ / G;
         const bool valid_ = r_ < QT * G && q0 + qi_ < sm.q_len;
-        const int64_t at = ((int64_t)(sm.q_start + q0 + qi_) * p.Hq + h * G + r_ % G);
-        const bool split = p.n_split > 1;
+        const int at = (sm.q_start + q0 + qi_) * p.Hq + h * G + r_ % G;
+        const bool split = p.n_split > 1, had = n_tiles > chain;
+        const float c = had ? rebase(ref->x, __float_as_int(ref->y), st.m, st.E) : 1.0f;
+        float4 old[8];  // the sums set aside
+        if (had) {
+            __threadfence();
+#pragma unroll
+            for (int i = 0; i < 8; i++) old[i] = __ldcg(aside + i * (2 * kM));
+        }
         if (active && n_tiles > 0 && ok && warp_wait(pv_done + 8 * X_, (uint32_t)((n_tiles - 1) & 1), abort_flag)) {
             tc_fence_after();
             // the row's sums from its two threads
-            x_mine[2 * 4 * kM] = st.l;
-            x_mine[3 * 4 * kM] = st.z;
+            const float l_mine = st.l.x + st.l.y, z_mine = st.z.x + st.z.y;
+            x_mine[2 * 4 * kM] = l_mine;
+            x_mine[3 * 4 * kM] = z_mine;
             __syncwarp();
             if (lane == 0) bar_arrive(pair);
             warp_wait(pair, (uint32_t)((n_tiles + 1) & 1), abort_flag);
-            const float l = st.l + x_mine[2 * 4 * kM + x_other], z = st.z + x_mine[3 * 4 * kM + x_other];
+            const float l = l_mine + x_mine[2 * 4 * kM + x_other], z = z_mine + x_mine[3 * 4 * kM + x_other];
             const float back = pow2(st.E - 127 - kVUp);
-            const int64_t row = split ? (int64_t)blockIdx.z * p.n_rows * p.Hq + at : at;
-            float* dst = (split ? p.part_o : p.out) + row * D + half_ * (D / 2);
             const float inv = split ? 1.0f : 1.0f / l;
             if (split && valid_ && half_ == 0) {
-                p.part_ml[row * 2] = st.m;
-                p.part_ml[row * 2 + 1] = l;
+                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2] = st.m;
+                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2 + 1] = l;
             }
-            const bool vec = ((uintptr_t)dst & 15) == 0, had = n_tiles > chain;
-            const float c = had ? rebase(ref->x, __float_as_int(ref->y), st.m, st.E) : 1.0f;
-            if (had) __threadfence();
+            // Half rows go through this warp's part of q's tiles (every product
+            // that read q is done), so that a row's columns are written together.
+            float4* stage = reinterpret_cast<float4*>(smem + C::kOffQ) + (tid_ >> 5) * (32 * D / 8);
+            constexpr int LR = D / 8;  // lanes a half row
 #pragma unroll 1
-            for (int d = 0; d < D / 8; d += 4) {
-                float ov[16];
-                float4 old[4];
-                if (had)
+            for (int d = 0; d < D / 8; d += 8) {
+                float ov[32];
+                if (had && d)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) old[i] = __ldcg(aside + (d + i) * (2 * kM));
+                    for (int i = 0; i < 8; i++) old[i] = __ldcg(aside + (d + i) * (2 * kM));
                 tmem_ld16(tO + 4 * d, ov);
+                tmem_ld16(tO + 4 * d + 16, ov + 16);
                 tmem_ld_wait16(ov);
+                tmem_ld_wait16(ov + 16);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 8; i++) {
                     float4 o = make_float4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
                     if (had)
                         o = make_float4(fmaf(old[i].x, c, o.x), fmaf(old[i].y, c, o.y), fmaf(old[i].z, c, o.z), fmaf(old[i].w, c, o.w));
-                    o = make_float4(fmaf(o.x, back, z) * inv, fmaf(o.y, back, z) * inv, fmaf(o.z, back, z) * inv,
-                                    fmaf(o.w, back, z) * inv);
-                    if (!valid_) continue;
-                    if (vec) {
-                        *reinterpret_cast<float4*>(dst + 4 * (d + i)) = o;
-                    } else {
-                        dst[4 * (d + i)] = o.x, dst[4 * (d + i) + 1] = o.y;
-                        dst[4 * (d + i) + 2] = o.z, dst[4 * (d + i) + 3] = o.w;
-                    }
+                    stage[lane * LR + ((d + i) ^ (lane & 7))] = make_float4(fmaf(o.x, back, z) * inv, fmaf(o.y, back, z) * inv,
+                                                                            fmaf(o.z, back, z) * inv, fmaf(o.w, back, z) * inv);
                 }
+            }
+            __syncwarp();
+            float* dst = (split ? p.part_o + (int64_t)blockIdx.y * p.n_rows * p.Hq * D : p.out) + half_ * (D / 2) + 4 * (lane % LR);
+            const bool vec = ((uintptr_t)dst & 15) == 0;
+            const int row_at = valid_ ? at : -1;
+#pragma unroll 4
+            for (int j = 0; j < 32; j += 32 / LR) {
+                const int row = j + lane / LR, to = __shfl_sync(0xffffffffu, row_at, row);
+                const float4 o = stage[row * LR + ((lane % LR) ^ (row & 7))];
+                if (to < 0) continue;
+                float* d = dst + (int64_t)to * D;
+                if (vec)
+                    *reinterpret_cast<float4*>(d) = o;
+                else
+                    d[0] = o.x, d[1] = o.y, d[2] = o.z, d[3] = o.w;
             }
         }
         if (active && n_tiles == 0 && valid_) {  // an empty share of a split
-            const int64_t row = (int64_t)blockIdx.z * p.n_rows * p.Hq + at;
+            const int64_t row = (int64_t)blockIdx.y * p.n_rows * p.Hq + at;
             for (int d = 0; d < D / 2; d++) p.part_o[row * D + half_ * (D / 2) + d] = 0.0f;
             p.part_ml[row * 2] = -INFINITY;
             p.part_ml[row * 2 + 1] = 0.0f;
@@ -880,14 +911,15 @@ bool prefill_q4_supported(int D, int G, int block_size) {
 }
 
 template <int D>
-static int launch_prefill(const PrefillQ4Params& p, int n_seqs, cudaStream_t stream) {
+static int launch_prefill(const PrefillQ4Params& p, cudaStream_t stream) {
     static std::atomic<uint64_t> attr_set{0};  // per device
     int st = once_per_device(attr_set, [] {
         S1KV_CUDA(cudaFuncSetAttribute(prefill_q4_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
         return S1KV_OK;
     });
     if (st) return st;
-    const dim3 grid((unsigned)(n_seqs * p.max_chunks), (unsigned)p.Hkv, (unsigned)p.n_split);
+    if ((int64_t)p.n_seqs * p.max_chunks * p.Hkv > INT32_MAX) return set_error(S1KV_EINVAL, "attention: too many query chunks");
+    const dim3 grid((unsigned)(p.n_seqs * p.max_chunks * p.Hkv), (unsigned)p.n_split);
     S1KV_CUDA(launch_pdl(prefill_q4_kernel<D>, grid, dim3(kThreads), Cfg<D>::kSmem, stream, p));
     g_launches++;
     if (p.n_split > 1) {
@@ -910,6 +942,7 @@ int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, 
     p.kbase = pool->k + (size_t)layer * pool->layer_bytes;
     p.vbase = pool->v + (size_t)layer * pool->layer_bytes;
     p.n_rows = b->n_rows;
+    p.n_seqs = b->n_seqs;
     p.max_bps = pool->max_bps;
     p.max_blocks = (int32_t)pool->desc.max_blocks;
     p.Hq = Hq;
@@ -946,7 +979,7 @@ int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, 
         p.part_o = (float*)pool->scratch.p;
         p.part_ml = p.part_o + rows * D;
     }
-    return D == 128 ? launch_prefill<128>(p, b->n_seqs, stream) : launch_prefill<64>(p, b->n_seqs, stream);
+    return D == 128 ? launch_prefill<128>(p, stream) : launch_prefill<64>(p, stream);
 }
 
 }  // namespace s1kv

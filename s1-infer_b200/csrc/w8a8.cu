@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     using C = TcCfg<NT, SPLIT>;
     constexpr int ST = C::kStages;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem = smem_raw + (-su32(smem_raw) & 1023u);  // (a sum: the compiler still sees shared memory)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
     uint64_t* empty = full + ST;
     uint64_t* acc_full = empty + ST;    // [2]

@@ -201,6 +201,32 @@ def test_chunks(s1kv, cuda, hq, hkv, dim):
     attend(s1kv, [1025, 20], [2, 3], hq, hkv, dim, 52)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", ["up", "down", "steps"])
+def test_scores_that_rise(s1kv, cuda, dim, shape):
+    """Scores over 60 log2 units, up or down the sequence or in jumps inside
+    tiles, so that the running maximum moves again and again, for decode rows
+    and chunks (scores stay within 32 of zero)."""
+    rng = np.random.default_rng(65)
+    hkv, hq, n = 1, 4, 700
+    u = rng.standard_normal(dim).astype(np.float32)
+    u *= np.float32(np.sqrt(dim) / np.linalg.norm(u))
+    ramp = np.linspace(-1, 1, n)
+    if shape == "down":
+        ramp = ramp[::-1]
+    elif shape == "steps":
+        ramp = np.sign(np.sin(np.arange(n) / 23.0)) * np.linspace(0.1, 1, n)
+    top = 28 * np.log(2) / np.sqrt(dim)  # q.k / sqrt(dim) in log2 units: 28 at the ends
+    k = (ramp[:, None] * u * top)[:, None].astype(np.float32)
+    v = rng.standard_normal((n, hkv, dim)).astype(np.float32)
+    pool = pool_of(s1kv, hkv, dim, 50)
+    fill(pool, [n], k, v)
+    for r in (1, 200):
+        q = np.tile(u, (r, hq, 1)) + 0.05 * rng.standard_normal((r, hq, dim)).astype(np.float32)
+        got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
+        check_close(got, LB.attention64(q, LB.q4_values(k), LB.q4_values(v)))
+
+
 def test_scales_far_apart(s1kv, cuda):
     """V rows of one sequence differing by 2^80 in size, the large ones seldom
     and early or late: the running power of two must follow."""
