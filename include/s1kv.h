@@ -480,11 +480,8 @@ int s1kv_quantize_tokens(const float* x, int64_t M, int64_t K, int8_t* q, int64_
  * that order; the same bits on every run.  Weights are rows of an output
  * channel (an nn.Linear weight's order): s1kv_quantize_rows of that [N][K]
  * matrix makes q and scales.  K is the padded row length: a multiple of 16
- * up to 131072, xq zero past the true K (w may hold anything there); xq and w
- * 16-byte aligned.  The products are programmatic dependent launches that
- * request weights while the previous kernel of the stream is still running: a
- * caller's own programmatic-dependent kernel that writes weights must not come
- * directly before them. */
+ * up to 131072, xq zero past the true K (w may hold anything there) and no code
+ * -128; xq and w 16-byte aligned. */
 int s1kv_matmul_w8a8(const int8_t* xq, const float* x_scales, int64_t M, int64_t K, const int8_t* w,
                      const float* w_scales, int64_t N, float* out, void* stream);
 /* Both in one call: x [M][K] fp32 (any K up to 131072) quantised per token and

@@ -131,15 +131,16 @@ int launch_quantize(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq
 // channel's (and its token's) row: weights go from global memory to the
 // instruction's registers in 16-byte loads, nothing is staged or shuffled.
 // A CTA owns 16 channels, its 8 warps split K by 128-byte steps; the warps'
-// integer sums meet in shared memory.  The first steps' weights are
-// requested before the wait for the previous kernel (the token quantiser):
-// they do not depend on it.
+// integer sums meet in shared memory.  Behind this call's own token quantiser
+// (EARLY) the first steps' weights are requested before the wait for it: the
+// quantiser has waited for all that came before it and writes no weights.
 // FUSED (one token of up to kFusedK values): each CTA quantises the token
-// itself, from x through L2 into its shared memory, while its first weights
-// are on their way: one launch instead of two.
+// itself, from x through L2 into its shared memory: one launch instead of two.
+// What runs before it may write anything, so its first weights are only
+// brought to L2 before the wait.
 // Three CTAs an SM with two steps in flight a warp stream better than two with
 // four (8 tokens, K = 4096, 6144 channels: 7.8 against 11.0 us, 3.3 TB/s).
-constexpr int kFusedK = 4096, kFusedM = 1;
+constexpr int kFusedK = 1024;  // four values a thread
 constexpr int kGemvWarps = 8;
 constexpr int kGemvPre = 2;  // 128-byte steps in flight a warp
 
@@ -151,12 +152,12 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NTILE, bool FUSED>
+template <int NTILE, bool FUSED, bool EARLY>  // (neither: the caller's codes)
 __global__ void __launch_bounds__(kGemvWarps * 32, 3)
     w8a8_gemv_kernel(const float* __restrict__ x, int x_len, const int8_t* __restrict__ xq, const float* __restrict__ sx, int M,
                      int K, const __grid_constant__ W8Group grp) {
-    extern __shared__ uint4 own[];  // FUSED: the tokens' codes, K bytes each
-    __shared__ float part[8], own_scale[kFusedM];
+    __shared__ uint4 own[FUSED ? kFusedK / 16 : 1];  // the token's codes
+    __shared__ float part[8], own_scale;
     __shared__ int red[kGemvWarps][16][8 * NTILE + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int mi = 0;
@@ -180,33 +181,24 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 3)
             r[hf][1] = in ? __ldcs(reinterpret_cast<const uint4*>(w1 + k)) : make_uint4(0, 0, 0, 0);
         }
     };
+    auto fetch_first = [&] {
 #pragma unroll
-    for (int s = 0; s < kGemvPre; s++) fetch(s, a[s]);
+        for (int s = 0; s < kGemvPre; s++) fetch(s, a[s]);
+    };
+    if (EARLY) fetch_first();
+    if (FUSED && t < 2 && 128 * warp < K)  // all of a warp's row pieces: one step
+        asm volatile("prefetch.global.L2 [%0];" ::"l"((t ? w1 : w0) + 128 * warp));
     pdl_wait_trigger();
+    if (!EARLY) fetch_first();
     if (FUSED) {
-        for (int m = 0; m < M; m++) {
-            const float* src = x + (int64_t)m * x_len;
-            float4 v[kFusedK / 1024];  // a row of up to 16 K values, 64 a thread: only what K needs is touched
-            float mx = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kFusedK / 1024; i++) {
-                if (i * 1024 >= K) break;
-                const int k = 4 * (threadIdx.x + 256 * i);
-                v[i] = k < x_len ? *reinterpret_cast<const float4*>(src + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                mx = top_of(top_of(top_of(top_of(mx, v[i].x), v[i].y), v[i].z), v[i].w);
-            }
-            mx = cta_max(mx, part);
-            const bool fine = mx < INFINITY;
-            const float s = token_scale(mx), inv = __frcp_rn(s);
-            if (threadIdx.x == 0) own_scale[m] = fine ? s : __uint_as_float(0x7FC00000u);
-#pragma unroll
-            for (int i = 0; i < kFusedK / 1024; i++) {
-                if (i * 1024 >= K) break;
-                const int k = 4 * (threadIdx.x + 256 * i);
-                if (k < K) reinterpret_cast<uint32_t*>(own)[(m * K + k) / 4] = fine ? token_codes4(v[i], s, inv) : 0u;
-            }
-            __syncthreads();  // codes written; part free for the next row
-        }
+        const int k = 4 * threadIdx.x;
+        const float4 v = k < x_len ? *reinterpret_cast<const float4*>(x + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float mx = cta_max(top_of(top_of(top_of(top_of(0.0f, v.x), v.y), v.z), v.w), part);
+        const bool fine = mx < INFINITY;
+        const float s = token_scale(mx), inv = __frcp_rn(s);
+        if (threadIdx.x == 0) own_scale = fine ? s : __uint_as_float(0x7FC00000u);
+        if (k < K) reinterpret_cast<uint32_t*>(own)[threadIdx.x] = fine ? token_codes4(v, s, inv) : 0u;
+        __syncthreads();
     }
     int acc[NTILE][4] = {};
     for (int s0 = 0; s0 < steps; s0 += kGemvPre) {
@@ -242,7 +234,7 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 3)
 #pragma unroll
         for (int w = 0; w < kGemvWarps; w++) sum += red[w][n][m];
         if (m < M && n0 + n < mat.N)
-            mat.out[(int64_t)m * mat.N + n0 + n] = __fmul_rn(__fmul_rn((float)sum, FUSED ? own_scale[m] : sx[m]), mat.scales[n0 + n]);
+            mat.out[(int64_t)m * mat.N + n0 + n] = __fmul_rn(__fmul_rn((float)sum, FUSED ? own_scale : sx[m]), mat.scales[n0 + n]);
     }
 }
 
@@ -286,6 +278,7 @@ struct TcParams {
     const float* sx;
     int M, k_blocks;   // stages of K
     int ch_tiles, tok_tiles;
+    int early;         // this call's token quantiser runs before: weights may be read before the wait for it
 };
 struct TcMaps {
     CUtensorMap x, w[kMaxMats];
@@ -426,10 +419,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ================= TMA producer =================
         int it = 0;  // stages used so far
         bool ok = true;
-        // the weights of the first stages do not depend on the kernel before
-        // this one (the token quantiser): requested before the wait for it
+        // the weights of the first stages do not depend on this call's token
+        // quantiser: requested before the wait for it
         int pre = 0;
-        {
+        if (p.early) {
             int ch, tok;
             tile_at(blockIdx.x, ch, tok);
             const int mi = mat_of(ch), n0 = (ch - p.grp.m[mi].tile0) * kCh;
@@ -591,7 +584,8 @@ int encode_rows(CUtensorMap* m, const int8_t* base, int64_t rows, int64_t K, int
 }
 
 template <int NT, bool SPLIT>
-int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int ch_tiles, int cs, cudaStream_t stream) {
+int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int ch_tiles, int cs, bool early,
+              cudaStream_t stream) {
     auto kern = w8a8_tc_kernel<NT, SPLIT>;
     static std::atomic<uint64_t> attr_set{0};  // per device
     int st = once_per_device(attr_set, [&] {
@@ -603,6 +597,7 @@ int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& gr
     TcParams p{};
     p.grp = grp;
     p.sx = sx;
+    p.early = early;
     p.M = M;
     p.k_blocks = (K + kKB - 1) / kKB;
     p.ch_tiles = ch_tiles;
@@ -635,11 +630,11 @@ int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& gr
     return S1KV_OK;
 }
 
-template <int NTILE, bool FUSED>
+template <int NTILE, bool FUSED, bool EARLY>
 int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int tiles,
                 cudaStream_t stream) {
-    S1KV_CUDA(launch_pdl(w8a8_gemv_kernel<NTILE, FUSED>, dim3((unsigned)tiles), dim3(kGemvWarps * 32),
-                         FUSED ? (size_t)M * K : 0, stream, x, x_len, xq, sx, M, K, grp));
+    S1KV_CUDA(launch_pdl(w8a8_gemv_kernel<NTILE, FUSED, EARLY>, dim3((unsigned)tiles), dim3(kGemvWarps * 32), 0, stream, x,
+                         x_len, xq, sx, M, K, grp));
     g_launches++;
     return S1KV_OK;
 }
@@ -667,30 +662,35 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
             S1KV_CUDA(cudaMemsetAsync(grp.m[i].out, 0, sizeof(float) * (size_t)M * grp.m[i].N, stream));
         return S1KV_OK;
     }
-    // One token: a kernel of its own for the codes costs more than making them
-    // in every CTA as long as all CTAs are resident at once (K = 1024, 4096
-    // channels: 2.6 against 3.3 us; K = 4096, 6144 channels: 7.2 against 7.4;
-    // 14336 channels: 15.6 against 14.8).
-    if (x && M <= kFusedM && K <= kFusedK && tiles <= 3 * 148 && x_len % 4 == 0 && ((uintptr_t)x & 15) == 0)
-        return launch_gemv<1, true>(x, x_len, nullptr, nullptr, M, K, grp, (int)tiles, stream);
+    // One short token: a kernel of its own for the codes costs more than making
+    // them in every CTA (K = 1024, 4096 channels: 3.3 us against 3.0; K = 2048:
+    // 4.1 against 4.6), as long as all CTAs are resident at once.
+    if (x && M == 1 && K <= kFusedK && tiles <= 3 * 148 && x_len % 4 == 0 && ((uintptr_t)x & 15) == 0)
+        return launch_gemv<1, true, false>(x, x_len, nullptr, nullptr, M, K, grp, (int)tiles, stream);
     if (x) {
         const int st = launch_quantize(x, M, x_len, xq, K, sx, stream);
         if (st) return st;
     }
-    if (M <= 8) return launch_gemv<1, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
-    if (M <= 16) return launch_gemv<2, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
-    if (M <= 32) return launch_gemv<4, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 8)
+        return x ? launch_gemv<1, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
+                 : launch_gemv<1, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 16)
+        return x ? launch_gemv<2, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
+                 : launch_gemv<2, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
+    if (M <= 32)
+        return x ? launch_gemv<4, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
+                 : launch_gemv<4, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
     int cs = 1;
     if (NT <= 128)
         while (cs < 8 && tiles * ((M + NT - 1) / NT) * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
 #define S1KV_TC(NT_)                                                                                       \
     if (NT == NT_)                                                                                         \
-        return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, stream)                     \
-                      : launch_tc<NT_, false>(xq, sx, M, K, grp, (int)tiles, 1, stream);
+        return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, x != nullptr, stream)       \
+                      : launch_tc<NT_, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
     S1KV_TC(32) S1KV_TC(64) S1KV_TC(128)
 #undef S1KV_TC
-    return launch_tc<256, false>(xq, sx, M, K, grp, (int)tiles, 1, stream);
+    return launch_tc<256, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
 }
 
 }  // namespace
