@@ -468,7 +468,9 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                 }
             }
         }
-        __syncthreads();  // before the next pass's copies overwrite the partial rows
+        // before the next pass's copies overwrite the partial rows
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
     }
     pdl_trigger();
     if (p.counters && rm.n_split > 1) {
