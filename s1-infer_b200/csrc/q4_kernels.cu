@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
                 tile = q4_tile(part == 0 ? p.kpool : p.vpool, slot, h, p.Hkv, p.block_size, D, &tt);
             }
         }
+        if (ROPE) __syncwarp();  // a row's lanes have all read it (q_out may be q_in)
         if (ok && part == 2)
 #pragma unroll
             for (int i = 0; i < NQ; i++) {

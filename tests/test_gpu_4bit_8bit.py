@@ -116,6 +116,21 @@ def test_rope_append_is_rope_then_append(s1kv, cuda, dim, hkv, hq):
         np.testing.assert_array_equal(got[i], LB.q4_values(want[i]))
 
 
+@pytest.mark.parametrize("dim", [64, 128, 40])
+def test_rope_append_of_q_in_place(s1kv, cuda, dim):
+    rng = np.random.default_rng(7)
+    n, hkv, hq = 700, 2, 6
+    k, v = kv(rng, n, hkv, dim)
+    q = dev(rng.standard_normal((n, hq, dim)).astype(np.float32))
+    pool = pool_of(s1kv, hkv, dim, 100)
+    with pool.batch([0], [n]) as b:
+        want = b.rope_append(0, dev(k), dev(v), q)
+    pool.truncate(0, 0)
+    with pool.batch([0], [n]) as b:
+        got = b.rope_append(0, dev(k), dev(v), q, q)
+    np.testing.assert_array_equal(got.cpu().numpy(), want.cpu().numpy())
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_norm_rope_append_is_the_fp32_pools_rows(s1kv, cuda, dim):
     rng = np.random.default_rng(6)
@@ -225,6 +240,33 @@ def test_scores_that_rise(s1kv, cuda, dim, shape):
         q = np.tile(u, (r, hq, 1)) + 0.05 * rng.standard_normal((r, hq, dim)).astype(np.float32)
         got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
         check_close(got, LB.attention64(q, LB.q4_values(k), LB.q4_values(v)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", ["up", "steps"])
+def test_long_chunks(s1kv, cuda, dim, shape):
+    """As many chunks as SMs, so that none is split and a chunk passes over up
+    to 13 tiles: scores that rise by 56 log2 units and V rows that grow by
+    2^12 on the way, so what earlier tiles left is brought to new references
+    (scores stay within 32 of zero)."""
+    rng = np.random.default_rng(66)
+    hkv, hq, n, r = 8, 32, 1570, 1301
+    u = rng.standard_normal(dim).astype(np.float32)
+    u *= np.float32(np.sqrt(dim) / np.linalg.norm(u))
+    ramp = np.linspace(-1, 1, n)
+    if shape == "steps":
+        ramp = np.sign(np.sin(np.arange(n) / 93.0)) * np.linspace(0.1, 1, n)
+    k = np.repeat((ramp[:, None] * u * (28 * np.log(2) / np.sqrt(dim)))[:, None].astype(np.float32), hkv, 1)
+    k[:, 1::2] *= np.float32(0.1)  # flat scores: every tile counts
+    v = rng.standard_normal((n, hkv, dim)).astype(np.float32)
+    v *= np.exp2(np.floor(np.arange(n) * 13 / n)).astype(np.float32)[:, None, None]
+    q = np.tile(u, (r, hq, 1)) + 0.05 * rng.standard_normal((r, hq, dim)).astype(np.float32)
+    pool = pool_of(s1kv, hkv, dim, 100)
+    fill(pool, [n], k, v)
+    got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
+    for h in (0, 3, 6):
+        heads = slice(4 * h, 4 * h + 4)
+        check_close(got[:, heads], LB.attention64(q[:, heads], LB.q4_values(k[:, h:h + 1]), LB.q4_values(v[:, h:h + 1])))
 
 
 def test_scales_far_apart(s1kv, cuda):
@@ -424,7 +466,7 @@ def test_token_codes(s1kv, cuda, m, k):
     assert (q.cpu().numpy()[:, k:] == 0).all()
 
 
-PRODUCTS = [(1, 16, 1), (1, 1024, 2048), (2, 100, 77), (7, 48, 130), (8, 4096, 256), (9, 512, 300), (16, 2000, 129), (17, 64, 64),
+PRODUCTS = [(1, 16, 1), (1, 1024, 2048), (1, 1020, 333), (1, 1022, 50), (1, 1040, 70), (2, 100, 77), (7, 48, 130), (8, 4096, 256), (9, 512, 300), (16, 2000, 129), (17, 64, 64),
             (33, 1000, 777), (64, 4096, 512), (65, 272, 200), (128, 128, 128), (129, 1040, 385), (256, 1536, 1000),
             (300, 4096, 520), (1000, 80, 50), (2049, 512, 640), (5, 131072, 40)]
 
