@@ -114,11 +114,12 @@ __device__ __forceinline__ int q4_k_quad(int t, int quad, int D) { return t * (D
 __device__ __forceinline__ int q4_v_quad(int t, int quad, int D) { return (t >> 1) * D + quad * 4 + (t & 1) * 2; }
 __device__ __forceinline__ int q4_param(int t, int bs, int D) { return bs * (D / 2) + t * 4; }
 
-// Tile of (slot, head) in one layer's storage and the token's place in it.
+// Tile of (slot, head) in one layer's storage and the token's place in it.  (A
+// pool has fewer than 2^31 slots: one 32-bit division.)
 __device__ __forceinline__ char* q4_tile(void* base, int64_t slot, int h, int Hkv, int bs, int D, int* t) {
-    const int64_t blk = slot / bs;
-    *t = (int)(slot - blk * bs);
-    return reinterpret_cast<char*>(base) + (blk * Hkv + h) * q4_tile_bytes(bs, D);
+    const uint32_t blk = (uint32_t)slot / (uint32_t)bs;
+    *t = (int)((uint32_t)slot - blk * (uint32_t)bs);
+    return reinterpret_cast<char*>(base) + ((int64_t)blk * Hkv + h) * q4_tile_bytes(bs, D);
 }
 
 // Quantises one row held by `LANES` adjacent lanes of a warp, NQ quads a
@@ -163,8 +164,8 @@ __device__ __forceinline__ void q4_store_row(const float (&x)[NQ][4], int nq, ch
     if (lr == 0) *reinterpret_cast<uint32_t*>(tile + q4_param(t, bs, D)) = r.packed;
 }
 
-// The same for a row held by D / 16 adjacent lanes, 16 contiguous values
-// (four quads) a lane: a warp takes 512 / D rows, so the reductions and the
+// The same for a row held by LANES = D / 16 adjacent lanes, quads lane_in_row +
+// i LANES (x[4 i ..]): a warp takes 512 / D rows, so the reductions and the
 // 64-bit arithmetic of the parameters serve that many rows at once (a row a
 // warp ran at a quarter of the speed).  Codes are made in packed fp32:
 // (x - m) / s + 8, rounded by adding 1.5 * 2^23; a row with a value within
@@ -215,12 +216,10 @@ __device__ __forceinline__ void q4_store_row16(const float (&x)[16], char* tile,
             for (int e = 0; e < 4; e++) c[q] |= q4_code(x[4 * q + e], r, inv) << (4 * e);
         }
     }
-    if (is_v) {
+    char* at = tile + (is_v ? q4_v_quad(t, lr, D) : q4_k_quad(t, lr, D));
+    const int step = (is_v ? 4 : 2) * LANES;
 #pragma unroll
-        for (int q = 0; q < 4; q++) *reinterpret_cast<uint16_t*>(tile + q4_v_quad(t, 4 * lr + q, D)) = (uint16_t)c[q];
-    } else {
-        *reinterpret_cast<uint2*>(tile + q4_k_quad(t, 4 * lr, D)) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-    }
+    for (int q = 0; q < 4; q++) *reinterpret_cast<uint16_t*>(at + q * step) = (uint16_t)c[q];
     if (lr == 0) *reinterpret_cast<uint32_t*>(tile + q4_param(t, bs, D)) = r.packed;
 }
 

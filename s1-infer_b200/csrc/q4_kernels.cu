@@ -10,16 +10,20 @@ constexpr int kSMs = 148;
 
 // -------------------------------------------------------------- append ----
 // A row (one token and head of k, v or, rotated only, q) on LANES lanes.
-// LANES = D / 16 (D of 64, 128, 256): 16 contiguous values a lane.  LANES = 32,
-// any other D: two quads a lane, 128 values apart.  RoPE (src/nn/RoPE.cpp:32-33:
-// out1 = x1 c - x2 s, out2 = x2 c + x1 s, each operation rounded on its own)
-// reads its partner values D / 2 away through the L1 cache, before the
-// quantisation.  Bound by the fp32 rows read (8 bytes a K and V value pair
-// against 1 written).
+// LANES = D / 16 (D of 64, 128, 256): four quads of values a lane, LANES quads
+// apart, so that a row's lanes read 16 LANES adjacent bytes at a time and a
+// value's RoPE partner D / 2 away is the lane's own (17000 tokens of 8 heads of
+// 128: 34.5 us, 4.6 TB/s, with RoPE 39.2; 16 contiguous values a lane and
+// partners read again: 36.9 and 57.4).  LANES = 32, any other D: two quads a lane, 128 values apart,
+// partners read through the L1 cache.  RoPE (src/nn/RoPE.cpp:32-33: out1 =
+// x1 c - x2 s, out2 = x2 c + x1 s, each operation rounded on its own) comes
+// before the quantisation.  Bound by the fp32 rows read (8 bytes a K and V
+// value pair against 1 written) and by the instructions that find a row's
+// parameters and codes, 56% of the issue slots.
 template <int LANES, bool ROPE>
-__global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 5) append_q4_kernel(const AppendParams p) {
     pdl_wait_trigger();
-    constexpr bool kWide = LANES < 32;               // 16 contiguous values
+    constexpr bool kWide = LANES < 32;
     constexpr int NQ = kWide ? 4 : 2, RPW = 32 / LANES;
     const int D = p.D, half = D / 2, nq = D / 4;
     const int lane = threadIdx.x & 31, lr = lane % LANES;
@@ -42,39 +46,49 @@ __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
             ok = false;
         }
         float x[4 * NQ];
+        if constexpr (kWide) {  // 16-byte aligned (launch_append_q4)
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const int quad = kWide ? 4 * lr + i : lr + i * LANES, d = 4 * quad;
-            x[4 * i] = x[4 * i + 1] = x[4 * i + 2] = x[4 * i + 3] = 0.0f;
-            if (quad >= nq || !ok) continue;
-            if (kWide) {  // 16-byte aligned (launch_append_q4)
-                const float4 f = *reinterpret_cast<const float4*>(src + d);
+            for (int i = 0; i < 4; i++) {
+                const float4 f = ok ? *reinterpret_cast<const float4*>(src + 4 * (lr + LANES * i)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 x[4 * i] = f.x, x[4 * i + 1] = f.y, x[4 * i + 2] = f.z, x[4 * i + 3] = f.w;
-            } else {
+            }
+            if (rot && ok) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {  // quads i and i + 2
+                    const float4* cs = reinterpret_cast<const float4*>(p.rope + (int64_t)pos * half + 4 * (lr + LANES * i));
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float4 c = __ldg(cs + e / 2);  // two (cos, sin)
+                        float &a0 = x[4 * i + e], &a1 = x[4 * i + e + 1], &b0 = x[4 * i + 8 + e], &b1 = x[4 * i + 9 + e];
+                        const float y0 = __fsub_rn(__fmul_rn(a0, c.x), __fmul_rn(b0, c.y));
+                        const float y1 = __fsub_rn(__fmul_rn(a1, c.z), __fmul_rn(b1, c.w));
+                        b0 = __fadd_rn(__fmul_rn(b0, c.x), __fmul_rn(a0, c.y));
+                        b1 = __fadd_rn(__fmul_rn(b1, c.z), __fmul_rn(a1, c.w));
+                        a0 = y0, a1 = y1;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                const int quad = lr + i * LANES, d = 4 * quad;
+                x[4 * i] = x[4 * i + 1] = x[4 * i + 2] = x[4 * i + 3] = 0.0f;
+                if (quad >= nq || !ok) continue;
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[4 * i + e] = src[d + e];
-            }
-            if (rot) {
-                const bool first = d < half;
-                const float* other = src + (first ? d + half : d - half);
-                const float2* cs = p.rope + (int64_t)pos * half + (first ? d : d - half);
-                float o[4];
-                if (kWide) {
-                    const float4 f = *reinterpret_cast<const float4*>(other);
-                    o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
-                } else {
+                if (rot) {
+                    const bool first = d < half;
+                    const float* other = src + (first ? d + half : d - half);
+                    const float2* cs = p.rope + (int64_t)pos * half + (first ? d : d - half);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = other[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float4 c = __ldg(reinterpret_cast<const float4*>(cs + e));  // two (cos, sin)
-                    const float a0 = __fmul_rn(x[4 * i + e], c.x), b0 = __fmul_rn(o[e], c.y);
-                    const float a1 = __fmul_rn(x[4 * i + e + 1], c.z), b1 = __fmul_rn(o[e + 1], c.w);
-                    x[4 * i + e] = first ? __fsub_rn(a0, b0) : __fadd_rn(a0, b0);
-                    x[4 * i + e + 1] = first ? __fsub_rn(a1, b1) : __fadd_rn(a1, b1);
+                    for (int e = 0; e < 4; e++) {
+                        const float2 c = __ldg(cs + e);
+                        const float a = __fmul_rn(x[4 * i + e], c.x), b = __fmul_rn(other[e], c.y);
+                        x[4 * i + e] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
+                    }
                 }
             }
+            if (ROPE) __syncwarp();  // a row's lanes have all read it (q_out may be q_in)
         }
         char* tile = nullptr;
         int tt = 0;
@@ -88,11 +102,10 @@ __global__ void __launch_bounds__(256) append_q4_kernel(const AppendParams p) {
                 tile = q4_tile(part == 0 ? p.kpool : p.vpool, slot, h, p.Hkv, p.block_size, D, &tt);
             }
         }
-        if (ROPE) __syncwarp();  // a row's lanes have all read it (q_out may be q_in)
         if (ok && part == 2)
 #pragma unroll
             for (int i = 0; i < NQ; i++) {
-                const int quad = kWide ? 4 * lr + i : lr + i * LANES;
+                const int quad = lr + i * LANES;
                 if (quad >= nq) continue;
                 float* dst = p.q_out + (int64_t)th * D + 4 * quad;
                 if (kWide) *reinterpret_cast<float4*>(dst) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
@@ -150,19 +163,22 @@ int launch_append_q4(const AppendParams& all, bool rope, cudaStream_t stream, bo
 
 // -------------------------------------------------------------- gather ----
 // Token i of a sequence (block-table row `trow`) or of a batch (`slots`), widened
-// to fp32: a warp a (token, head) row, one quad a lane at a time, several rows
-// in turn; the row's place is worked out once for its lanes.
+// to fp32: a warp eight (token, head) rows at a time, one quad a lane.  The
+// rows' places are worked out by a lane each, their codes and parameters all
+// requested before the first is widened (17000 tokens of 8 heads of 128: 16.6 us,
+// 4.7 TB/s; 4 or 16 rows: 18.7).
+constexpr int kGatherRows = 8;
 __global__ void __launch_bounds__(256) gather_q4_kernel(const char* __restrict__ base, bool is_v, const int32_t* __restrict__ trow,
                                                         const int32_t* __restrict__ slots, uint32_t n_rows, uint32_t row0, int bs,
                                                         int Hkv, int D, int64_t num_slots, float* __restrict__ out, int* err) {
     const int nq = D / 4, lane = threadIdx.x & 31;
     const uint32_t warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, warps = gridDim.x * (blockDim.x / 32);
     const bool vec = ((uintptr_t)out & 15) == 0;
-    for (uint32_t r0 = warp * 4; r0 < n_rows; r0 += warps * 4) {
-        // lane j < 4 looks row r0 + j up
+    for (uint32_t r0 = warp * kGatherRows; r0 < n_rows; r0 += warps * kGatherRows) {
+        // lane j looks row r0 + j up
         int64_t off = -1;
         int t = 0;
-        if (lane < 4 && r0 + lane < n_rows) {
+        if (lane < kGatherRows && r0 + lane < n_rows) {
             const uint32_t th = row0 + r0 + lane, i = th / Hkv;
             const int32_t slot = slots ? slots[i] : trow[i / bs] * bs + (int)(i % bs);
             if ((uint64_t)slot >= (uint64_t)num_slots) {
@@ -173,19 +189,23 @@ __global__ void __launch_bounds__(256) gather_q4_kernel(const char* __restrict__
                 off = ((int64_t)blk * Hkv + (int)(th - i * Hkv)) * q4_tile_bytes(bs, D);
             }
         }
+        for (int quad = lane; quad - lane < nq; quad += 32) {  // warp-uniform (shuffles inside)
+            uint32_t c[kGatherRows], sm[kGatherRows];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t at = __shfl_sync(0xffffffffu, off, j);
-            const int tt = __shfl_sync(0xffffffffu, t, j);
-            if (r0 + j >= n_rows) break;
-            const char* tile = base + at;
-            float2 sm = make_float2(0.0f, 0.0f);
-            if (at >= 0) sm = q4_unpack(*reinterpret_cast<const uint32_t*>(tile + q4_param(tt, bs, D)));
-            for (int quad = lane; quad < nq; quad += 32) {
-                uint32_t c = 0x8888u;  // zeros where the slot is out of range
-                if (at >= 0) c = *reinterpret_cast<const uint16_t*>(tile + (is_v ? q4_v_quad(tt, quad, D) : q4_k_quad(tt, quad, D)));
-                const float4 v = make_float4(q4_value(c & 15u, sm.x, sm.y), q4_value((c >> 4) & 15u, sm.x, sm.y),
-                                             q4_value((c >> 8) & 15u, sm.x, sm.y), q4_value(c >> 12, sm.x, sm.y));
+            for (int j = 0; j < kGatherRows; j++) {
+                const int64_t at = __shfl_sync(0xffffffffu, off, j);
+                const int tt = __shfl_sync(0xffffffffu, t, j);
+                c[j] = 0x8888u, sm[j] = 0;  // zeros where the slot is out of range
+                if (at < 0 || quad >= nq) continue;
+                sm[j] = *reinterpret_cast<const uint32_t*>(base + at + q4_param(tt, bs, D));
+                c[j] = *reinterpret_cast<const uint16_t*>(base + at + (is_v ? q4_v_quad(tt, quad, D) : q4_k_quad(tt, quad, D)));
+            }
+#pragma unroll
+            for (int j = 0; j < kGatherRows; j++) {
+                if (r0 + j >= n_rows || quad >= nq) continue;
+                const float2 p = q4_unpack(sm[j]);
+                const float4 v = make_float4(q4_value(c[j] & 15u, p.x, p.y), q4_value((c[j] >> 4) & 15u, p.x, p.y),
+                                             q4_value((c[j] >> 8) & 15u, p.x, p.y), q4_value(c[j] >> 12, p.x, p.y));
                 float* dst = out + (int64_t)(r0 + j) * D + 4 * quad;
                 if (vec) __stcs(reinterpret_cast<float4*>(dst), v);
                 else dst[0] = v.x, dst[1] = v.y, dst[2] = v.z, dst[3] = v.w;
@@ -202,7 +222,7 @@ int launch_gather_q4(s1kv_pool* p, int32_t layer, const int32_t* trow, const int
     if (rows > UINT32_MAX) return set_error(S1KV_EINVAL, "gather: more than 2^32 rows");
     for (int64_t r0 = 0; r0 < rows; r0 += (int64_t)1 << 30) {
         const uint32_t part = (uint32_t)std::min<int64_t>((int64_t)1 << 30, rows - r0);
-        const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)part + 31) / 32, kSMs * 16));
+        const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)part + 8 * kGatherRows - 1) / (8 * kGatherRows), kSMs * 32));
         gather_q4_kernel<<<grid, 256, 0, stream>>>(base, which != 0, trow, slots, part, (uint32_t)r0, p->desc.block_size,
                                                    p->desc.num_kv_heads, p->desc.head_dim, p->num_slots,
                                                    out + r0 * p->desc.head_dim, p->d_err);
