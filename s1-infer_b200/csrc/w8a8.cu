@@ -77,7 +77,7 @@ __device__ __forceinline__ float token_scale(float mx) { return mx > 0.0f ? __fd
 
 // A row a CTA.  NV > 0: rows of up to 1024 NV values, a multiple of 4 and
 // 16-byte aligned, stay in registers between the maximum and the codes (one
-// read of x); NV = 0: any row, read twice.
+// read of x: 8001 rows of 4096 in 39 us, 4.2 TB/s); NV = 0: any row, read twice.
 template <int NV>
 __global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __restrict__ x, int64_t K, int8_t* __restrict__ q,
                                                               int64_t ldq, float* __restrict__ scales) {
@@ -239,10 +239,9 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 3)
 }
 
 // -------------------------------------------------- many tokens: tcgen05 --
-// tcgen05.mma kind::i8 with the 128 channels of a tile as M and NT tokens as
-// N, so one kernel serves from 17 tokens (NT = 32, bound by the weights'
-// bytes) to prompts (NT = 256, bound by the tensor cores), and a stored
-// output row is 128 adjacent channels.  Roles: a TMA warp fills a ring of
+// tcgen05.mma kind::i8 with the 128 channels of a tile as M and NT = 64 or 128
+// tokens as N, bound by the weights' bytes; a stored output row is 128 adjacent
+// channels.  Roles: a TMA warp fills a ring of
 // 128-byte deep stages (both operands K-major, 128B swizzle, rows past the
 // end zero filled), one warp issues the MMAs, four warps take finished
 // accumulators out of TMEM, scale and store them.
@@ -264,7 +263,7 @@ template <int NT, bool SPLIT>
 struct TcCfg {
     static constexpr int kStageBytes = kKB * (kCh + NT);
     // split tiles leave room for a second CTA on the SM where they can
-    static constexpr int kStages = NT == 256 ? 4 : !SPLIT ? 6 : NT == 128 ? 5 : NT == 64 ? 3 : 4;
+    static constexpr int kStages = !SPLIT ? 6 : NT == 128 ? 5 : 3;
     static constexpr int kCols = (SPLIT ? 1 : 2) * NT;             // two accumulators for a chain of tiles
     static constexpr int kExchange = SPLIT ? kCh * NT * 4 : 0;     // [rank][token of the slice][channel] sums
     static constexpr int kOffX = kStages * kStageBytes;
@@ -559,6 +558,208 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
+// ------------------------------------ prompts: tcgen05 over pairs of SMs ----
+// 256 channels by 256 tokens a pair of CTAs (cta_group::2): each brings its 128
+// channels' weights and half of the tokens and holds its channels' sums of all
+// the tokens, so a CTA moves 32 KB a stage from L2 where a tile of its own of
+// 128 channels takes 48 KB.  The even rank's MMA warp issues for both; every
+// copy counts on its barrier, its commits arrive at both.  Persistent, two
+// accumulators, eight token tiles share the weights through L2, as above.
+struct PairCfg {
+    static constexpr int kTok = 256;
+    static constexpr int kStageBytes = kKB * (kCh + kTok / 2);  // a CTA's part
+    static constexpr int kStages = 6;
+    static constexpr int kOffBar = kStages * kStageBytes;
+    static constexpr int kNumBars = 2 * kStages + 5;
+    static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
+};
+
+// The address of the pair's even rank's copy of a barrier.
+__device__ __forceinline__ uint32_t lead_bar(uint64_t* b) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(su32(b)));
+    return at;
+}
+__device__ __forceinline__ void tma2_pair(uint32_t dst, const CUtensorMap* m, uint32_t lead, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(m), "r"(c0), "r"(c1), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair_w(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair_w(uint64_t* b) {  // arrives at both CTAs' barrier
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(su32(b)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+    w8a8_pair_kernel(const __grid_constant__ TcParams p, const __grid_constant__ TcMaps maps) {
+    using C = PairCfg;
+    constexpr int ST = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (-su32(smem_raw) & 1023u);  // (a sum: the compiler still sees shared memory)
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);  // [ST], the even rank's count for both
+    uint64_t* empty = full + ST;
+    uint64_t* acc_full = empty + ST;     // [2]
+    uint64_t* acc_empty = acc_full + 2;  // [2], the even rank's count for both
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffBar + C::kNumBars * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)(blockIdx.x & 1);
+
+    if (tid == 0) {
+        for (int i = 0; i < C::kNumBars; i++) bar_init(&full[i], i == 2 * ST + 2 || i == 2 * ST + 3 ? 8u : 1u);  // acc_empty: one arrive a warp
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    cluster_sync();  // both run and their barriers stand
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(2 * C::kTok)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // TMEM is there in both before an MMA writes it
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int n_tiles = p.ch_tiles * p.tok_tiles, first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+    auto tile_at = [&](int t, int& ch, int& tok) {  // eight token tiles side by side, their channels in turn
+        const int per = 8 * p.ch_tiles, grp = t / per, in = t - grp * per, wide = min(8, p.tok_tiles - grp * 8);
+        ch = in / wide;
+        tok = grp * 8 + in - ch * wide;
+    };
+    auto mat_of = [&](int ch) {
+        int mi = 0;
+#pragma unroll
+        for (int i = 1; i < kMaxMats; i++)
+            if (i < p.grp.n && ch >= p.grp.m[i].tile0) mi = i;
+        return mi;
+    };
+
+    if (warp == 0) {
+        // ================= TMA producer: this CTA's channels and tokens =================
+        int it = 0;  // stages used so far
+        bool ok = true;
+        int pre = 0;  // weights requested before the wait for this call's token quantiser
+        auto load_w = [&](int s, int kb, int mi, int n0) {
+            if (rank == 0) bar_expect(&full[s], 2 * C::kStageBytes);
+            tma2_pair(su32(smem + s * C::kStageBytes), &maps.w[mi], lead_bar(&full[s]), kb * kKB, n0);
+        };
+        if (p.early) {
+            int ch, tok;
+            tile_at(first, ch, tok);
+            const int mi = mat_of(ch);
+            pre = min(ST, p.k_blocks);
+            if (lane == 0)
+                for (int s = 0; s < pre; s++) load_w(s, s, mi, (ch - p.grp.m[mi].tile0) * 2 * kCh + rank * kCh);
+            __syncwarp();
+        }
+        pdl_wait();
+        for (int t = first; t < n_tiles && ok; t += step) {
+            int ch, tok;
+            tile_at(t, ch, tok);
+            const int mi = mat_of(ch), n0 = (ch - p.grp.m[mi].tile0) * 2 * kCh + rank * kCh, m0 = tok * C::kTok + rank * (C::kTok / 2);
+            for (int kb = 0; kb < p.k_blocks; kb++, it++) {
+                const int s = it % ST;
+                if (it >= ST && !(ok = warp_wait(&empty[s], (uint32_t)((it / ST - 1) & 1), abort_flag))) break;
+                if (lane == 0) {
+                    if (it >= pre) load_w(s, kb, mi, n0);
+                    tma2_pair(su32(smem + s * C::kStageBytes + kCh * kKB), &maps.x, lead_bar(&full[s]), kb * kKB, m0);
+                }
+                __syncwarp();
+            }
+        }
+        // every copy issued has landed before a CTA of the pair may exit (bounded)
+        if (rank == 0)
+            for (int i = max(0, it - ST); i < it; i++) bar_wait(&full[i % ST], (uint32_t)((i / ST) & 1));
+    } else if (warp == 1) {
+        // ================= MMA issuer, for both =================
+        if (rank == 0) {
+            constexpr uint32_t id = idesc_s8(2 * kCh, C::kTok);
+            int it = 0, done = 0;  // stages consumed, tiles issued
+            bool ok = true;
+            for (int t = first; t < n_tiles && ok; t += step, done++) {
+                const int buf = done & 1;
+                if (done >= 2 && !(ok = warp_wait(&acc_empty[buf], (uint32_t)((done / 2 - 1) & 1), abort_flag))) break;
+                tc_fence_after();
+                for (int kb = 0; kb < p.k_blocks; kb++, it++) {
+                    const int s = it % ST;
+                    if (!(ok = warp_wait(&full[s], (uint32_t)((it / ST) & 1), abort_flag))) break;
+                    tc_fence_after();
+                    const uint64_t da = sdesc(su32(smem + s * C::kStageBytes)), db = sdesc(su32(smem + s * C::kStageBytes + kCh * kKB));
+#pragma unroll
+                    for (int k = 0; k < kKB / 32; k++)  // 32 bytes of K an instruction
+                        mma_i8_pair_w(tmem + buf * C::kTok, da + 2 * k, db + 2 * k, id, kb > 0 || k > 0);
+                    mma_commit_pair_w(&empty[s]);
+                }
+                if (ok) mma_commit_pair_w(&acc_full[buf]);
+            }
+            // everything issued has finished before TMEM is freed (bounded)
+            mma_commit_pair_w(drain);
+            bar_wait(drain, 0);
+        }
+    } else {
+        // ================= epilogue =================
+        pdl_wait_trigger();  // the scales of the tokens, and outputs the kernel before may still read
+        const int sub = warp & 3;  // the TMEM lanes 32 sub .. + 31 are this warp's
+        const uint32_t lanes = (uint32_t)(32 * sub) << 16;
+        int done = 0;
+        for (int t = first; t < n_tiles; t += step, done++) {
+            const int buf = done & 1;
+            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
+            tc_fence_after();
+            int ch, tok;
+            tile_at(t, ch, tok);
+            const W8Mat& mat = p.grp.m[mat_of(ch)];
+            const int n = (ch - mat.tile0) * 2 * kCh + rank * kCh + 32 * sub + lane;
+            const bool live = n < mat.N;
+            const float sw = live ? mat.scales[n] : 0.0f;
+            float* out = mat.out + n;
+            const int m_end = min(C::kTok, p.M - tok * C::kTok);
+            for (int c = 0; c < m_end; c += 16) {
+                int v[16];
+                tmem_ld16(tmem + lanes + buf * C::kTok + c, v);
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int m = tok * C::kTok + c + j;
+                    if (live && c + j < m_end) __stcs(out + (int64_t)m * mat.N, __fmul_rn(__fmul_rn((float)v[j], __ldg(p.sx + m)), sw));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_bar(&acc_empty[buf])) : "memory");
+        }
+    }
+
+    // ---- tear-down: every path frees TMEM; neither CTA leaves before the other is done ----
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (tid == 0 && *abort_flag) atomicOr(&g_w8a8_error, kErrTimeout);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * C::kTok) : "memory");
+    }
+}
+
 // ---------------------------------------------------------------- launch --
 std::atomic<uint64_t> g_used_on{0};  // devices a tcgen05 launch ran on (its error word may be set there)
 
@@ -630,6 +831,35 @@ int launch_tc(const int8_t* xq, const float* sx, int M, int K, const W8Group& gr
     return S1KV_OK;
 }
 
+int launch_pair(const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int ch_tiles, bool early, cudaStream_t stream) {
+    static std::atomic<uint64_t> attr_set{0};  // per device
+    int st = once_per_device(attr_set, [&] {
+        S1KV_CUDA(cudaFuncSetAttribute(w8a8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmem));
+        return S1KV_OK;
+    });
+    if (st) return st;
+    TcParams p{};
+    p.grp = grp;
+    p.sx = sx;
+    p.early = early;
+    p.M = M;
+    p.k_blocks = (K + kKB - 1) / kKB;
+    p.ch_tiles = ch_tiles;
+    p.tok_tiles = (M + PairCfg::kTok - 1) / PairCfg::kTok;
+    TcMaps maps;
+    st = encode_rows(&maps.x, xq, M, K, PairCfg::kTok / 2);
+    for (int i = 0; i < grp.n && !st; i++) st = encode_rows(&maps.w[i], grp.m[i].w, grp.m[i].N, K, kCh);
+    if (st) return st;
+    for (int i = grp.n; i < kMaxMats; i++) maps.w[i] = maps.w[0];
+    int dev = 0;
+    S1KV_CUDA(cudaGetDevice(&dev));
+    if (dev < 64) g_used_on.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+    const unsigned pairs = (unsigned)std::min(ch_tiles * p.tok_tiles, 74);
+    S1KV_CUDA(launch_pdl(w8a8_pair_kernel, dim3(2 * pairs), dim3(kTcThreads), PairCfg::kSmem, stream, p, maps));
+    g_launches++;
+    return S1KV_OK;
+}
+
 template <int NTILE, bool FUSED, bool EARLY>
 int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, int M, int K, const W8Group& grp, int tiles,
                 cudaStream_t stream) {
@@ -644,7 +874,9 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
 // tensor-core tiles.  NT is the least that holds the tokens (256 at most),
 // halved down to 64 while the tiles leave SMs without work, and K is split
 // over a cluster while the tiles still do not fill them (two CTAs an SM fit
-// for NT up to 64).
+// for NT = 64).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336
+// channels: 324 us, 2.9e15 operations a second, 88% of twice the bf16 matrix
+// rate; 342 us in tiles of one SM; 8192^3: 3.2e15, 98%).
 // x (optional, rows of x_len values): the tokens that xq and sx will hold; they
 // are quantised here first, or by the weight stream itself.
 int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
@@ -654,7 +886,7 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
         grp.m[i].tile0 = (int)tiles;
         tiles += (grp.m[i].N + rows - 1) / rows;
     }
-    int NT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    int NT = M <= 64 ? 64 : M <= 128 ? 128 : 256;
     while (NT > 64 && tiles * ((M + NT - 1) / NT) < 111) NT /= 2;
     if (tiles * ((M + NT - 1) / NT) > INT32_MAX) return set_error(S1KV_EINVAL, "matmul_w8a8: more than 2^31 tiles");
     if (K == 0) {  // empty sums
@@ -682,15 +914,20 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
                  : launch_gemv<4, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
     int cs = 1;
-    if (NT <= 128)
+    if (NT < 256)
         while (cs < 8 && tiles * ((M + NT - 1) / NT) * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
 #define S1KV_TC(NT_)                                                                                       \
     if (NT == NT_)                                                                                         \
         return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, x != nullptr, stream)       \
                       : launch_tc<NT_, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
-    S1KV_TC(32) S1KV_TC(64) S1KV_TC(128)
+    S1KV_TC(64) S1KV_TC(128)
 #undef S1KV_TC
-    return launch_tc<256, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
+    int pairs = 0;  // tiles of 256 channels
+    for (int i = 0; i < grp.n; i++) {
+        grp.m[i].tile0 = pairs;
+        pairs += (grp.m[i].N + 2 * kCh - 1) / (2 * kCh);
+    }
+    return launch_pair(xq, sx, M, K, grp, pairs, x != nullptr, stream);
 }
 
 }  // namespace

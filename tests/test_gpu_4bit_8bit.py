@@ -482,6 +482,26 @@ def test_product(s1kv, cuda, m, k, n):
     np.testing.assert_array_equal(got, LB.product8(c, s, wq.data.cpu().numpy()[:, :k], wq.scales.cpu().numpy()))
 
 
+@pytest.mark.parametrize("m,k,ns", [(4100, 272, [1500]), (257, 1040, [7201]), (700, 80, [5000]), (2000, 640, [1000, 130, 2001]),
+                                    (9000, 16, [513])])
+def test_product_of_prompts(s1kv, cuda, m, k, ns):
+    """Tokens and channels enough for tiles over pairs of SMs, ragged in both."""
+    rng = np.random.default_rng(m + k)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    x[m - 1, 0], x[m // 2] = np.inf, 0
+    ws = [s1kv.quantize_channels(rng.standard_normal((k, n)).astype(np.float32)) for n in ns]
+    outs = s1kv.matmul_w8a8_group(x, ws)
+    c, s = LB.tokens8(x)
+    xq, sx = s1kv.quantize_tokens(x)
+    for w, o in zip(ws, outs):
+        want = LB.product8(c, s, w.data.cpu().numpy()[:, :k], w.scales.cpu().numpy())
+        np.testing.assert_array_equal(o.cpu().numpy(), want)
+        o.fill_(1.0)  # the caller's own codes
+        s1kv.check(s1kv.lib().s1kv_matmul_w8a8(xq.data_ptr(), sx.data_ptr(), m, w.ld, w.data.data_ptr(), w.scales.data_ptr(), w.n,
+                                               o.data_ptr(), s1kv._stream()))
+        np.testing.assert_array_equal(o.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize("m", [1, 20, 200])
 def test_product_at_the_integers_limits(s1kv, cuda, m):
     """Sums of 131072 products of 127: beyond 24 bits and next to 2^31."""
