@@ -2,13 +2,15 @@
 // q4.cuh) on warp-level tensor-core instructions (mma.sync m16n8k16, fp16 x
 // fp16 -> fp32).
 //
-// With u the raw codes, k = m_k + s_k (u - 8) and v = m_v + s_v (u - 8):
-//   score_t = s_k (q . u_t) + (m_k - 8 s_k) sum(q)
-//   out     = sum_t (p_t s_v) (u_t - 8) + sum_t p_t m_v,   over sum_t p_t
+// With c = u - 8 the centred codes, k = m_k + s_k c and v = m_v + s_v c:
+//   score_t = s_k (q . c_t) + m_k sum(q)
+//   out     = sum_t (p_t s_v) c_t + sum_t p_t m_v,   over sum_t p_t
 // so the products run over small integers, exact in fp16, and the scales
-// act on scores.  V's codes are centred before the product (out is a small
-// sum of terms of both signs; 15-level unsigned sums would cancel against
-// 8 sum(p s_v) and lose 7 to 8 bits for a few thousand tokens).
+// act on scores.  The codes are centred before the products: unsigned sums
+// would cancel against 8 sum(q) and 8 sum(p s_v).  (K's raw codes as fp16
+// subnormals, u 2^-24, need no arithmetic, but contexts of a few tokens were
+// off by up to 1.2e-6, now 2e-7, for 89 against 86 us on 64 rows of up to 8192
+// tokens.)
 //
 // Precision: q (times log2(e) / sqrt(D)) and p s_v are each split into two
 // fp16 parts, 22 bits, of values scaled by a power of two that puts the
@@ -24,12 +26,11 @@
 //   K: lane (g, t) = (L / 4, L % 4) takes dims 32 t .. 32 t + 31 of tokens g
 //      and g + 8.  The sum over dims does not care for their order, so q's
 //      fragments simply follow K's: nibbles n and n + 4 of a word are the
-//      halves of one fp16x2 register.  (w & 0x000f000f) read as fp16 is
-//      u 2^-24 (a subnormal, exact), (w & 0x00f000f0) is u 2^-20: one
-//      instruction per two codes, the factors go into q and the scores.
+//      halves of one fp16x2 register.
 //   V: lane (g, t) takes dims 16 g .. 16 g + 15 of token pairs t and t + 4;
-//      a word holds four dims of the two adjacent tokens.  (w & 0x000f000f) |
-//      0x6400 is 1024 + u, and one fp16x2 operation makes it u - 8.
+//      a word holds four dims of the two adjacent tokens.
+//   (w & 0x000f000f) | 0x64006400 is 1024 + u in both halves, and one fp16x2
+//   operation makes it u - 8 (q4_centred).
 // Query heads fill the N = 8 side: up to four heads take one mma with both
 // parts of q (or p) side by side in its columns, five to eight take two.
 //
@@ -54,8 +55,9 @@ constexpr uint32_t kSpin = 1u << 22;
 constexpr int kNS = 3;                 // stages a warp, of two tiles each
 // CTAs an SM, within 64K registers and 227 KB, as far as nothing spills in the
 // loop (a fifth CTA for D = 128 with two stages a warp: 90.7 against 85.7 us on
-// 64 rows of up to 8192 tokens).
-constexpr int ctas_per_sm(int D) { return D == 64 ? 6 : 4; }
+// 64 rows of up to 8192 tokens; a sixth for D = 64: 31.9 against 30.6 us on 200
+// rows of 1024 tokens, 4 KV heads).
+constexpr int ctas_per_sm(int D) { return D == 64 ? 5 : 4; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         // power of two that puts the pass's largest |q| in [2^14, 2^15)
         const int qe = min(max((int)(__float_as_uint(amax) >> 23), 40), 240);
         const float qscale = __uint_as_float((uint32_t)(127 + 14 + 127 - qe) << 23);
-        const float unscale = __uint_as_float((uint32_t)(qe - 14 + 24) << 23);  // 2^24 / qscale
+        const float unscale = __uint_as_float((uint32_t)(qe - 14) << 23);  // 1 / qscale
         uint32_t qf[NT][KS][2];
 #pragma unroll
         for (int wi = 0; wi < NWD; wi++)
@@ -234,9 +236,8 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     const int d = 8 * wi + 2 * j + b;
-                    const float f = qscale * (b ? 0.0625f : 1.0f);
                     uint32_t hi, lo;
-                    split_h2(x[d] * f, x[d + 4] * f, hi, lo);
+                    split_h2(x[d] * qscale, x[d + 4] * qscale, hi, lo);
                     if (NT == 1) {
                         qf[0][2 * wi + j][b] = gq < 4 ? hi : lo;
                     } else {
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         // lanes of a head), this lane's share of sum(p) and sum(p m_v)
         float m0 = -INFINITY, m1 = -INFINITY;
         float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
-        const float2 un2 = make_float2(unscale, unscale), qs2 = make_float2(qs0, qs1), off2 = make_float2(-8.0f * qs0, -8.0f * qs1);
+        const float2 un2 = make_float2(unscale, unscale), qs2 = make_float2(qs0, qs1);
         const float2 low = NT == 1 ? (tq < 2 ? make_float2(0.f, 0.f) : make_float2(-1.f, -1.f)) : make_float2(-1.f, -1.f);
         int E = kMinExp;  // V scales are taken relative to 2^(E - 127)
         float vmul = __uint_as_float((uint32_t)(260 - E) << 23);  // 2^(133 - E): the largest scaled s_v in [2^6, 2^7)
@@ -284,28 +285,27 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                 vb[u] = q4_unpack(vp[8]);
                 float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int wi = 0; wi < NWD; wi++)
+                for (int wi = 0; wi < NWD; wi++) {
+                    uint32_t c0[4], c1[4];
+                    q4_centred(k0[wi], c0);
+                    q4_centred(k1[wi], c1);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t a = k0[wi] >> (8 * j), b = k1[wi] >> (8 * j);
-                        const uint32_t a0 = a & 0x000F000Fu, a1 = b & 0x000F000Fu, a2 = a & 0x00F000F0u, a3 = b & 0x00F000F0u;
+                    for (int j = 0; j < 2; j++) {  // (small parts first: the sums are cut, not rounded)
+                        float(&sum)[4] = j ? sb : sa;
                         const int ks = 2 * wi + j;
-                        if (NT == 1) {
-                            mma16816(j ? sb : sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
-                        } else {
-                            mma16816(sa, a0, a1, a2, a3, qf[0][ks][0], qf[0][ks][1]);
-                            mma16816(sb, a0, a1, a2, a3, qf[NT - 1][ks][0], qf[NT - 1][ks][1]);
-                        }
+                        if (NT == 2) mma16816(sum, c0[2 * j], c1[2 * j], c0[2 * j + 1], c1[2 * j + 1], qf[NT - 1][ks][0], qf[NT - 1][ks][1]);
+                        mma16816(sum, c0[2 * j], c1[2 * j], c0[2 * j + 1], c1[2 * j + 1], qf[0][ks][0], qf[0][ks][1]);
                     }
+                }
                 float2 s0 = __fadd2_rn(make_float2(sa[0], sa[1]), make_float2(sb[0], sb[1]));
                 float2 s1 = __fadd2_rn(make_float2(sa[2], sa[3]), make_float2(sb[2], sb[3]));
                 if (NT == 1) {  // high + low part of q
                     s0 = __fadd2_rn(s0, make_float2(__shfl_xor_sync(kFull, s0.x, 2), __shfl_xor_sync(kFull, s0.y, 2)));
                     s1 = __fadd2_rn(s1, make_float2(__shfl_xor_sync(kFull, s1.x, 2), __shfl_xor_sync(kFull, s1.y, 2)));
                 }
-                // s (q . u - 8 sum(q)) + m sum(q)
-                x[u][0] = __ffma2_rn(make_float2(ka.x, ka.x), __ffma2_rn(s0, un2, off2), __fmul2_rn(make_float2(ka.y, ka.y), qs2));
-                x[u][1] = __ffma2_rn(make_float2(kb.x, kb.x), __ffma2_rn(s1, un2, off2), __fmul2_rn(make_float2(kb.y, kb.y), qs2));
+                // s (q . c) + m sum(q)
+                x[u][0] = __ffma2_rn(make_float2(ka.x, ka.x), __fmul2_rn(s0, un2), __fmul2_rn(make_float2(ka.y, ka.y), qs2));
+                x[u][1] = __ffma2_rn(make_float2(kb.x, kb.x), __fmul2_rn(s1, un2), __fmul2_rn(make_float2(kb.y, kb.y), qs2));
             }
             if (rest < 2 * kTile) {  // rows past the end hold anything, NaN included
 #pragma unroll
