@@ -46,14 +46,23 @@ int check_layer(const s1kv_pool* p, int32_t layer) {
 // kMaxSplitsPerRow splits of the longest row (the merge's counters and
 // groups are sized for that).
 // 4-bit pools: a tile is a quarter of bf16's bytes, so what a CTA costs besides
-// its tiles weighs more.  About two CTAs an SM until a CTA has 32 tiles, then
-// longer splits only past the 8 waves: 33 rows of up to 2049 tokens, 4 KV heads
-// of 64, took 17.7 us at 8 waves and 11.1 at two CTAs an SM; 64 rows of up to
-// 8192, 8 KV heads of 128, 85.7 at 8 waves, 125 at two CTAs an SM.
-int32_t plan_split_tiles(int64_t total_tiles, int64_t max_row_tiles, int32_t Hkv, int nw, bool q4) {
+// its tiles weighs more (as much as some 30 tiles).  The fewest full waves of
+// resident CTAs that keep a split within 32 tiles per warp, and until a CTA has
+// 32 tiles about two CTAs an SM; whole steps of every warp.  8 KV heads of 128,
+// us at one wave and at two of them: 16 rows of up to 8192 tokens 27.0 and 32.6,
+// 2 of 131072 (64 heads) 92.3 and 97.8, 64 of 8192 (one wave is past the limit)
+// 145 and 135.7; 33 rows of up to 2049 tokens, 4 KV heads of 64: 17.7 at two
+// waves, 11.1 at two CTAs an SM.
+int32_t plan_split_tiles(int64_t total_tiles, int64_t max_row_tiles, int32_t Hkv, int nw, int64_t q4_resident) {
+    const int64_t work = total_tiles * Hkv;
     int64_t target = (int64_t)kSMs * 8;
-    int64_t s = (total_tiles * Hkv + target - 1) / target;
-    if (q4) s = std::max<int64_t>(s, std::min<int64_t>(32, (total_tiles * Hkv + 2 * kSMs - 1) / (2 * kSMs)));
+    int64_t s = (work + target - 1) / target;
+    if (q4_resident) {
+        const int64_t waves = std::max<int64_t>(1, (work + 32 * nw * q4_resident - 1) / (32 * nw * q4_resident));
+        s = (work + waves * q4_resident - 1) / (waves * q4_resident);
+        s = std::max<int64_t>(s, std::min<int64_t>(32, (work + 2 * kSMs - 1) / (2 * kSMs)));
+        s = (s + nw - 1) / nw * nw;
+    }
     s = std::max<int64_t>(s, nw);
     s = std::min<int64_t>(s, 32 * nw);
     s = std::max<int64_t>(s, (max_row_tiles + kMaxSplitsPerRow - 1) / kMaxSplitsPerRow);
@@ -73,7 +82,7 @@ void plan_items(const s1kv_pool* p, s1kv_batch* b) {
         max_row_tiles = std::max<int64_t>(max_row_tiles, (m.kv_len + bs - 1) / bs);
     }
     b->split_tokens = plan_split_tiles(total_tiles, max_row_tiles, p->desc.num_kv_heads, nw,
-                                       p->desc.dtype == S1KV_DTYPE_Q4) * 16;
+                                       p->desc.dtype == S1KV_DTYPE_Q4 ? kSMs * decode_q4_ctas_per_sm(p->desc.head_dim) : 0) * 16;
     std::vector<WorkItem>& items = b->items;
     items.clear();
     int64_t n_part = 0;

@@ -454,6 +454,7 @@ int launch_gather_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const 
 int launch_rows_q4(s1kv_pool* pool, int32_t layer, const int32_t* trow, const int32_t* slots, int64_t n, int which,
                    void* rows, bool to_pool, cudaStream_t stream);
 bool decode_q4_supported(int D, int G, int block_size);
+int decode_q4_ctas_per_sm(int D);
 bool prefill_q4_supported(int D, int G, int block_size);
 int launch_prefill_q4(s1kv_batch* b, int32_t layer, const float* q, float* out, int32_t Hq, float scale_log2, int32_t max_kv,
                       cudaStream_t stream);

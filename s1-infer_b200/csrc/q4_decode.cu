@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
     const uint32_t bars = su32(smem) + kRing + warp * kNS * 8;
     int* flag = reinterpret_cast<int*>(smem + kRing + kNW * kNS * 8);
     const int gq = lane >> 2, tq = lane & 3;
-    const int h = blockIdx.y;
-    const WorkItem item = p.items[blockIdx.x];
+    const int h = blockIdx.x % p.Hkv;  // (an item's heads together: the longest items of all heads come first)
+    const WorkItem item = p.items[blockIdx.x / p.Hkv];
     const int tok0 = item.split * p.split_tokens;
     const int tok1 = min(tok0 + p.split_tokens, item.kv_len);
     const int n_tiles = (tok1 - tok0 + kTile - 1) / kTile;
@@ -549,6 +549,8 @@ bool decode_q4_supported(int D, int G, int block_size) {
     return (D == 64 || D == 128) && block_size == kTile && G >= 1 && G <= kMaxG;
 }
 
+int decode_q4_ctas_per_sm(int D) { return ctas_per_sm(D); }
+
 template <int D, int NT>
 static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
     constexpr int smem = kNW * kNS * (4 * kTile * (D / 2 + 4) + 8) + 16;
@@ -558,8 +560,8 @@ static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
         return S1KV_OK;
     });
     if (st) return st;
-    const dim3 grid((unsigned)p.n_items, (unsigned)p.Hkv);
-    S1KV_CUDA(launch_pdl(decode_q4_kernel<D, NT>, grid, dim3(kNW * 32), smem, stream, p, G));
+    if ((int64_t)p.n_items * p.Hkv > INT32_MAX) return set_error(S1KV_EINVAL, "decode: too many work items");
+    S1KV_CUDA(launch_pdl(decode_q4_kernel<D, NT>, dim3((unsigned)(p.n_items * p.Hkv)), dim3(kNW * 32), smem, stream, p, G));
     g_launches++;
     S1KV_CUDA(cudaGetLastError());
     return S1KV_OK;
