@@ -9,8 +9,7 @@
 // act on scores.  The codes are centred before the products: unsigned sums
 // would cancel against 8 sum(q) and 8 sum(p s_v).  (K's raw codes as fp16
 // subnormals, u 2^-24, need no arithmetic, but contexts of a few tokens were
-// off by up to 1.2e-6, now 2e-7, for 89 against 86 us on 64 rows of up to 8192
-// tokens.)
+// off by up to 1.2e-6, now 2e-7, for 4% more time.)
 //
 // Precision: q (times log2(e) / sqrt(D)) and p s_v are each split into two
 // fp16 parts, 22 bits, of values scaled by a power of two that puts the
@@ -37,6 +36,11 @@
 // Work: as the other decode kernels, a CTA takes one split-K item (row,
 // token range) of one KV head, its 4 warps the range's tiles in turn; warps
 // merge through shared memory, splits through combine.cuh.
+//
+// Bound: K's and V's bytes, and the instructions that widen them (46% of the
+// issue slots, ALU 45%, 16 warps an SM): 64 rows of 8192 tokens, 32 heads on 8
+// of 128, 136 us, 4.2 TB/s (bf16 pools: 314 us); 2 of 131072, 64 heads, 97 us,
+// 2.9 TB/s; 16 of up to 8192, 27 us.
 #include <cmath>
 
 #include "combine.cuh"
@@ -54,9 +58,8 @@ constexpr int kMinExp = 8;             // least exponent (biased) the V scales a
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kNS = 3;                 // stages a warp, of two tiles each
 // CTAs an SM, within 64K registers and 227 KB, as far as nothing spills in the
-// loop (a fifth CTA for D = 128 with two stages a warp: 90.7 against 85.7 us on
-// 64 rows of up to 8192 tokens; a sixth for D = 64: 31.9 against 30.6 us on 200
-// rows of 1024 tokens, 4 KV heads).
+// loop (a fifth CTA for D = 128 with two stages a warp: 6% slower on 64 rows of
+// up to 8192 tokens; a sixth for D = 64: 4% on 200 rows of 1024).
 constexpr int ctas_per_sm(int D) { return D == 64 ? 5 : 4; }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -374,22 +377,45 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                     b0[u][1] = movt(e0), b1[u][1] = movt(e1);
                 }
             }
-            // ---- O^T += V^T P^T: M = 16 dims per m-block, K = the 16 tokens ----
+            // ---- O^T += V^T P^T: M = 16 dims per m-block, K = 16 tokens.  The tensor
+            // cores cut what lies below the running sum.  NT = 2 (two products a tile):
+            // a pair's sum is taken apart, small parts first, and added with rounding
+            // (2 rows of 131072 tokens: error 1.3e-6 -> 1e-7 for 97 against 92 us); NT = 1
+            // stays within 3.3e-7 without. ----
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < (NT == 1 ? 2 : 1); u++) {
                 const char* at = kt + u * 2 * kTileBytes + kTileBytes;
-                uint32_t v0[NWD], v1[NWD];
-                load_words<NWD>(at + tq * D + gq * (4 * NWD), v0);
-                load_words<NWD>(at + (tq + 4) * D + gq * (4 * NWD), v1);
+                constexpr int NU = NT == 1 ? 1 : 2;
+                uint32_t v0[NU][NWD], v1[NU][NWD];
+#pragma unroll
+                for (int i = 0; i < NU; i++) {
+                    load_words<NWD>(at + i * 2 * kTileBytes + tq * D + gq * (4 * NWD), v0[i]);
+                    load_words<NWD>(at + i * 2 * kTileBytes + (tq + 4) * D + gq * (4 * NWD), v1[i]);
+                }
 #pragma unroll
                 for (int wi = 0; wi < NWD; wi++) {
-                    uint32_t c0[4], c1[4];
-                    q4_centred(v0[wi], c0);
-                    q4_centred(v1[wi], c1);
+                    uint32_t c0[NU][4], c1[NU][4];
+#pragma unroll
+                    for (int i = 0; i < NU; i++) {
+                        q4_centred(v0[i][wi], c0[i]);
+                        q4_centred(v1[i][wi], c1[i]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], b0[u][0], b1[u][0]);
-                        if (NT == 2) mma16816(o[2 * wi + j], c0[2 * j], c0[2 * j + 1], c1[2 * j], c1[2 * j + 1], b0[u][1], b1[u][1]);
+                        float(&acc)[4] = o[2 * wi + j];
+                        if constexpr (NT == 1) {
+                            mma16816(acc, c0[0][2 * j], c0[0][2 * j + 1], c1[0][2 * j], c1[0][2 * j + 1], b0[u][0], b1[u][0]);
+                        } else {
+                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int part = 1; part >= 0; part--)
+#pragma unroll
+                                for (int i = 0; i < 2; i++)
+                                    mma16816(sum, c0[i][2 * j], c0[i][2 * j + 1], c1[i][2 * j], c1[i][2 * j + 1], b0[i][part], b1[i][part]);
+                            const float2 x0 = __fadd2_rn(make_float2(acc[0], acc[1]), make_float2(sum[0], sum[1]));
+                            const float2 x1 = __fadd2_rn(make_float2(acc[2], acc[3]), make_float2(sum[2], sum[3]));
+                            acc[0] = x0.x, acc[1] = x0.y, acc[2] = x1.x, acc[3] = x1.y;
+                        }
                     }
                 }
             }
