@@ -419,7 +419,9 @@ int s1kv_batch_append(s1kv_batch* batch, int32_t layer, const float* k, const fl
  * append while the previous kernel of the stream is still running; every
  * kernel of this library that writes the pool elsewhere completes before a
  * later kernel starts.  A caller's own programmatic-dependent kernel that
- * writes the pool must therefore not come directly before this call. */
+ * writes the pool must therefore not come directly before this call.
+ * Attention calls of one pool share its scratch memory: order those on
+ * different streams. */
 int s1kv_batch_attention(s1kv_batch* batch, int32_t layer, const float* q, float* out, int32_t n_q_heads,
                          void* stream);
 /* End-to-end layer step with HOST buffers (pinned for full speed): copies

@@ -447,6 +447,48 @@ def test_graph_replay_and_another_stream(s1kv, cuda):
     plain.end()
 
 
+def test_prompts_captured_on_two_streams_at_once(s1kv, cuda):
+    """Chunk attention of two pools and prompt-sized products, captured into a
+    graph each and replayed at once on two streams, again and again."""
+    torch = cuda
+    rng = np.random.default_rng(75)
+    hkv, hq, dim, n = 4, 16, 64, 900
+    w = s1kv.quantize_channels(rng.standard_normal((hq * dim, 5000)).astype(np.float32))
+    runs = []
+    for i in range(2):
+        k, v = kv(rng, n, hkv, dim)
+        pool = pool_of(s1kv, hkv, dim, 60)
+        fill(pool, [n], k, v)
+        q = dev(rng.standard_normal((n - 100, hq, dim)).astype(np.float32))
+        b = pool.batch([0], None, [n - 100])
+        o, y = torch.empty_like(q), torch.empty((n - 100, 5000), device="cuda")
+
+        def step(b=b, q=q, o=o, y=y):
+            b.attention(0, q, o)
+            s1kv.matmul_w8a8(o.reshape(n - 100, -1), w, y)
+
+        step()
+        torch.cuda.synchronize()
+        want = o.clone(), y.clone()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            b.end()
+            b = pool.batch([0], None, [n - 100])
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step(b=b)
+        runs.append((stream, graph, o, y, want, b, q))
+    for _ in range(5):
+        for stream, graph, o, y, *_ in runs:
+            with torch.cuda.stream(stream):
+                o.zero_(), y.zero_()
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, o, y, want, b, _ in runs:
+        assert torch.equal(o, want[0]) and torch.equal(y, want[1])
+        b.end()
+
+
 # --------------------------------------------------------------- products --
 
 @pytest.mark.parametrize("m,k", [(1, 1), (3, 16), (5, 33), (1, 4096), (130, 1000), (2, 131072)])
