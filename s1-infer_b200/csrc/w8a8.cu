@@ -114,10 +114,11 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __res
 }
 
 int launch_quantize(const float* x, int64_t M, int64_t K, int8_t* q, int64_t ldq, float* scales, cudaStream_t stream) {
-    const int nv = K % 4 || ((uintptr_t)x & 15) || ldq > 8192 ? 0 : ldq <= 1024 ? 1 : ldq <= 2048 ? 2 : ldq <= 4096 ? 4 : 8;
+    const int nv = K % 4 || ((uintptr_t)x & 15) || ldq > 16384 ? 0 : ldq <= 1024 ? 1 : ldq <= 2048 ? 2 : ldq <= 4096 ? 4 : ldq <= 8192 ? 8 : 16;
     auto kern = nv == 0 ? quantize_tokens_kernel<0>
                         : nv == 1 ? quantize_tokens_kernel<1>
-                                  : nv == 2 ? quantize_tokens_kernel<2> : nv == 4 ? quantize_tokens_kernel<4> : quantize_tokens_kernel<8>;
+                                  : nv == 2 ? quantize_tokens_kernel<2>
+                                  : nv == 4 ? quantize_tokens_kernel<4> : nv == 8 ? quantize_tokens_kernel<8> : quantize_tokens_kernel<16>;
     S1KV_CUDA(launch_pdl(kern, dim3((unsigned)M), dim3(256), 0, stream, x, K, q, ldq, scales));
     g_launches++;
     return S1KV_OK;
@@ -262,8 +263,8 @@ constexpr int kTcThreads = 192;      // TMA warp, MMA warp, 4 epilogue warps
 template <int NT, bool SPLIT>
 struct TcCfg {
     static constexpr int kStageBytes = kKB * (kCh + NT);
-    // split tiles leave room for a second CTA on the SM where they can
-    static constexpr int kStages = !SPLIT ? 6 : NT == 128 ? 5 : 3;
+    // split tiles leave room for a second CTA on the SM
+    static constexpr int kStages = SPLIT ? 3 : 6;
     static constexpr int kCols = (SPLIT ? 1 : 2) * NT;             // two accumulators for a chain of tiles
     static constexpr int kExchange = SPLIT ? kCh * NT * 4 : 0;     // [rank][token of the slice][channel] sums
     static constexpr int kOffX = kStages * kStageBytes;
@@ -418,6 +419,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // ================= TMA producer =================
         int it = 0;  // stages used so far
         bool ok = true;
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w[0]) : "memory");
+        }
         // the weights of the first stages do not depend on this call's token
         // quantiser: requested before the wait for it
         int pre = 0;
@@ -514,13 +519,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     int v[16];
                     tmem_ld16(tmem + lanes + c, v);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int owner = (c + j) / per;
+                    for (int j0 = 0; j0 < 16; j0 += 8) {  // per is 8 or more
+                        const int owner = (c + j0) / per;
                         uint32_t at;
                         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                                      : "=r"(at)
-                                     : "r"(mine + (uint32_t)((c + j - owner * per) * kCh * 4)), "r"(owner));
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+                                     : "r"(mine + (uint32_t)((c + j0 - owner * per) * kCh * 4)), "r"(owner));
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + j * kCh * 4), "r"(v[j0 + j]) : "memory");
                     }
                 }
             }
@@ -532,21 +539,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     // ---- tear-down: every path frees TMEM ----
     __syncthreads();
-    if (SPLIT) {  // every rank's sums have arrived
+    if (SPLIT) {
+        // this rank's slice: a token a warp, four channels a lane; the scales are
+        // on their way while the other ranks' sums arrive
         pdl_wait();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         int ch, tok;
         tile_at(blockIdx.x, ch, tok);
         const W8Mat& mat = p.grp.m[mat_of(ch)];
-        const int per = NT / cs;
-        const int* got = reinterpret_cast<const int*>(smem + C::kOffX);
-        for (int i = tid; i < per * kCh; i += kTcThreads) {
-            const int c = i / kCh, n = (ch - mat.tile0) * kCh + i % kCh, m = tok * NT + rank * per + c;
-            int sum = 0;
-            for (int r = 0; r < cs; r++) sum += got[r * per * kCh + i];
-            if (m < p.M && n < mat.N)
-                mat.out[(int64_t)m * mat.N + n] = __fmul_rn(__fmul_rn((float)sum, __ldg(p.sx + m)), mat.scales[n]);
+        constexpr int kWarps = kTcThreads / 32, kMost = (NT / 2 + kWarps - 1) / kWarps;
+        const int per = NT / cs, n = (ch - mat.tile0) * kCh + 4 * lane, m0 = tok * NT + rank * per;
+        float sw[4], sm[kMost];
+#pragma unroll
+        for (int j = 0; j < 4; j++) sw[j] = n + j < mat.N ? mat.scales[n + j] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMost; i++) {
+            const int c = warp + kWarps * i;
+            sm[i] = c < per && m0 + c < p.M ? __ldg(p.sx + m0 + c) : 0.0f;
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        const int* got = reinterpret_cast<const int*>(smem + C::kOffX) + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < kMost; i++) {
+            const int c = warp + kWarps * i, m = m0 + c;
+            if (c >= per || m >= p.M) break;
+            int sum[4] = {0, 0, 0, 0};
+            for (int r = 0; r < cs; r++) {
+                const int4 v = *reinterpret_cast<const int4*>(got + (r * per + c) * kCh);
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            }
+            float* out = mat.out + (int64_t)m * mat.N + n;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (n + j < mat.N) out[j] = __fmul_rn(__fmul_rn((float)sum[j], sm[i]), sw[j]);
         }
     }
     tc_fence_before();
@@ -872,9 +897,12 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
 // Which kernel, by the tokens: up to 32 the weight stream (32 tokens, K = 4096,
 // 6144 channels: 13.8 us against 14.6 in tiles; 16: 9.3 us); above, the
 // tensor-core tiles.  NT is the least that holds the tokens (256 at most),
-// halved down to 64 while the tiles leave SMs without work, and K is split
-// over a cluster while the tiles still do not fill them (two CTAs an SM fit
-// for NT = 64).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336
+// halved down to 64 while there are fewer than 90 tiles (256 tokens, K = 4096,
+// 6144 channels: 96 tiles of 128 tokens 15.6 us, 192 of 64 19.8; 4096 channels:
+// 64 tiles 15.0, 128 of 64 12.6); then K is split
+// over a cluster, at least two stages a CTA, two CTAs an SM, if the tiles are
+// fewer than two thirds of the SMs (64 tokens, K = 4096: 48 tiles 10.1 us split
+// in four, 12.6 unsplit; 112 tiles 16.5 in two, 15.5 unsplit).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336
 // channels: 324 us, 2.9e15 operations a second, 88% of twice the bf16 matrix
 // rate; 342 us in tiles of one SM; 8192^3: 3.2e15, 98%).
 // x (optional, rows of x_len values): the tokens that xq and sx will hold; they
@@ -887,7 +915,7 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
         tiles += (grp.m[i].N + rows - 1) / rows;
     }
     int NT = M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    while (NT > 64 && tiles * ((M + NT - 1) / NT) < 111) NT /= 2;
+    while (NT > 64 && tiles * ((M + NT - 1) / NT) < 90) NT /= 2;
     if (tiles * ((M + NT - 1) / NT) > INT32_MAX) return set_error(S1KV_EINVAL, "matmul_w8a8: more than 2^31 tiles");
     if (K == 0) {  // empty sums
         for (int i = 0; i < grp.n; i++)
@@ -913,15 +941,14 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
         return x ? launch_gemv<4, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
                  : launch_gemv<4, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
-    int cs = 1;
-    if (NT < 256)
-        while (cs < 8 && tiles * ((M + NT - 1) / NT) * cs * 2 <= (NT == 128 ? 148 : 296) && k_blocks >= cs * 4) cs *= 2;
-#define S1KV_TC(NT_)                                                                                       \
-    if (NT == NT_)                                                                                         \
-        return cs > 1 ? launch_tc<NT_, true>(xq, sx, M, K, grp, (int)tiles, cs, x != nullptr, stream)       \
-                      : launch_tc<NT_, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
-    S1KV_TC(64) S1KV_TC(128)
-#undef S1KV_TC
+    const int64_t all = tiles * ((M + NT - 1) / NT);
+    if (NT == 64) {
+        int cs = 1;
+        while (cs < 8 && all <= 98 && all * cs * 2 <= 296 && k_blocks >= cs * 4) cs *= 2;
+        return cs > 1 ? launch_tc<64, true>(xq, sx, M, K, grp, (int)tiles, cs, x != nullptr, stream)
+                      : launch_tc<64, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
+    }
+    if (NT == 128) return launch_tc<128, false>(xq, sx, M, K, grp, (int)tiles, 1, x != nullptr, stream);
     int pairs = 0;  // tiles of 256 channels
     for (int i = 0; i < grp.n; i++) {
         grp.m[i].tile0 = pairs;
