@@ -894,22 +894,25 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
     return S1KV_OK;
 }
 
-// Which kernel, by the tokens: up to 32 the weight stream (32 tokens, K = 4096,
-// 6144 channels: 13.8 us against 14.6 in tiles; 16: 9.3 us); above, the
-// tensor-core tiles.  NT is the least that holds the tokens (256 at most),
-// halved down to 64 while there are fewer than 90 tiles (256 tokens, K = 4096,
-// 6144 channels: 96 tiles of 128 tokens 15.6 us, 192 of 64 19.8; 4096 channels:
-// 64 tiles 15.0, 128 of 64 12.6); then K is split
-// over a cluster, at least two stages a CTA, two CTAs an SM, if the tiles are
-// fewer than two thirds of the SMs (64 tokens, K = 4096: 48 tiles 10.1 us split
-// in four, 12.6 unsplit; 112 tiles 16.5 in two, 15.5 unsplit).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336
-// channels: 324 us, 2.9e15 operations a second, 88% of twice the bf16 matrix
-// rate; 342 us in tiles of one SM; 8192^3: 3.2e15, 98%).
+// Which kernel, by the tokens: up to 16 the weight stream, and up to 32 while the
+// weights are small (32 tokens, with the quantiser: 4 MB 6.0 us against 8.0 in
+// tiles, 25 MB 13.7 and 12.3, 59 MB 29 and 16); above, the tensor-core tiles.
+// NT is the least that holds the tokens (256 at most), halved down to 64 while
+// there are fewer than 90 tiles (256 tokens, K = 4096, 6144 channels: 96 tiles of
+// 128 tokens 15.6 us, 192 of 64 19.8; 4096 channels: 64 tiles 15.0, 128 of 64
+// 12.6); then K is split over a cluster, at least two stages a CTA, two CTAs an
+// SM, if the tiles are fewer than two thirds of the SMs (64 tokens, K = 4096: 48
+// tiles 10.1 us split in four, 12.6 unsplit; 112 tiles 16.5 in two, 15.5
+// unsplit).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336 channels:
+// 324 us, 2.9e15 operations a second, 88% of twice the bf16 matrix rate; 342 us
+// in tiles of one SM; 8192^3: 3.2e15, 98%).
 // x (optional, rows of x_len values): the tokens that xq and sx will hold; they
 // are quantised here first, or by the weight stream itself.
 int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
-    const int rows = M <= 32 || K == 0 ? 16 : kCh;
-    int64_t tiles = 0;
+    int64_t channels = 0, tiles = 0;
+    for (int i = 0; i < grp.n; i++) channels += grp.m[i].N;
+    const bool stream_w = M <= 16 || (M <= 32 && channels * K <= (20 << 20));
+    const int rows = stream_w || K == 0 ? 16 : kCh;
     for (int i = 0; i < grp.n; i++) {
         grp.m[i].tile0 = (int)tiles;
         tiles += (grp.m[i].N + rows - 1) / rows;
@@ -937,7 +940,7 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
     if (M <= 16)
         return x ? launch_gemv<2, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
                  : launch_gemv<2, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
-    if (M <= 32)
+    if (stream_w)
         return x ? launch_gemv<4, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
                  : launch_gemv<4, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     const int k_blocks = (K + kKB - 1) / kKB;
