@@ -894,9 +894,10 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
     return S1KV_OK;
 }
 
-// Which kernel, by the tokens: up to 16 the weight stream, and up to 32 while the
-// weights are small (32 tokens, with the quantiser: 4 MB 6.0 us against 8.0 in
-// tiles, 25 MB 13.7 and 12.3, 59 MB 29 and 16); above, the tensor-core tiles.
+// Which kernel, by the tokens: up to 8 the weight stream, and up to 32 while the
+// weights are small (with the quantiser, in tiles beside it: 16 tokens, 25 MB 9.3
+// us and 12.9, 59 MB 18.6 and 16.5, 67 MB 24.3 and 19.1; 32 tokens, 4 MB 6.0 and
+// 8.0, 25 MB 13.7 and 12.3, 59 MB 29 and 16); above, the tensor-core tiles.
 // NT is the least that holds the tokens (256 at most), halved down to 64 while
 // there are fewer than 90 tiles (256 tokens, K = 4096, 6144 channels: 96 tiles of
 // 128 tokens 15.6 us, 192 of 64 19.8; 4096 channels: 64 tiles 15.0, 128 of 64
@@ -911,7 +912,7 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
 int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
     int64_t channels = 0, tiles = 0;
     for (int i = 0; i < grp.n; i++) channels += grp.m[i].N;
-    const bool stream_w = M <= 16 || (M <= 32 && channels * K <= (20 << 20));
+    const bool stream_w = M <= 8 || (M <= 32 && channels * K <= (M <= 16 ? 48 : 20) << 20);
     const int rows = stream_w || K == 0 ? 16 : kCh;
     for (int i = 0; i < grp.n; i++) {
         grp.m[i].tile0 = (int)tiles;
@@ -937,7 +938,7 @@ int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, 
     if (M <= 8)
         return x ? launch_gemv<1, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
                  : launch_gemv<1, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
-    if (M <= 16)
+    if (stream_w && M <= 16)
         return x ? launch_gemv<2, false, true>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream)
                  : launch_gemv<2, false, false>(nullptr, 0, xq, sx, M, K, grp, (int)tiles, stream);
     if (stream_w)

@@ -511,7 +511,7 @@ def test_token_codes(s1kv, cuda, m, k):
 PRODUCTS = [(1, 16, 1), (1, 1024, 2048), (1, 1020, 333), (1, 1022, 50), (1, 1040, 70), (2, 100, 77), (7, 48, 130), (8, 4096, 256), (9, 512, 300), (16, 2000, 129), (17, 64, 64),
             (33, 1000, 777), (64, 4096, 512), (65, 272, 200), (128, 128, 128), (129, 1040, 385), (256, 1536, 1000),
             (300, 4096, 520), (1000, 80, 50), (2049, 512, 640), (5, 131072, 40), (50, 600, 200), (100, 48, 11700), (3, 14336, 70),
-            (34, 131072, 130), (20, 4096, 5200), (32, 512, 300)]
+            (34, 131072, 130), (20, 4096, 5200), (32, 512, 300), (11, 8192, 6200)]
 
 
 @pytest.mark.parametrize("m,k,n", PRODUCTS)
