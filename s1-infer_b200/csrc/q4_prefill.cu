@@ -68,7 +68,7 @@ struct Cfg {
     static constexpr int kOffK = 4 * kQBytes;
     static constexpr int kOffV = kOffK + kKBytes;
     static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
-    static constexpr int kOffXch = kOffPar + 2 * (kN * 12 + 32);  // floats [4][2 halves][256 rows]
+    static constexpr int kOffXch = kOffPar + 2 * (kN * 16 + 48);  // floats [4][2 halves][256 rows]
     static constexpr int kOffRef = kOffXch + 4 * 4 * 2 * kM * 2;  // float2 [512] (max, exponent)
     static constexpr int kOffIds = kOffRef + 512 * 8;
     static constexpr int kOffBar = kOffIds + kIdsCached * 4;
@@ -236,7 +236,9 @@ struct RowState {
 struct TilePar {
     float mk[kN], mv[kN];
     float sv[kN];   // s_v 2^(133 - E)
-    float f[4];     // K's tokens 32 g .. + 31 stand in the tile as s_k c / f[g], a power of two
+    float fk[kN];   // K's token t stands in the tile as s_k c / fk[t], a power of two
+    float f[4];     // fk of all the tokens 32 g .. + 31 where uneven[g] is 0
+    int uneven[4];  // 1: these tokens' s_k and m_k lie too far apart for one power of two (or s_k is 0)
     int E;          // largest exponent of s_v so far
     int pad[3];
 };
@@ -275,10 +277,13 @@ __device__ __forceinline__ void scale_p(uint32_t tS, int cols, float f) {
 // is scaled; at the end the row's two threads agree on the larger reference.
 // (A pass of its own for the maximum, agreed on before the weights, took 2200
 // of 5400 cycles a tile.)  The loop stays rolled: unrolled over all scores the
-// code runs from beyond the instruction cache.  EDGE: only tokens up to `last`
-// (of this tile) are seen; the others may hold anything, NaN included.  fresh:
-// O starts anew with this tile.
-template <bool EDGE, int D>
+// code runs from beyond the instruction cache.  ANY: only tokens up to `last`
+// (of this tile) are seen, the others may hold anything, NaN included; and K's
+// rows may have any scales: the score is v (un fk) + m_k (qs un), so that m_k is
+// not divided by a scale (0, for a row of equal values).  Else m_k qs / f joins
+// v in units of 1 / (un f), one operation a score.  fresh: O starts anew with
+// this tile.
+template <bool ANY, int D>
 __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int t0, int last, RowState& st,
                                              bool fresh, float* xch, int xch_other, uint32_t pair, uint32_t phase,
                                              uint32_t p_full, uint32_t abort_flag, int lane) {
@@ -288,7 +293,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
     tmem_ld16(tS, v[0]);
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
-        const float f = par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f), un = st.un * f;
+        const float f = ANY ? 1.0f : par.f[(t0 + c) / 32], qs = ANY ? st.qs * st.un : __fdividef(st.qs, f), un = ANY ? 1.0f : st.un * f;
         const float2 qs2 = make_float2(qs, qs), un2 = make_float2(un, un);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -300,9 +305,19 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + 2 * i]);
-                x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, make_float2(v[u][2 * i], v[u][2 * i + 1]));
-                x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, make_float2(v[u][2 * i + 2], v[u][2 * i + 3]));
-                if (EDGE) {
+                x[i] = make_float2(v[u][2 * i], v[u][2 * i + 1]);
+                x[i + 1] = make_float2(v[u][2 * i + 2], v[u][2 * i + 3]);
+                if (ANY) {
+                    const float4 fk = *reinterpret_cast<const float4*>(&par.fk[c0 + 2 * i]);
+                    const float2 a = __fmul2_rn(make_float2(fk.x, fk.y), make_float2(st.un, st.un));
+                    const float2 b = __fmul2_rn(make_float2(fk.z, fk.w), make_float2(st.un, st.un));
+                    x[i] = __ffma2_rn(x[i], a, __fmul2_rn(make_float2(k.x, k.y), qs2));
+                    x[i + 1] = __ffma2_rn(x[i + 1], b, __fmul2_rn(make_float2(k.z, k.w), qs2));
+                } else {
+                    x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, x[i]);
+                    x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, x[i + 1]);
+                }
+                if (ANY) {
                     if (c0 + 2 * i > last) x[i].x = -INFINITY;
                     if (c0 + 2 * i + 1 > last) x[i].y = -INFINITY;
                     if (c0 + 2 * i + 2 > last) x[i + 1].x = -INFINITY;
@@ -310,7 +325,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                 }
                 top = fmaxf(fmaxf(top, fmaxf(x[i].x, x[i].y)), fmaxf(x[i + 1].x, x[i + 1].y));
             }
-            top *= un;
+            if (!ANY) top *= un;
             const bool raise = top > m + kRescaleAt;
             if (__any_sync(0xffffffffu, raise)) {
                 const float mn = raise ? ceilf(top) : m, r = from_max(m, mn);
@@ -328,9 +343,9 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                 const float4 sv = *reinterpret_cast<const float4*>(&par.sv[c0 + 2 * i]);
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    const float2 y = __ffma2_rn(x[i + w], un2, nm2);
+                    const float2 y = ANY ? __fadd2_rn(x[i + w], nm2) : __ffma2_rn(x[i + w], un2, nm2);
                     float2 mm = w ? make_float2(mv.z, mv.w) : make_float2(mv.x, mv.y);
-                    if (EDGE) {  // 0 times what an unseen token holds
+                    if (ANY) {  // 0 times what an unseen token holds
                         if (c0 + 2 * (i + w) > last) mm.x = 0.0f;
                         if (c0 + 2 * (i + w) + 1 > last) mm.y = 0.0f;
                     }
@@ -422,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
     volatile int* aside_slot = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 8);
     TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
-    static_assert(sizeof(TilePar) == kN * 12 + 32, "two tiles' parameters");
+    static_assert(sizeof(TilePar) == kN * 16 + 48, "two tiles' parameters");
     int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -613,10 +628,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             // reaches the rows that see it through m
             par_t.sv[i] = va.x < INFINITY ? va.x * pow2(127 + kVUp - E) : 0.0f;
             if (i == 0) par_t.E = E;
-            const uint32_t ek = __reduce_max_sync(0xffffffffu, ka.x < INFINITY ? __float_as_uint(ka.x) >> 23 : 0u);
-            const uint32_t kx = max(ek, (uint32_t)kMinExp);
-            if (lane == 0) par_t.f[wi] = pow2((int)kx - 127 - kUp);
-            const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - (int)kx));
+            // one power of two for the 32 tokens if their scales are within 2^20 of
+            // the largest (8 of fp16's bits carry the code and s) and m / s is not so large
+            // nor s so small that m qs / f could overflow; else one a token
+            const bool held = ka.x < INFINITY;
+            const uint32_t et = held ? __float_as_uint(ka.x) >> 23 : 0u, em = held ? __float_as_uint(fabsf(ka.y)) >> 23 : 0u;
+            const uint32_t ek = __reduce_max_sync(0xffffffffu, et);
+            const bool uneven = ek < 64 || __any_sync(0xffffffffu, held && (et + 20 < ek || em > ek + 40));
+            const int kx = max((int)(uneven ? et : ek), kMinExp);
+            const float fk = pow2(kx - 127 - kUp);
+            par_t.fk[i] = fk;
+            if (lane == 0) {
+                par_t.f[wi] = fk;
+                par_t.uneven[wi] = uneven;
+            }
+            const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - kx));
             uint8_t* kt = smem + C::kOffK;
 #pragma unroll
             for (int c = 0; c < NK; c++) {
@@ -791,7 +817,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             tc_fence_after();
             const int base = (tb + t) * kN;
             // (the pair's phase 0 was q's)
-            if (base + kN - 1 > prefix + q0)  // some row of the chunk does not see all of it
+            const int4 uneven = *reinterpret_cast<const int4*>(par[ph].uneven);
+            if (base + kN - 1 > prefix + q0 || (uneven.x | uneven.y | uneven.z | uneven.w))  // some row of the chunk does not see all of it
                 ok = softmax_tile<true, D>(tS, tO, par[ph], 64 * half, row_limit - base, st, fresh, x_mine + ph * 4 * kM, x_other, pair,
                                            ph ^ 1u, p_full + 8 * X, abort_flag, lane);
             else

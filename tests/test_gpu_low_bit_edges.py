@@ -1,0 +1,89 @@
+"""GPU tests of the 4-bit cache and the 8-bit product where they can go wrong:
+rows of equal values, scales far apart, and what the pool's other calls meet.
+
+Tolerance of attention: as in test_gpu_4bit_8bit.py a weight is off by S 2^-21
+at most, relative, for scores of up to S < 32 in log2 units: 1.5e-5; the sums
+and the two fp16 parts of p s_v leave a few 2^-23 more.  So an output element
+is within 2e-5 of sum_t p_t |v_t|, taken as its largest over the row's dims:
+each row and head is held to its own size, whatever the others hold."""
+import numpy as np
+import pytest
+
+from oracle import lowbit as LB
+from test_gpu_4bit_8bit import dev, fill, kv, pool_of
+
+pytestmark = pytest.mark.gpu
+TOL = 2e-5
+
+
+def check_rows(got, q, k, v, lens=None):
+    """got [rows, Hq, D] against 64 bits on what the cache holds of k and v."""
+    k, v = LB.q4_values(k), LB.q4_values(v)
+    want, size = LB.attention64(q, k, v), LB.attention64(q, k, np.abs(v)).max(-1, keepdims=True)
+    assert got.shape == want.shape and np.isfinite(want).all()
+    assert np.isfinite(got).all(), "not finite"
+    err = (np.abs(got - want) / np.maximum(size, 1e-300)).max()
+    assert err <= TOL, err
+
+
+def attend_and_check(s1kv, k, v, r, hq, seed=0, q=None):
+    n, hkv, dim = k.shape
+    if q is None:
+        q = np.random.default_rng(seed).standard_normal((r, hq, dim)).astype(np.float32)
+    pool = pool_of(s1kv, hkv, dim, -(-n // 16) + 4)
+    fill(pool, [n], k, v)
+    got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
+    assert pool.check_device() == 0
+    check_rows(got, q, k, v)
+
+
+# ------------------------------------------------------ keys of scale zero --
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("r", [1, 3, 60, 170])
+@pytest.mark.parametrize("kind", ["zeros", "ones", "value", "head", "group", "last", "tiny", "first"])
+def test_keys_of_equal_values(s1kv, cuda, dim, r, kind):
+    """K rows whose values are all the same are held with s = 0 (or a tiny s):
+    their scores are m sum(q) alone."""
+    rng = np.random.default_rng(80)
+    hkv, hq, n = 2, 8, 193  # the last group of 32 keys holds one
+    k, v = kv(rng, n, hkv, dim)
+    if kind == "zeros":
+        k[:] = 0
+    elif kind == "ones":
+        k[:] = 1
+    elif kind == "value":
+        k[:] = 3.3 / 8  # not a bf16 number
+    elif kind == "head":
+        k[:, 1] = 0
+    elif kind == "group":
+        k[32:64] = 0
+        k[96:128, 0] = -0.5
+    elif kind == "last":
+        k[192] = 0
+    elif kind == "tiny":
+        k *= np.float32(1e-35)
+    else:
+        k[:40] = 0
+    attend_and_check(s1kv, k, v, r, hq)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 33, 64])
+def test_short_prompts_of_zero_keys(s1kv, cuda, dim, n):
+    v = kv(np.random.default_rng(81), n, 1, dim)[1]
+    attend_and_check(s1kv, np.zeros((n, 1, dim), np.float32), v, n, 4)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("r", [1, 150])
+def test_keys_of_scales_far_apart(s1kv, cuda, dim, r):
+    """Keys of 2^-40 beside ordinary ones in every group, and keys with a large
+    common value beside a small spread (m / s of 2^9 and, seldom, 2^20)."""
+    rng = np.random.default_rng(82)
+    k, v = kv(rng, 300, 2, dim)
+    k[::3] *= np.float32(2.0 ** -40)
+    k[1::7] = k[1::7] * np.float32(2.0 ** -11) + np.float32(0.25)
+    k[5::50] = np.float32(0.25)
+    k[5::50, :, 0] += np.float32(2.0 ** -22)
+    attend_and_check(s1kv, k, v, r, 8)
