@@ -54,7 +54,10 @@ constexpr int kNW = 4;
 constexpr int kTile = 16;
 constexpr int kMaxG = 128;             // query heads per KV head the merge's scratch covers (least: 36 G of 6912 floats)
 constexpr float kRescaleAt = 8.0f;     // log2 units
-constexpr int kMinExp = 8;             // least exponent (biased) the V scales are taken relative to
+constexpr int kMinExp = 8;             // least exponent (biased) V's rows are taken relative to
+// A V row counts by the exponent of max(s, |m| / 2^kBelowM); rows kEven below the
+// largest or more are weighed each by its own, down to kFar below.
+constexpr int kBelowM = 8, kEven = 6, kFar = 80;
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kNS = 3;                 // stages a warp, of two tiles each
 // CTAs an SM, within 64K registers and 227 KB, as far as nothing spills in the
@@ -116,6 +119,13 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                  "r"(bytes), "r"(b)
                  : "memory");
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+// What the V rows of (s, m) a and b count by (a NaN row: NaN).
+__device__ __forceinline__ float2 q4_size(float2 a, float2 b) {
+    return make_float2(fmaxf(a.x, fabsf(a.y) * (1.0f / (1 << kBelowM))), fmaxf(b.x, fabsf(b.y) * (1.0f / (1 << kBelowM))));
+}
+// Biased exponent of x >= 0; 0 of a NaN.
+__device__ __forceinline__ int exponent_of(float x) { return x < INFINITY ? (int)(__float_as_uint(x) >> 23) : 0; }
 template <int NWD>
 __device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[NWD]) {
     if constexpr (NWD == 4) {
@@ -318,29 +328,62 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                 }
             }
             // the reference max of a head moves only when a score outgrows it
-            // by 2^8, and E only when an s_v outgrows it: both are rare
+            // by 2^8, and E only when a V row outgrows it: both are rare, and so
+            // are V rows of 2^kEven below E
             float mx0 = fmaxf(fmaxf(x[0][0].x, x[0][1].x), fmaxf(x[1][0].x, x[1][1].x));
             float mx1 = fmaxf(fmaxf(x[0][0].y, x[0][1].y), fmaxf(x[1][0].y, x[1][1].y));
-            const float sv = fmaxf(fmaxf(va[0].x, vb[0].x), fmaxf(va[1].x, vb[1].x));
-            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || (int)(__float_as_uint(sv) >> 23) > E)) {
+            // a V row counts by max(s, |m| / 2^kBelowM)
+            const float2 ra = q4_size(va[0], va[1]), rb = q4_size(vb[0], vb[1]);
+            const float most = fmaxf(fmaxf(ra.x, ra.y), fmaxf(rb.x, rb.y)), least = fminf(fminf(ra.x, ra.y), fminf(rb.x, rb.y));
+            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || exponent_of(most) > E || exponent_of(least) + kEven < E)) {
+                // The reference is one for the weights p s_v, which must fit fp16:
+                // scores plus V's exponents relative to E (down to -kFar).  A V row
+                // that is hardly weighed then takes no bits from the others,
+                // however large it is; p may pass 2^8 by as much as V's exponents
+                // lie below E.
+                float c0 = 1.0f, c1 = 1.0f;
+                const int ne = max(E, (int)__reduce_max_sync(kFull, (unsigned)exponent_of(most)));
+                if (ne > E) {
+                    // m falls by as much, which leaves the sums of p s_v as they are,
+                    // as far as l and z stay in range (l to 2^100, z to 2^113)
+                    int u0 = max(exponent_of(l2.x) + 13, exponent_of(fabsf(z2.x))), u1 = max(exponent_of(l2.y) + 13, exponent_of(fabsf(z2.y)));
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) {
+                        u0 = max(u0, __shfl_xor_sync(kFull, u0, off));
+                        u1 = max(u1, __shfl_xor_sync(kFull, u1, off));
+                    }
+                    const int d = ne - E, by0 = max(min(min(d, 120), 237 - u0), 0), by1 = max(min(min(d, 120), 237 - u1), 0);
+                    m0 -= (float)by0;
+                    m1 -= (float)by1;
+                    l2 = make_float2(l2.x * pow2(by0), l2.y * pow2(by1));
+                    z2 = make_float2(z2.x * pow2(by0), z2.y * pow2(by1));
+                    c0 = by0 - d < -126 ? 0.0f : pow2(by0 - d);
+                    c1 = by1 - d < -126 ? 0.0f : pow2(by1 - d);
+                    E = ne;
+                    vmul = __uint_as_float((uint32_t)(260 - E) << 23);
+                }
+                mx0 = mx1 = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float r = i ? (u ? rb.y : rb.x) : (u ? ra.y : ra.x), ev = (float)max(exponent_of(r) - E, -kFar);
+                        mx0 = fmaxf(mx0, x[u][i].x + ev);
+                        mx1 = fmaxf(mx1, x[u][i].y + ev);
+                    }
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     mx0 = fmaxf(mx0, __shfl_xor_sync(kFull, mx0, off));
                     mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, off));
                 }
                 const bool r0 = mx0 > m0 + kRescaleAt, r1 = mx1 > m1 + kRescaleAt;
-                float c0 = r0 ? ex2(m0 - mx0) : 1.0f, c1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
+                const float f0 = r0 ? ex2(m0 - mx0) : 1.0f, f1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
                 if (r0) m0 = mx0;
                 if (r1) m1 = mx1;
-                l2 = make_float2(l2.x * c0, l2.y * c1);
-                z2 = make_float2(z2.x * c0, z2.y * c1);
-                const int e = min((int)(__float_as_uint(sv) >> 23), 254);
-                const int ne = max(E, (int)__reduce_max_sync(kFull, (unsigned)e));
-                const float ce = ne - E > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (ne - E)) << 23);
-                E = ne;
-                vmul = __uint_as_float((uint32_t)(260 - E) << 23);
-                c0 *= ce;
-                c1 *= ce;
+                l2 = make_float2(l2.x * f0, l2.y * f1);
+                z2 = make_float2(z2.x * f0, z2.y * f1);
+                c0 *= f0;
+                c1 *= f1;
 #pragma unroll
                 for (int mb = 0; mb < KS; mb++) {
                     o[mb][0] *= c0;
@@ -445,12 +488,19 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             z0 += __shfl_xor_sync(kFull, z0, off);
             z1 += __shfl_xor_sync(kFull, z1, off);
         }
+        // a sum of more than 2^40 goes into the reference: the merges take that for the scores' maximum
+        const int up0 = l0 > 1.0995116e12f ? exponent_of(l0) - 127 : 0, up1 = l1 > 1.0995116e12f ? exponent_of(l1) - 127 : 0;
+        const float down0 = pow2(-max(up0, 0)), down1 = pow2(-max(up1, 0));
+        m0 += (float)max(up0, 0);
+        m1 += (float)max(up1, 0);
+        l0 *= down0;
+        l1 *= down1;
 #pragma unroll
         for (int mb = 0; mb < KS; mb++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if (NT == 1) o[mb][i] += __shfl_xor_sync(kFull, o[mb][i], 2);
-                o[mb][i] = fmaf(o[mb][i], back, i & 1 ? z1 : z0);
+                o[mb][i] = fmaf(o[mb][i], back, i & 1 ? z1 : z0) * (i & 1 ? down1 : down0);
             }
         __syncthreads();  // every warp's tiles are consumed
         if (2 * tq < GP) {  // dims D / 8 gq + 2 mb (rows g) and + 1 (rows g + 8) of heads 2 tq, 2 tq + 1

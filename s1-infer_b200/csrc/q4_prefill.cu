@@ -57,6 +57,9 @@ constexpr float kRescaleAt = 8.0f;
 constexpr int kMinExp = 20;         // least exponent (biased) scales are taken relative to
 constexpr int kUp = 11;             // K's largest s stands as 2^11 .. 2^12 in its fp16 tile: 8 s below 2^15
 constexpr int kVUp = 6;             // V's largest s counts as 2^6 .. 2^7 beside p: p s below 2^15
+// A V row counts by the exponent of max(s, |m| / 2^kBelowM): rows kEven below the
+// largest or more are weighed each by its own, down to kFar below.
+constexpr int kBelowM = 8, kEven = 6, kFar = 80;
 constexpr int kIdsCached = 1024;   // block ids kept in shared memory (16K tokens)
 
 template <int D>
@@ -68,7 +71,7 @@ struct Cfg {
     static constexpr int kOffK = 4 * kQBytes;
     static constexpr int kOffV = kOffK + kKBytes;
     static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
-    static constexpr int kOffXch = kOffPar + 2 * (kN * 16 + 48);  // floats [4][2 halves][256 rows]
+    static constexpr int kOffXch = kOffPar + 2 * (kN * 20 + 48);  // floats [4][2 halves][256 rows]
     static constexpr int kOffRef = kOffXch + 4 * 4 * 2 * kM * 2;  // float2 [512] (max, exponent)
     static constexpr int kOffIds = kOffRef + 512 * 8;
     static constexpr int kOffBar = kOffIds + kIdsCached * 4;
@@ -236,10 +239,11 @@ struct RowState {
 struct TilePar {
     float mk[kN], mv[kN];
     float sv[kN];   // s_v 2^(133 - E)
+    float ev[kN];   // V's exponent less E, -kFar at least
     float fk[kN];   // K's token t stands in the tile as s_k c / fk[t], a power of two
     float f[4];     // fk of all the tokens 32 g .. + 31 where uneven[g] is 0
-    int uneven[4];  // 1: these tokens' s_k and m_k lie too far apart for one power of two (or s_k is 0)
-    int E;          // largest exponent of s_v so far
+    int uneven[4];  // 1: these tokens' s_k and m_k lie too far apart for one power of two (or s_k is 0), or V's exponents do
+    int E;          // largest exponent of V so far
     int pad[3];
 };
 
@@ -247,9 +251,10 @@ struct TilePar {
 __device__ __forceinline__ float from_max(float m_old, float m) {
     return m_old == m ? 1.0f : m - m_old < 127.0f ? pow2((int)(m_old - m)) : 0.0f;  // (0 from m' = -inf)
 }
-// 2^(m' - m) 2^(E' - E): from sums that refer to (m', E') to (m, E).
+// 2^(m' - m) 2^(E' - E): from sums that refer to (m', E') to (m, E); never more than 1.
 __device__ __forceinline__ float rebase(float m_old, int e_old, float m, int e) {
-    return e - e_old > 126 ? 0.0f : from_max(m_old, m) * pow2(e_old - e);
+    const float k = (m_old - m) + (float)(e_old - e);
+    return k > -127.0f ? pow2((int)fminf(k, 0.0f)) : 0.0f;  // (0 from m' = -inf)
 }
 
 // The first `cols` columns of this thread's P times a power of two (exact but
@@ -283,6 +288,11 @@ __device__ __forceinline__ void scale_p(uint32_t tS, int cols, float f) {
 // not divided by a scale (0, for a row of equal values).  Else m_k qs / f joins
 // v in units of 1 / (un f), one operation a score.  fresh: O starts anew with
 // this tile.
+// The reference is one for the weights p s_v, which must fit fp16: m follows the
+// largest score plus V's exponent relative to E, so a V row that a token does not
+// see, or hardly weighs, takes no bits from the others however large it is.
+// Where the rows' exponents are even the scores alone will do.  Then p may pass
+// 2^8, by as much as V's exponents lie below E.
 template <bool ANY, int D>
 __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const TilePar& par, int t0, int last, RowState& st,
                                              bool fresh, float* xch, int xch_other, uint32_t pair, uint32_t phase,
@@ -291,6 +301,16 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
     float m = st.m;
     float2 l2 = st.l, z2 = st.z;
     tmem_ld16(tS, v[0]);
+    if (par.E != st.E) {
+        // E has risen: m falls by as much, which leaves the sums of p s_v as they
+        // are, as far as l and z stay in range (l to 2^100, z to 2^113)
+        const int el = (int)(__float_as_uint(l2.x + l2.y) >> 23) + 13, ez = (int)(__float_as_uint(fmaxf(fabsf(z2.x), fabsf(z2.y))) >> 23);
+        const int room = max(min(min(par.E - st.E, 120), 240 - max(el, ez)), 0);
+        const float f = pow2(room);
+        m -= (float)room;
+        l2 = make_float2(l2.x * f, l2.y * f);
+        z2 = make_float2(z2.x * f, z2.y * f);
+    }
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
         const float f = ANY ? 1.0f : par.f[(t0 + c) / 32], qs = ANY ? st.qs * st.un : __fdividef(st.qs, f), un = ANY ? 1.0f : st.un * f;
@@ -317,13 +337,17 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                     x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, x[i]);
                     x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, x[i + 1]);
                 }
+                float2 w0 = x[i], w1 = x[i + 1];
                 if (ANY) {
                     if (c0 + 2 * i > last) x[i].x = -INFINITY;
                     if (c0 + 2 * i + 1 > last) x[i].y = -INFINITY;
                     if (c0 + 2 * i + 2 > last) x[i + 1].x = -INFINITY;
                     if (c0 + 2 * i + 3 > last) x[i + 1].y = -INFINITY;
+                    const float4 ev = *reinterpret_cast<const float4*>(&par.ev[c0 + 2 * i]);
+                    w0 = __fadd2_rn(x[i], make_float2(ev.x, ev.y));
+                    w1 = __fadd2_rn(x[i + 1], make_float2(ev.z, ev.w));
                 }
-                top = fmaxf(fmaxf(top, fmaxf(x[i].x, x[i].y)), fmaxf(x[i + 1].x, x[i + 1].y));
+                top = fmaxf(fmaxf(top, fmaxf(w0.x, w0.y)), fmaxf(w1.x, w1.y));
             }
             if (!ANY) top *= un;
             const bool raise = top > m + kRescaleAt;
@@ -437,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
     volatile int* aside_slot = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 8);
     TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
-    static_assert(sizeof(TilePar) == kN * 16 + 48, "two tiles' parameters");
+    static_assert(sizeof(TilePar) == kN * 20 + 48, "two tiles' parameters");
     int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -570,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         uint4 kr[NK];  // one tile of K or V at a time: K's next loads wait for V's conversion, registers are short
         uint4 (&vr)[NK] = kr;
         uint32_t pk = 0, pv[4];  // this thread's token of K; V's tokens lane + 32 j (every warp works out the tile's largest s_v)
-        int E = kMinExp;         // largest exponent of s_v so far
+        int E = kMinExp;         // largest exponent of V so far
         auto block = [&](int t, int b) -> int32_t {  // block b of local tile t
             const int j = t * (kN / 16) + b;
             return j < kIdsCached ? ids[j] : lookup(b0 + j);
@@ -613,15 +637,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             // them (S(t - 1), which k_empty tracks, was issued after it)
             TilePar& par_t = par[ph];
             const float2 ka = q4_unpack(pk);
-            uint32_t ev = 0;
+            const int wi = warp & 3;
+            uint32_t top_v = 0, low_v = 255, ev = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float x = q4_unpack(pv[j]).x;
-                ev = max(ev, x < INFINITY ? __float_as_uint(x) >> 23 : 0u);
+                const float2 a = q4_unpack(pv[j]);
+                const uint32_t x = a.x < INFINITY ? __float_as_uint(fmaxf(a.x, fabsf(a.y) * (1.0f / (1 << kBelowM)))) >> 23 : 0u;
+                top_v = max(top_v, x);
+                low_v = min(low_v, x);
+                if (j == wi) ev = x;
             }
-            E = max(E, (int)__reduce_max_sync(0xffffffffu, ev));
-            const int wi = warp & 3;
+            E = max(E, (int)__reduce_max_sync(0xffffffffu, top_v));
+            const bool uneven_v = (int)__reduce_min_sync(0xffffffffu, low_v) + kEven < E;
             const float2 va = q4_unpack(wi == 0 ? pv[0] : wi == 1 ? pv[1] : wi == 2 ? pv[2] : pv[3]);
+            par_t.ev[i] = (float)max((int)ev - E, -kFar);
             par_t.mk[i] = ka.y;
             par_t.mv[i] = va.y;
             // a V row that cannot be held (s = m = NaN) counts as zeros here: its NaN
@@ -640,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             par_t.fk[i] = fk;
             if (lane == 0) {
                 par_t.f[wi] = fk;
-                par_t.uneven[wi] = uneven;
+                par_t.uneven[wi] = uneven || uneven_v;
             }
             const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - kx));
             uint8_t* kt = smem + C::kOffK;
@@ -849,10 +878,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             warp_wait(pair, (uint32_t)((n_tiles + 1) & 1), abort_flag);
             const float l = l_mine + x_mine[2 * 4 * kM + x_other], z = z_mine + x_mine[3 * 4 * kM + x_other];
             const float back = pow2(st.E - 127 - kVUp);
-            const float inv = split ? 1.0f : 1.0f / l;
+            // (a split's l of more than 2^40 goes into its reference: the join takes that for the scores' maximum)
+            const int up = l > 1.0995116e12f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
+            const float inv = split ? pow2(-up) : 1.0f / l;
             if (split && valid_ && half_ == 0) {
-                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2] = st.m;
-                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2 + 1] = l;
+                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2] = st.m + (float)up;
+                p.part_ml[((int64_t)blockIdx.y * p.n_rows * p.Hq + at) * 2 + 1] = l * pow2(-up);
             }
             // Half rows go through this warp's part of q's tiles (every product
             // that read q is done), so that a row's columns are written together.

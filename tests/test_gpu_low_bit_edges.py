@@ -87,3 +87,97 @@ def test_keys_of_scales_far_apart(s1kv, cuda, dim, r):
     k[5::50] = np.float32(0.25)
     k[5::50, :, 0] += np.float32(2.0 ** -22)
     attend_and_check(s1kv, k, v, r, 8)
+
+
+# ------------------------------------------------- values of far-off scales --
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("r", [1, 40, 200])
+@pytest.mark.parametrize("at,grow", [(230, 16), (230, 20), (230, 40), (230, 70), (100, 30), (299, 60), (0, 40)])
+def test_a_large_value_row(s1kv, cuda, dim, r, at, grow):
+    """One V row 2^16 to 2^70 larger than the others: query rows before it do
+    not see it and keep their precision, whatever the tile holds."""
+    rng = np.random.default_rng(83)
+    k, v = kv(rng, 300, 2, dim)
+    v[at] *= np.float32(2.0 ** grow)
+    attend_and_check(s1kv, k, v, r, 8)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hq", [4, 8])
+@pytest.mark.parametrize("r", [1, 90])
+@pytest.mark.parametrize("grow", [20, 40, 60])
+@pytest.mark.parametrize("where", ["early", "late", "both"])
+def test_a_large_value_row_that_weighs_little(s1kv, cuda, dim, hq, r, grow, where):
+    """The large V rows are seen, but their scores lie 56 log2 units below the
+    others': what they add is small, and the others keep their precision."""
+    rng = np.random.default_rng(84)
+    n, hkv = 600, 1
+    u = rng.standard_normal(dim).astype(np.float32)
+    u *= np.float32(np.sqrt(dim) / np.linalg.norm(u))
+    side = np.ones(n, np.float32)
+    for i in {"early": (3, 17), "late": (500,), "both": (0, 200, 509)}[where]:
+        side[i] = -1
+    top = 28 * np.log(2) / np.sqrt(dim)
+    k = ((side[:, None] * u * top) + 0.01 * rng.standard_normal((n, dim))).astype(np.float32)[:, None]
+    v = rng.standard_normal((n, hkv, dim)).astype(np.float32)
+    v[side < 0] *= np.float32(2.0 ** grow)
+    q = (np.tile(u, (r, hq, 1)) + 0.02 * rng.standard_normal((r, hq, dim))).astype(np.float32)
+    attend_and_check(s1kv, k, v, r, hq, q=q)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("r", [1, 300])
+@pytest.mark.parametrize("shape", ["rise", "fall", "constants", "huge", "offset"])
+def test_value_rows_of_all_sizes(s1kv, cuda, dim, r, shape):
+    """V rows that grow or shrink by 2^100 over the sequence, rows of equal
+    values (s = 0) among others, rows next to fp32's end, rows of a large
+    common value."""
+    rng = np.random.default_rng(85)
+    n = 500
+    k, v = kv(rng, n, 2, dim)
+    if shape in ("rise", "fall"):
+        steps = np.linspace(-60, 40, n) * (1 if shape == "rise" else -1)
+        v *= np.exp2(np.floor(steps)).astype(np.float32)[:, None, None]
+    elif shape == "constants":
+        v[::2] = np.float32(3.3)
+        v[1::6] = 0
+    elif shape == "huge":
+        v *= np.float32(1e34)
+        v[::5] = np.float32(3.3)
+        v[3::5] = np.float32(1e36)
+    else:
+        v = v * np.float32(2.0 ** -10) + np.float32(4.0)
+    attend_and_check(s1kv, k, v, r, 4)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_chunks_with_large_value_rows(s1kv, cuda, dim):
+    """As many chunks as SMs, so that none is split and sums are set aside on
+    the way: V rows of 2^50 here and there, and a steady growth of 2^40."""
+    rng = np.random.default_rng(86)
+    hkv, hq, n, r = 8, 32, 1570, 1301
+    k, v = kv(rng, n, hkv, dim)
+    k *= np.float32(0.2)
+    v[:, 2] *= np.exp2(np.floor(np.arange(n) * 41 / n)).astype(np.float32)[:, None]
+    v[[700, 1400], 0] *= np.float32(2.0 ** 50)
+    v[[300, 301, 1569], 5] *= np.float32(2.0 ** 24)
+    q = rng.standard_normal((r, hq, dim)).astype(np.float32)
+    pool = pool_of(s1kv, hkv, dim, 100)
+    fill(pool, [n], k, v)
+    got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
+    for h in (0, 2, 5):
+        heads = slice(4 * h, 4 * h + 4)
+        check_rows(got[:, heads], q[:, heads], k[:, h:h + 1], v[:, h:h + 1])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_decode_with_large_value_rows(s1kv, cuda, dim):
+    """Rows split over CTAs: the splits' references differ by far."""
+    rng = np.random.default_rng(87)
+    k, v = kv(rng, 9000, 1, dim)
+    v[[5, 4000, 8990]] *= np.float32(2.0 ** 40)
+    v[3000:3500] *= np.float32(2.0 ** -50)
+    attend_and_check(s1kv, k, v, 1, 4)
+    attend_and_check(s1kv, k, v, 1, 12)
+    attend_and_check(s1kv, k, v, 3, 4)
