@@ -55,9 +55,9 @@ constexpr int kTile = 16;
 constexpr int kMaxG = 128;             // query heads per KV head the merge's scratch covers (least: 36 G of 6912 floats)
 constexpr float kRescaleAt = 8.0f;     // log2 units
 constexpr int kMinExp = 8;             // least exponent (biased) V's rows are taken relative to
-// A V row counts by the exponent of max(s, |m| / 2^kBelowM); rows kEven below the
-// largest or more are weighed each by its own, down to kFar below.
-constexpr int kBelowM = 8, kEven = 6, kFar = 80;
+// A V row counts by the exponent of max(s, |m| / 2^kBelowM) where rows are uneven,
+// some s kEven powers of two below the largest or more; kFar below it at least.
+constexpr int kBelowM = 8, kEven = 6, kFar = 80, kAbove = 60;
 constexpr uint32_t kSpin = 1u << 22;
 constexpr int kNS = 3;                 // stages a warp, of two tiles each
 // CTAs an SM, within 64K registers and 227 KB, as far as nothing spills in the
@@ -120,10 +120,6 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
-// What the V rows of (s, m) a and b count by (a NaN row: NaN).
-__device__ __forceinline__ float2 q4_size(float2 a, float2 b) {
-    return make_float2(fmaxf(a.x, fabsf(a.y) * (1.0f / (1 << kBelowM))), fmaxf(b.x, fabsf(b.y) * (1.0f / (1 << kBelowM))));
-}
 // Biased exponent of x >= 0; 0 of a NaN.
 __device__ __forceinline__ int exponent_of(float x) { return x < INFINITY ? (int)(__float_as_uint(x) >> 23) : 0; }
 template <int NWD>
@@ -270,8 +266,10 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
         const float2 un2 = make_float2(unscale, unscale), qs2 = make_float2(qs0, qs1);
         const float2 low = NT == 1 ? (tq < 2 ? make_float2(0.f, 0.f) : make_float2(-1.f, -1.f)) : make_float2(-1.f, -1.f);
-        int E = kMinExp;  // V scales are taken relative to 2^(E - 127)
-        float vmul = __uint_as_float((uint32_t)(260 - E) << 23);  // 2^(133 - E): the largest scaled s_v in [2^6, 2^7)
+        // V's scales are taken relative to 2^(E - 127), E the largest exponent of an s_v so far: vmul =
+        // 2^(133 - E) puts the largest in [2^6, 2^7)
+        float vmul = __uint_as_float((uint32_t)(260 - kMinExp) << 23);
+        auto exponent_v = [&] { return 260 - (int)(__float_as_uint(vmul) >> 23); };  // E
         int done = 0;
         for (int k = 0; k < pairs; k++) {
             const int it = it0 + k, stage = it % kNS;
@@ -332,42 +330,37 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             // are V rows of 2^kEven below E
             float mx0 = fmaxf(fmaxf(x[0][0].x, x[0][1].x), fmaxf(x[1][0].x, x[1][1].x));
             float mx1 = fmaxf(fmaxf(x[0][0].y, x[0][1].y), fmaxf(x[1][0].y, x[1][1].y));
-            // a V row counts by max(s, |m| / 2^kBelowM)
-            const float2 ra = q4_size(va[0], va[1]), rb = q4_size(vb[0], vb[1]);
-            const float most = fmaxf(fmaxf(ra.x, ra.y), fmaxf(rb.x, rb.y)), least = fminf(fminf(ra.x, ra.y), fminf(rb.x, rb.y));
-            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || exponent_of(most) > E || exponent_of(least) + kEven < E)) {
+            const float most = fmaxf(fmaxf(va[0].x, vb[0].x), fmaxf(va[1].x, vb[1].x));
+            const float least = fminf(fminf(va[0].x, vb[0].x), fminf(va[1].x, vb[1].x));
+            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || most * vmul >= 128.0f || least * vmul < 64.0f / (1 << kEven))) {
                 // The reference is one for the weights p s_v, which must fit fp16:
                 // scores plus V's exponents relative to E (down to -kFar).  A V row
                 // that is hardly weighed then takes no bits from the others,
                 // however large it is; p may pass 2^8 by as much as V's exponents
                 // lie below E.
-                float c0 = 1.0f, c1 = 1.0f;
-                const int ne = max(E, (int)__reduce_max_sync(kFull, (unsigned)exponent_of(most)));
-                if (ne > E) {
-                    // m falls by as much, which leaves the sums of p s_v as they are,
-                    // as far as l and z stay in range (l to 2^100, z to 2^113)
-                    int u0 = max(exponent_of(l2.x) + 13, exponent_of(fabsf(z2.x))), u1 = max(exponent_of(l2.y) + 13, exponent_of(fabsf(z2.y)));
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        u0 = max(u0, __shfl_xor_sync(kFull, u0, off));
-                        u1 = max(u1, __shfl_xor_sync(kFull, u1, off));
-                    }
-                    const int d = ne - E, by0 = max(min(min(d, 120), 237 - u0), 0), by1 = max(min(min(d, 120), 237 - u1), 0);
-                    m0 -= (float)by0;
-                    m1 -= (float)by1;
-                    l2 = make_float2(l2.x * pow2(by0), l2.y * pow2(by1));
-                    z2 = make_float2(z2.x * pow2(by0), z2.y * pow2(by1));
-                    c0 = by0 - d < -126 ? 0.0f : pow2(by0 - d);
-                    c1 = by1 - d < -126 ? 0.0f : pow2(by1 - d);
-                    E = ne;
-                    vmul = __uint_as_float((uint32_t)(260 - E) << 23);
+                float c = 1.0f;
+                const int d = (int)__reduce_max_sync(kFull, (unsigned)exponent_of(most)) - exponent_v();
+                if (d > 0) {
+                    // m falls by as much as E rises, which leaves the sums of p s_v as
+                    // they are, as far as l and z stay in range (l to 2^100, z to 2^113)
+                    const int u = max(exponent_of(fmaxf(l2.x, l2.y)) + 13, exponent_of(fmaxf(fabsf(z2.x), fabsf(z2.y))));
+                    const int by = max(min(min(d, 120), 237 - (int)__reduce_max_sync(kFull, (unsigned)u)), 0);
+                    const float g = pow2(by);
+                    m0 -= (float)by;
+                    m1 -= (float)by;
+                    l2 = make_float2(l2.x * g, l2.y * g);
+                    z2 = make_float2(z2.x * g, z2.y * g);
+                    c = by - d < -126 ? 0.0f : pow2(by - d);
+                    vmul = __uint_as_float(__float_as_uint(vmul) - ((uint32_t)d << 23));
                 }
                 mx0 = mx1 = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        const float r = i ? (u ? rb.y : rb.x) : (u ? ra.y : ra.x), ev = (float)max(exponent_of(r) - E, -kFar);
+                        const float2 r = i ? vb[u] : va[u];
+                        const int e = exponent_of(fmaxf(r.x, fabsf(r.y) * (1.0f / (1 << kBelowM)))) - exponent_v();
+                        const float ev = (float)min(max(e, -kFar), kAbove);
                         mx0 = fmaxf(mx0, x[u][i].x + ev);
                         mx1 = fmaxf(mx1, x[u][i].y + ev);
                     }
@@ -377,13 +370,13 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                     mx1 = fmaxf(mx1, __shfl_xor_sync(kFull, mx1, off));
                 }
                 const bool r0 = mx0 > m0 + kRescaleAt, r1 = mx1 > m1 + kRescaleAt;
-                const float f0 = r0 ? ex2(m0 - mx0) : 1.0f, f1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
+                float c0 = r0 ? ex2(m0 - mx0) : 1.0f, c1 = r1 ? ex2(m1 - mx1) : 1.0f;  // 0 from m = -inf
                 if (r0) m0 = mx0;
                 if (r1) m1 = mx1;
-                l2 = make_float2(l2.x * f0, l2.y * f1);
-                z2 = make_float2(z2.x * f0, z2.y * f1);
-                c0 *= f0;
-                c1 *= f1;
+                l2 = make_float2(l2.x * c0, l2.y * c1);
+                z2 = make_float2(z2.x * c0, z2.y * c1);
+                c0 *= c;
+                c1 *= c;
 #pragma unroll
                 for (int mb = 0; mb < KS; mb++) {
                     o[mb][0] *= c0;
@@ -480,7 +473,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         it0 += pairs;
         float l0 = l2.x, l1 = l2.y, z0 = z2.x, z1 = z2.y;
         // ---- merge the warps through shared memory (over the rings) ----
-        const float back = __uint_as_float((uint32_t)(E - 6) << 23);  // 1 / vmul
+        const float back = __uint_as_float((254u << 23) - __float_as_uint(vmul));  // 1 / vmul
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
             l0 += __shfl_xor_sync(kFull, l0, off);

@@ -57,9 +57,12 @@ constexpr float kRescaleAt = 8.0f;
 constexpr int kMinExp = 20;         // least exponent (biased) scales are taken relative to
 constexpr int kUp = 11;             // K's largest s stands as 2^11 .. 2^12 in its fp16 tile: 8 s below 2^15
 constexpr int kVUp = 6;             // V's largest s counts as 2^6 .. 2^7 beside p: p s below 2^15
-// A V row counts by the exponent of max(s, |m| / 2^kBelowM): rows kEven below the
-// largest or more are weighed each by its own, down to kFar below.
-constexpr int kBelowM = 8, kEven = 6, kFar = 80;
+// A V row counts by the exponent of max(s, |m| / 2^kBelowM) where rows are uneven,
+// some s kEven powers of two below the largest or more; kFar below it at least.
+constexpr int kBelowM = 8, kEven = 6, kFar = 80, kAbove = 60;
+// Keys of uneven scales: scores are summed in units of 2^kUnit / un, where neither
+// m_k sum(q) of the largest keys overflows nor that of the smallest is lost.
+constexpr int kUnit = 28, kMinExpK = 40;
 constexpr int kIdsCached = 1024;   // block ids kept in shared memory (16K tokens)
 
 template <int D>
@@ -71,7 +74,7 @@ struct Cfg {
     static constexpr int kOffK = 4 * kQBytes;
     static constexpr int kOffV = kOffK + kKBytes;
     static constexpr int kOffPar = kOffV + kKBytes;    // TilePar [2]
-    static constexpr int kOffXch = kOffPar + 2 * (kN * 20 + 48);  // floats [4][2 halves][256 rows]
+    static constexpr int kOffXch = kOffPar + 2 * (kN * 20 + 32);  // floats [4][2 halves][256 rows]
     static constexpr int kOffRef = kOffXch + 4 * 4 * 2 * kM * 2;  // float2 [512] (max, exponent)
     static constexpr int kOffIds = kOffRef + 512 * 8;
     static constexpr int kOffBar = kOffIds + kIdsCached * 4;
@@ -239,12 +242,12 @@ struct RowState {
 struct TilePar {
     float mk[kN], mv[kN];
     float sv[kN];   // s_v 2^(133 - E)
-    float ev[kN];   // V's exponent less E, -kFar at least
-    float fk[kN];   // K's token t stands in the tile as s_k c / fk[t], a power of two
-    float f[4];     // fk of all the tokens 32 g .. + 31 where uneven[g] is 0
-    int uneven[4];  // 1: these tokens' s_k and m_k lie too far apart for one power of two (or s_k is 0), or V's exponents do
-    int E;          // largest exponent of V so far
-    int pad[3];
+    float ev[kN];   // exponents of V less E, from -kFar to kAbove
+    float fk[kN];   // K's token t stands in the tile as s_k c 2^-kUnit / fk[t], a power of two
+    float f[4];     // 2^kUnit fk of all the tokens 32 g .. + 31 where uneven[g] is 0
+    uint8_t uneven[4];  // 1: these tokens' s_k and m_k lie too far apart for one power of two (or s_k is 0), or V's exponents do
+    int E;              // largest exponent of s_v so far
+    int pad[2];
 };
 
 // 2^(m' - m): from what refers to m' to m; reference maxima are whole numbers.
@@ -284,9 +287,9 @@ __device__ __forceinline__ void scale_p(uint32_t tS, int cols, float f) {
 // of 5400 cycles a tile.)  The loop stays rolled: unrolled over all scores the
 // code runs from beyond the instruction cache.  ANY: only tokens up to `last`
 // (of this tile) are seen, the others may hold anything, NaN included; and K's
-// rows may have any scales: the score is v (un fk) + m_k (qs un), so that m_k is
-// not divided by a scale (0, for a row of equal values).  Else m_k qs / f joins
-// v in units of 1 / (un f), one operation a score.  fresh: O starts anew with
+// rows may have any scales: the score is (v fk + m_k qs 2^-kUnit) (un 2^kUnit), so
+// that m_k is not divided by a scale (0, for a row of equal values).  Else m_k qs
+// / f joins v in units of 1 / (un f), one operation a score.  fresh: O starts anew with
 // this tile.
 // The reference is one for the weights p s_v, which must fit fp16: m follows the
 // largest score plus V's exponent relative to E, so a V row that a token does not
@@ -313,7 +316,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
     }
 #pragma unroll 1
     for (int c = 0; c < 64; c += 32) {
-        const float f = ANY ? 1.0f : par.f[(t0 + c) / 32], qs = ANY ? st.qs * st.un : __fdividef(st.qs, f), un = ANY ? 1.0f : st.un * f;
+        const float f = ANY ? pow2(kUnit) : par.f[(t0 + c) / 32], qs = __fdividef(st.qs, f), un = st.un * f;
         const float2 qs2 = make_float2(qs, qs), un2 = make_float2(un, un);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -322,6 +325,12 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
             float top = -INFINITY;
             tmem_ld_wait16(v[u]);
             if (u == 0 || c == 0) tmem_ld16(tS + c + 16 * u + 16, v[u ^ 1]);
+            if (ANY && __all_sync(0xffffffffu, c0 > last)) {  // none of these rows sees any of the 16
+                const uint32_t none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                tmem_st8(tS + c + 16 * u, none);
+                tmem_st8(tS + c + 16 * u + 8, none);
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 const float4 k = *reinterpret_cast<const float4*>(&par.mk[c0 + 2 * i]);
@@ -329,14 +338,11 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                 x[i + 1] = make_float2(v[u][2 * i + 2], v[u][2 * i + 3]);
                 if (ANY) {
                     const float4 fk = *reinterpret_cast<const float4*>(&par.fk[c0 + 2 * i]);
-                    const float2 a = __fmul2_rn(make_float2(fk.x, fk.y), make_float2(st.un, st.un));
-                    const float2 b = __fmul2_rn(make_float2(fk.z, fk.w), make_float2(st.un, st.un));
-                    x[i] = __ffma2_rn(x[i], a, __fmul2_rn(make_float2(k.x, k.y), qs2));
-                    x[i + 1] = __ffma2_rn(x[i + 1], b, __fmul2_rn(make_float2(k.z, k.w), qs2));
-                } else {
-                    x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, x[i]);
-                    x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, x[i + 1]);
+                    x[i] = __fmul2_rn(x[i], make_float2(fk.x, fk.y));
+                    x[i + 1] = __fmul2_rn(x[i + 1], make_float2(fk.z, fk.w));
                 }
+                x[i] = __ffma2_rn(make_float2(k.x, k.y), qs2, x[i]);
+                x[i + 1] = __ffma2_rn(make_float2(k.z, k.w), qs2, x[i + 1]);
                 float2 w0 = x[i], w1 = x[i + 1];
                 if (ANY) {
                     if (c0 + 2 * i > last) x[i].x = -INFINITY;
@@ -344,8 +350,8 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                     if (c0 + 2 * i + 2 > last) x[i + 1].x = -INFINITY;
                     if (c0 + 2 * i + 3 > last) x[i + 1].y = -INFINITY;
                     const float4 ev = *reinterpret_cast<const float4*>(&par.ev[c0 + 2 * i]);
-                    w0 = __fadd2_rn(x[i], make_float2(ev.x, ev.y));
-                    w1 = __fadd2_rn(x[i + 1], make_float2(ev.z, ev.w));
+                    w0 = __ffma2_rn(x[i], un2, make_float2(ev.x, ev.y));
+                    w1 = __ffma2_rn(x[i + 1], un2, make_float2(ev.z, ev.w));
                 }
                 top = fmaxf(fmaxf(top, fmaxf(w0.x, w0.y)), fmaxf(w1.x, w1.y));
             }
@@ -367,7 +373,7 @@ __device__ __forceinline__ bool softmax_tile(uint32_t tS, uint32_t tO, const Til
                 const float4 sv = *reinterpret_cast<const float4*>(&par.sv[c0 + 2 * i]);
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    const float2 y = ANY ? __fadd2_rn(x[i + w], nm2) : __ffma2_rn(x[i + w], un2, nm2);
+                    const float2 y = __ffma2_rn(x[i + w], un2, nm2);
                     float2 mm = w ? make_float2(mv.z, mv.w) : make_float2(mv.x, mv.y);
                     if (ANY) {  // 0 times what an unseen token holds
                         if (c0 + 2 * (i + w) > last) mm.x = 0.0f;
@@ -461,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
     float* xch = reinterpret_cast<float*>(smem + C::kOffXch);
     volatile int* aside_slot = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 8);
     TilePar* par = reinterpret_cast<TilePar*>(smem + C::kOffPar);
-    static_assert(sizeof(TilePar) == kN * 20 + 48, "two tiles' parameters");
+    static_assert(sizeof(TilePar) == kN * 20 + 32, "two tiles' parameters");
     int32_t* ids = reinterpret_cast<int32_t*>(smem + C::kOffIds);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
         uint4 kr[NK];  // one tile of K or V at a time: K's next loads wait for V's conversion, registers are short
         uint4 (&vr)[NK] = kr;
         uint32_t pk = 0, pv[4];  // this thread's token of K; V's tokens lane + 32 j (every warp works out the tile's largest s_v)
-        int E = kMinExp;         // largest exponent of V so far
+        int E = kMinExp;         // largest exponent of s_v so far
         auto block = [&](int t, int b) -> int32_t {  // block b of local tile t
             const int j = t * (kN / 16) + b;
             return j < kIdsCached ? ids[j] : lookup(b0 + j);
@@ -638,19 +644,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             TilePar& par_t = par[ph];
             const float2 ka = q4_unpack(pk);
             const int wi = warp & 3;
-            uint32_t top_v = 0, low_v = 255, ev = 0;
+            uint32_t top_v = 0, low_v = 255;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float2 a = q4_unpack(pv[j]);
-                const uint32_t x = a.x < INFINITY ? __float_as_uint(fmaxf(a.x, fabsf(a.y) * (1.0f / (1 << kBelowM)))) >> 23 : 0u;
-                top_v = max(top_v, x);
-                low_v = min(low_v, x);
-                if (j == wi) ev = x;
+                const float x = q4_unpack(pv[j]).x;
+                const uint32_t e = x < INFINITY ? __float_as_uint(x) >> 23 : 0u;
+                top_v = max(top_v, e);
+                low_v = min(low_v, e);
             }
             E = max(E, (int)__reduce_max_sync(0xffffffffu, top_v));
-            const bool uneven_v = (int)__reduce_min_sync(0xffffffffu, low_v) + kEven < E;
             const float2 va = q4_unpack(wi == 0 ? pv[0] : wi == 1 ? pv[1] : wi == 2 ? pv[2] : pv[3]);
-            par_t.ev[i] = (float)max((int)ev - E, -kFar);
+            const int ev = va.x < INFINITY ? (int)(__float_as_uint(fmaxf(va.x, fabsf(va.y) * (1.0f / (1 << kBelowM)))) >> 23) : 0;
+            par_t.ev[i] = (float)min(max(ev - E, -kFar), kAbove);
             par_t.mk[i] = ka.y;
             par_t.mv[i] = va.y;
             // a V row that cannot be held (s = m = NaN) counts as zeros here: its NaN
@@ -664,11 +669,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             const uint32_t et = held ? __float_as_uint(ka.x) >> 23 : 0u, em = held ? __float_as_uint(fabsf(ka.y)) >> 23 : 0u;
             const uint32_t ek = __reduce_max_sync(0xffffffffu, et);
             const bool uneven = ek < 64 || __any_sync(0xffffffffu, held && (et + 20 < ek || em > ek + 40));
-            const int kx = max((int)(uneven ? et : ek), kMinExp);
-            const float fk = pow2(kx - 127 - kUp);
-            par_t.fk[i] = fk;
+            const bool uneven_v = __any_sync(0xffffffffu, (int)low_v + kEven < E);
+            const int kx = max((int)(uneven ? et : ek), kMinExpK);
+            par_t.fk[i] = pow2(kx - 127 - kUp - kUnit);
             if (lane == 0) {
-                par_t.f[wi] = fk;
+                par_t.f[wi] = pow2(kx - 127 - kUp);
                 par_t.uneven[wi] = uneven || uneven_v;
             }
             const __half2 sk = __float2half2_rn(ka.x * pow2(127 + kUp - kx));
@@ -846,8 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
             tc_fence_after();
             const int base = (tb + t) * kN;
             // (the pair's phase 0 was q's)
-            const int4 uneven = *reinterpret_cast<const int4*>(par[ph].uneven);
-            if (base + kN - 1 > prefix + q0 || (uneven.x | uneven.y | uneven.z | uneven.w))  // some row of the chunk does not see all of it
+            if (base + kN - 1 > prefix + q0 || *reinterpret_cast<const uint32_t*>(par[ph].uneven))  // some row of the chunk does not see all of it
                 ok = softmax_tile<true, D>(tS, tO, par[ph], 64 * half, row_limit - base, st, fresh, x_mine + ph * 4 * kM, x_other, pair,
                                            ph ^ 1u, p_full + 8 * X, abort_flag, lane);
             else
