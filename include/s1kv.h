@@ -56,8 +56,8 @@ extern "C" {
                                s = fp32(max((hi - m) / 7, (m - lo) / 8)), rounded up to bf16;
                                code = 8 + the integer nearest to (x - m) / s (ties to even; 8 where s = 0);
                                value = fp32(m + s (code - 8)), within s / 2 of x.
-                             A row holding a NaN, an infinity or a magnitude beyond bf16's largest reads back
-                             as NaN throughout.  head_dim a multiple of 8 up to 256, block_size a multiple
+                             A row holding a NaN or an infinity, or whose m or s passes bf16's largest (3.39e38),
+                             reads back as NaN throughout.  head_dim a multiple of 8 up to 256, block_size a multiple
                              of 4.  Every call of a pool takes it; attention reads the held values with
                              fp32-level accuracy.  The no-allocation decode takes F32 and BF16 storage only. */
 

@@ -12,9 +12,9 @@
 // row's offset.  One (s, m) pair a row (4 bytes beside D / 2 bytes of codes)
 // keeps K's scale and zero term out of the tensor-core products: they act
 // on whole scores.  bf16 for both because its range is fp32's; the bound
-// above holds for the rounded pair.  A row with a NaN or an infinity (or a
-// value beyond bf16's largest, 3.39e38) is held as s = m = NaN: the whole
-// row reads back as NaN.
+// above holds for the rounded pair.  A row with a NaN or an infinity, or whose
+// m or s passes bf16's largest (3.39e38), is held as s = m = NaN: the whole row
+// reads back as NaN.
 //
 // Storage: one tile per (block, KV head), K and V apart:
 //   codes  bs * D / 2 bytes, then the rows' params  bs * {bf16 s, bf16 m}.
@@ -207,8 +207,9 @@ __device__ __forceinline__ void q4_store_row16(const float (&x)[16], char* tile,
         }
         c[q] = (uint32_t)fmaf(4096.f, u[3], fmaf(256.f, u[2], fmaf(16.f, u[1], u[0])));
     }
-    // (not finite where s is 0 or too small to invert, or the row is spoilt)
-    if (!(far < 0.4999f) || !(fabsf(inv) < INFINITY)) {
+    // (inv is not finite where s is 0 or too small to invert, or the row is spoilt;
+    // m - lo passes fp32 where the row spans nearly all of it)
+    if (!(far < 0.4999f) || !(fabsf(inv) < INFINITY) || !(r.m - lo < INFINITY)) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             c[q] = 0;

@@ -181,3 +181,26 @@ def test_long_decode_with_large_value_rows(s1kv, cuda, dim):
     attend_and_check(s1kv, k, v, 1, 4)
     attend_and_check(s1kv, k, v, 1, 12)
     attend_and_check(s1kv, k, v, 3, 4)
+
+
+# ------------------------------------------------------- rows of wide spread --
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 40])
+@pytest.mark.parametrize("rope", [False, True])
+def test_rows_that_span_fp32(s1kv, cuda, dim, rope):
+    """x - m passes fp32's largest at the low end: the codes are the format's."""
+    rng = np.random.default_rng(88)
+    n, hkv = 6, 2
+    x = rng.standard_normal((n, hkv, dim)).astype(np.float32)
+    x[0, 0] = np.linspace(-3.3e38, 3.3e38, dim)
+    x[1, 1, ::3], x[1, 1, 5] = -3.2e38, 3.3e38
+    x[2, 0, :2] = 3.3e38, -3.3e38
+    x[3] *= np.float32(7e37)
+    x[4, 1, -1] = -3.3e38
+    pool = pool_of(s1kv, hkv, dim, 10)
+    for i in range(n):  # (position 0: RoPE leaves the values as they are)
+        with pool.batch([i], [1]) as b:
+            one = dev(x[i:i + 1])
+            b.rope_append(0, one, one) if rope else b.append(0, one, one)
+            for which in (s1kv.K, s1kv.V):
+                np.testing.assert_array_equal(b.gather(0, which).cpu().numpy(), LB.q4_values(x[i:i + 1]))
