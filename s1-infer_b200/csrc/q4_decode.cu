@@ -231,9 +231,9 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         }
         qsum += __shfl_xor_sync(kFull, qsum, 1);
         qsum += __shfl_xor_sync(kFull, qsum, 2);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
-        // power of two that puts the pass's largest |q| in [2^14, 2^15)
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+        // power of two that puts the head's largest |q| in [2^14, 2^15)
         const int qe = min(max((int)(__float_as_uint(amax) >> 23), 40), 240);
         const float qscale = __uint_as_float((uint32_t)(127 + 14 + 127 - qe) << 23);
         const float unscale = __uint_as_float((uint32_t)(qe - 14) << 23);  // 1 / qscale
@@ -254,8 +254,17 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                         qf[NT - 1][2 * wi + j][b] = lo;
                     }
                 }
-        // sum(q) of the two heads whose scores this lane holds (columns 2 tq, 2 tq + 1)
-        const float qs0 = __shfl_sync(kFull, qsum, (2 * tq) * 4 & 31), qs1 = __shfl_sync(kFull, qsum, (2 * tq + 1) * 4 & 31);
+        // scale and sum(q) of the two heads whose scores this lane holds (columns 2 tq, 2 tq + 1);
+        // NT = 2 is short of registers and reads them every step
+        const float4* heads = reinterpret_cast<const float4*>(smem + kRing + kNW * kNS * 8 + 16) + 4 * warp;
+        float4 hq;
+        if (NT == 1) {
+            hq = make_float4(__shfl_sync(kFull, unscale, 8 * tq & 31), __shfl_sync(kFull, qsum, 8 * tq & 31),
+                             __shfl_sync(kFull, unscale, 8 * tq + 4 & 31), __shfl_sync(kFull, qsum, 8 * tq + 4 & 31));
+        } else {
+            if (tq == 0) reinterpret_cast<float2*>(const_cast<float4*>(heads))[gq] = make_float2(unscale, qsum);
+            __syncwarp();
+        }
 
         float o[KS][4];
 #pragma unroll
@@ -264,7 +273,6 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         // lanes of a head), this lane's share of sum(p) and sum(p m_v)
         float m0 = -INFINITY, m1 = -INFINITY;
         float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
-        const float2 un2 = make_float2(unscale, unscale), qs2 = make_float2(qs0, qs1);
         const float2 low = NT == 1 ? (tq < 2 ? make_float2(0.f, 0.f) : make_float2(-1.f, -1.f)) : make_float2(-1.f, -1.f);
         // V's scales are taken relative to 2^(E - 127), E the largest exponent of an s_v so far: vmul =
         // 2^(133 - E) puts the largest in [2^6, 2^7)
@@ -281,6 +289,8 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             const char* kt = ring + stage * kStage;
             const int rest = tok1 - (tok0 + (warp + k * kNW) * 2 * kTile);  // tokens of the pair: 32, fewer at the end
 
+            if (NT == 2) hq = heads[tq];
+            const float2 un2 = make_float2(hq.x, hq.z), qs2 = make_float2(hq.y, hq.w);
             // ---- scores: M = the 16 tokens of a tile, N = the 8 columns ----
             float2 x[2][2], va[2], vb[2];  // [tile][token gq, gq + 8] of heads (2 tq, 2 tq + 1); (s_v, m_v) of the tokens
 #pragma unroll
@@ -622,7 +632,7 @@ int decode_q4_ctas_per_sm(int D) { return ctas_per_sm(D); }
 
 template <int D, int NT>
 static int launch_q4(const AttnParams& p, int G, cudaStream_t stream) {
-    constexpr int smem = kNW * kNS * (4 * kTile * (D / 2 + 4) + 8) + 16;
+    constexpr int smem = kNW * kNS * (4 * kTile * (D / 2 + 4) + 8) + 16 + kNW * 64;
     static std::atomic<uint64_t> attr_set{0};  // per device
     const int st = once_per_device(attr_set, [] {
         S1KV_CUDA(cudaFuncSetAttribute(decode_q4_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));

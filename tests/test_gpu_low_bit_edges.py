@@ -204,3 +204,30 @@ def test_rows_that_span_fp32(s1kv, cuda, dim, rope):
             b.rope_append(0, one, one) if rope else b.append(0, one, one)
             for which in (s1kv.K, s1kv.V):
                 np.testing.assert_array_equal(b.gather(0, which).cpu().numpy(), LB.q4_values(x[i:i + 1]))
+
+
+# ------------------------------------------------------- heads of a KV head --
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("g", [2, 4, 8, 9])
+@pytest.mark.parametrize("r", [1, 20])
+@pytest.mark.parametrize("factor", [2.0 ** 30, 2.0 ** 90, np.inf, np.nan])
+def test_one_heads_query_leaves_the_others_alone(s1kv, cuda, dim, g, r, factor):
+    """Query heads that share a KV head, one of them far larger or not finite:
+    the others are held to their own precision."""
+    rng = np.random.default_rng(89)
+    hkv, n = 2, 150
+    k, v = kv(rng, n, hkv, dim)
+    q = rng.standard_normal((r, g * hkv, dim)).astype(np.float32)
+    odd = [1, g * hkv - 1]
+    rest = [h for h in range(g * hkv) if h not in odd]
+    plain = q.copy()
+    with np.errstate(invalid="ignore"):
+        q[:, odd, 3:5] *= np.float32(factor)
+    pool = pool_of(s1kv, hkv, dim, 14)
+    fill(pool, [n], k, v)
+    got = pool.attention(0, [0], [r], dev(q), g * hkv).cpu().numpy()
+    for h in rest:
+        check_rows(got[:, [h]], plain[:, [h]], k[:, [h // g]], v[:, [h // g]])
+    if not np.isfinite(factor):
+        assert np.isnan(got[:, odd]).all()
