@@ -281,11 +281,9 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         int done = 0;
         for (int k = 0; k < pairs; k++) {
             const int it = it0 + k, stage = it % kNS;
-            if (!bar_wait(bars + 8 * stage, (uint32_t)((it / kNS) & 1))) {
-                failed = true;
-                break;
-            }
-            done = k + 1;
+            // Each lane polls for itself; a timeout goes into the vote below, so that
+            // the warp leaves as one.
+            const bool late = !bar_wait(bars + 8 * stage, (uint32_t)((it / kNS) & 1));
             const char* kt = ring + stage * kStage;
             const int rest = tok1 - (tok0 + (warp + k * kNW) * 2 * kTile);  // tokens of the pair: 32, fewer at the end
 
@@ -342,7 +340,12 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             float mx1 = fmaxf(fmaxf(x[0][0].y, x[0][1].y), fmaxf(x[1][0].y, x[1][1].y));
             const float most = fmaxf(fmaxf(va[0].x, vb[0].x), fmaxf(va[1].x, vb[1].x));
             const float least = fminf(fminf(va[0].x, vb[0].x), fminf(va[1].x, vb[1].x));
-            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || most * vmul >= 128.0f || least * vmul < 64.0f / (1 << kEven))) {
+            if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || most * vmul >= 128.0f || least * vmul < 64.0f / (1 << kEven) ||
+                                  late)) {
+                if (__any_sync(kFull, late)) {
+                    failed = true;
+                    break;
+                }
                 // The reference is one for the weights p s_v, which must fit fp16:
                 // scores plus V's exponents relative to E (down to -kFar).  A V row
                 // that is hardly weighed then takes no bits from the others,
@@ -395,6 +398,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                     o[mb][3] *= c1;
                 }
             }
+            done = k + 1;
             // p, then p s_v in two fp16 parts: rows of P^T, transposed in
             // registers into the B fragments of O^T += V^T P^T.  NT = 1: lanes
             // of columns 0-3 give the high part, of 4-7 the low part.
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         if (failed && pairs > 0) {
             // copies still in flight land before the CTA exits (bounded)
             if (lane == 0) atomicOr(p.err, kErrTimeout);
-            for (int k = done + 1; k < min(pairs, done + kNS); k++) bar_wait(bars + 8 * ((it0 + k) % kNS), (uint32_t)(((it0 + k) / kNS) & 1));
+            for (int k = done; k < min(pairs, done + kNS); k++) bar_wait(bars + 8 * ((it0 + k) % kNS), (uint32_t)(((it0 + k) / kNS) & 1));
             m0 = m1 = -INFINITY;
             l2 = z2 = make_float2(0.f, 0.f);
         }
