@@ -415,10 +415,10 @@ int s1kv_batch_gather(s1kv_batch* batch, int32_t layer, int32_t which, float* ou
 int s1kv_batch_append(s1kv_batch* batch, int32_t layer, const float* k, const float* v, void* stream);
 /* Paged GQA attention of the batch's query rows (post-RoPE q).  For decode
  * batches (at most one query row per sequence) the kernel is a programmatic
- * dependent launch that may request the K/V of tokens this batch did not
- * append while the previous kernel of the stream is still running; every
- * kernel of this library that writes the pool elsewhere completes before a
- * later kernel starts.  A caller's own programmatic-dependent kernel that
+ * dependent launch that may request the K/V of tokens that neither this batch
+ * nor another one open when it began appends, while the previous kernel of
+ * the stream is still running; every kernel of this library that writes the
+ * pool elsewhere completes before a later kernel starts.  A caller's own programmatic-dependent kernel that
  * writes the pool must therefore not come directly before this call.
  * Attention calls of one pool share its scratch memory: order those on
  * different streams. */

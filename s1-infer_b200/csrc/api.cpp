@@ -261,6 +261,33 @@ int s1kv_batch_begin(s1kv_pool* p, const uint64_t* seqs, const int32_t* n_append
     b->items_uploaded = b->items_planned;
     b->d_pseqs = (const PrefillSeq*)(b->seg->d + o_pseq);
     b->d_qpos = b->rows_are_tokens ? nullptr : (const int32_t*)(b->seg->d + o_qpos);
+    // Tokens that a decode row may not request before its wait: the last
+    // max_append, unless another open batch may still append to the row's
+    // blocks or the batch names a sequence twice.
+    b->prewait_margin = b->max_append;
+    bool look = b->decode_rows && p->open_appends > 0;
+    if (n_tok) {
+        const int64_t bs = p->desc.block_size;
+        if (p->appending.empty()) {
+            p->appending.resize(p->desc.max_blocks);
+            p->row_seen.resize(p->desc.max_seqs);
+        }
+        const uint64_t serial = ++p->batch_serial;
+        for (int64_t i = 0, t = 0; i < n_seqs; i++) {
+            if (n_append[i] == 0) continue;
+            look |= b->decode_rows && p->row_seen[trow[i]] == serial;
+            p->row_seen[trow[i]] = serial;
+            for (const int64_t end = t + n_append[i]; t < end;) {
+                const int32_t blk = (int32_t)(slots[t] / bs);
+                p->appending[blk]++;
+                b->append_blocks.push_back(blk);
+                t = std::min(end, t + bs - slots[t] % bs);
+            }
+        }
+        p->open_appends++;
+    }
+    for (int32_t i = 0; look && i < n_seqs; i++)
+        b->prewait_margin = std::max<int64_t>(b->prewait_margin, lens[i] - first_appending(p, seqs[i]));
     *out = b;
     return S1KV_OK;
 }
@@ -432,17 +459,20 @@ static int split_k_attention(s1kv_batch* b, int32_t layer, const float* q, float
     ap.scale_log2 = scale_log2(D);
     ap.err = p->d_err;
     // Decode rows: the kernels request the K/V tiles that lie entirely below
-    // the last max_append tokens of each row before their wait for the
+    // the last prewait_margin tokens of each row before their wait for the
     // previous kernel of the stream.  Safe because the kernels of this
-    // library that may still run then write the pool only at this batch's
-    // appended tokens (the batch's RoPE + append of any layer; the decode
-    // kernels read it): every other write of the pool -- single-call
-    // appends, copy-on-write copies, block-table updates, prefix loads -- is
-    // a plain launch or a copy, complete before any later kernel starts, and
-    // the step's metadata is uploaded before the batch's first kernel.
+    // library that may still run then write the pool only at tokens above:
+    // those that this batch appends, and those of batches that were open when
+    // it began (their RoPE + append of any layer; the decode kernels read it).
+    // A batch that ended before has its appends ahead of this one's upload of
+    // metadata, one that begins later appends behind the row.  Every other
+    // write of the pool -- single-call appends, copy-on-write copies,
+    // block-table updates, prefix loads -- is a plain launch or a copy,
+    // complete before any later kernel starts, and the step's metadata is
+    // uploaded before the batch's first kernel.
     if (b->decode_rows) {
         ap.prewait = 1;
-        ap.prewait_margin = b->max_append;
+        ap.prewait_margin = (int32_t)b->prewait_margin;
     }
     const size_t cbytes = (size_t)b->n_rows * Hkv * kCounterStride * sizeof(int32_t);
     if (p->counters.cap < cbytes) {
@@ -595,6 +625,8 @@ int s1kv_batch_end(s1kv_batch* b, void* stream) {
         if (cudaStreamWaitEvent((cudaStream_t)stream, b->pool->io_ev[4 + s], 0) != cudaSuccess)
             st = set_error(S1KV_ECUDA, "s1kv_batch_end: waiting for host copies");
     if (b->seg) st = b->pool->stager.release(b->seg, (cudaStream_t)stream);
+    for (int32_t blk : b->append_blocks) b->pool->appending[blk]--;
+    if (!b->append_blocks.empty()) b->pool->open_appends--;
     delete b;
     return st;
 }

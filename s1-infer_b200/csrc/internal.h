@@ -179,9 +179,9 @@ struct AttnParams {
     uint32_t epoch;
     // Copies issued before the wait for the previous kernel (decode rows of
     // a batch): when prewait is set, a tile whose tokens all lie below
-    // kv_len - prewait_margin (the tokens appended by this batch are the
-    // last prewait_margin of each sequence) is requested before
-    // griddepcontrol.wait.  See split_k_attention for why that is safe.
+    // kv_len - prewait_margin (the tokens appended by this batch, and by
+    // others that were open when it began, are the last prewait_margin of each
+    // sequence) is requested before griddepcontrol.wait.  See split_k_attention for why that is safe.
     int32_t prewait;
     int32_t prewait_margin;
 };
@@ -298,6 +298,11 @@ struct s1kv_pool {
     s1kv_pool_desc desc{};
     int device = 0;
     bool host_only = false;
+    // Open batches that append, and per block how many of them append to it.
+    int32_t open_appends = 0;
+    std::vector<uint16_t> appending;
+    uint64_t batch_serial = 0;
+    std::vector<uint64_t> row_seen;  // per block-table row, the last batch that appended to it
     // device storage
     char* k = nullptr;
     char* v = nullptr;
@@ -379,6 +384,8 @@ struct s1kv_batch {
     bool decode_rows = true;  // every row has q_len 1 for its sequence
     bool rows_are_tokens = true;  // q_len == n_append for every sequence: query row i is appended token i
     int32_t max_append = 0;   // the most tokens any sequence appends in this batch
+    int64_t prewait_margin = 0;  // tokens at each row's end that this or another open batch may be appending
+    std::vector<int32_t> append_blocks;  // the blocks its tokens go to, counted in pool->appending until its end
     const int32_t* d_qpos = nullptr;  // position of each query row (kv_len - 1), when rows are not the tokens
     // device views into seg->d
     const int32_t* d_slots = nullptr;
@@ -444,6 +451,9 @@ int launch_decode_mma(const AttnParams& p, const CUtensorMap& tk_sw, const CUten
 // Exchange fields of a decode launch that publishes its rows (exchange.cu).
 int exchange_params(const s1kv_exchange* ex, uint32_t epoch, int32_t head0, int32_t heads_total, AttnParams* ap);
 void exchange_record(s1kv_exchange* ex, uint32_t epoch, int64_t words);
+
+// The first token of sequence `id` in a block that an open batch appends to (its length if there is none).
+int64_t first_appending(const s1kv_pool* p, uint64_t id);
 
 // 4-bit pools (q4_kernels.cu, q4_decode.cu).
 int launch_append_q4(const AppendParams& p, bool rope, cudaStream_t stream, bool pdl);

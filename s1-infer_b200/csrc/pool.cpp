@@ -339,6 +339,14 @@ int seq_row(const s1kv_pool* p, uint64_t id, int32_t* row, int64_t* len) {
     return S1KV_OK;
 }
 
+int64_t first_appending(const s1kv_pool* p, uint64_t id) {
+    const Seq* s = find_seq(p, id);
+    if (!s) return 0;
+    for (size_t i = 0; i < s->table.size(); i++)
+        if (p->appending[s->table[i]]) return std::min<int64_t>((int64_t)i * p->desc.block_size, seq_len(p, s));
+    return seq_len(p, s);
+}
+
 int reserve_internal(s1kv_pool* p, uint64_t id, int64_t n, int32_t* slots, int64_t* n_done) {
     return reserve(p, id, n, slots, n_done);
 }

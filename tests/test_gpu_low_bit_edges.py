@@ -231,3 +231,56 @@ def test_one_heads_query_leaves_the_others_alone(s1kv, cuda, dim, g, r, factor):
         check_rows(got[:, [h]], plain[:, [h]], k[:, [h // g]], v[:, [h // g]])
     if not np.isfinite(factor):
         assert np.isnan(got[:, odd]).all()
+
+
+# ------------------------------------------------- batches open at one time --
+
+def plain_rows(pool, kk, vv, q):
+    """Attention of q's rows, the last tokens of kk, vv, as the pool holds them."""
+    if pool.dtype == 2:
+        kk, vv = LB.q4_values(kk), LB.q4_values(vv)
+    elif pool.dtype == 1:
+        kk, vv = (LB._bf16_rn(x) for x in (kk, vv))
+    return LB.attention64(q, kk, vv)
+
+
+@pytest.mark.parametrize("dtype", ["q4", "bf16", "f32"])
+def test_decode_beside_an_open_batch_that_appends(s1kv, cuda, dtype):
+    """One batch appends (its kernel lets the next start early), another that
+    began before that append reads its tokens, right behind it."""
+    rng = np.random.default_rng(90)
+    hkv, hq, dim, n, new = 8, 32, 128, 900, 700
+    k, v = kv(rng, 4 * n, hkv, dim)
+    k2, v2 = kv(rng, 4 * new, hkv, dim)
+    q = rng.standard_normal((5, hq, dim)).astype(np.float32)
+    pool = s1kv.Pool(1, hkv, dim, 600, 16, dtype=dtype)
+    with pool.batch([0, 1, 2, 3], [n] * 4, [0] * 4) as b:
+        b.append(0, dev(k), dev(v))
+    grow = pool.batch([0, 1, 2, 3], [new] * 4, [0] * 4)
+    pool.fork(1, 9, n + new)  # shares blocks that `grow` fills
+    read = pool.batch([0, 1, 2, 3, 9], None, [1] * 5)
+    dk, dv, dq = dev(k2), dev(v2), dev(q)
+    grow.append(0, dk, dv)
+    got = read.attention(0, dq).cpu().numpy()
+    grow.end()
+    read.end()
+    for row, i in enumerate((0, 1, 2, 3, 1)):
+        kk = np.concatenate([k[i * n:(i + 1) * n], k2[i * new:(i + 1) * new]])
+        vv = np.concatenate([v[i * n:(i + 1) * n], v2[i * new:(i + 1) * new]])
+        want = plain_rows(pool, kk, vv, q[row:row + 1])
+        assert np.abs(got[row] - want[0]).max() <= 2e-5 * np.abs(vv).max()
+
+
+@pytest.mark.parametrize("dtype", ["q4", "bf16", "f32"])
+def test_decode_of_a_sequence_named_twice(s1kv, cuda, dtype):
+    rng = np.random.default_rng(91)
+    hkv, hq, dim = 8, 32, 128
+    k, v = kv(rng, 840, hkv, dim)
+    q = rng.standard_normal((2, hq, dim)).astype(np.float32)
+    pool = s1kv.Pool(1, hkv, dim, 80, 16, dtype=dtype)
+    with pool.batch([0, 0], [400, 440], [1, 1]) as b:
+        b.append(0, dev(k), dev(v))
+        got = b.attention(0, dev(q)).cpu().numpy()
+    for row, n in enumerate((400, 840)):
+        want = plain_rows(pool, k[:n], v[:n], q[row:row + 1])
+        assert np.abs(got[row] - want[0]).max() <= 2e-5 * np.abs(v).max()
