@@ -79,8 +79,7 @@ __device__ __forceinline__ float token_scale(float mx) { return mx > 0.0f ? __fd
 // 16-byte aligned, stay in registers between the maximum and the codes (one
 // read of x: 8001 rows of 4096 in 39 us, 4.2 TB/s); NV = 0: any row, read twice.
 template <int NV>
-__global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* __restrict__ x, int64_t K, int8_t* __restrict__ q,
-                                                              int64_t ldq, float* __restrict__ scales) {
+__global__ void __launch_bounds__(256) quantize_tokens_kernel(const float* x, int64_t K, int8_t* q, int64_t ldq, float* scales) {
     pdl_wait_trigger();
     __shared__ float part[8];
     const int64_t m = blockIdx.x;
@@ -155,8 +154,7 @@ __device__ __forceinline__ void imma16832(int (&c)[4], uint32_t a0, uint32_t a1,
 
 template <int NTILE, bool FUSED, bool EARLY>  // (neither: the caller's codes)
 __global__ void __launch_bounds__(kGemvWarps * 32, 3)
-    w8a8_gemv_kernel(const float* __restrict__ x, int x_len, const int8_t* __restrict__ xq, const float* __restrict__ sx, int M,
-                     int K, const __grid_constant__ W8Group grp) {
+    w8a8_gemv_kernel(const float* x, int x_len, const int8_t* xq, const float* sx, int M, int K, const __grid_constant__ W8Group grp) {
     __shared__ uint4 own[FUSED ? kFusedK / 16 : 1];  // the token's codes
     __shared__ float part[8], own_scale;
     __shared__ int red[kGemvWarps][16][8 * NTILE + 1];
@@ -216,7 +214,7 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 3)
                     // tokens past the last read the last one's bytes; their columns are not stored
                     const int64_t at = (int64_t)min(8 * nt + g, M - 1) * K + k;
                     const uint4 b = k >= K ? make_uint4(0, 0, 0, 0)
-                                           : FUSED ? own[at >> 4] : __ldg(reinterpret_cast<const uint4*>(xq + at));
+                                           : FUSED ? own[at >> 4] : *reinterpret_cast<const uint4*>(xq + at);
                     imma16832(acc[nt], x.x, y.x, x.y, y.y, b.x, b.y);
                     imma16832(acc[nt], x.z, y.z, x.w, y.w, b.z, b.w);
                 }
@@ -239,6 +237,10 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 3)
     }
 }
 
+// (Tokens' codes and scales, and x, are read by ordinary loads throughout: the
+// kernel that writes them may run while this one waits, which the read-only
+// path does not allow for.)
+//
 // -------------------------------------------------- many tokens: tcgen05 --
 // tcgen05.mma kind::i8 with the 128 channels of a tile as M and NT = 64 or 128
 // tokens as N, bound by the weights' bytes; a stored output row is 128 adjacent
@@ -268,7 +270,8 @@ struct TcCfg {
     static constexpr int kCols = (SPLIT ? 1 : 2) * NT;             // two accumulators for a chain of tiles
     static constexpr int kExchange = SPLIT ? kCh * NT * 4 : 0;     // [rank][token of the slice][channel] sums
     static constexpr int kOffX = kStages * kStageBytes;
-    static constexpr int kOffBar = kOffX + kExchange;
+    static constexpr int kOffScales = kOffX + kExchange;           // [4 warps][token]
+    static constexpr int kOffBar = kOffScales + (SPLIT ? 0 : 4 * NT * 4);
     static constexpr int kNumBars = 2 * kStages + 5;
     static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
 };
@@ -361,6 +364,37 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, int (&r)[16]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+
+// The scales of n tokens from token m0 into this warp's part of shared memory
+// (the kernel that wrote them may have run beside this one's start, so they are
+// read by ordinary loads, which are slow next to every store of an output).
+__device__ __forceinline__ void bring_scales(float* to, const float* sx, int m0, int n, int M) {
+    __syncwarp();  // the last tile's are read
+    for (int i = threadIdx.x & 31; i < n; i += 32) to[i] = m0 + i < M ? sx[m0 + i] : 0.0f;
+    __syncwarp();
+}
+// A lane's channel of m_end tokens out of TMEM, scaled, to out (rows of N).
+__device__ __forceinline__ void store_tile(uint32_t taddr, int m_end, const float* scales, float* out, int N, bool live, float sw) {
+    for (int c = 0; c < m_end; c += 16) {
+        int v[16];
+        float sx[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(sx + j) = *reinterpret_cast<const float4*>(scales + c + j);
+        tmem_ld16(taddr + c, v);
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            sx[j] = __fmul_rn(__fmul_rn((float)v[j], sx[j]), sw);
+        float* at = out + (int64_t)c * N;
+        if (live && c + 16 <= m_end) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) __stcs(at + (int64_t)j * N, sx[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (live && c + j < m_end) __stcs(at + (int64_t)j * N, sx[j]);
+        }
+    }
 }
 
 template <int NT, bool SPLIT>
@@ -488,29 +522,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         pdl_wait_trigger();  // the scales of the tokens, and outputs the kernel before may still read
         const int sub = warp & 3;  // the TMEM lanes 32 sub .. + 31 are this warp's
         const uint32_t lanes = (uint32_t)(32 * sub) << 16;
+        float* scales = reinterpret_cast<float*>(smem + C::kOffScales) + sub * NT;
         int done = 0;
         for (int t = blockIdx.x; t < n_tiles; t += gridDim.x, done++) {
             const int buf = done & 1;
-            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
-            tc_fence_after();
             int ch, tok;
             tile_at(t, ch, tok);
             const W8Mat& mat = p.grp.m[mat_of(ch)];
             const int n = (ch - mat.tile0) * kCh + 32 * sub + lane;
             const bool live = n < mat.N;
+            const float sw = !SPLIT && live ? mat.scales[n] : 0.0f;
+            if (!SPLIT) bring_scales(scales, p.sx, tok * NT, NT, p.M);
+            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
+            tc_fence_after();
             if (!SPLIT) {
-                const float sw = live ? mat.scales[n] : 0.0f;
-                float* out = mat.out + n;
-                const int m_end = min(NT, p.M - tok * NT);
-                for (int c = 0; c < m_end; c += 16) {
-                    int v[16];
-                    tmem_ld16(tmem + lanes + buf * NT + c, v);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int m = tok * NT + c + j;
-                        if (live && c + j < m_end) __stcs(out + (int64_t)m * mat.N, __fmul_rn(__fmul_rn((float)v[j], __ldg(p.sx + m)), sw));
-                    }
-                }
+                store_tile(tmem + lanes + buf * NT, min(NT, p.M - tok * NT), scales, mat.out + (int64_t)tok * NT * mat.N + n,
+                           mat.N, live, sw);
             } else {
                 // columns [r * per, (r + 1) * per) of this tile are rank r's: [rank][column][channel]
                 const int per = NT / cs;
@@ -554,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int i = 0; i < kMost; i++) {
             const int c = warp + kWarps * i;
-            sm[i] = c < per && m0 + c < p.M ? __ldg(p.sx + m0 + c) : 0.0f;
+            sm[i] = c < per && m0 + c < p.M ? p.sx[m0 + c] : 0.0f;
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -594,7 +621,8 @@ struct PairCfg {
     static constexpr int kTok = 256;
     static constexpr int kStageBytes = kKB * (kCh + kTok / 2);  // a CTA's part
     static constexpr int kStages = 6;
-    static constexpr int kOffBar = kStages * kStageBytes;
+    static constexpr int kOffScales = kStages * kStageBytes;  // [4 warps][token]
+    static constexpr int kOffBar = kOffScales + 4 * kTok * 4;
     static constexpr int kNumBars = 2 * kStages + 5;
     static constexpr int kSmem = kOffBar + kNumBars * 8 + 16 + 1024;
 };
@@ -745,28 +773,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         pdl_wait_trigger();  // the scales of the tokens, and outputs the kernel before may still read
         const int sub = warp & 3;  // the TMEM lanes 32 sub .. + 31 are this warp's
         const uint32_t lanes = (uint32_t)(32 * sub) << 16;
+        float* scales = reinterpret_cast<float*>(smem + C::kOffScales) + sub * C::kTok;
         int done = 0;
         for (int t = first; t < n_tiles; t += step, done++) {
             const int buf = done & 1;
-            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
-            tc_fence_after();
             int ch, tok;
             tile_at(t, ch, tok);
             const W8Mat& mat = p.grp.m[mat_of(ch)];
             const int n = (ch - mat.tile0) * 2 * kCh + rank * kCh + 32 * sub + lane;
             const bool live = n < mat.N;
             const float sw = live ? mat.scales[n] : 0.0f;
-            float* out = mat.out + n;
-            const int m_end = min(C::kTok, p.M - tok * C::kTok);
-            for (int c = 0; c < m_end; c += 16) {
-                int v[16];
-                tmem_ld16(tmem + lanes + buf * C::kTok + c, v);
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int m = tok * C::kTok + c + j;
-                    if (live && c + j < m_end) __stcs(out + (int64_t)m * mat.N, __fmul_rn(__fmul_rn((float)v[j], __ldg(p.sx + m)), sw));
-                }
-            }
+            bring_scales(scales, p.sx, tok * C::kTok, C::kTok, p.M);
+            if (!warp_wait(&acc_full[buf], (uint32_t)((done / 2) & 1), abort_flag)) break;
+            tc_fence_after();
+            store_tile(tmem + lanes + buf * C::kTok, min(C::kTok, p.M - tok * C::kTok), scales, mat.out + (int64_t)tok * C::kTok * mat.N + n, mat.N, live, sw);
             tc_fence_before();
             __syncwarp();
             if (lane == 0)

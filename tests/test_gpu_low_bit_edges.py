@@ -284,3 +284,26 @@ def test_decode_of_a_sequence_named_twice(s1kv, cuda, dtype):
     for row, n in enumerate((400, 840)):
         want = plain_rows(pool, k[:n], v[:n], q[row:row + 1])
         assert np.abs(got[row] - want[0]).max() <= 2e-5 * np.abs(v).max()
+
+
+# ----------------------------------------------------------------- products --
+
+@pytest.mark.parametrize("m", [1, 2, 8, 20, 64, 200, 700])
+@pytest.mark.parametrize("k", [512, 2048])
+def test_products_one_behind_the_other(s1kv, cuda, m, k):
+    """Calls without a pause, each quantising other tokens into the workspace
+    that the one before used: every product is of its own tokens."""
+    torch = cuda
+    rng = np.random.default_rng(m + k)
+    n, turns = 384, 12
+    w = s1kv.quantize_channels(rng.standard_normal((k, n)).astype(np.float32))
+    xs = [dev((rng.standard_normal((m, k)) * 3.0 ** i).astype(np.float32)) for i in range(turns)]
+    outs = [torch.empty((m, n), device="cuda") for _ in xs]
+    for _ in range(3):
+        for x, o in zip(xs, outs):
+            s1kv.matmul_w8a8(x, w, o)
+        torch.cuda.synchronize()
+        for x, o in zip(xs, outs):
+            c, s = LB.tokens8(x.cpu().numpy())
+            np.testing.assert_array_equal(o.cpu().numpy(), LB.product8(c, s, w.data.cpu().numpy()[:, :k], w.scales.cpu().numpy()))
+            o.zero_()
