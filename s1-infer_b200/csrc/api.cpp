@@ -420,12 +420,12 @@ static int split_k_attention(s1kv_batch* b, int32_t layer, const float* q, float
         // tensor-core prefill does not take): plan and upload its work list.
         if (!b->items_planned) plan_items(p, b);
         const size_t rb = b->rows.size() * sizeof(RowMeta), ib = b->items.size() * sizeof(WorkItem);
-        st = p->late_meta.ensure(align16(rb) + ib + 16);
+        st = p->late_stager.acquire(align16(rb) + ib + 16, &b->late);
         if (st) return st;
-        char* d = (char*)p->late_meta.p;
-        S1KV_CUDA(cudaMemcpyAsync(d, b->rows.data(), rb, cudaMemcpyHostToDevice, stream));
-        S1KV_CUDA(cudaMemcpyAsync(d + align16(rb), b->items.data(), ib, cudaMemcpyHostToDevice, stream));
-        S1KV_CUDA(cudaStreamSynchronize(stream));  // the host vectors are pageable
+        char *h = b->late->h, *d = b->late->d;
+        std::memcpy(h, b->rows.data(), rb);
+        std::memcpy(h + align16(rb), b->items.data(), ib);
+        S1KV_CUDA(cudaMemcpyAsync(d, h, align16(rb) + ib, cudaMemcpyHostToDevice, stream));
         b->d_rows = (const RowMeta*)d;
         b->d_items = (const WorkItem*)(d + align16(rb));
         b->items_uploaded = true;
@@ -625,6 +625,10 @@ int s1kv_batch_end(s1kv_batch* b, void* stream) {
         if (cudaStreamWaitEvent((cudaStream_t)stream, b->pool->io_ev[4 + s], 0) != cudaSuccess)
             st = set_error(S1KV_ECUDA, "s1kv_batch_end: waiting for host copies");
     if (b->seg) st = b->pool->stager.release(b->seg, (cudaStream_t)stream);
+    if (b->late) {
+        const int st2 = b->pool->late_stager.release(b->late, (cudaStream_t)stream);
+        if (!st) st = st2;
+    }
     for (int32_t blk : b->append_blocks) b->pool->appending[blk]--;
     if (!b->append_blocks.empty()) b->pool->open_appends--;
     delete b;

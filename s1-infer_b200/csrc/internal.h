@@ -345,7 +345,7 @@ struct s1kv_pool {
     s1kv::Stager stager;
     s1kv::DevBuf scratch;             // split-K partials
     s1kv::DevBuf counters;            // split-K arrival counters (kept at zero)
-    s1kv::DevBuf late_meta;           // rows + work list planned after batch_begin
+    s1kv::Stager late_stager;         // rows + work lists planned after batch_begin, one segment a batch
     s1kv::DevBuf aside;               // 4-bit prefill: sums set aside by running CTAs, and their slots' locks
     s1kv::DevBuf io;                  // host-pointer step buffers: two slots
     // s1kv_batch_layer_host: inputs go up on copy_stream and outputs come back
@@ -375,6 +375,7 @@ struct s1kv_exchange {
 struct s1kv_batch {
     s1kv_pool* pool = nullptr;
     s1kv::StageSeg* seg = nullptr;
+    s1kv::StageSeg* late = nullptr;   // work list planned after batch_begin
     int64_t n_tokens = 0;     // appended tokens
     int64_t n_rows = 0;       // attention query rows
     int64_t n_items = 0;      // split-K work items

@@ -518,7 +518,7 @@ int s1kv_pool_destroy(s1kv_pool* p) {
         p->stager.destroy();
         p->scratch.destroy();
         p->counters.destroy();
-        p->late_meta.destroy();
+        p->late_stager.destroy();
         p->aside.destroy();
         p->io.destroy();
         if (p->k) cudaFree(p->k);

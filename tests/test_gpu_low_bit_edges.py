@@ -307,3 +307,28 @@ def test_products_one_behind_the_other(s1kv, cuda, m, k):
             c, s = LB.tokens8(x.cpu().numpy())
             np.testing.assert_array_equal(o.cpu().numpy(), LB.product8(c, s, w.data.cpu().numpy()[:, :k], w.scales.cpu().numpy()))
             o.zero_()
+
+
+# ----------------------------------------------- chunk batches side by side --
+
+@pytest.mark.parametrize("dtype,dim,bs", [("q4", 40, 16), ("q4", 128, 8), ("f32", 64, 16), ("bf16", 40, 16)])
+def test_chunk_batches_of_odd_shapes_keep_their_own_rows(s1kv, cuda, dtype, dim, bs):
+    """Shapes without a chunk kernel plan their rows at the first attention
+    call: another open batch's plan must not take their place."""
+    rng = np.random.default_rng(92)
+    hkv, hq = 2, 4
+    pool = s1kv.Pool(2, hkv, dim, 100, bs, dtype=dtype)
+    lens, rows = {0: 90, 1: 61}, {0: 7, 1: 11}
+    kvs = {i: kv(rng, n, hkv, dim) for i, n in lens.items()}
+    with pool.batch([0, 1], [90, 61], [0, 0]) as b:
+        for layer in (0, 1):
+            b.append(layer, *(dev(np.concatenate([kvs[0][j], kvs[1][j]])) for j in (0, 1)))
+    q = {i: rng.standard_normal((r, hq, dim)).astype(np.float32) for i, r in rows.items()}
+    open_ = {i: pool.batch([i], None, [rows[i]]) for i in (0, 1)}
+    got = [(i, open_[i].attention(layer, dev(q[i])).cpu().numpy()) for layer in (0, 1) for i in (0, 1)]
+    for b in open_.values():
+        b.end()
+    for i, o in got:
+        want = plain_rows(pool, *kvs[i], q[i])
+        assert np.abs(o - want).max() <= 2e-5 * np.abs(kvs[i][1]).max()
+    assert pool.check_device() == 0
