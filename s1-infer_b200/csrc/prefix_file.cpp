@@ -79,13 +79,19 @@ uint64_t payload_row(uint32_t dtype, uint64_t heads, uint64_t dim) {
     return dtype == S1KV_DTYPE_Q4 ? heads * (dim / 2 + 4) : heads * dim * (dtype == S1KV_DTYPE_F32 ? 4 : 2);
 }
 
-// Reads and checks a whole file: header, token ids, payload as fp32 and as
-// it stands in the file.
+// Reads and checks a whole file: header, token ids, payload as fp32.  With
+// `whole`, a 4-bit file is given back as it stands (its payload is the end)
+// and not widened.
 int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, std::vector<float>* payload,
-              std::vector<unsigned char>* raw = nullptr) {
+              std::vector<unsigned char>* whole = nullptr) {
     FILE* f = std::fopen(path, "rb");
     if (!f) return set_error(S1KV_EINVAL, "prefix file: cannot open %s", path);
     std::vector<unsigned char> all;
+    if (std::fseek(f, 0, SEEK_END) == 0) {
+        const long size = std::ftell(f);
+        if (size > 0) all.reserve((size_t)size);
+        std::rewind(f);
+    }
     unsigned char buf[1 << 16];
     size_t got;
     while ((got = std::fread(buf, 1, sizeof(buf), f)) > 0) all.insert(all.end(), buf, buf + got);
@@ -117,8 +123,9 @@ int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, st
         if (tok_bytes) std::memcpy(tokens->data(), p, tok_bytes);
     }
     p += tok_bytes;
-    if (raw) raw->assign(p, p + (body - tok_bytes));
-    if (payload) {
+    if (whole && hd->dtype == S1KV_DTYPE_Q4) {
+        *whole = std::move(all);
+    } else if (payload) {
         const uint64_t n = 2ull * hd->num_layers * (uint64_t)hd->n_tokens * row;
         payload->resize(n);
         if (hd->dtype == S1KV_DTYPE_F32) {
@@ -243,8 +250,8 @@ int s1kv_prefix_load_v1(s1kv_pool* p, uint64_t seq, const char* path, int32_t re
     FileHeader hd{};
     std::vector<int32_t> tokens;
     std::vector<float> payload;
-    std::vector<unsigned char> raw;
-    int st = read_file(path, &hd, &tokens, &payload, &raw);
+    std::vector<unsigned char> whole;  // a 4-bit file for a 4-bit pool: its rows go in as they are
+    int st = read_file(path, &hd, &tokens, &payload, p->desc.dtype == S1KV_DTYPE_Q4 ? &whole : nullptr);
     if (st) return st;
     if ((int32_t)hd.num_layers != p->desc.num_layers || (int32_t)hd.num_kv_heads != p->desc.num_kv_heads ||
         (int32_t)hd.head_dim != p->desc.head_dim)
@@ -264,13 +271,13 @@ int s1kv_prefix_load_v1(s1kv_pool* p, uint64_t seq, const char* path, int32_t re
     const int32_t na = (int32_t)n_tok, ql = 0;
     st = s1kv_batch_begin(p, &seq, &na, &ql, 1, nullptr, &b);
     if (st) return st;
-    float* d = nullptr;
-    cudaError_t e = cudaMalloc(&d, std::max<size_t>(2 * n, 1) * sizeof(float));
-    // a 4-bit file's rows go into a 4-bit pool as they are
-    const bool as_is = hd.dtype == S1KV_DTYPE_Q4 && p->desc.dtype == S1KV_DTYPE_Q4;
+    const bool as_is = !whole.empty();
     const size_t bytes = (size_t)n_tok * payload_row(hd.dtype, hd.num_kv_heads, hd.head_dim);
+    const unsigned char* rows = as_is ? whole.data() + whole.size() - 2 * bytes * hd.num_layers : nullptr;
+    float* d = nullptr;
+    cudaError_t e = cudaMalloc(&d, std::max<size_t>(as_is ? bytes : 2 * n * sizeof(float), 1));
     for (int32_t i = 0; i < 2 * p->desc.num_layers && as_is && e == cudaSuccess && st == S1KV_OK; i++) {
-        e = cudaMemcpy(d, raw.data() + bytes * i, bytes, cudaMemcpyHostToDevice);
+        e = cudaMemcpy(d, rows + bytes * i, bytes, cudaMemcpyHostToDevice);
         if (e == cudaSuccess) st = launch_rows_q4(p, i / 2, nullptr, b->d_slots, n_tok, i % 2, d, true, nullptr);
         if (e == cudaSuccess && st == S1KV_OK) e = cudaDeviceSynchronize();
     }

@@ -332,3 +332,46 @@ def test_chunk_batches_of_odd_shapes_keep_their_own_rows(s1kv, cuda, dtype, dim,
         want = plain_rows(pool, *kvs[i], q[i])
         assert np.abs(o - want).max() <= 2e-5 * np.abs(kvs[i][1]).max()
     assert pool.check_device() == 0
+
+
+# ------------------------------------------------------------- prefix files --
+
+LOAD = """
+import re, sys
+import torch
+import s1kv
+
+def status(key):
+    return int(re.search(key + r":\\s+(\\d+) kB", open("/proc/self/status").read()).group(1)) * 1024
+
+dtype, path, small, layers = sys.argv[1], sys.argv[2], sys.argv[3], int(sys.argv[4])
+pool = s1kv.Pool(layers, 8, 128, 600, 16, dtype=dtype)
+assert pool.prefix_load_v1(1, small) == 16
+before = status("VmRSS")
+assert pool.prefix_load_v1(2, path) == 4096
+print(status("VmHWM") - before)
+"""
+
+
+@pytest.mark.parametrize("dtype,layers,most", [("q4", 16, 2.0), ("f32", 4, 2.6)])
+def test_a_prefix_file_is_held_once(s1kv, cuda, tmp_path, dtype, layers, most):
+    """Host memory of a load: the file, and its rows in fp32 where the pool
+    takes those; a 4-bit file for a 4-bit pool is not widened."""
+    import os
+    import subprocess
+    import sys
+    torch = cuda
+    pool = s1kv.Pool(layers, 8, 128, 600, 16, dtype=dtype)
+    paths = []
+    for seq, n in ((1, 16), (2, 4096)):
+        with pool.batch([seq], [n], [0]) as b:
+            for layer in range(layers):
+                b.append(layer, *(torch.randn((n, 8, 128), device="cuda") for _ in range(2)))
+        paths.append(tmp_path / f"{seq}.s1kv")
+        pool.prefix_save_v1(seq, paths[-1], np.arange(n))
+    size = os.path.getsize(paths[1])
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(s1kv.__file__)))
+    r = subprocess.run([sys.executable, "-c", LOAD, dtype, str(paths[1]), str(paths[0]), str(layers)], env=env,
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert int(r.stdout) <= most * size + (32 << 20), (int(r.stdout), size)
