@@ -111,7 +111,9 @@ int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, st
     const uint64_t row_bytes = payload_row(hd->dtype, hd->num_kv_heads, hd->head_dim);
     const uint64_t tok_bytes = (hd->flags & kHasTokens) ? (uint64_t)hd->n_tokens * 4 : 0;
     const uint64_t body = tok_bytes + 2ull * hd->num_layers * (uint64_t)hd->n_tokens * row_bytes;
-    if (all.size() - kHeaderBytes != body)
+    // (in floating point too: the header's numbers may pass 64 bits together)
+    const double about = (double)tok_bytes + 2.0 * hd->num_layers * (double)hd->n_tokens * hd->num_kv_heads * hd->head_dim / 2;
+    if (all.size() - kHeaderBytes != body || about > (double)all.size())
         return set_error(S1KV_EINVAL, "prefix file %s: %llu payload bytes, header says %llu", path,
                          (unsigned long long)(all.size() - kHeaderBytes), (unsigned long long)body);
     Fnv fnv;
@@ -123,6 +125,17 @@ int read_file(const char* path, FileHeader* hd, std::vector<int32_t>* tokens, st
         if (tok_bytes) std::memcpy(tokens->data(), p, tok_bytes);
     }
     p += tok_bytes;
+    if (hd->dtype == S1KV_DTYPE_Q4) {
+        // What append writes: s from 0 up and m finite, or both NaN.
+        const uint64_t bytes = hd->head_dim / 2 + 4, n = (body - tok_bytes) / bytes;
+        for (uint64_t r = 0; r < n; r++) {
+            uint16_t sm[2];
+            std::memcpy(sm, p + r * bytes + bytes - 4, 4);
+            if ((sm[0] >= 0x7f80 || (sm[1] & 0x7fff) >= 0x7f80) && !(sm[0] == 0x7fc0 && sm[1] == 0x7fc0))
+                return set_error(S1KV_EINVAL, "prefix file %s: row %llu is not a 4-bit row (s 0x%04x, m 0x%04x)", path,
+                                 (unsigned long long)r, sm[0], sm[1]);
+        }
+    }
     if (whole && hd->dtype == S1KV_DTYPE_Q4) {
         *whole = std::move(all);
     } else if (payload) {
