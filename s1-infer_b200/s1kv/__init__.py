@@ -199,13 +199,18 @@ def device_check(device=0):
 
 # ==================================================================== Pool ==
 
+_POOL_DTYPES = {"f32": DTYPE_F32, "fp32": DTYPE_F32, "float32": DTYPE_F32, str(DTYPE_F32): DTYPE_F32, "bf16": DTYPE_BF16,
+                "bfloat16": DTYPE_BF16, str(DTYPE_BF16): DTYPE_BF16, "q4": DTYPE_Q4, str(DTYPE_Q4): DTYPE_Q4}
+
+
 class Pool:
     """A device-resident block pool of ``num_layers`` layers sharing one block
     table per sequence (include/s1kv.h)."""
 
     def __init__(self, num_layers, num_kv_heads, head_dim, max_blocks, block_size=16, dtype="f32", device=None,
                  max_seqs=1024, max_seq_len=0, rope_theta=1.0e6, initial_free_list=None, host_only=False):
-        """dtype "f32", "bf16" or "q4" (4 bits a value, S1KV_DTYPE_Q4).  device
+        """dtype "f32", "bf16" or "q4" (4 bits a value, S1KV_DTYPE_Q4), the
+        DTYPE_* numbers, or torch's float32 and bfloat16.  device
         None = torch's current CUDA device (0 for a host-only pool)."""
         self.L = lib()
         if device is None:
@@ -216,8 +221,9 @@ class Pool:
                 device = torch.cuda.current_device()
         self.num_layers, self.Hkv, self.D = num_layers, num_kv_heads, head_dim
         self.max_blocks, self.bs = max_blocks, block_size
-        self.dtype = (DTYPE_F32 if dtype in ("f32", "fp32", "float32", DTYPE_F32) else
-                      DTYPE_Q4 if dtype in ("q4", DTYPE_Q4) else DTYPE_BF16)
+        self.dtype = _POOL_DTYPES.get(str(dtype).removeprefix("torch."))
+        if self.dtype is None:
+            raise S1KVError(EINVAL, f"Pool: dtype {dtype!r} (\"f32\", \"bf16\" or \"q4\")")
         self.device = device
         d = PoolDesc(num_layers, num_kv_heads, head_dim, block_size, max_blocks, self.dtype, max_seqs, max_seq_len,
                      rope_theta, POOL_HOST_ONLY if host_only else 0, None)

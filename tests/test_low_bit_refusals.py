@@ -39,3 +39,20 @@ def test_sizes_that_pass_64_bits(s1kv, tmp_path, n, heads, dim, layers, dtype):
     with pytest.raises(s1kv.S1KVError) as e:
         s1kv.prefix_file_info(q4_file(tmp_path / "a", b"", n, heads, dim, layers, dtype))
     assert e.value.status == s1kv.EINVAL
+
+
+@pytest.mark.parametrize("dtype", ["int4", "Q4", "q8", "float16", "half", "", 3, None, "fp8"])
+def test_pools_of_an_unknown_type(s1kv, dtype):
+    with pytest.raises(s1kv.S1KVError) as e:
+        s1kv.Pool(1, 2, 64, 4, 16, dtype=dtype, host_only=True)
+    assert e.value.status == s1kv.EINVAL and "dtype" in str(e.value)
+
+
+def test_pools_of_known_types(s1kv):
+    import torch
+    for dtypes, want in ((("f32", "fp32", "float32", 0, torch.float32), s1kv.DTYPE_F32),
+                         (("bf16", "bfloat16", 1, torch.bfloat16), s1kv.DTYPE_BF16), (("q4", 2), s1kv.DTYPE_Q4)):
+        for d in dtypes:
+            pool = s1kv.Pool(1, 2, 64, 4, 16, dtype=d, host_only=True)
+            assert pool.dtype == want
+            pool.close()
