@@ -264,11 +264,14 @@ struct Stager {
     void destroy();
 };
 
-// Growable device buffer.  Growth is geometric and keeps the smaller buffers
-// until destroy(): a captured graph may still use them.
+// Growable device buffer.  Growth is geometric.  The smaller buffers stay until
+// destroy(), as a captured graph may still use them, unless no graph can hold
+// them (keep = false).
 struct DevBuf {
     void* p = nullptr;
     size_t cap = 0;
+    size_t held = 0;  // bytes of p and old
+    bool keep = true;
     std::vector<void*> old;
     int ensure(size_t bytes);
     void destroy();
@@ -347,7 +350,7 @@ struct s1kv_pool {
     s1kv::DevBuf counters;            // split-K arrival counters (kept at zero)
     s1kv::Stager late_stager;         // rows + work lists planned after batch_begin, one segment a batch
     s1kv::DevBuf aside;               // 4-bit prefill: sums set aside by running CTAs, and their slots' locks
-    s1kv::DevBuf io;                  // host-pointer step buffers: two slots
+    s1kv::DevBuf io;                  // host-pointer step buffers: two slots (their events and streams keep them out of a capture)
     // s1kv_batch_layer_host: inputs go up on copy_stream and outputs come back
     // on d2h_stream, overlapped with the kernels of neighbouring calls.
     // io_ev: [0,1] inputs of slot s landed, [2,3] slot s's kernels done,

@@ -126,11 +126,13 @@ int DevBuf::ensure(size_t bytes) {
     if (cap >= bytes) return S1KV_OK;
     S1KV_CUDA(cudaDeviceSynchronize());
     const size_t c = std::max<size_t>({bytes + bytes / 4, 2 * cap, size_t(16) << 20});
+    if (!keep) destroy();
     void* np = nullptr;
     S1KV_CUDA(cudaMalloc(&np, c));
     if (p) old.push_back(p);
     p = np;
     cap = c;
+    held += c;
     return S1KV_OK;
 }
 
@@ -139,7 +141,7 @@ void DevBuf::destroy() {
     for (void* o : old) cudaFree(o);
     old.clear();
     p = nullptr;
-    cap = 0;
+    cap = held = 0;
 }
 
 // ------------------------------------------------------ block primitives --
@@ -422,6 +424,7 @@ int s1kv_pool_create(const s1kv_pool_desc* d, int device, s1kv_pool** out) {
     int64_t slots = d->max_blocks * (int64_t)d->block_size;
     if (slots > INT32_MAX) return set_error(S1KV_EINVAL, "s1kv_pool_create: more than 2^31 slots per layer");
     auto* p = new s1kv_pool();
+    p->io.keep = false;
     p->desc = *d;
     p->desc.initial_free_list = nullptr;
     if (p->desc.max_seqs <= 0) p->desc.max_seqs = 1024;
@@ -549,8 +552,8 @@ int s1kv_pool_stats_get(const s1kv_pool* p, s1kv_pool_stats* out) {
     out->evictions = p->evictions;
     out->device_bytes = p->host_only ? 0
                                      : (int64_t)(2 * p->layer_bytes * p->desc.num_layers +
-                                                 (size_t)p->desc.max_seqs * p->max_bps * 4 + p->scratch.cap +
-                                                 p->aside.cap + p->io.cap);
+                                                 (size_t)p->desc.max_seqs * p->max_bps * 4 + p->scratch.held +
+                                                 p->counters.held + p->aside.held + p->io.held);
     return S1KV_OK;
 }
 

@@ -375,3 +375,41 @@ def test_a_prefix_file_is_held_once(s1kv, cuda, tmp_path, dtype, layers, most):
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
     assert int(r.stdout) <= most * size + (32 << 20), (int(r.stdout), size)
+
+
+# ------------------------------------------------------------ device memory --
+
+@pytest.mark.parametrize("dtype", ["q4", "bf16"])
+def test_device_bytes_are_what_the_pool_holds(s1kv, cuda, dtype):
+    """Host-buffer steps and split rows of growing size: the statistic follows
+    the device's free memory, and outgrown host-step buffers are given back."""
+    torch = cuda
+    hkv, hq, dim = 8, 32, 128
+    sizes = (100, 900, 3000)
+    pool = s1kv.Pool(1, hkv, dim, 3000, 16, dtype=dtype, max_seqs=300)
+    h = [torch.randn((sizes[-1], x, dim)).pin_memory() for x in (hq, hkv, hkv)]
+    out = torch.empty_like(h[0]).pin_memory()
+    long = torch.randn((40000, hkv, dim), device="cuda")
+    q = torch.randn((256, hq, dim), device="cuda")
+    o = torch.empty_like(q)
+    with pool.batch([999], [40000], [0]) as b:
+        b.append(0, long, long)
+    torch.cuda.synchronize()
+    free, told = torch.cuda.mem_get_info()[0], pool.stats()["device_bytes"]
+    slot = 0
+    for i, n in enumerate(sizes):
+        with pool.batch([i], [n]) as b:
+            b.layer_host(0, *(x[:n] for x in h), out[:n], hq)
+        torch.cuda.synchronize()
+        slot = 4 * n * dim * (3 * hq + 2 * hkv)
+        for s in range(1000, 1000 + (1, 16, 250)[i]):
+            if not pool.length(s):
+                pool.fork(999, s, 40000)
+        seqs = list(range(1000, 1000 + (1, 16, 250)[i]))
+        with pool.batch(seqs, None, [1] * len(seqs)) as b:
+            b.attention(0, q[:len(seqs)], o[:len(seqs)])
+        torch.cuda.synchronize()
+        held = free - torch.cuda.mem_get_info()[0]
+        assert abs(held - (pool.stats()["device_bytes"] - told)) <= 48 << 20
+    grown = pool.stats()["device_bytes"] - told
+    assert 2 * slot <= grown
