@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_q4_kernel(const __grid_co
                 const int at = (int)((sm_id + i) % p.n_aside);
                 if (atomicCAS(&p.aside_lock[at], 0, 1) == 0) got = at;
             }
+            __threadfence();  // what the slot's last CTA left lies behind
         }
         *aside_slot = got;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
