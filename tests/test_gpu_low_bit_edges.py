@@ -89,6 +89,18 @@ def test_keys_of_scales_far_apart(s1kv, cuda, dim, r):
     attend_and_check(s1kv, k, v, r, 8)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("r", [1, 40, 200])
+@pytest.mark.parametrize("at,grow", [(230, 24), (230, 40), (230, 90), (100, 40), (299, 40), (0, 60)])
+def test_a_large_key(s1kv, cuda, dim, r, at, grow):
+    """One key 2^24 to 2^90 larger: a row that sees it gives it all its weight or
+    none, rows before it are as they would be without."""
+    rng = np.random.default_rng(79)
+    k, v = kv(rng, 300, 2, dim)
+    k[at] *= np.float32(2.0 ** grow)
+    attend_and_check(s1kv, k, v, r, 8)
+
+
 # ------------------------------------------------- values of far-off scales --
 
 @pytest.mark.parametrize("dim", [64, 128])
@@ -413,3 +425,71 @@ def test_device_bytes_are_what_the_pool_holds(s1kv, cuda, dtype):
         assert abs(held - (pool.stats()["device_bytes"] - told)) <= 48 << 20
     grown = pool.stats()["device_bytes"] - told
     assert 2 * slot <= grown
+
+
+# --------------------------------------------------- addresses and alignment --
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("g", [4, 8])
+@pytest.mark.parametrize("r", [1, 50])
+def test_pointers_of_four_bytes(s1kv, cuda, dim, g, r):
+    """k, v, q and out that are aligned to their elements only; what lies
+    before and behind out stays."""
+    torch = cuda
+    rng = np.random.default_rng(93)
+    hkv, n = 2, 130
+    k, v = kv(rng, n, hkv, dim)
+    q = rng.standard_normal((r, g * hkv, dim)).astype(np.float32)
+
+    def odd(x, fill=None):
+        buf = torch.full((x.size + 2,), 7.0, device="cuda")
+        t = buf[1:-1].view(x.shape)
+        if fill is None:
+            t.copy_(torch.from_numpy(x))
+        return t, buf
+
+    pool = pool_of(s1kv, hkv, dim, 14)
+    with pool.batch([0], [n], [0]) as b:
+        b.append(0, odd(k)[0], odd(v)[0])
+        for which, x in ((s1kv.K, k), (s1kv.V, v)):
+            np.testing.assert_array_equal(b.gather(0, which, odd(k, 0)[0]).cpu().numpy(), LB.q4_values(x))
+    out, buf = odd(q, 0)
+    with pool.batch([0], None, [r]) as b:
+        b.attention(0, odd(q)[0], out)
+    check_rows(out.cpu().numpy(), q, k, v)
+    assert buf[0] == 7 and buf[-1] == 7
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_blocks_beyond_four_gigabytes(s1kv, cuda, dim):
+    rng = np.random.default_rng(94)
+    hkv, hq, n = 8, 16, 300
+    blocks = (9 << 29) // (hkv * 16 * (dim // 2 + 4))  # 4.5 GB of K, and of V
+    pool = s1kv.Pool(1, hkv, dim, blocks, 16, dtype="q4", max_seqs=4, max_seq_len=4096)  # (the last blocks come first)
+    k, v = kv(rng, n, hkv, dim)
+    q = rng.standard_normal((70, hq, dim)).astype(np.float32)
+    fill(pool, [n], k, v)
+    assert pool.block_table(0).min() > blocks - 40
+    for which, x in ((s1kv.K, k), (s1kv.V, v)):
+        np.testing.assert_array_equal(pool.gather(0, 0, which).cpu().numpy(), LB.q4_values(x))
+    for r in (1, 70):
+        check_rows(pool.attention(0, [0], [r], dev(q[:r]), hq).cpu().numpy(), q[:r], k, v)
+    assert pool.check_device() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunks_over_long_contexts(s1kv, cuda, dim):
+    """More tokens than a CTA keeps block ids of (16384), with and without the
+    tiles split over CTAs."""
+    rng = np.random.default_rng(95)
+    hkv, hq, n = 4, 16, 19000
+    k, v = kv(rng, n, hkv, dim)
+    pool = pool_of(s1kv, hkv, dim, 1200)
+    fill(pool, [n], k, v)
+    for r in (5, 2600):
+        q = rng.standard_normal((r, hq, dim)).astype(np.float32)
+        got = pool.attention(0, [0], [r], dev(q), hq).cpu().numpy()
+        for row in {0, r // 2, r - 1}:
+            seen = n - r + row + 1
+            check_rows(got[row:row + 1, :4], q[row:row + 1, :4], k[:seen, :1], v[:seen, :1])
+            check_rows(got[row:row + 1, 12:], q[row:row + 1, 12:], k[:seen, 3:], v[:seen, 3:])
