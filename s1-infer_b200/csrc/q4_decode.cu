@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
         // 2^(133 - E) puts the largest in [2^6, 2^7)
         float vmul = __uint_as_float((uint32_t)(260 - kMinExp) << 23);
         auto exponent_v = [&] { return 260 - (int)(__float_as_uint(vmul) >> 23); };  // E
-        int done = 0;
-        for (int k = 0; k < pairs; k++) {
+        int k = 0;
+        for (; k < pairs; k++) {
             const int it = it0 + k, stage = it % kNS;
             // Each lane polls for itself; a timeout goes into the vote below, so that
             // the warp leaves as one.
@@ -298,10 +298,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                 load_words<NWD>(at + gq * (D / 2) + tq * (4 * NWD), k0);
                 load_words<NWD>(at + (gq + 8) * (D / 2) + tq * (4 * NWD), k1);
                 const uint32_t* kp = reinterpret_cast<const uint32_t*>(at + kParams) + gq;
-                const uint32_t* vp = reinterpret_cast<const uint32_t*>(at + kTileBytes + kParams) + gq;
                 const float2 ka = q4_unpack(kp[0]), kb = q4_unpack(kp[8]);
-                va[u] = q4_unpack(vp[0]);
-                vb[u] = q4_unpack(vp[8]);
                 float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int wi = 0; wi < NWD; wi++) {
@@ -326,11 +323,18 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                 x[u][0] = __ffma2_rn(make_float2(ka.x, ka.x), __fmul2_rn(s0, un2), __fmul2_rn(make_float2(ka.y, ka.y), qs2));
                 x[u][1] = __ffma2_rn(make_float2(kb.x, kb.x), __fmul2_rn(s1, un2), __fmul2_rn(make_float2(kb.y, kb.y), qs2));
             }
-            if (rest < 2 * kTile) {  // rows past the end hold anything, NaN included
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint32_t* vp = reinterpret_cast<const uint32_t*>(kt + (2 * u + 1) * kTileBytes + kParams) + gq;
+                va[u] = q4_unpack(vp[0]);
+                vb[u] = q4_unpack(vp[8]);
+            }
+            if (rest < 2 * kTile) {  // rows past the end hold anything, NaN included: score -inf, s_v even with E, m_v 0
+                const float2 past = make_float2(__uint_as_float((260u << 23) - __float_as_uint(vmul)), 0.0f);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    if (16 * u + gq >= rest) x[u][0] = make_float2(-INFINITY, -INFINITY), va[u] = make_float2(0.f, 0.f);
-                    if (16 * u + gq + 8 >= rest) x[u][1] = make_float2(-INFINITY, -INFINITY), vb[u] = make_float2(0.f, 0.f);
+                    if (16 * u + gq >= rest) x[u][0] = make_float2(-INFINITY, -INFINITY), va[u] = past;
+                    if (16 * u + gq + 8 >= rest) x[u][1] = make_float2(-INFINITY, -INFINITY), vb[u] = past;
                 }
             }
             // the reference max of a head moves only when a score outgrows it
@@ -342,10 +346,7 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             const float least = fminf(fminf(va[0].x, vb[0].x), fminf(va[1].x, vb[1].x));
             if (__any_sync(kFull, mx0 > m0 + kRescaleAt || mx1 > m1 + kRescaleAt || most * vmul >= 128.0f || least * vmul < 64.0f / (1 << kEven) ||
                                   late)) {
-                if (__any_sync(kFull, late)) {
-                    failed = true;
-                    break;
-                }
+                if (__any_sync(kFull, late)) break;
                 // The reference is one for the weights p s_v, which must fit fp16:
                 // scores plus V's exponents relative to E (down to -kFar).  A V row
                 // that is hardly weighed then takes no bits from the others,
@@ -398,7 +399,6 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
                     o[mb][3] *= c1;
                 }
             }
-            done = k + 1;
             // p, then p s_v in two fp16 parts: rows of P^T, transposed in
             // registers into the B fragments of O^T += V^T P^T.  NT = 1: lanes
             // of columns 0-3 give the high part, of 4-7 the low part.
@@ -477,10 +477,11 @@ __global__ void __launch_bounds__(kNW * 32, ctas_per_sm(D)) decode_q4_kernel(con
             }
         }
 
-        if (failed && pairs > 0) {
+        if (k < pairs) {  // pair k did not come
             // copies still in flight land before the CTA exits (bounded)
             if (lane == 0) atomicOr(p.err, kErrTimeout);
-            for (int k = done; k < min(pairs, done + kNS); k++) bar_wait(bars + 8 * ((it0 + k) % kNS), (uint32_t)(((it0 + k) / kNS) & 1));
+            failed = true;
+            for (int i = k; i < min(pairs, k + kNS); i++) bar_wait(bars + 8 * ((it0 + i) % kNS), (uint32_t)(((it0 + i) / kNS) & 1));
             m0 = m1 = -INFINITY;
             l2 = z2 = make_float2(0.f, 0.f);
         }
