@@ -59,7 +59,8 @@ extern "C" {
                              A row holding a NaN or an infinity, or whose m or s passes bf16's largest (3.39e38),
                              reads back as NaN throughout.  head_dim a multiple of 8 up to 256, block_size a multiple
                              of 4.  Every call of a pool takes it; attention reads the held values with
-                             fp32-level accuracy.  The no-allocation decode takes F32 and BF16 storage only. */
+                             fp32-level accuracy (rows of V that weigh and are smaller than 2^-80 of the largest
+                             seen or unseen one lose bits).  The no-allocation decode takes F32 and BF16 storage only. */
 
 /* ---- pool flags ---- */
 #define S1KV_POOL_HOST_ONLY 1 /* bookkeeping only: no device memory; kernel calls fail */

@@ -13,12 +13,14 @@
 //
 // Precision: q (times log2(e) / sqrt(D)) and p s_v are each split into two
 // fp16 parts, 22 bits, of values scaled by a power of two that puts the
-// largest at 2^15: scores and outputs carry fp32-level error.
+// largest of a head's q, or of its weights p s_v so far, at 2^15: scores and
+// outputs carry fp32-level error, whatever other heads or V rows that hardly
+// weigh hold (V rows down to 2^kFar below the largest).
 //
 // Layout: one 16-token tile of a KV head is 16 D / 2 + 64 bytes of K and as
 // many of V, contiguous, and the storage order is the fragments' own: a lane's
-// codes of the whole tile are two 16-byte reads of K and two of V (D = 128),
-// without bank conflicts.  Each warp brings pairs of tiles, two bulk copies a
+// codes of the whole tile are two 16-byte reads of K and two of V (D = 128; V's
+// meet four to a bank).  Each warp brings pairs of tiles, two bulk copies a
 // tile, into a ring of its own in shared memory, kNS pairs ahead, and takes a
 // pair at a time: what a step costs besides the codes (waits, the maximum's
 // vote) is shared by 32 tokens.
@@ -37,10 +39,10 @@
 // token range) of one KV head, its 4 warps the range's tiles in turn; warps
 // merge through shared memory, splits through combine.cuh.
 //
-// Bound: K's and V's bytes, and the instructions that widen them (46% of the
-// issue slots, ALU 45%, 16 warps an SM): 64 rows of 8192 tokens, 32 heads on 8
-// of 128, 136 us, 4.2 TB/s (bf16 pools: 314 us); 2 of 131072, 64 heads, 97 us,
-// 2.9 TB/s; 16 of up to 8192, 27 us.
+// Bound: nothing is full (46% of the issue slots, ALU 45% with widening, memory
+// 57% of the copy rate, 16 warps an SM that wait for their own chain of loads,
+// products and votes): 64 rows of 8192 tokens, 32 heads on 8 of 128, 138 us, 4.1
+// TB/s (bf16 pools: 314 us); 2 of 131072, 64 heads, 98 us, 2.9 TB/s.
 #include <cmath>
 
 #include "combine.cuh"

@@ -919,14 +919,14 @@ int launch_gemv(const float* x, int x_len, const int8_t* xq, const float* sx, in
 // us and 12.9, 59 MB 18.6 and 16.5, 67 MB 24.3 and 19.1; 32 tokens, 4 MB 6.0 and
 // 8.0, 25 MB 13.7 and 12.3, 59 MB 29 and 16); above, the tensor-core tiles.
 // NT is the least that holds the tokens (256 at most), halved down to 64 while
-// there are fewer than 90 tiles (256 tokens, K = 4096, 6144 channels: 96 tiles of
-// 128 tokens 15.6 us, 192 of 64 19.8; 4096 channels: 64 tiles 15.0, 128 of 64
-// 12.6); then K is split over a cluster, at least two stages a CTA, two CTAs an
-// SM, if the tiles are fewer than two thirds of the SMs (64 tokens, K = 4096: 48
-// tiles 10.1 us split in four, 12.6 unsplit; 112 tiles 16.5 in two, 15.5
-// unsplit).  NT = 256 runs on pairs of SMs (8001 tokens, K = 4096, 14336 channels:
-// 324 us, 2.9e15 operations a second, 88% of twice the bf16 matrix rate; 342 us
-// in tiles of one SM; 8192^3: 3.2e15, 98%).
+// there are fewer than 90 tiles (products alone: 256 tokens, K = 4096, 6144
+// channels: 96 tiles of 128 tokens 12.7 us, 192 of 64 20.0; 4096 channels: 32
+// tiles of 256 tokens 14.8, 128 of 64 11.3); then K is split over a cluster, at
+// least two stages a CTA, two CTAs an SM, if the tiles are fewer than two thirds of
+// the SMs (64 tokens, K = 4096: 48 tiles 9.4 us split in four, 10.8 unsplit; 112
+// tiles 12.0 in two, 11.4 unsplit).  NT = 256 runs on pairs of SMs (8001 tokens, K
+// = 4096, 14336 channels: 326 us, 2.9e15 operations a second, 88% of twice the bf16
+// matrix rate; 442 us in tiles of 128 tokens of one SM; 8192^3: 3.3e15, 99%).
 // x (optional, rows of x_len values): the tokens that xq and sx will hold; they
 // are quantised here first, or by the weight stream itself.
 int matmul_w8a8(const float* x, int x_len, int8_t* xq, float* sx, int M, int K, W8Group& grp, cudaStream_t stream) {
